@@ -1,0 +1,170 @@
+// C-ABI host dispatch of the serving operators (include/fav4_serving.h): the
+// argument checks, before any HIP call, and the launches.
+#include "fav4_serving.h"
+#include "serving_kernel.hpp"
+
+#include <algorithm>
+#include <atomic>
+#include <climits>
+#include <cmath>
+#include <cstdint>
+
+namespace {
+
+constexpr int64_t MAX_GRID = int64_t(1) << 22;
+constexpr int64_t MAX_BYTES = int64_t(1) << 48;
+
+// CU count of the current device (256 if it cannot be read), cached per
+// device after the first query.
+int device_cus() {
+    static std::atomic<int> cache[64];
+    int dev = 0, cus = 0;
+    if (hipGetDevice(&dev) != hipSuccess) return 256;
+    const bool slot = dev >= 0 && dev < 64;
+    if (slot && (cus = cache[dev].load(std::memory_order_relaxed)) > 0) return cus;
+    if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus <= 0) cus = 256;
+    if (slot) cache[dev].store(cus, std::memory_order_relaxed);
+    return cus;
+}
+
+template <class... P>
+bool aligned(uintptr_t to, P... p) {
+    return ((... | reinterpret_cast<uintptr_t>(p)) & (to - 1)) == 0;
+}
+
+// ---- append ------------------------------------------------------------------
+bool append_ok(const Fav4AppendArgs* a) {
+    if (!a || !a->k || !a->v || !a->k_cache || !a->v_cache || !a->cu_seqlens_q || !a->seqlens_k || !a->block_table ||
+        !a->q != !a->q_out)
+        return false;
+    if (a->batch < 1 || a->heads < 1 || a->kv_heads < 1 || a->total_q < 1 || a->num_pages < 1 || a->page_size < 1 ||
+        a->max_pages_per_seq < 1 || a->rotary_dim < 0 || a->rotary_dim > fav4::D || a->rotary_dim % 16 ||
+        (a->interleaved != 0 && a->interleaved != 1))
+        return false;
+    if (a->rotary_dim > 0 ? !a->cos || !a->sin || a->rotary_rows < 1 : a->cos || a->sin) return false;
+    const int64_t rows = (a->q ? int64_t(a->heads) : 0) + 2 * int64_t(a->kv_heads);
+    if (rows * a->total_q > INT_MAX) return false;
+    auto stride_ok = [&](long long stride, int heads) {
+        return stride >= int64_t(heads) * fav4::D && (stride & 7) == 0 &&
+               static_cast<__int128>(stride) * a->total_q * 2 < MAX_BYTES;
+    };
+    if (!stride_ok(a->k_stride, a->kv_heads) || !stride_ok(a->v_stride, a->kv_heads)) return false;
+    if (a->q && (!stride_ok(a->q_stride, a->heads) || !stride_ok(a->q_out_stride, a->heads) ||
+                 (a->q == a->q_out && a->q_stride != a->q_out_stride)))
+        return false;
+    if (static_cast<__int128>(a->num_pages) * a->page_size * a->kv_heads * fav4::ROW_BYTES >= MAX_BYTES) return false;
+    return aligned(16, a->q, a->k, a->v, a->q_out, a->k_cache, a->v_cache, a->cos, a->sin) &&
+           aligned(4, a->cu_seqlens_q, a->seqlens_k, a->block_table, a->positions);
+}
+
+// ---- attention behind shared prefixes ------------------------------------------
+constexpr int BOTTOM_RIGHT = 2;
+constexpr int WAVES = 4, BM = WAVES * 32, BN = 64;
+constexpr int MIN_TILES = 4;
+
+bool prefix_shape_ok(const Fav4PrefixArgs* args, int causal) {
+    if (!args) return false;
+    const Fav4PagedArgs& a = args->paged;
+    if (a.batch < 1 || a.heads < 1 || a.kv_heads < 1 || a.heads % a.kv_heads || a.max_seqlen_q < 1 ||
+        a.max_seqlen_k < 1 || a.total_q < 1 || a.total_k < 0 || a.num_pages < 1 || a.page_size < 1 ||
+        a.max_pages_per_seq < 1 || args->num_prefixes < 1 || args->max_pages_per_prefix < 1 ||
+        (causal != 0 && causal != BOTTOM_RIGHT) || !std::isfinite(a.scale) || a.scale <= 0)
+        return false;
+    if (a.page_size % 32 || a.max_seqlen_k > int64_t(a.max_pages_per_seq) * a.page_size ||
+        a.heads > INT_MAX / fav4::D || int64_t(a.total_q) * a.heads > INT_MAX ||
+        int64_t(a.kv_heads) * fav4::ROW_BYTES * 32 > INT_MAX ||
+        static_cast<__int128>(a.num_pages) * a.page_size * a.kv_heads * fav4::ROW_BYTES >= MAX_BYTES)
+        return false;
+    return true;
+}
+
+struct PrefixSizes {
+    fav4::PrefixPlan plan;
+    int64_t part_rows, note_rows, bytes;
+    bool ok;
+};
+PrefixSizes prefix_sizes(const Fav4PrefixArgs& args, int causal) {
+    const Fav4PagedArgs& a = args.paged;
+    const int64_t group = a.heads / a.kv_heads, rows = a.total_q * group;
+    PrefixSizes s{};
+    s.plan.br = causal == BOTTOM_RIGHT;
+    s.plan.ranges = std::max(1, 2 * device_cus() / a.kv_heads);
+    s.plan.min_tiles = MIN_TILES;
+    // Row tiles that the rows of n families can have.
+    auto tiles = [&](int64_t n, int64_t most) {
+        return std::min(n * ((most + BM - 1) / BM), (rows + n * (BM - 1)) / BM);
+    };
+    const int64_t own_rows = std::min<int64_t>(BM, a.max_seqlen_q * group);
+    const int64_t prefix_segs = tiles(args.num_prefixes, rows), own_segs = tiles(a.batch, a.max_seqlen_q * group);
+    const int64_t prefix_keys = std::min<int64_t>(int64_t(args.max_pages_per_prefix) * a.page_size, a.max_seqlen_k);
+    const int64_t extra = 1 + fav4::SEG_TILES;
+    const int64_t prefix_blocks = prefix_segs + s.plan.ranges, own_blocks = own_segs + s.plan.ranges;
+    s.part_rows = a.kv_heads * (prefix_blocks * BM + own_blocks * own_rows);
+    s.ok = prefix_segs * (prefix_keys / BN + extra) + own_segs * (a.max_seqlen_k / BN + extra) < (1 << 30) &&
+           prefix_blocks * BM <= INT_MAX && own_blocks * own_rows <= INT_MAX;
+    s.plan.prefix_blocks = int(prefix_blocks);
+    s.plan.own_blocks = int(own_blocks);
+    s.plan.own_rows = int(own_rows);
+    s.note_rows = rows;
+    s.bytes = s.part_rows * (fav4::D * 4 + 8) + s.note_rows * 16;
+    return s;
+}
+
+template <bool LSE>
+void launch_prefix(const Fav4PrefixArgs& args, const fav4::PrefixPlan& plan, hipStream_t stream) {
+    const dim3 grid(unsigned(args.paged.kv_heads) * unsigned(plan.ranges));
+    hipLaunchKernelGGL((fav4::prefix_kernel<LSE, WAVES>), grid, dim3(WAVES * 64), 0, stream, args, plan);
+}
+
+}  // namespace
+
+extern "C" __attribute__((visibility("default"))) int fav4_bshd_append_paged(const Fav4AppendArgs* a,
+                                                                            hipStream_t stream) {
+    if (!append_ok(a)) return hipErrorInvalidValue;
+    const int rows = (a->q ? a->heads : 0) + 2 * a->kv_heads, units = (rows + 7) / 8;
+    const int64_t total = int64_t(units) * a->total_q, blocks = std::min((total + 3) / 4, MAX_GRID);
+    if (a->interleaved)
+        hipLaunchKernelGGL(fav4::append_kernel<true>, dim3(unsigned(blocks)), dim3(256), 0, stream, *a, units, total);
+    else
+        hipLaunchKernelGGL(fav4::append_kernel<false>, dim3(unsigned(blocks)), dim3(256), 0, stream, *a, units, total);
+    return hipGetLastError();
+}
+
+extern "C" __attribute__((visibility("default"))) long long fav4_bshd_prefix_paged_workspace_size(
+    const Fav4PrefixArgs* args, int causal) {
+    if (!prefix_shape_ok(args, causal)) return -1;
+    const PrefixSizes s = prefix_sizes(*args, causal);
+    return s.ok ? s.bytes : -1;
+}
+
+extern "C" __attribute__((visibility("default"))) int fav4_bshd_forward_prefix_paged(const Fav4PrefixArgs* args,
+                                                                                    int causal, void* workspace,
+                                                                                    size_t workspace_bytes,
+                                                                                    hipStream_t stream) {
+    if (!prefix_shape_ok(args, causal)) return hipErrorInvalidValue;
+    const Fav4PagedArgs& a = args->paged;
+    if (!a.q || !a.k_cache || !a.v_cache || !a.o || !a.cu_seqlens_q || !a.seqlens_k || !a.block_table ||
+        !args->prefix_table || !args->prefix_lens || !args->cu_prefix_seqs ||
+        !aligned(16, a.q, a.k_cache, a.v_cache, a.o) ||
+        !aligned(4, a.lse, a.cu_seqlens_q, a.seqlens_k, a.block_table, args->prefix_table, args->prefix_lens,
+                 args->cu_prefix_seqs))
+        return hipErrorInvalidValue;
+    PrefixSizes s = prefix_sizes(*args, causal);
+    if (!s.ok || !workspace || !aligned(256, workspace) || uint64_t(s.bytes) > workspace_bytes)
+        return hipErrorInvalidValue;
+    s.plan.o_part = static_cast<float*>(workspace);
+    s.plan.lse_part = s.plan.o_part + s.part_rows * fav4::D;
+    s.plan.notes = reinterpret_cast<int2*>(s.plan.lse_part + s.part_rows * 2);
+    if (a.lse) launch_prefix<true>(*args, s.plan, stream);
+    else launch_prefix<false>(*args, s.plan, stream);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    const int64_t rows = int64_t(a.total_q) * a.heads;
+    const int per = rows <= 2048 ? 4 : 1;
+    const unsigned blocks = unsigned(std::min((rows * per + 7) / 8, MAX_GRID));
+    if (per == 4)
+        hipLaunchKernelGGL(fav4::prefix_merge_kernel<4>, dim3(blocks), dim3(256), 0, stream, *args, s.plan, BM);
+    else
+        hipLaunchKernelGGL(fav4::prefix_merge_kernel<1>, dim3(blocks), dim3(256), 0, stream, *args, s.plan, BM);
+    return hipGetLastError();
+}

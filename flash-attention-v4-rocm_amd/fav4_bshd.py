@@ -34,6 +34,7 @@ HIPCC_FLAGS = [
 ]
 KAT_LIB_PATH = ROOT / "build" / "libfav4_loader_kat.so"
 CEILING_LIB_PATH = ROOT / "build" / "libfav4_mfma_ceiling.so"
+SERVING_LIB_PATH = ROOT / "build" / "libfav4_serving.so"
 RESOURCE_LOG = ROOT / "build" / "resource-usage.txt"
 MANIFEST = ROOT / "build" / "build-manifest.json"
 
@@ -56,6 +57,22 @@ class PagedArgs(C.Structure):
                                           "block_table")] + [
         (n, C.c_int) for n in ("batch", "heads", "kv_heads", "max_seqlen_q", "max_seqlen_k", "total_q", "total_k",
                                "num_pages", "page_size", "max_pages_per_seq")] + [("scale", C.c_float)]
+
+
+class AppendArgs(C.Structure):
+    """``struct Fav4AppendArgs`` (include/fav4_serving.h): 12 pointers, 4 long longs, 10 ints."""
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v", "q_out", "k_cache", "v_cache", "cos", "sin", "cu_seqlens_q",
+                                          "seqlens_k", "block_table", "positions")] + [
+        (n, C.c_longlong) for n in ("q_stride", "k_stride", "v_stride", "q_out_stride")] + [
+        (n, C.c_int) for n in ("batch", "heads", "kv_heads", "total_q", "num_pages", "page_size", "max_pages_per_seq",
+                               "rotary_dim", "rotary_rows", "interleaved")]
+
+
+class PrefixArgs(C.Structure):
+    """``struct Fav4PrefixArgs`` (include/fav4_serving.h): PagedArgs, 3 pointers, 2 ints."""
+    _fields_ = [("paged", PagedArgs)] + [(n, C.c_void_p) for n in ("prefix_table", "prefix_lens",
+                                                                   "cu_prefix_seqs")] + [
+        (n, C.c_int) for n in ("num_prefixes", "max_pages_per_prefix")]
 
 
 class Strides(C.Structure):
@@ -82,6 +99,7 @@ def parse_resource_usage(text: str) -> dict:
 
 def build_library(out: Path = LIB_PATH, verbose: bool = False) -> Path:
     """Compile ``csrc/bshd.hip`` for gfx950 into ``build/libfav4_bshd.so``, the
+    serving operators ``csrc/serving.hip`` into ``build/libfav4_serving.so``, the
     loader probe ``csrc/loader_kat.hip`` into ``build/libfav4_loader_kat.so``
     (a test library) and the MFMA-only probe ``csrc/mfma_ceiling.hip`` into
     ``build/libfav4_mfma_ceiling.so`` (a measurement library, read by
@@ -94,7 +112,7 @@ def build_library(out: Path = LIB_PATH, verbose: bool = False) -> Path:
     import time
     out.parent.mkdir(parents=True, exist_ok=True)
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-    jobs = {out: CSRC / "bshd.hip", KAT_LIB_PATH: CSRC / "loader_kat.hip",
+    jobs = {out: CSRC / "bshd.hip", SERVING_LIB_PATH: CSRC / "serving.hip", KAT_LIB_PATH: CSRC / "loader_kat.hip",
             CEILING_LIB_PATH: CSRC / "mfma_ceiling.hip"}
     procs = {}
     for lib, src in jobs.items():
@@ -114,7 +132,7 @@ def build_library(out: Path = LIB_PATH, verbose: bool = False) -> Path:
     RESOURCE_LOG.write_text(text)
     sha = lambda p: hashlib.sha256(Path(p).read_bytes()).hexdigest()
     version = subprocess.run([hipcc, "--version"], capture_output=True, text=True).stdout
-    sources = sorted(CSRC.glob("*.hip")) + sorted(CSRC.glob("*.hpp")) + [INCLUDE / "fav4_bshd.h"]
+    sources = sorted(CSRC.glob("*.hip")) + sorted(CSRC.glob("*.hpp")) + sorted(INCLUDE.glob("*.h"))
     manifest = {
         "built_at": time.strftime("%Y-%m-%dT%H:%M:%SZ", time.gmtime()),
         "host": platform.node(),
@@ -196,6 +214,31 @@ def load_library(path: Path = LIB_PATH) -> C.CDLL:
         lib.fav4_bshd_splitkv_paged_select.restype = C.c_int
         _LIB = lib
     return _LIB
+
+
+_SERVING = None
+
+
+def load_serving_library(path: Path = SERVING_LIB_PATH) -> C.CDLL:
+    """Load the serving operators' library (raises OSError if it is missing); torch first, as load_library says."""
+    global _SERVING
+    if _SERVING is None or Path(_SERVING._name) != Path(path):
+        if not Path(path).exists():
+            raise OSError(f"{path} not built; run __graft_entry__.build() first")
+        try:
+            import torch  # noqa: F401
+        except ImportError:
+            pass
+        lib = C.CDLL(str(path))
+        lib.fav4_bshd_append_paged.argtypes = [C.POINTER(AppendArgs), C.c_void_p]
+        lib.fav4_bshd_append_paged.restype = C.c_int
+        lib.fav4_bshd_forward_prefix_paged.argtypes = [C.POINTER(PrefixArgs), C.c_int, C.c_void_p, C.c_size_t,
+                                                       C.c_void_p]
+        lib.fav4_bshd_forward_prefix_paged.restype = C.c_int
+        lib.fav4_bshd_prefix_paged_workspace_size.argtypes = [C.POINTER(PrefixArgs), C.c_int]
+        lib.fav4_bshd_prefix_paged_workspace_size.restype = C.c_longlong
+        _SERVING = lib
+    return _SERVING
 
 
 class Runner:
@@ -454,6 +497,106 @@ class Runner:
                                                            nbytes, stream)
         if status:
             raise RuntimeError(f"splitkv paged splits {splits}: HIP status {status}")
+        return workspace
+
+    # ---- serving operators on paged K/V caches (include/fav4_serving.h; no reference counterpart) ----
+    @property
+    def serving(self) -> C.CDLL:
+        return load_serving_library()
+
+    @staticmethod
+    def _one_device(*tensors):
+        """All tensors (None left out) on the current device, which the library launches on."""
+        import torch
+        devices = {x.device for x in tensors if x is not None}
+        if devices != {torch.device("cuda", torch.cuda.current_device())}:
+            raise ValueError(f"tensors on {sorted(map(str, devices))}, current device cuda:{torch.cuda.current_device()}")
+
+    def append_args(self, q, k, v, q_out, k_cache, v_cache, cu_q, seqlens_k, block_table, cos=None, sin=None,
+                    interleaved=False, positions=None) -> AppendArgs:
+        """q/q_out: [total_q, heads, 128] or both None; k/v: [total_q, kv_heads, 128] (BF16; any stride between
+        tokens, heads and dims contiguous); k_cache/v_cache: [num_pages, page_size, kv_heads, 128] (BF16, contiguous);
+        cu_q: int32 [batch+1]; seqlens_k: int32 [batch], new tokens included; block_table: int32 [batch, max_pages];
+        cos/sin: FP32 [rows, rotary_dim / 2] or None; positions: int32 [total_q] or None."""
+        import torch
+        bf16, f32, i32 = torch.bfloat16, torch.float32, torch.int32
+        self._one_device(q, k, v, q_out, k_cache, v_cache, cu_q, seqlens_k, block_table, cos, sin, positions)
+        tq, kvh = k.shape[0], k.shape[1]
+        for x in (q, k, v, q_out):
+            assert x is None or (x.dtype == bf16 and x.dim() == 3 and x.shape[0] == tq and x.shape[2] == D
+                                 and x.stride(2) == 1 and (x.shape[1] == 1 or x.stride(1) == D))
+        assert v.shape == k.shape and (q is None) == (q_out is None) and (q is None or q.shape == q_out.shape)
+        assert k_cache.dtype == v_cache.dtype == bf16 and k_cache.is_contiguous() and v_cache.is_contiguous()
+        assert k_cache.dim() == 4 and k_cache.shape == v_cache.shape and tuple(k_cache.shape[2:]) == (kvh, D)
+        assert all(c.dtype == i32 and c.is_contiguous() for c in (cu_q, seqlens_k, block_table))
+        assert block_table.dim() == 2 and cu_q.numel() == seqlens_k.numel() + 1 == block_table.shape[0] + 1
+        assert (cos is None) == (sin is None)
+        assert cos is None or (cos.dtype == sin.dtype == f32 and cos.dim() == 2 and cos.shape == sin.shape
+                               and cos.is_contiguous() and sin.is_contiguous())
+        assert positions is None or (positions.dtype == i32 and positions.is_contiguous() and positions.numel() == tq)
+        # A single token has no stride that counts.
+        stride = lambda x: 0 if x is None else x.stride(0) if tq > 1 else x.shape[1] * D
+        ptr = lambda x: None if x is None else x.data_ptr()
+        return AppendArgs(ptr(q), ptr(k), ptr(v), ptr(q_out), ptr(k_cache), ptr(v_cache), ptr(cos), ptr(sin),
+                          ptr(cu_q), ptr(seqlens_k), ptr(block_table), ptr(positions), stride(q), stride(k), stride(v),
+                          stride(q_out), seqlens_k.numel(), 1 if q is None else q.shape[1], kvh, tq, k_cache.shape[0],
+                          k_cache.shape[1], block_table.shape[1], 0 if cos is None else 2 * cos.shape[1],
+                          0 if cos is None else cos.shape[0], int(interleaved))
+
+    def call_append_paged(self, q, k, v, q_out, k_cache, v_cache, cu_q, seqlens_k, block_table, cos=None, sin=None,
+                          interleaved=False, positions=None, stream=None):
+        """fav4_bshd_append_paged: store the new tokens' K and V in the caches, K and Q rotated on the way (tensors as
+        for append_args).  q_out may be q: rotated in place."""
+        import torch
+        a = self.append_args(q, k, v, q_out, k_cache, v_cache, cu_q, seqlens_k, block_table, cos, sin, interleaved,
+                             positions)
+        if stream is None:
+            stream = torch.cuda.current_stream().cuda_stream
+        status = self.serving.fav4_bshd_append_paged(C.byref(a), stream)
+        if status:
+            raise RuntimeError(f"append paged: HIP status {status}")
+
+    def prefix_args(self, q, k_cache, v_cache, o, lse, cu_q, seqlens_k, block_table, prefix_table, prefix_lens,
+                    cu_prefix_seqs, max_q, max_k, total_k=None, scale=None) -> PrefixArgs:
+        """Tensors as for paged_args; prefix_table: int32 [num_prefixes, max_pages]; prefix_lens: int32
+        [num_prefixes]; cu_prefix_seqs: int32 [num_prefixes + 1]."""
+        import torch
+        self._one_device(q, k_cache, v_cache, o, lse, cu_q, seqlens_k, block_table, prefix_table, prefix_lens,
+                         cu_prefix_seqs)
+        paged = self.paged_args(q, k_cache, v_cache, o, lse, cu_q, seqlens_k, block_table, max_q, max_k, total_k, scale)
+        assert all(c.dtype == torch.int32 and c.is_contiguous() for c in (prefix_table, prefix_lens, cu_prefix_seqs))
+        n, pages = prefix_table.shape
+        assert prefix_lens.numel() == n and cu_prefix_seqs.numel() == n + 1
+        return PrefixArgs(paged, prefix_table.data_ptr(), prefix_lens.data_ptr(), cu_prefix_seqs.data_ptr(), n, pages)
+
+    def prefix_paged_workspace_size(self, batch, heads, kv_heads, max_q, max_k, total_q, page_size, max_pages,
+                                    num_pages, num_prefixes, max_prefix_pages, causal=0) -> int:
+        a = PrefixArgs(self.paged_shape_args(batch, heads, kv_heads, max_q, max_k, total_q, 0, page_size, max_pages,
+                                             num_pages), None, None, None, num_prefixes, max_prefix_pages)
+        return self.serving.fav4_bshd_prefix_paged_workspace_size(C.byref(a), int(causal))
+
+    def call_prefix_paged(self, q, k_cache, v_cache, o, lse, cu_q, seqlens_k, block_table, prefix_table, prefix_lens,
+                          cu_prefix_seqs, max_q, max_k, workspace=None, total_k=None, scale=None, stream=None,
+                          causal=0):
+        """fav4_bshd_forward_prefix_paged: call_splitkv_paged for sequences that share leading pages (tensors as for
+        prefix_args; causal 0 dense, 2 bottom-right).  `workspace` as for call_splitkv (None: allocated here);
+        returned for the next call."""
+        import torch
+        a = self.prefix_args(q, k_cache, v_cache, o, lse, cu_q, seqlens_k, block_table, prefix_table, prefix_lens,
+                             cu_prefix_seqs, max_q, max_k, total_k, scale)
+        if workspace is None:
+            need = self.serving.fav4_bshd_prefix_paged_workspace_size(C.byref(a), int(causal))
+            if need < 0:
+                raise RuntimeError("prefix paged: arguments rejected")
+            # Allocated for the stream that uses it, which then orders its reuse.
+            with torch.cuda.stream(None if stream is None else torch.cuda.ExternalStream(stream)):
+                workspace = torch.empty(need, device=q.device, dtype=torch.uint8)
+        if stream is None:
+            stream = torch.cuda.current_stream().cuda_stream
+        status = self.serving.fav4_bshd_forward_prefix_paged(
+            C.byref(a), int(causal), workspace.data_ptr(), workspace.numel() * workspace.element_size(), stream)
+        if status:
+            raise RuntimeError(f"prefix paged: HIP status {status}")
         return workspace
 
 
