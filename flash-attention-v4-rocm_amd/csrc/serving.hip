@@ -59,8 +59,8 @@ bool append_ok(const Fav4AppendArgs* a) {
 
 // ---- attention behind shared prefixes ------------------------------------------
 constexpr int BOTTOM_RIGHT = 2;
-constexpr int WAVES = 4, BM = WAVES * 32, BN = 64;
-constexpr int MIN_TILES = 4;
+constexpr int PREFIX_WAVE_ROWS = 32;  // up to this many rows of a prefix (the mean): its keys are, too
+constexpr int WAVE_ROWS = 64;      // up to this many rows of a sequence: its own keys are read by single waves
 
 bool prefix_shape_ok(const Fav4PrefixArgs* args, int causal) {
     if (!args) return false;
@@ -80,7 +80,9 @@ bool prefix_shape_ok(const Fav4PrefixArgs* args, int causal) {
 
 struct PrefixSizes {
     fav4::PrefixPlan plan;
-    int64_t part_rows, note_rows, bytes;
+    int64_t part_rows, note_rows, bytes, prefix_segs, prefix_ranges;
+    int waves, prefix_rows;    // of a workgroup, of a prefix block
+    fav4::Cut cut;
     bool ok;
 };
 PrefixSizes prefix_sizes(const Fav4PrefixArgs& args, int causal) {
@@ -88,32 +90,69 @@ PrefixSizes prefix_sizes(const Fav4PrefixArgs& args, int causal) {
     const int64_t group = a.heads / a.kv_heads, rows = a.total_q * group;
     PrefixSizes s{};
     s.plan.br = causal == BOTTOM_RIGHT;
-    s.plan.ranges = std::max(1, 2 * device_cus() / a.kv_heads);
-    s.plan.min_tiles = MIN_TILES;
+    s.cut = a.max_seqlen_q * group > WAVE_ROWS                     ? fav4::MANY
+            : rows <= int64_t(args.num_prefixes) * PREFIX_WAVE_ROWS ? fav4::FEWEST
+                                                                    : fav4::FEW;
+    // 256-row tiles where the prefixes or the sequences have that many rows, else 128.
+    s.waves = s.cut == fav4::MANY || (s.cut == fav4::FEW && rows > int64_t(args.num_prefixes) * 128) ? 8 : 4;
+    const int WAVES = s.waves, BM = s.prefix_rows = s.cut == fav4::FEWEST ? 32 : WAVES * 32;
+    const bool own_waves = s.cut != fav4::MANY;
+    // As many workgroups as are resident at once; at least one for each line.
+    s.plan.ranges = std::min(1024, std::max(2, (WAVES == 8 ? 1 : 2) * device_cus() / a.kv_heads));
     // Row tiles that the rows of n families can have.
-    auto tiles = [&](int64_t n, int64_t most) {
-        return std::min(n * ((most + BM - 1) / BM), (rows + n * (BM - 1)) / BM);
+    auto tiles = [&](int64_t n, int64_t most, int bm) {
+        return std::min(n * ((most + bm - 1) / bm), (rows + n * (bm - 1)) / bm);
     };
-    const int64_t own_rows = std::min<int64_t>(BM, a.max_seqlen_q * group);
-    const int64_t prefix_segs = tiles(args.num_prefixes, rows), own_segs = tiles(a.batch, a.max_seqlen_q * group);
+    const int own_bm = own_waves ? 32 : BM;
+    const int64_t own_rows = std::min<int64_t>(own_bm, a.max_seqlen_q * group);
+    const int64_t prefix_segs = s.prefix_segs = tiles(args.num_prefixes, rows, BM);
+    const int64_t own_segs = tiles(a.batch, a.max_seqlen_q * group, own_bm);
     const int64_t prefix_keys = std::min<int64_t>(int64_t(args.max_pages_per_prefix) * a.page_size, a.max_seqlen_k);
     const int64_t extra = 1 + fav4::SEG_TILES;
-    const int64_t prefix_blocks = prefix_segs + s.plan.ranges, own_blocks = own_segs + s.plan.ranges;
-    s.part_rows = a.kv_heads * (prefix_blocks * BM + own_blocks * own_rows);
-    s.ok = prefix_segs * (prefix_keys / BN + extra) + own_segs * (a.max_seqlen_k / BN + extra) < (1 << 30) &&
+    s.prefix_ranges = s.plan.ranges * (s.cut == fav4::FEWEST ? WAVES : 1);
+    const int64_t prefix_blocks = prefix_segs + s.prefix_ranges;
+    const int64_t own_blocks = own_segs + s.plan.ranges * (own_waves ? WAVES : 1);
+    s.part_rows = (a.kv_heads * (prefix_blocks * BM + own_blocks * own_rows) + 1) & ~int64_t(1);   // notes 16-byte aligned
+    s.ok = prefix_segs * (prefix_keys / 32 + extra) < (1 << 30) && own_segs * (a.max_seqlen_k / 32 + extra) < (1 << 30) &&
            prefix_blocks * BM <= INT_MAX && own_blocks * own_rows <= INT_MAX;
     s.plan.prefix_blocks = int(prefix_blocks);
     s.plan.own_blocks = int(own_blocks);
     s.plan.own_rows = int(own_rows);
+    s.plan.group = int(group);
+    s.plan.by_kv_heads = fav4::fast_div(a.kv_heads);
+    s.plan.by_group = fav4::fast_div(int(group));
+    s.plan.by_page = fav4::fast_div(a.page_size);
+    s.plan.by_heads = fav4::fast_div(a.heads);
+    s.plan.by_bm = fav4::fast_div(BM);
+    s.plan.by_own_rows = fav4::fast_div(int(own_rows));
     s.note_rows = rows;
     s.bytes = s.part_rows * (fav4::D * 4 + 8) + s.note_rows * 16;
     return s;
 }
 
-template <bool LSE>
-void launch_prefix(const Fav4PrefixArgs& args, const fav4::PrefixPlan& plan, hipStream_t stream) {
-    const dim3 grid(unsigned(args.paged.kv_heads) * unsigned(plan.ranges));
-    hipLaunchKernelGGL((fav4::prefix_kernel<LSE, WAVES>), grid, dim3(WAVES * 64), 0, stream, args, plan);
+void launch_prefix(const Fav4PrefixArgs& args, const PrefixSizes& s, hipStream_t stream) {
+    const dim3 grid(unsigned(args.paged.kv_heads) * unsigned(s.plan.ranges));
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(s.waves * 64), 0, stream, args, s.plan); };
+    auto with_lse = [&](auto waves, auto cut, auto cached) {
+        constexpr int W = decltype(waves)::value;
+        constexpr fav4::Cut CUT = decltype(cut)::value;
+        constexpr bool C = decltype(cached)::value;
+        if (args.paged.lse) go(fav4::prefix_kernel<true, W, CUT, C>);
+        else go(fav4::prefix_kernel<false, W, CUT, C>);
+    };
+    auto with_waves = [&](auto cached) {
+        using Four = std::integral_constant<int, 4>;
+        using Eight = std::integral_constant<int, 8>;
+        using Many = std::integral_constant<fav4::Cut, fav4::MANY>;
+        using Few = std::integral_constant<fav4::Cut, fav4::FEW>;
+        using Fewest = std::integral_constant<fav4::Cut, fav4::FEWEST>;
+        if (s.cut == fav4::MANY) with_lse(Eight{}, Many{}, cached);
+        else if (s.cut == fav4::FEWEST) with_lse(Four{}, Fewest{}, cached);
+        else if (s.waves == 8) with_lse(Eight{}, Few{}, cached);
+        else with_lse(Four{}, Few{}, cached);
+    };
+    if (args.paged.batch <= fav4::PLAN_SEQS && args.num_prefixes <= fav4::PLAN_PREFIXES) with_waves(std::true_type{});
+    else with_waves(std::false_type{});
 }
 
 }  // namespace
@@ -155,16 +194,23 @@ extern "C" __attribute__((visibility("default"))) int fav4_bshd_forward_prefix_p
     s.plan.o_part = static_cast<float*>(workspace);
     s.plan.lse_part = s.plan.o_part + s.part_rows * fav4::D;
     s.plan.notes = reinterpret_cast<int2*>(s.plan.lse_part + s.part_rows * 2);
-    if (a.lse) launch_prefix<true>(*args, s.plan, stream);
-    else launch_prefix<false>(*args, s.plan, stream);
+    launch_prefix(*args, s, stream);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    const int64_t rows = int64_t(a.total_q) * a.heads;
-    const int per = rows <= 2048 ? 4 : 1;
+    // Lane groups per merged row, by the parts that a prefix's row tile has when the
+    // prefixes take every range, as long as the rows leave the GPU some for it.
+    const int64_t rows = int64_t(a.total_q) * a.heads, parts = s.prefix_ranges / std::max<int64_t>(1, s.prefix_segs);
+    const int per = rows <= 1024 || (parts > 16 && rows <= 2048) ? 8
+                    : rows <= 2048 || (parts > 8 && rows <= 4096) ? 4
+                    : rows <= 4096                                ? 2
+                                                                  : 1;
     const unsigned blocks = unsigned(std::min((rows * per + 7) / 8, MAX_GRID));
-    if (per == 4)
-        hipLaunchKernelGGL(fav4::prefix_merge_kernel<4>, dim3(blocks), dim3(256), 0, stream, *args, s.plan, BM);
-    else
-        hipLaunchKernelGGL(fav4::prefix_merge_kernel<1>, dim3(blocks), dim3(256), 0, stream, *args, s.plan, BM);
+    auto merge = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(blocks), dim3(256), 0, stream, *args, s.plan, s.prefix_rows);
+    };
+    if (per == 8) merge(fav4::prefix_merge_kernel<8>);
+    else if (per == 4) merge(fav4::prefix_merge_kernel<4>);
+    else if (per == 2) merge(fav4::prefix_merge_kernel<2>);
+    else merge(fav4::prefix_merge_kernel<1>);
     return hipGetLastError();
 }

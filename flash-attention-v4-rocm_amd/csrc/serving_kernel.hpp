@@ -8,6 +8,20 @@ namespace fav4 {
 
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
+// Division of 0 <= n < 2^31 by a divisor d >= 1 that the host knows: with l =
+// ceil(log2 d) and m = floor(2^(31 + l) / d) + 1 (below 2^32), n / d is
+// floor(n m / 2^(31 + l)).
+struct FastDiv {
+    uint32_t m;
+    int l;
+    __device__ __forceinline__ int operator()(int n) const { return int(__umulhi(uint32_t(n) * 2, m) >> l); }
+};
+inline FastDiv fast_div(int d) {
+    int l = 0;
+    while ((int64_t(1) << l) < d) ++l;
+    return {uint32_t((uint64_t(1) << (31 + l)) / uint32_t(d) + 1), l};
+}
+
 // How many of the non-decreasing cu[1..n] are <= x, found by the whole wave: 64
 // entries at a time, so two rounds of loads up to 4096 entries.  For x >=
 // cu[0] that is the index of the range [cu[i], cu[i + 1]) that holds x, or n
@@ -111,15 +125,23 @@ __global__ __launch_bounds__(256) void append_kernel(Fav4AppendArgs a, int units
 // Attention behind shared prefixes.  Rows are (token, query head of the K/V
 // head's group), r = token * group + head: the rows of all sequences of a
 // prefix are neighbours, and so are those of one sequence.  A segment is a row
-// tile of BM rows of one prefix against the prefix's keys, or of one sequence
+// tile of one prefix against the prefix's keys (BM rows), or of one sequence
 // against the sequence's own keys; it costs its key tiles and SEG_TILES more,
-// laid before them, for what its start and end cost.  The segments of a K/V
-// head, prefixes first, are laid end to end and cut into ranges of one length,
-// one per workgroup, whatever segments they cross.
+// laid before them, for what its start and end cost (without keys, one tile).
+// The segments of a K/V head are laid end to end, the prefixes' on one line,
+// the sequences' own on another, and each line is cut into ranges of one
+// length, whatever segments they cross.
+//
+// A prefix range is a workgroup's: its WAVES waves take 32 rows each of the
+// row tile and share the K/V tiles.  An own range is a workgroup's too
+// (OWN_WAVES false: many rows per sequence), or a single wave's (up to 64 rows
+// of a sequence): the wave streams 32-key tiles through 16 KiB of LDS of its
+// own, with no barrier, and the eight such waves of a CU hide each other's
+// latency.
 //
 // A segment's part that lies in range w writes its O (normalised, FP32) and two
 // log-sums (log2: of the BF16 weights, and of the FP32 ones) to partial block
-// (segment + w) of its kind: segments and ranges both only grow along the line,
+// (segment + w) of its line: segments and ranges both only grow along the line,
 // so no two parts have the same sum, and the blocks number segments + ranges.
 // The part that holds a segment's first key tile also notes for each of its rows
 // where its partials start and how many there are; prefix_merge_kernel goes by
@@ -128,122 +150,235 @@ __global__ __launch_bounds__(256) void append_kernel(Fav4AppendArgs a, int units
 struct PrefixPlan {
     float *o_part, *lse_part;         // prefix blocks of all K/V heads (BM rows each), then own blocks (own_rows each)
     int2* notes;                      // [total_q * group][2]: first partial row and parts, prefix and own
-    int ranges, min_tiles;            // ranges of a K/V head; shortest range
+    int group;                        // query heads of a K/V head
+    int ranges;                       // workgroups of a K/V head
+    FastDiv by_kv_heads, by_group, by_page, by_heads, by_bm, by_own_rows;
     int prefix_blocks, own_blocks;    // partial blocks of a K/V head
     int own_rows;                     // rows of an own block
     int br;                           // bottom-right causal
 };
 
-// Tokens, rows and key tiles of one segment family: a prefix or a sequence.
-struct Family {
-    int t0, tokens;                   // first token, tokens
-    int k0, k1;                       // keys [k0, k1)
+constexpr int SEG_TILES = 4, OWN_SEG_TILES = 2;        // OWN_SEG_TILES: of a single wave's segment
+constexpr int MIN_PREFIX_TILES = 2, MIN_OWN_TILES = 2;  // shortest ranges
+// What a prefix's key tile costs, in own key tiles of a wave (its share of the
+// workgroups follows): 32 keys by four waves, 64 keys by eight.
+constexpr float PREFIX_COST_4 = 1.5f, PREFIX_COST_8 = 4.f;
+// Sequences and prefixes whose lengths are kept in LDS (others are read again
+// from memory where they are needed).
+constexpr int PLAN_SEQS = 1024, PLAN_PREFIXES = 256;
+struct PlanLds {
+    int cu[PLAN_SEQS + 1], keys[PLAN_SEQS], shared[PLAN_SEQS], first_seq[PLAN_PREFIXES + 1], prefix_keys[PLAN_PREFIXES];
 };
 
-// Prefix p's sequences [s0, s1) and keys.
-struct PrefixSpan {
-    int s0, s1, keys;
-};
-__device__ __forceinline__ PrefixSpan prefix_span(const Fav4PrefixArgs& a, int p) {
-    const int n = a.paged.batch, page = a.paged.page_size;
-    const int s0 = min(max(a.cu_prefix_seqs[p], 0), n), s1 = min(max(a.cu_prefix_seqs[p + 1], s0), n);
-    const int most = int(min(int64_t(a.max_pages_per_prefix) * page, int64_t(a.paged.max_seqlen_k)));
-    return {s0, s1, min(max(a.prefix_lens[p], 0), most) / page * page};
-}
-__device__ __forceinline__ int clamp_token(const Fav4PrefixArgs& a, int x) { return min(max(x, 0), a.paged.total_q); }
+// The batch as read on the device, clamped: tokens to [0, total_q], keys to
+// [0, max_seqlen_k], a prefix's keys to whole pages of its table.
+template <bool CACHED>
+struct PrefixBatch {
+    const Fav4PrefixArgs& a;
+    const PrefixPlan& pl;
+    const PlanLds& lds;
+    bool hidden;                      // a sequence may not see all of its prefix
 
-__device__ __forceinline__ Family prefix_family(const Fav4PrefixArgs& a, int p) {
-    const PrefixSpan s = prefix_span(a, p);
-    const int t0 = clamp_token(a, a.paged.cu_seqlens_q[s.s0]), t1 = max(t0, clamp_token(a, a.paged.cu_seqlens_q[s.s1]));
-    return {t0, s.keys > 0 ? t1 - t0 : 0, 0, s.keys};
-}
-// Shared keys of sequence b.
-__device__ __forceinline__ int shared_keys(const Fav4PrefixArgs& a, int b) {
-    int lo = 0, hi = a.num_prefixes;                           // the last prefix that starts at or before b
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (a.cu_prefix_seqs[mid] <= b) lo = mid;
-        else hi = mid;
+    __device__ __forceinline__ int load_cu(int b) const {
+        return min(max(a.paged.cu_seqlens_q[b], 0), a.paged.total_q);
     }
-    const PrefixSpan s = prefix_span(a, lo);
-    return s.s0 <= b && b < s.s1 ? s.keys : 0;
-}
-struct OwnFamily {
-    Family f;
-    int sq, sk, shared;
+    __device__ __forceinline__ int load_keys(int b) const {
+        return min(max(a.paged.seqlens_k[b], 0), a.paged.max_seqlen_k);
+    }
+    __device__ __forceinline__ int load_first_seq(int p) const {
+        return min(max(a.cu_prefix_seqs[p], 0), a.paged.batch);
+    }
+    __device__ __forceinline__ int load_prefix_keys(int p) const {
+        const int page = a.paged.page_size;
+        const int most = int(min(int64_t(a.max_pages_per_prefix) * page, int64_t(a.paged.max_seqlen_k)));
+        return pl.by_page(min(max(a.prefix_lens[p], 0), most)) * page;
+    }
+    __device__ __forceinline__ int cu(int b) const { return CACHED ? lds.cu[b] : load_cu(b); }
+    __device__ __forceinline__ int keys(int b) const { return CACHED ? lds.keys[b] : load_keys(b); }
+    __device__ __forceinline__ int first_seq(int p) const { return CACHED ? lds.first_seq[p] : load_first_seq(p); }
+    __device__ __forceinline__ int prefix_keys(int p) const { return CACHED ? lds.prefix_keys[p] : load_prefix_keys(p); }
+    // Shared keys of sequence b: of the last prefix that starts at or before it.
+    __device__ __forceinline__ int find_shared(int b) const {
+        int lo = 0, hi = a.num_prefixes;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (first_seq(mid) <= b) lo = mid;
+            else hi = mid;
+        }
+        return first_seq(lo) <= b && b < first_seq(lo + 1) ? prefix_keys(lo) : 0;
+    }
+    __device__ __forceinline__ int shared(int b) const { return CACHED ? lds.shared[b] : find_shared(b); }
 };
-__device__ __forceinline__ OwnFamily own_family(const Fav4PrefixArgs& a, int b) {
-    const int t0 = clamp_token(a, a.paged.cu_seqlens_q[b]);
-    const int t1 = min(max(clamp_token(a, a.paged.cu_seqlens_q[b + 1]), t0), t0 + a.paged.max_seqlen_q);
-    const int sk = min(max(a.paged.seqlens_k[b], 0), a.paged.max_seqlen_k), shared = shared_keys(a, b);
-    return {{t0, t1 - t0, min(shared, sk), sk}, t1 - t0, sk, shared};
+
+// A prefix or a sequence: its tokens and the keys [k0, k1) that they read here.
+struct Family {
+    int t0, tokens, k0, k1;
+};
+template <class B>
+__device__ __forceinline__ Family prefix_family(const B& x, int p) {
+    const int s0 = x.first_seq(p), s1 = max(x.first_seq(p + 1), s0), t0 = x.cu(s0), keys = x.prefix_keys(p);
+    return {t0, keys > 0 ? max(0, x.cu(s1) - t0) : 0, 0, keys};
+}
+template <class B>
+__device__ __forceinline__ Family own_family(const B& x, int b) {
+    const int t0 = x.cu(b), sk = x.keys(b);
+    return {t0, min(max(x.cu(b + 1) - t0, 0), x.a.paged.max_seqlen_q), min(x.shared(b), sk), sk};
 }
 
-constexpr int SEG_TILES = 4;
+// A line of families' segments: row tiles of ROWS rows, key tiles of BN keys,
+// LEAD units before each segment's key tiles.
+template <class B, bool OWN, int ROWS, int BN, int LEAD>
+struct Line {
+    const B& x;
+    int count, group;
+    __device__ __forceinline__ Family family(int i) const { return OWN ? own_family(x, i) : prefix_family(x, i); }
+    __device__ __forceinline__ int tiles(const Family& f) const { return int(uint32_t(f.tokens * group + ROWS - 1) / ROWS); }
+    __device__ __forceinline__ int key_tiles(const Family& f) const { return int(uint32_t(f.k1 - f.k0 + BN - 1) / BN); }
+    __device__ __forceinline__ int seg_cost(const Family& f) const { return max(1, key_tiles(f)) + LEAD; }
 
-template <bool LSE, int WAVES>
-__global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
-void prefix_kernel(Fav4PrefixArgs a, PrefixPlan pl) {
-    constexpr int BN = 64, BM = WAVES * 32;
+    // Up to 64 families from i on in the wave's lanes: the units and segments up to and with each.
+    struct Sums {
+        int cost, segs, cost_end, segs_end;
+    };
+    __device__ __forceinline__ Sums sums(int i, int lane) const {
+        Family f{};
+        if (i + lane < count) f = family(i + lane);
+        const int s = tiles(f), c = s * seg_cost(f);
+        return {c, s, wave_scan(c), wave_scan(s)};
+    }
+    // The line's length; `head` gets the first families' sums.
+    __device__ __forceinline__ int length(int lane, Sums& head) const {
+        head = sums(0, lane);
+        int total = __builtin_amdgcn_readlane(head.cost_end, 63);
+        for (int i = 64; i < count; i += 64) total += __builtin_amdgcn_readlane(sums(i, lane).cost_end, 63);
+        return total;
+    }
+    // The family that holds unit `at`, the unit where it starts and the segments before it.
+    struct Place {
+        int idx, base, seg;
+    };
+    __device__ __forceinline__ Place find(int at, int lane, const Sums& head) const {
+        Sums v = head;
+        Place p{0, 0, 0};
+        for (;;) {
+            const uint64_t hit = __builtin_amdgcn_ballot_w64(p.base + v.cost_end > at);
+            if (hit) {
+                const int l = __builtin_ctzll(hit);
+                return {uniform(p.idx + l), uniform(p.base + __builtin_amdgcn_readlane(v.cost_end - v.cost, l)),
+                        uniform(p.seg + __builtin_amdgcn_readlane(v.segs_end - v.segs, l))};
+            }
+            p.base += __builtin_amdgcn_readlane(v.cost_end, 63);
+            p.seg += __builtin_amdgcn_readlane(v.segs_end, 63);
+            p.idx += 64;
+            if (p.idx >= count) return {count, 0, 0};
+            v = sums(p.idx, lane);
+        }
+    }
+};
+
+// Number of a page table's entries, 64 of them in the wave's lanes; key tiles
+// are taken in ascending order.
+struct PageWalk {
+    const int* table;
+    int entries, page_size, num_pages, pages, slot0, slot, in_page;
+    __device__ __forceinline__ void load(int lane) {
+        slot0 = slot;
+        pages = min(max(table[min(slot + lane, entries - 1)], 0), num_pages - 1);
+    }
+    __device__ __forceinline__ void start(const int* t, int n, int key, const FastDiv& by_page, int lane) {
+        table = t;
+        entries = n;
+        slot = by_page(key);
+        in_page = key - slot * page_size;
+        load(lane);
+    }
+    // The cache row of the present key; then on by `step` keys.
+    __device__ __forceinline__ int64_t row(int step, int lane) {
+        if (slot - slot0 >= 64) load(lane);
+        const int64_t r = int64_t(__builtin_amdgcn_readlane(pages, slot - slot0)) * page_size + in_page;
+        in_page += step;
+        while (in_page >= page_size) in_page -= page_size, ++slot;
+        return r;
+    }
+};
+
+__device__ __forceinline__ void load_q(const Fav4PagedArgs& pg, int tok, int head, int half, bf16x8 (&qr)[8]) {
+    const char* qp = static_cast<const char*>(pg.q) + (int64_t(tok) * pg.heads + head) * ROW_BYTES + half * 16;
+#pragma unroll
+    for (int c = 0; c < 8; ++c) qr[c] = *reinterpret_cast<const bf16x8*>(qp + c * 32);
+}
+
+__device__ __forceinline__ void clear(RowState& st) {
+#pragma unroll
+    for (int db = 0; db < 4; ++db) st.o[db] = f32x16{};
+    st.m = -__builtin_inff();
+    st.lb = 0.f;
+    st.l = 0.f;
+}
+
+// The keys that rows [first, last] of a family see: the last one of the row of
+// token `tok` (a lane's own); all rows see those of the family's keys below
+// `plain`, and none sees any from `end` on.
+struct Visible {
+    int lim, plain, end;
+};
+template <bool OWN, class B>
+__device__ __forceinline__ Visible visible(const B& x, const PrefixPlan& pl, const Family& f, int idx, int first,
+                                           int last, int tok) {
+    if constexpr (OWN) {
+        if (!pl.br) return {f.k1 - 1, uniform(f.k1), uniform(f.k1)};
+        const int shift = f.k1 - f.tokens;                             // last visible key of query 0
+        const int i0 = pl.by_group(first), i1 = pl.by_group(last);
+        return {shift + tok - f.t0, uniform(max(f.k0, min(f.k1, shift + i0 + 1))),
+                uniform(max(f.k0, min(f.k1, shift + i1 + 1)))};
+    } else {
+        if (!x.hidden) return {INT_MAX, uniform(f.k1), uniform(f.k1)};
+        // The last of the prefix's sequences that starts at or before tok.
+        int lo = x.first_seq(idx), hi = max(x.first_seq(idx + 1), lo + 1);
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (x.cu(mid) <= tok) lo = mid;
+            else hi = mid;
+        }
+        return {x.keys(lo) - (pl.br ? x.cu(lo + 1) - tok : 1), 0, uniform(f.k1)};
+    }
+}
+
+// The partial rows of one wave's 32 rows (`live` of them exist), to partial row prow on.
+template <bool LSE, int TILE_BYTES>
+__device__ __forceinline__ void store_parts(const RowState& st, const PrefixPlan& pl, int64_t prow, int live,
+                                            unsigned char* smem, uint32_t slot, int lane) {
+    if (live <= 0) return;
+    const rsrc_t rp = make_rsrc(pl.o_part + prow * D, uint32_t(live) * D * 4);
+    const float inv = st.lb > 0.f ? 1.f / st.lb : 0.f;
+    store_part_rows<TILE_BYTES, true>(st, inv, smem, slot, rp, 0, live, lane);
+    if (lane < 32 && lane < live) {
+        const float sb = st.m + __builtin_amdgcn_logf(st.lb);
+        reinterpret_cast<float2*>(pl.lse_part)[prow + lane] =
+            float2{sb, LSE ? st.m + __builtin_amdgcn_logf(st.l) : sb};
+    }
+}
+
+// The segments of the range [g0, g0 + per) of a line, each by WAVES waves that
+// share its key tiles: prefixes (OWN false) or sequences.  aligned: the units
+// of a segment of the line's only family, a multiple of per (0: seg_cost).
+template <bool LSE, int WAVES, bool OWN, int BN, int STAGES, class B, class L>
+__device__ __forceinline__ void attend_shared(const B& x, const PrefixPlan& pl, const L& line,
+                                              const typename L::Sums& head, int range, int per, int aligned, int kvh,
+                                              unsigned char* smem) {
+    constexpr int BM = WAVES * 32, AHEAD = STAGES - 1;         // prefetch distance in tiles
     constexpr int TILE_BYTES = BN * ROW_BYTES, STAGE_BYTES = 2 * TILE_BYTES;
     constexpr int DMA = BN / 4 / WAVES, SLAB = DMA * 4;        // this wave's key rows of a tile
     static_assert(DMA >= 2, "a wave's DMA slots hold 2 KiB per matrix (O staging)");
     static_assert(32 % SLAB == 0, "a wave's rows of a tile lie in one page");
-    __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * STAGE_BYTES];
-
+    const Fav4PrefixArgs& a = x.a;
     const Fav4PagedArgs& pg = a.paged;
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
-    const int col = lane & 31, half = lane >> 5;
-    const int group = pg.heads / pg.kv_heads;
+    const int col = lane & 31, half = lane >> 5, group = line.group;
     const uint32_t kv_row_bytes = uint32_t(pg.kv_heads) * ROW_BYTES;
     const float scale2 = pg.scale * LOG2E;
     const uint32_t smem_base = lds_addr(smem);
-    const int kvh = uniform(int(blockIdx.x) % pg.kv_heads), w = uniform(int(blockIdx.x) / pg.kv_heads);
-
-    auto row_tiles = [&](int tokens) { return int((int64_t(tokens) * group + BM - 1) / BM); };
-    auto cost = [&](const Family& f) { return row_tiles(f.tokens) * (max(1, (f.k1 - f.k0 + BN - 1) / BN) + SEG_TILES); };
-
-    // The line: its length, and where the prefixes' part ends.
-    int prefix_end = 0, prefix_segs = 0, total = 0;
-    for (int p0 = 0; p0 < a.num_prefixes; p0 += 64) {
-        Family f{};
-        if (p0 + lane < a.num_prefixes) f = prefix_family(a, p0 + lane);
-        prefix_end += wave_total(cost(f));
-        prefix_segs += wave_total(row_tiles(f.tokens));
-    }
-    total = prefix_end;
-    for (int b0 = 0; b0 < pg.batch; b0 += 64) {
-        Family f{};
-        if (b0 + lane < pg.batch) f = own_family(a, b0 + lane).f;
-        total += wave_total(cost(f));
-    }
-    const int per = max((total + pl.ranges - 1) / pl.ranges, pl.min_tiles);
-    if (int64_t(w) * per >= total) return;
-    const int g0 = w * per, g1 = g0 + per;
-
-    // The family that holds unit g0, the unit that it starts at and the
-    // segments of its kind before it.
-    bool own = g0 >= prefix_end;
-    int idx = 0, base = own ? prefix_end : 0, seg0 = 0;
-    {
-        const int count = own ? pg.batch : a.num_prefixes;
-        for (int i0 = 0; i0 < count; i0 += 64) {
-            Family f{};
-            if (i0 + lane < count) f = own ? own_family(a, i0 + lane).f : prefix_family(a, i0 + lane);
-            const int c = cost(f), s = row_tiles(f.tokens), end = wave_scan(c), segs = wave_scan(s);
-            const uint64_t hit = __builtin_amdgcn_ballot_w64(base + end > g0);
-            if (hit) {
-                const int l = __builtin_ctzll(hit);
-                idx = i0 + l;
-                base += __builtin_amdgcn_readlane(end - c, l);
-                seg0 += __builtin_amdgcn_readlane(segs - s, l);
-                break;
-            }
-            base += __builtin_amdgcn_readlane(end, 63);
-            seg0 += __builtin_amdgcn_readlane(segs, 63);
-        }
-    }
-    base = uniform(base), seg0 = uniform(seg0), idx = uniform(idx);
+    const int g0 = range * per, g1 = g0 + per;
 
     const LdsOffsets off = lds_offsets(lane);
     DmaOffsets<DMA> dofs;
@@ -253,263 +388,391 @@ void prefix_kernel(Fav4PrefixArgs a, PrefixPlan pl) {
         dofs.k[i] = in_slab * kv_row_bytes + ((p ^ k_swz(r)) << 4);
         dofs.v[i] = in_slab * kv_row_bytes + ((p ^ v_swz(r)) << 4);
     }
-
-    for (;;) {
-        // The next family that has rows, from idx on.
-        const int count = own ? pg.batch : a.num_prefixes;
-        if (idx >= count) {
-            if (own) break;
-            own = true, idx = 0, seg0 = 0, base = prefix_end;
-            continue;
-        }
-        OwnFamily o{};
-        if (own) o = own_family(a, idx);
-        else o.f = prefix_family(a, idx);
-        const int t0 = uniform(o.f.t0), tokens = uniform(o.f.tokens), k0 = uniform(o.f.k0), k1 = uniform(o.f.k1);
-        const int sq = uniform(o.sq), sk = uniform(o.sk), shared = uniform(o.shared);
-        const int tiles = row_tiles(tokens), ktiles = (k1 - k0 + BN - 1) / BN;
-        const int seg_cost = max(1, ktiles) + SEG_TILES;
+    typename L::Place at = aligned ? typename L::Place{0, 0, 0} : line.find(g0, lane, head);
+    for (; at.idx < line.count && at.base < g1; ++at.idx) {
+        const Family f = line.family(at.idx);
+        const int t0 = uniform(f.t0), tokens = uniform(f.tokens), k0 = uniform(f.k0), k1 = uniform(f.k1);
+        const int tiles = uniform(line.tiles(f)), ktiles = uniform(line.key_tiles(f)),
+                  seg_cost = aligned ? aligned : uniform(line.seg_cost(f));
         const int rows = tokens * group;
         // The first row tile whose units reach past g0 (bad offsets may overlap the
         // families and overflow the line: every index stays in bounds all the same).
-        int rt = base < g0 ? max(0, (g0 - base) / seg_cost) : 0;
-        const PrefixSpan ps = own ? PrefixSpan{} : prefix_span(a, idx);
-        const int s0 = uniform(ps.s0), s1 = uniform(ps.s1);
-        for (; rt < tiles; ++rt) {
-            const int first = base + rt * seg_cost + SEG_TILES;        // unit of its first key tile
+        for (int rt = at.base < g0 ? max(0, (g0 - at.base) / seg_cost) : 0; rt < tiles; ++rt) {
+            const int first = at.base + (rt + 1) * seg_cost - max(ktiles, 1);     // unit of its first key tile
             if (first >= g1) break;
             if (first + max(ktiles, 1) <= g0) continue;
             const int a0 = max(0, g0 - first), a1 = min(ktiles, g1 - first);
-            const bool starts = first >= g0;
             const int q0 = rt * BM, qw = q0 + wave * 32, row = qw + col;
             const int srow = min(row, rows - 1);
-            const int tok = t0 + srow / group, hg = srow - (srow / group) * group;
+            const int trow = pl.by_group(srow), tok = t0 + trow, qhead = kvh * group + srow - trow * group;
 
-            // Visible keys: the last one of this lane's row; all rows of the tile see
-            // those below `plain`, and none sees any from `end` on.
-            int lim, plain, end = k1;
-            if (own) {
-                const int shift = pl.br ? sk - sq : sk - 1;            // last visible key of query 0
-                const int i0 = q0 / group, i1 = min(rows - 1, q0 + BM - 1) / group;
-                lim = pl.br ? shift + tok - t0 : shift;
-                plain = min(k1, (pl.br ? shift + i0 : shift) + 1);
-                end = min(k1, (pl.br ? shift + i1 : shift) + 1);
-            } else {
-                int low = INT_MAX;
-                for (int b0 = s0; b0 < s1; b0 += 64) {
-                    const int b = min(b0 + lane, s1 - 1);
-                    const int n = max(0, pg.cu_seqlens_q[b + 1] - pg.cu_seqlens_q[b]);
-                    const int keys = min(max(pg.seqlens_k[b], 0), pg.max_seqlen_k);
-                    if (n > 0) low = min(low, pl.br ? keys - n : keys - 1);
-                }
-#pragma unroll
-                for (int m = 32; m >= 1; m >>= 1) low = min(low, __shfl_xor(low, m));
-                low = uniform(low);
-                plain = min(k1, max(-1, low) + 1);
-                lim = INT_MAX;
-                if (plain < k1) {
-                    // Some sequence has fewer keys than its prefix: each row's own limit.
-                    int lo = s0, hi = s1;                              // the last sequence that starts at or before tok
-                    while (hi - lo > 1) {
-                        const int mid = (lo + hi) >> 1;
-                        if (pg.cu_seqlens_q[mid] <= tok) lo = mid;
-                        else hi = mid;
-                    }
-                    const int keys = min(max(pg.seqlens_k[lo], 0), pg.max_seqlen_k);
-                    lim = pl.br ? keys - (pg.cu_seqlens_q[lo + 1] - tok) : keys - 1;
-                }
-            }
-            plain = uniform(max(plain, k0)), end = uniform(max(end, k0));
-            const int nfull = (plain - k0) / BN;
+            const Visible see = visible<OWN>(x, pl, f, at.idx, q0, min(rows, q0 + BM) - 1, tok);
+            const int plain = see.plain, end = see.end, lim = see.lim;
+            const int nfull = max(0, plain - k0) / BN;
             const int e1 = min(a1, (end - k0 + BN - 1) / BN);          // past what any row sees: nothing to do
 
             RowState st;
-#pragma unroll
-            for (int db = 0; db < 4; ++db) st.o[db] = f32x16{};
-            st.m = -__builtin_inff();
-            st.lb = 0.f;
-            st.l = 0.f;
+            clear(st);
             if (a0 < e1) {
-                const int* table = own ? pg.block_table + int64_t(idx) * pg.max_pages_per_seq
-                                       : a.prefix_table + int64_t(idx) * a.max_pages_per_prefix;
-                const int entries = own ? pg.max_pages_per_seq : a.max_pages_per_prefix;
-                int pages = 0, page0 = 0;                              // lane l holds the page of slot page0 + l
-                auto load_pages = [&](int slot) {
-                    page0 = slot;
-                    pages = min(max(table[min(slot + lane, entries - 1)], 0), pg.num_pages - 1);
-                };
-                load_pages((k0 + a0 * BN + wave * SLAB) / pg.page_size);
-                auto issue = [&](int t) {
-                    const int key = k0 + t * BN + wave * SLAB;         // this wave's first key row of the tile
-                    const int slot = key / pg.page_size, in_page = key - slot * pg.page_size;
-                    if (slot - page0 >= 64) load_pages(slot);
-                    const int64_t r0 =
-                        int64_t(__builtin_amdgcn_readlane(pages, slot - page0)) * pg.page_size + in_page;
-                    const int left = min(k1 - key, SLAB);
-                    const uint32_t bytes = left > 0 ? uint32_t(left - 1) * kv_row_bytes + ROW_BYTES : 0u;
-                    const int64_t at = (r0 * pg.kv_heads + kvh) * ROW_BYTES;
-                    const u32x4 rk = make_desc(static_cast<const char*>(pg.k_cache) + at, bytes);
-                    const u32x4 rv = make_desc(static_cast<const char*>(pg.v_cache) + at, bytes);
-                    dma_tile<DMA, TILE_BYTES>(rk, rv, smem_base + ((t - a0) & 1) * STAGE_BYTES, wave, dofs);
-                };
-                issue(a0);
+                PageWalk walk{nullptr, 0, pg.page_size, pg.num_pages};
+                const int key0 = k0 + a0 * BN + wave * SLAB;           // this wave's first key row
+                if constexpr (OWN)
+                    walk.start(pg.block_table + int64_t(at.idx) * pg.max_pages_per_seq, pg.max_pages_per_seq, key0,
+                               pl.by_page, lane);
+                else
+                    walk.start(a.prefix_table + int64_t(at.idx) * a.max_pages_per_prefix, a.max_pages_per_prefix,
+                               key0, pl.by_page, lane);
                 bf16x8 qr[8];
-                {
-                    const char* qp = static_cast<const char*>(pg.q) +
-                                     (int64_t(tok) * pg.heads + kvh * group + hg) * ROW_BYTES + half * 16;
+                load_q(pg, tok, qhead, half, qr);
+                // Q and the pages have landed before the first tile is asked for, so that
+                // the loop's only outstanding loads are its tiles.
 #pragma unroll
-                    for (int c = 0; c < 8; ++c) qr[c] = *reinterpret_cast<const bf16x8*>(qp + c * 32);
-#pragma unroll
-                    for (int c = 0; c < 8; ++c) asm volatile("" ::"v"(qr[c]));
-                }
-                const bool idle = qw >= rows;                          // all of this wave's rows are past the family's
-                auto step = [&](auto stage_c, auto masked_c, int t) {
-                    constexpr int STAGE = decltype(stage_c)::value;
-                    constexpr bool MASKED = decltype(masked_c)::value;
-                    const unsigned char* cur = smem + STAGE * STAGE_BYTES;
-                    wait_vmem();
-                    __syncthreads();
-                    if (t + 1 < e1) issue(t + 1);
-                    if (!idle)
-                        attend_fused<BN, MASKED, true, LSE, true>(cur, cur + TILE_BYTES, off, qr, st, t == a0,
-                                                                  k0 + t * BN, k1, lim, half, scale2);
+                for (int c = 0; c < 8; ++c) asm volatile("" ::"v"(qr[c]));
+                asm volatile("" ::"v"(walk.pages));
+                // Tiles past the last one read nothing (the descriptors' bound is 0) and land
+                // in a stage that no later step reads, which keeps the vmcnt count uniform.
+                auto issue = [&](int t, int stage) {
+                    const int left = t < e1 ? min(k1 - (k0 + t * BN + wave * SLAB), SLAB) : 0;
+                    const uint32_t bytes = left > 0 ? uint32_t(left - 1) * kv_row_bytes + ROW_BYTES : 0u;
+                    const int64_t byte = t < e1 ? (walk.row(BN, lane) * pg.kv_heads + kvh) * ROW_BYTES : 0;
+                    const u32x4 rk = make_desc(static_cast<const char*>(pg.k_cache) + byte, bytes);
+                    const u32x4 rv = make_desc(static_cast<const char*>(pg.v_cache) + byte, bytes);
+                    dma_tile<DMA, TILE_BYTES>(rk, rv, smem_base + stage * STAGE_BYTES, wave, dofs);
                 };
-                using S0 = std::integral_constant<int, 0>;
-                using S1 = std::integral_constant<int, 1>;
-                using Plain = std::integral_constant<bool, false>;
-                using Masked = std::integral_constant<bool, true>;
-                int t = a0;
-                for (; t + 1 < min(e1, nfull); t += 2) {
-                    step(S0{}, Plain{}, t);
-                    step(S1{}, Plain{}, t + 1);
-                }
-                for (; t + 1 < e1; t += 2) {
-                    step(S0{}, Masked{}, t);
-                    step(S1{}, Masked{}, t + 1);
-                }
-                if (t < e1) step(S0{}, Masked{}, t);
-                // Every wave has read its last tile before any stages O or loads the
-                // next segment's first one.
+#pragma unroll
+                for (int i = 0; i < AHEAD; ++i) issue(a0 + i, i);
+                const bool idle = qw >= rows;                          // all of this wave's rows are past the family's
+                int t = a0, stage = 0;
+                auto steps = [&](auto masked_c, int to) {
+                    for (; t < to; ++t) {
+                        const unsigned char* cur = smem + stage * STAGE_BYTES;
+                        wait_vmem_keep<2 * DMA * (AHEAD - 1)>();
+                        __syncthreads();
+                        issue(t + AHEAD, stage == 0 ? AHEAD : stage - 1);
+                        if (!idle)
+                            attend_fused<BN, decltype(masked_c)::value, true, LSE, true>(
+                                cur, cur + TILE_BYTES, off, qr, st, t == a0, k0 + t * BN, k1, lim, half, scale2);
+                        stage = stage == STAGES - 1 ? 0 : stage + 1;
+                    }
+                };
+                steps(std::integral_constant<bool, false>{}, min(e1, nfull));
+                steps(std::integral_constant<bool, true>{}, e1);
+                // The prefetches past the end have landed, and every wave has read its last
+                // tile, before any stages O or loads the next segment's first one.
+                wait_vmem();
                 __syncthreads();
             }
             // The part's partial rows, and the segment's notes.
-            const int seg = seg0 + rt, block = seg + w;
-            const int stride = own ? pl.own_rows : BM, blocks = own ? pl.own_blocks : pl.prefix_blocks;
-            const int live = min(min(BM, stride), rows - q0);          // rows of the tile
+            const int block = at.seg + rt + range;
+            const int stride = OWN ? pl.own_rows : BM, blocks = OWN ? pl.own_blocks : pl.prefix_blocks;
+            const int live = min(min(32, stride - wave * 32), rows - qw);      // of this wave's rows
             if (ktiles > 0 && uint32_t(block) < uint32_t(blocks)) {
-                const int64_t prow0 = (own ? int64_t(pg.kv_heads) * pl.prefix_blocks * BM : 0) +
-                                      (int64_t(kvh) * blocks + block) * stride;
-                const rsrc_t rp = make_rsrc(pl.o_part + prow0 * D, uint32_t(live) * D * 4);
-                const float inv = st.lb > 0.f ? 1.f / st.lb : 0.f;
-                store_part_rows<TILE_BYTES, true>(st, inv, smem, wave * DMA * 1024, rp, wave * 32, live - wave * 32,
-                                                  lane);
-                if (half == 0 && wave * 32 + col < live) {
-                    float* lp = pl.lse_part + (prow0 + wave * 32 + col) * 2;
-                    const float sb = st.m + __builtin_amdgcn_logf(st.lb);
-                    lp[0] = sb;
-                    lp[1] = LSE ? st.m + __builtin_amdgcn_logf(st.l) : sb;
-                }
+                const int64_t prow = (OWN ? int64_t(pg.kv_heads) * pl.prefix_blocks * BM : 0) +
+                                     (int64_t(kvh) * blocks + block) * stride + wave * 32;
+                store_parts<LSE, TILE_BYTES>(st, pl, prow, live, smem, wave * DMA * 1024, lane);
             }
-            if (kvh == 0 && starts && half == 0 && wave * 32 + col < live) {
+            if (kvh == 0 && first >= g0 && lane < 32 && lane < live) {
                 const int parts = ktiles > 0 ? (first + ktiles - 1) / per - first / per + 1 : 0;
-                const int64_t r = int64_t(t0) * group + row;
-                pl.notes[r * 2 + own] = int2{block * stride + wave * 32 + col, parts};
-                if (own && shared == 0) pl.notes[r * 2] = int2{0, 0};
+                int2* note = pl.notes + (int64_t(t0) * group + row) * 2;
+                note[OWN] = int2{block * stride + wave * 32 + lane, parts};
+                if (OWN && k0 == 0 && x.shared(at.idx) == 0) note[0] = int2{0, 0};
             }
             // The staging has been read (its values were stored) before this wave's
             // next copy into its slots.
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         }
-        base += tiles * seg_cost;
-        seg0 += tiles;
-        ++idx;
-        if (base >= g1) break;
+        at.base += tiles * seg_cost;
+        at.seg += tiles;
     }
 }
 
-// Merge: PER groups of 32 lanes share one (row, K/V head), 4 dims a lane.
+// The segments of the range [g0, g0 + per) of a line by one wave: 32-row tiles,
+// 32-key tiles in the wave's own 16 KiB of LDS at `slot`.  The line starts at
+// unit `origin`; partial blocks of `stride` rows from row part0 on, `blocks` of
+// them per K/V head.  Neighbouring families are taken with neighbouring K/V
+// heads: a wave that stays with one head reads one eighth of the memory
+// channels, and some of them are slower (128 sequences of 64..4096 own keys
+// behind 32768, H32 KVH8: the slowest head's tiles took 3.48 us, the fastest's
+// 2.75; 159 -> 146 us for the call).
+template <bool LSE, bool OWN, class B, class L>
+__device__ __forceinline__ void attend_wave(const B& x, const PrefixPlan& pl, const L& line,
+                                            const typename L::Sums& head, int origin, int range, int per, int turn,
+                                            unsigned char* smem, uint32_t slot, int64_t part0, int blocks,
+                                            int stride) {
+    constexpr int BN = 32, BM = 32, TILE_BYTES = BN * ROW_BYTES, DMA = BN / 4;
+    const Fav4PagedArgs& pg = x.a.paged;
+    const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, group = line.group;
+    const uint32_t kv_row_bytes = uint32_t(pg.kv_heads) * ROW_BYTES;
+    const float scale2 = pg.scale * LOG2E;
+    const uint32_t stage = lds_addr(smem) + slot;
+    const int g0 = range * per, g1 = g0 + per;
+
+    const LdsOffsets off = lds_offsets(lane);
+    const DmaOffsets<DMA> dofs = dma_offsets<DMA>(0, lane, kv_row_bytes, kv_row_bytes);
+    typename L::Place at = line.find(max(0, g0 - origin), lane, head);
+    for (at.base += origin; at.idx < line.count && at.base < g1; ++at.idx) {
+        const Family f = line.family(at.idx);
+        const int t0 = uniform(f.t0), tokens = uniform(f.tokens), k0 = uniform(f.k0), k1 = uniform(f.k1);
+        const int tiles = uniform(line.tiles(f)), ktiles = uniform(line.key_tiles(f)), seg_cost = uniform(line.seg_cost(f));
+        const int rows = tokens * group;
+        const int kvh = uniform(turn + at.idx - pl.by_kv_heads(turn + at.idx) * pg.kv_heads);
+        for (int rt = at.base < g0 ? max(0, (g0 - at.base) / seg_cost) : 0; rt < tiles; ++rt) {
+            const int first = at.base + (rt + 1) * seg_cost - max(ktiles, 1);
+            if (first >= g1) break;
+            if (first + max(ktiles, 1) <= g0) continue;
+            const int a0 = max(0, g0 - first), a1 = min(ktiles, g1 - first);
+            const int q0 = rt * BM, row = q0 + col, srow = min(row, rows - 1);
+            const int trow = pl.by_group(srow), tok = t0 + trow, qhead = kvh * group + srow - trow * group;
+            const Visible see = visible<OWN>(x, pl, f, at.idx, q0, min(rows, q0 + BM) - 1, tok);
+            const int lim = see.lim, nfull = max(0, see.plain - k0) / BN, e1 = min(a1, (see.end - k0 + BN - 1) / BN);
+
+            RowState st;
+            clear(st);
+            if (a0 < e1) {
+                PageWalk walk{nullptr, 0, pg.page_size, pg.num_pages};
+                if constexpr (OWN)
+                    walk.start(pg.block_table + int64_t(at.idx) * pg.max_pages_per_seq, pg.max_pages_per_seq,
+                               k0 + a0 * BN, pl.by_page, lane);
+                else
+                    walk.start(x.a.prefix_table + int64_t(at.idx) * x.a.max_pages_per_prefix, x.a.max_pages_per_prefix,
+                               a0 * BN, pl.by_page, lane);
+                bf16x8 qr[8];
+                load_q(pg, tok, qhead, half, qr);
+#pragma unroll
+                for (int c = 0; c < 8; ++c) asm volatile("" ::"v"(qr[c]));
+                auto issue = [&](int t) {
+                    const int left = min(k1 - (k0 + t * BN), BN);
+                    const uint32_t bytes = uint32_t(left - 1) * kv_row_bytes + ROW_BYTES;
+                    const int64_t byte = (walk.row(BN, lane) * pg.kv_heads + kvh) * ROW_BYTES;
+                    const u32x4 rk = make_desc(static_cast<const char*>(pg.k_cache) + byte, bytes);
+                    const u32x4 rv = make_desc(static_cast<const char*>(pg.v_cache) + byte, bytes);
+                    dma_tile<DMA, TILE_BYTES, true>(rk, rv, stage, 0, dofs);
+                };
+                issue(a0);
+                const unsigned char* ks = smem + slot;
+                auto step = [&](auto masked_c, int t) {
+                    wait_vmem();
+                    attend_fused<BN, decltype(masked_c)::value, true, LSE, true>(ks, ks + TILE_BYTES, off, qr, st, t == a0,
+                                                                                 k0 + t * BN, k1, lim, half, scale2);
+                    // The tile has been read: the next one may land in its place.
+                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                    if (t + 1 < e1) issue(t + 1);
+                };
+                int t = a0;
+                for (; t < min(e1, nfull); ++t) step(std::integral_constant<bool, false>{}, t);
+                for (; t < e1; ++t) step(std::integral_constant<bool, true>{}, t);
+            }
+            const int block = at.seg + rt + range, live = min(min(32, stride), rows - q0);
+            if (ktiles > 0 && uint32_t(block) < uint32_t(blocks))
+                store_parts<LSE, TILE_BYTES>(st, pl, part0 + (int64_t(kvh) * blocks + block) * stride, live, smem, slot,
+                                             lane);
+            if (kvh == 0 && first >= g0 && lane < 32 && lane < live) {
+                const int parts = ktiles > 0 ? (first + ktiles - 1) / per - first / per + 1 : 0;
+                int2* note = pl.notes + (int64_t(t0) * group + row) * 2;
+                note[OWN] = int2{block * stride + lane, parts};
+                if (OWN && k0 == 0 && x.shared(at.idx) == 0) note[0] = int2{0, 0};
+            }
+            // The staging has been read (its values were stored) before the next copy.
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        }
+        at.base += tiles * seg_cost;
+        at.seg += tiles;
+    }
+}
+
+// How a call's lines are cut (by the host, from the sizes): MANY rows per
+// sequence, both lines by whole workgroups; FEW, the prefixes' by workgroups
+// and the sequences' own by waves; FEWEST (a prefix's rows, too, few), both
+// by waves, as one line.
+enum Cut { MANY, FEW, FEWEST };
+
+template <bool LSE, int WAVES, Cut CUT, bool CACHED>
+__global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void prefix_kernel(Fav4PrefixArgs a, PrefixPlan pl) {
+    constexpr bool OWN_WAVES = CUT != MANY;
+    constexpr int BN = WAVES == 4 ? 32 : 64, STAGES = 4;               // three tiles in flight
+    constexpr int BM = CUT == FEWEST ? 32 : WAVES * 32;                // rows of a prefix segment
+    constexpr int OWN_RANGES = OWN_WAVES ? WAVES : 1;                  // of a workgroup
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[STAGES * 2 * BN * ROW_BYTES];
+    __shared__ PlanLds lds;
+    static_assert(!OWN_WAVES || sizeof(smem) >= WAVES * 64 * ROW_BYTES, "a 32-key tile of K and V for each wave");
+    const Fav4PagedArgs& pg = a.paged;
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+    const int w = uniform(pl.by_kv_heads(blockIdx.x)), kvh = uniform(int(blockIdx.x) - w * pg.kv_heads);
+    const int group = pl.group;
+
+    PrefixBatch<CACHED> x{a, pl, lds, true};
+    if constexpr (CACHED) {
+        // One round of loads for as many sequences as the workgroup has lanes.
+        for (int i = threadIdx.x; i <= max(pg.batch, a.num_prefixes); i += WAVES * 64) {
+            const int cu = x.load_cu(min(i, pg.batch)), keys = x.load_keys(min(i, pg.batch - 1));
+            const int first = x.load_first_seq(min(i, a.num_prefixes));
+            const int prefix_keys = x.load_prefix_keys(min(i, a.num_prefixes - 1));
+            if (i <= pg.batch) lds.cu[i] = cu;
+            if (i < pg.batch) lds.keys[i] = keys;
+            if (i <= a.num_prefixes) lds.first_seq[i] = first;
+            if (i < a.num_prefixes) lds.prefix_keys[i] = prefix_keys;
+        }
+        __syncthreads();
+        int hidden = 0;
+        for (int i = threadIdx.x; i < pg.batch; i += WAVES * 64) {
+            const int shared = x.find_shared(i), n = lds.cu[i + 1] - lds.cu[i];
+            lds.shared[i] = shared;
+            hidden |= n > 0 && lds.keys[i] - (pl.br ? n : 1) < shared - 1;
+        }
+        x.hidden = __syncthreads_or(hidden);
+    }
+    using B = PrefixBatch<CACHED>;
+    const Line<B, false, BM, BN, CUT == FEWEST ? OWN_SEG_TILES : SEG_TILES> prefixes{x, a.num_prefixes, group};
+    const Line<B, true, OWN_WAVES ? 32 : BM, OWN_WAVES ? 32 : BN, OWN_WAVES ? OWN_SEG_TILES : SEG_TILES> own{
+        x, pg.batch, group};
+    typename decltype(prefixes)::Sums prefix_head;
+    typename decltype(own)::Sums own_head;
+    const int prefix_units = prefixes.length(lane, prefix_head), own_units = own.length(lane, own_head);
+
+    const int64_t own_part0 = int64_t(pg.kv_heads) * pl.prefix_blocks * BM;
+    if constexpr (CUT == FEWEST) {
+        const int ranges = pl.ranges * WAVES, range = w * WAVES + wave, total = prefix_units + own_units;
+        const int per = max(int(uint32_t(total + ranges - 1) / uint32_t(ranges)), MIN_OWN_TILES);
+        const uint32_t slot = wave * 64 * ROW_BYTES;
+        if (range * per < prefix_units)
+            attend_wave<LSE, false>(x, pl, prefixes, prefix_head, 0, range, per, kvh, smem, slot, 0, pl.prefix_blocks, BM);
+        if ((range + 1) * per > prefix_units)
+            attend_wave<LSE, true>(x, pl, own, own_head, prefix_units, range, per, kvh, smem, slot, own_part0,
+                                   pl.own_blocks, pl.own_rows);
+        return;
+    } else {
+    // The workgroups of either line, by what its tiles cost; the two kinds alternate,
+    // so that a CU has both.
+    const float cost = prefix_units * (OWN_WAVES ? WAVES == 4 ? PREFIX_COST_4 : PREFIX_COST_8 : 1.f);
+    int pw = min(max(int(cost / (cost + own_units) * pl.ranges + 0.5f), 1), pl.ranges - 1);
+    if (prefix_units <= 0) pw = 0;
+    int per = max(int(uint32_t(prefix_units + pw - 1) / uint32_t(max(pw, 1))), MIN_PREFIX_TILES);
+    int aligned = 0;
+    if (a.num_prefixes == 1 && pw >= uniform(prefixes.tiles(prefixes.family(0)))) {
+        // One prefix, a range or more for each row tile: they are cut at the same keys (the lead units take up the
+        // rest), so that they read them at the same time and share them in L2.
+        const Family f = prefixes.family(0);
+        const int cost = uniform(prefixes.seg_cost(f)), cuts = pw / uniform(max(prefixes.tiles(f), 1));
+        per = max(int(uint32_t(cost + cuts - 1) / uint32_t(cuts)), MIN_PREFIX_TILES);
+        aligned = int(uint32_t(cost + per - 1) / uint32_t(per)) * per;
+    }
+    // w pw / ranges, exact: both factors are at most 1024.
+    const float step = 1.f / pl.ranges;
+    const int before = int((w * pw + 0.5f) * step);
+    if (int(((w + 1) * pw + 0.5f) * step) > before) {
+        attend_shared<LSE, WAVES, false, BN, STAGES>(x, pl, prefixes, prefix_head, before, per, aligned, kvh,
+                                                     smem);
+    } else {
+        const int ranges = (pl.ranges - pw) * OWN_RANGES, range = w - before;
+        per = max(int(uint32_t(own_units + ranges - 1) / uint32_t(ranges)), MIN_OWN_TILES);
+        if constexpr (OWN_WAVES)
+            attend_wave<LSE, true>(x, pl, own, own_head, 0, range * WAVES + wave, per, kvh, smem, wave * 64 * ROW_BYTES,
+                                   own_part0, pl.own_blocks, pl.own_rows);
+        else
+            attend_shared<LSE, WAVES, true, BN, STAGES>(x, pl, own, own_head, range, per, 0, kvh, smem);
+    }
+    }
+}
+
+// Merge of a row's parts: PER groups of 32 lanes share one row of one head, 4
+// dims a lane; a group takes every PER-th part, NS at a time with all their
+// loads in flight, and keeps the running maximum and sums of a softmax over
+// the parts' log-sums.
 template <int PER>
 __global__ __launch_bounds__(256) void prefix_merge_kernel(Fav4PrefixArgs a, PrefixPlan pl, int bm) {
-    constexpr int RPB = 8 / PER;
-    __shared__ float2 red[8];
+    constexpr int RPB = 8 / PER, NS = 4;
+    __shared__ float4 red[8];
     __shared__ f32x4 red_o[8][32];
     const Fav4PagedArgs& pg = a.paged;
     const int grp = threadIdx.x >> 5, q4 = threadIdx.x & 31;
-    const int slot = grp / PER, part = grp - slot * PER, team = part * 32 + q4;
-    const int group = pg.heads / pg.kv_heads;
+    const int slot = grp / PER, part = grp - slot * PER;
+    const int group = pl.group;
     const uint32_t rows = uint32_t(pg.total_q) * uint32_t(pg.heads), blocks = (rows + RPB - 1) / RPB;
     for (uint32_t blk = blockIdx.x; blk < blocks; blk += gridDim.x) {
         const uint32_t r = blk * RPB + slot;                   // token * heads + head
-        const int tok = int(r / uint32_t(pg.heads)), head = int(r - uint32_t(tok) * uint32_t(pg.heads));
-        const int kvh = head / group, hg = head - kvh * group;
-        const bool live = r < rows && tok >= pg.cu_seqlens_q[0] && tok < pg.cu_seqlens_q[pg.batch];
+        const int tok = pl.by_heads(r), head = int(r - uint32_t(tok) * uint32_t(pg.heads));
+        const int kvh = pl.by_group(head), hg = head - kvh * group;
         int first[2] = {}, n[2] = {};
+        bool live = r < rows;
         if (live) {
-            const int2* note = pl.notes + (int64_t(tok) * group + hg) * 2;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                // Clamped: bad offsets leave notes unwritten.
-                const int stride = i ? pl.own_rows : bm, last = (i ? pl.own_blocks : pl.prefix_blocks) * stride - 1;
-                first[i] = min(max(note[i].x, 0), last);
-                n[i] = min(max(note[i].y, 0), (last - first[i]) / stride + 1);
+            const int4 note = *reinterpret_cast<const int4*>(pl.notes + (int64_t(tok) * group + hg) * 2);
+            live = tok >= pg.cu_seqlens_q[0] && tok < pg.cu_seqlens_q[pg.batch];
+            // Clamped: bad offsets leave notes unwritten.
+            const int last_p = pl.prefix_blocks * bm - 1, last_o = pl.own_blocks * pl.own_rows - 1;
+            first[0] = min(max(note.x, 0), last_p);
+            first[1] = min(max(note.z, 0), last_o);
+            if (live) {
+                n[0] = min(max(note.y, 0), pl.prefix_blocks - pl.by_bm(first[0]));
+                n[1] = min(max(note.w, 0), pl.own_blocks - pl.by_own_rows(first[1]));
             }
         }
         const int total = n[0] + n[1];
-        const int64_t at[2] = {int64_t(kvh) * pl.prefix_blocks * bm + first[0],
-                               int64_t(pg.kv_heads) * pl.prefix_blocks * bm +
-                                   int64_t(kvh) * pl.own_blocks * pl.own_rows + first[1]};
-        auto row_of = [&](int c) {
-            return c < n[0] ? at[0] + int64_t(c) * bm : at[1] + int64_t(c - n[0]) * pl.own_rows;
-        };
-        auto sums = [&](int c) { return *reinterpret_cast<const float2*>(pl.lse_part + row_of(c) * 2); };
-        float mb = -__builtin_inff(), ml = mb;
-        for (int c = team; c < total; c += PER * 32) {
-            const float2 v = sums(c);
-            mb = fmaxf(mb, v.x), ml = fmaxf(ml, v.y);
+        const int64_t at_p = int64_t(kvh) * pl.prefix_blocks * bm + first[0];
+        const int64_t at_o = int64_t(pg.kv_heads) * pl.prefix_blocks * bm + int64_t(kvh) * pl.own_blocks * pl.own_rows +
+                             first[1];
+        float mb = -__builtin_inff(), ml = mb, den = 0.f, suml = 0.f;
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        for (int c0 = part; c0 < total; c0 += PER * NS) {
+            // Loads past the last part repeat it, with weight 0: no branch between the loads.
+            float2 v[NS];
+            f32x4 xo[NS];
+#pragma unroll
+            for (int i = 0; i < NS; ++i) {
+                const int c = min(c0 + i * PER, total - 1);
+                const int64_t row = c < n[0] ? at_p + int64_t(c) * bm : at_o + int64_t(c - n[0]) * pl.own_rows;
+                v[i] = reinterpret_cast<const float2*>(pl.lse_part)[row];
+                xo[i] = *reinterpret_cast<const f32x4*>(pl.o_part + row * D + q4 * 4);
+            }
+#pragma unroll
+            for (int i = 0; i < NS; ++i)
+                if (c0 + i * PER >= total) v[i] = float2{-__builtin_inff(), -__builtin_inff()};
+            float nb = mb, nl = ml;
+#pragma unroll
+            for (int i = 0; i < NS; ++i) nb = fmaxf(nb, v[i].x), nl = fmaxf(nl, v[i].y);
+            if (nb == -__builtin_inff()) continue;             // parts without a visible key
+            const float keep = exp2_native(mb - nb);
+            acc *= keep;
+            den *= keep;
+            suml *= exp2_native(ml - nl);
+            mb = nb, ml = nl;
+#pragma unroll
+            for (int i = 0; i < NS; ++i) {
+                const float wgt = exp2_native(v[i].x - mb);
+                if (wgt > 0.f) acc += wgt * xo[i];
+                den += wgt;
+                suml += exp2_native(v[i].y - ml);
+            }
         }
-        mb = max32(mb), ml = max32(ml);
         if constexpr (PER > 1) {
-            if (q4 == 0) red[grp] = float2{mb, ml};
+            if (q4 == 0) red[grp] = float4{mb, ml, den, suml};
+            red_o[grp][q4] = acc;
             __syncthreads();
 #pragma unroll
             for (int p = 0; p < PER; ++p) mb = fmaxf(mb, red[slot * PER + p].x), ml = fmaxf(ml, red[slot * PER + p].y);
-            __syncthreads();
-        }
-        // No key in any part: weights 2^-inf = 0, so O = 0 and LSE = -inf.
-        if (mb == -__builtin_inff()) mb = ml = 0.f;
-        float den = 0.f, suml = 0.f;
-        for (int c = team; c < total; c += PER * 32) {
-            const float2 v = sums(c);
-            den += exp2_native(v.x - mb), suml += exp2_native(v.y - ml);
-        }
-        den = sum32(den), suml = sum32(suml);
-        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-        for (int c = part; c < total; c += PER) {
-            const float wgt = exp2_native(sums(c).x - mb);
-            const f32x4 x = *reinterpret_cast<const f32x4*>(pl.o_part + row_of(c) * D + q4 * 4);
-            if (wgt > 0.f) acc += wgt * x;
-        }
-        if constexpr (PER > 1) {
-            if (q4 == 0) red[grp] = float2{den, suml};
-            red_o[grp][q4] = acc;
-            __syncthreads();
             den = suml = 0.f;
             acc = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int p = 0; p < PER; ++p) {
-                den += red[slot * PER + p].x, suml += red[slot * PER + p].y;
-                acc += red_o[slot * PER + p][q4];
+                const float4 o = red[slot * PER + p];
+                if (o.x == -__builtin_inff()) continue;
+                const float wgt = exp2_native(o.x - mb);
+                den += wgt * o.z;
+                suml += exp2_native(o.y - ml) * o.w;
+                acc += wgt * red_o[slot * PER + p][q4];
             }
             __syncthreads();
         }
         if (!live || part != 0) continue;
+        // No key in any part: O = 0, LSE = -inf.
         const float rden = den > 0.f ? 1.f / den : 0.f;
         const f32x4 y = acc * rden;
         const f32x2 y0 = {y[0], y[1]}, y1 = {y[2], y[3]};
         const bf16x2 b0 = __builtin_convertvector(y0, bf16x2), b1 = __builtin_convertvector(y1, bf16x2);
         *reinterpret_cast<bf16x4*>(static_cast<char*>(pg.o) + int64_t(r) * ROW_BYTES + q4 * 8) =
             bf16x4{b0[0], b0[1], b1[0], b1[1]};
-        if (pg.lse && q4 == 0) pg.lse[int64_t(head) * pg.total_q + tok] = (ml + __builtin_amdgcn_logf(suml)) * LN2;
+        if (pg.lse && q4 == 0) pg.lse[int64_t(head) * pg.total_q + tok] =
+            den > 0.f ? (ml + __builtin_amdgcn_logf(suml)) * LN2 : -__builtin_inff();
     }
 }
 

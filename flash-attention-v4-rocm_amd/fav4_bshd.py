@@ -12,6 +12,7 @@ from __future__ import annotations
 import ctypes as C
 import math
 import os
+import struct
 import subprocess
 from pathlib import Path
 
@@ -21,6 +22,7 @@ LIB_PATH = ROOT / "build" / "libfav4_bshd.so"
 CSRC = PKG / "csrc"
 INCLUDE = ROOT / "include"
 D = 128
+SCALE = 1 / math.sqrt(D)
 
 HIPCC_FLAGS = [
     "-O3", "-std=c++17", "--offload-arch=gfx950", "-fPIC", "-shared", "-fvisibility=hidden",
@@ -73,6 +75,11 @@ class PrefixArgs(C.Structure):
     _fields_ = [("paged", PagedArgs)] + [(n, C.c_void_p) for n in ("prefix_table", "prefix_lens",
                                                                    "cu_prefix_seqs")] + [
         (n, C.c_int) for n in ("num_prefixes", "max_pages_per_prefix")]
+
+
+# The same two structs, for packing in one step.
+_APPEND = struct.Struct("@12P4q10i")
+_PREFIX = struct.Struct("@8P10if3P2i0P")
 
 
 class Strides(C.Structure):
@@ -230,12 +237,12 @@ def load_serving_library(path: Path = SERVING_LIB_PATH) -> C.CDLL:
         except ImportError:
             pass
         lib = C.CDLL(str(path))
-        lib.fav4_bshd_append_paged.argtypes = [C.POINTER(AppendArgs), C.c_void_p]
+        # The argument blocks are passed as packed bytes or by reference.
+        lib.fav4_bshd_append_paged.argtypes = [C.c_void_p, C.c_void_p]
         lib.fav4_bshd_append_paged.restype = C.c_int
-        lib.fav4_bshd_forward_prefix_paged.argtypes = [C.POINTER(PrefixArgs), C.c_int, C.c_void_p, C.c_size_t,
-                                                       C.c_void_p]
+        lib.fav4_bshd_forward_prefix_paged.argtypes = [C.c_void_p, C.c_int, C.c_void_p, C.c_size_t, C.c_void_p]
         lib.fav4_bshd_forward_prefix_paged.restype = C.c_int
-        lib.fav4_bshd_prefix_paged_workspace_size.argtypes = [C.POINTER(PrefixArgs), C.c_int]
+        lib.fav4_bshd_prefix_paged_workspace_size.argtypes = [C.c_void_p, C.c_int]
         lib.fav4_bshd_prefix_paged_workspace_size.restype = C.c_longlong
         _SERVING = lib
     return _SERVING
@@ -500,77 +507,126 @@ class Runner:
         return workspace
 
     # ---- serving operators on paged K/V caches (include/fav4_serving.h; no reference counterpart) ----
+    # A decode step is a few microseconds of GPU time, so these calls keep the host's part short: the argument blocks
+    # are packed in one step, and every tensor's properties are read once.
     @property
     def serving(self) -> C.CDLL:
-        return load_serving_library()
+        lib = self.__dict__.get("_serving")
+        if lib is None:
+            lib = self._serving = load_serving_library()
+        return lib
 
     @staticmethod
-    def _one_device(*tensors):
-        """All tensors (None left out) on the current device, which the library launches on."""
-        import torch
-        devices = {x.device for x in tensors if x is not None}
-        if devices != {torch.device("cuda", torch.cuda.current_device())}:
-            raise ValueError(f"tensors on {sorted(map(str, devices))}, current device cuda:{torch.cuda.current_device()}")
+    def _stream(torch, device, stream):
+        """The stream to launch on (None: torch's current one), with `device`, the tensors', current."""
+        if device < 0 or device != torch.cuda.current_device():
+            raise ValueError(f"tensors on {'the host' if device < 0 else f'cuda:{device}'}, current device "
+                             f"cuda:{torch.cuda.current_device()}")
+        if stream is not None:
+            return stream
+        raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)       # without a Stream object
+        return raw(device) if raw is not None else torch.cuda.current_stream().cuda_stream
 
-    def append_args(self, q, k, v, q_out, k_cache, v_cache, cu_q, seqlens_k, block_table, cos=None, sin=None,
-                    interleaved=False, positions=None) -> AppendArgs:
-        """q/q_out: [total_q, heads, 128] or both None; k/v: [total_q, kv_heads, 128] (BF16; any stride between
-        tokens, heads and dims contiguous); k_cache/v_cache: [num_pages, page_size, kv_heads, 128] (BF16, contiguous);
-        cu_q: int32 [batch+1]; seqlens_k: int32 [batch], new tokens included; block_table: int32 [batch, max_pages];
-        cos/sin: FP32 [rows, rotary_dim / 2] or None; positions: int32 [total_q] or None."""
-        import torch
-        bf16, f32, i32 = torch.bfloat16, torch.float32, torch.int32
-        self._one_device(q, k, v, q_out, k_cache, v_cache, cu_q, seqlens_k, block_table, cos, sin, positions)
-        tq, kvh = k.shape[0], k.shape[1]
-        for x in (q, k, v, q_out):
-            assert x is None or (x.dtype == bf16 and x.dim() == 3 and x.shape[0] == tq and x.shape[2] == D
-                                 and x.stride(2) == 1 and (x.shape[1] == 1 or x.stride(1) == D))
-        assert v.shape == k.shape and (q is None) == (q_out is None) and (q is None or q.shape == q_out.shape)
-        assert k_cache.dtype == v_cache.dtype == bf16 and k_cache.is_contiguous() and v_cache.is_contiguous()
-        assert k_cache.dim() == 4 and k_cache.shape == v_cache.shape and tuple(k_cache.shape[2:]) == (kvh, D)
-        assert all(c.dtype == i32 and c.is_contiguous() for c in (cu_q, seqlens_k, block_table))
-        assert block_table.dim() == 2 and cu_q.numel() == seqlens_k.numel() + 1 == block_table.shape[0] + 1
+    @staticmethod
+    def _paged_batch(torch, device, cu_q, seqlens_k, block_table):
+        """Checks of a paged batch's index tensors; (batch, max_pages_per_seq)."""
+        i32 = torch.int32
+        for x in (cu_q, seqlens_k, block_table):
+            assert x.dtype is i32 and x.is_contiguous() and x.get_device() == device, "int32, contiguous, on one device"
+        batch, pages = block_table.shape
+        assert cu_q.shape == (batch + 1,) and seqlens_k.shape == (batch,)
+        return batch, pages
+
+    @staticmethod
+    def _caches(torch, device, k_cache, v_cache):
+        """Checks of the paged caches; their shape."""
+        shape = k_cache.shape
+        assert len(shape) == 4 and shape[3] == D and v_cache.shape == shape
+        assert k_cache.dtype is torch.bfloat16 and v_cache.dtype is torch.bfloat16
+        assert k_cache.is_contiguous() and v_cache.is_contiguous()
+        assert k_cache.get_device() == device and v_cache.get_device() == device
+        return shape
+
+    @staticmethod
+    def _rows(torch, device, x, tokens):
+        """Checks of [tokens, heads, 128] BF16 rows with any stride between tokens; (heads, stride)."""
+        n, heads, d = x.shape
+        s0, s1, s2 = x.stride()
+        assert n == tokens and d == D and x.dtype is torch.bfloat16 and x.get_device() == device
+        assert s2 == 1 and (s1 == D or heads == 1)
+        return heads, s0 if n > 1 else heads * D          # a single token has no stride that counts
+
+    def _append_block(self, torch, q, k, v, q_out, k_cache, v_cache, cu_q, seqlens_k, block_table, cos, sin,
+                      interleaved, positions) -> bytes:
+        device = k.get_device()
+        num_pages, page_size, kv_heads, _ = self._caches(torch, device, k_cache, v_cache)
+        batch, pages = self._paged_batch(torch, device, cu_q, seqlens_k, block_table)
+        tokens = k.shape[0]
+        k_heads, k_stride = self._rows(torch, device, k, tokens)
+        v_heads, v_stride = self._rows(torch, device, v, tokens)
+        assert k_heads == v_heads == kv_heads and (q is None) == (q_out is None)
+        heads, q_stride, o_stride, q_ptr, o_ptr = 1, 0, 0, 0, 0
+        if q is not None:
+            heads, q_stride = self._rows(torch, device, q, tokens)
+            o_heads, o_stride = self._rows(torch, device, q_out, tokens)
+            assert o_heads == heads
+            q_ptr, o_ptr = q.data_ptr(), q_out.data_ptr()
+        rows = half = c_ptr = s_ptr = p_ptr = 0
         assert (cos is None) == (sin is None)
-        assert cos is None or (cos.dtype == sin.dtype == f32 and cos.dim() == 2 and cos.shape == sin.shape
-                               and cos.is_contiguous() and sin.is_contiguous())
-        assert positions is None or (positions.dtype == i32 and positions.is_contiguous() and positions.numel() == tq)
-        # A single token has no stride that counts.
-        stride = lambda x: 0 if x is None else x.stride(0) if tq > 1 else x.shape[1] * D
-        ptr = lambda x: None if x is None else x.data_ptr()
-        return AppendArgs(ptr(q), ptr(k), ptr(v), ptr(q_out), ptr(k_cache), ptr(v_cache), ptr(cos), ptr(sin),
-                          ptr(cu_q), ptr(seqlens_k), ptr(block_table), ptr(positions), stride(q), stride(k), stride(v),
-                          stride(q_out), seqlens_k.numel(), 1 if q is None else q.shape[1], kvh, tq, k_cache.shape[0],
-                          k_cache.shape[1], block_table.shape[1], 0 if cos is None else 2 * cos.shape[1],
-                          0 if cos is None else cos.shape[0], int(interleaved))
+        if cos is not None:
+            rows, half = cos.shape
+            assert sin.shape == (rows, half) and cos.dtype is sin.dtype is torch.float32
+            assert cos.is_contiguous() and sin.is_contiguous() and cos.get_device() == sin.get_device() == device
+            c_ptr, s_ptr = cos.data_ptr(), sin.data_ptr()
+        if positions is not None:
+            assert positions.dtype is torch.int32 and positions.shape == (tokens,) and positions.is_contiguous()
+            assert positions.get_device() == device
+            p_ptr = positions.data_ptr()
+        return _APPEND.pack(q_ptr, k.data_ptr(), v.data_ptr(), o_ptr, k_cache.data_ptr(), v_cache.data_ptr(), c_ptr,
+                            s_ptr, cu_q.data_ptr(), seqlens_k.data_ptr(), block_table.data_ptr(), p_ptr, q_stride,
+                            k_stride, v_stride, o_stride, batch, heads, kv_heads, tokens, num_pages, page_size, pages,
+                            2 * half, rows, 1 if interleaved else 0)
 
     def call_append_paged(self, q, k, v, q_out, k_cache, v_cache, cu_q, seqlens_k, block_table, cos=None, sin=None,
                           interleaved=False, positions=None, stream=None):
-        """fav4_bshd_append_paged: store the new tokens' K and V in the caches, K and Q rotated on the way (tensors as
-        for append_args).  q_out may be q: rotated in place."""
+        """fav4_bshd_append_paged: store the new tokens' K and V in the caches, K and Q rotated by position on the way.
+        q/q_out: [total_q, heads, 128] or both None; k/v: [total_q, kv_heads, 128] (BF16; any stride between tokens);
+        k_cache/v_cache: [num_pages, page_size, kv_heads, 128] (BF16, contiguous); cu_q: int32 [batch+1]; seqlens_k:
+        int32 [batch], new tokens included; block_table: int32 [batch, max_pages]; cos/sin: FP32 [rows, rotary_dim / 2]
+        or None (no rotation); positions: int32 [total_q] or None (a token's slot).  q_out may be q: in place."""
         import torch
-        a = self.append_args(q, k, v, q_out, k_cache, v_cache, cu_q, seqlens_k, block_table, cos, sin, interleaved,
-                             positions)
-        if stream is None:
-            stream = torch.cuda.current_stream().cuda_stream
-        status = self.serving.fav4_bshd_append_paged(C.byref(a), stream)
+        block = self._append_block(torch, q, k, v, q_out, k_cache, v_cache, cu_q, seqlens_k, block_table, cos, sin,
+                                   interleaved, positions)
+        status = self.serving.fav4_bshd_append_paged(block, self._stream(torch, k.get_device(), stream))
         if status:
             raise RuntimeError(f"append paged: HIP status {status}")
 
-    def prefix_args(self, q, k_cache, v_cache, o, lse, cu_q, seqlens_k, block_table, prefix_table, prefix_lens,
-                    cu_prefix_seqs, max_q, max_k, total_k=None, scale=None) -> PrefixArgs:
-        """Tensors as for paged_args; prefix_table: int32 [num_prefixes, max_pages]; prefix_lens: int32
-        [num_prefixes]; cu_prefix_seqs: int32 [num_prefixes + 1]."""
-        import torch
-        self._one_device(q, k_cache, v_cache, o, lse, cu_q, seqlens_k, block_table, prefix_table, prefix_lens,
-                         cu_prefix_seqs)
-        paged = self.paged_args(q, k_cache, v_cache, o, lse, cu_q, seqlens_k, block_table, max_q, max_k, total_k, scale)
-        assert all(c.dtype == torch.int32 and c.is_contiguous() for c in (prefix_table, prefix_lens, cu_prefix_seqs))
-        n, pages = prefix_table.shape
-        assert prefix_lens.numel() == n and cu_prefix_seqs.numel() == n + 1
-        return PrefixArgs(paged, prefix_table.data_ptr(), prefix_lens.data_ptr(), cu_prefix_seqs.data_ptr(), n, pages)
+    def _prefix_block(self, torch, q, k_cache, v_cache, o, lse, cu_q, seqlens_k, block_table, prefix_table,
+                      prefix_lens, cu_prefix_seqs, max_q, max_k, total_k, scale) -> bytes:
+        device = q.get_device()
+        num_pages, page_size, kv_heads, _ = self._caches(torch, device, k_cache, v_cache)
+        batch, pages = self._paged_batch(torch, device, cu_q, seqlens_k, block_table)
+        tokens, heads, d = q.shape
+        assert d == D and o.shape == q.shape and q.dtype is o.dtype is torch.bfloat16
+        assert q.is_contiguous() and o.is_contiguous() and o.get_device() == device
+        lse_ptr = 0
+        if lse is not None:
+            assert lse.shape == (heads, tokens) and lse.is_contiguous() and lse.dtype is torch.float32
+            assert lse.get_device() == device
+            lse_ptr = lse.data_ptr()
+        prefixes, prefix_pages = prefix_table.shape
+        assert prefix_lens.shape == (prefixes,) and cu_prefix_seqs.shape == (prefixes + 1,)
+        for x in (prefix_table, prefix_lens, cu_prefix_seqs):
+            assert x.dtype is torch.int32 and x.is_contiguous() and x.get_device() == device
+        return _PREFIX.pack(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), o.data_ptr(), lse_ptr,
+                            cu_q.data_ptr(), seqlens_k.data_ptr(), block_table.data_ptr(), batch, heads, kv_heads,
+                            int(max_q), int(max_k), tokens, 0 if total_k is None else int(total_k), num_pages,
+                            page_size, pages, SCALE if scale is None else scale, prefix_table.data_ptr(),
+                            prefix_lens.data_ptr(), cu_prefix_seqs.data_ptr(), prefixes, prefix_pages)
 
     def prefix_paged_workspace_size(self, batch, heads, kv_heads, max_q, max_k, total_q, page_size, max_pages,
                                     num_pages, num_prefixes, max_prefix_pages, causal=0) -> int:
+        """Workspace bytes of call_prefix_paged for a batch of this shape (-1: rejected)."""
         a = PrefixArgs(self.paged_shape_args(batch, heads, kv_heads, max_q, max_k, total_q, 0, page_size, max_pages,
                                              num_pages), None, None, None, num_prefixes, max_prefix_pages)
         return self.serving.fav4_bshd_prefix_paged_workspace_size(C.byref(a), int(causal))
@@ -578,23 +634,24 @@ class Runner:
     def call_prefix_paged(self, q, k_cache, v_cache, o, lse, cu_q, seqlens_k, block_table, prefix_table, prefix_lens,
                           cu_prefix_seqs, max_q, max_k, workspace=None, total_k=None, scale=None, stream=None,
                           causal=0):
-        """fav4_bshd_forward_prefix_paged: call_splitkv_paged for sequences that share leading pages (tensors as for
-        prefix_args; causal 0 dense, 2 bottom-right).  `workspace` as for call_splitkv (None: allocated here);
-        returned for the next call."""
+        """fav4_bshd_forward_prefix_paged: call_splitkv_paged for sequences that share leading pages.  Tensors as for
+        paged_args, and prefix_table: int32 [num_prefixes, max_pages]; prefix_lens: int32 [num_prefixes];
+        cu_prefix_seqs: int32 [num_prefixes + 1].  causal 0 dense, 2 bottom-right.  `workspace` as for call_splitkv
+        (None: allocated here); returned for the next call."""
         import torch
-        a = self.prefix_args(q, k_cache, v_cache, o, lse, cu_q, seqlens_k, block_table, prefix_table, prefix_lens,
-                             cu_prefix_seqs, max_q, max_k, total_k, scale)
+        block = self._prefix_block(torch, q, k_cache, v_cache, o, lse, cu_q, seqlens_k, block_table, prefix_table,
+                                   prefix_lens, cu_prefix_seqs, max_q, max_k, total_k, scale)
+        raw = self._stream(torch, q.get_device(), stream)
+        causal = int(causal)
         if workspace is None:
-            need = self.serving.fav4_bshd_prefix_paged_workspace_size(C.byref(a), int(causal))
+            need = self.serving.fav4_bshd_prefix_paged_workspace_size(block, causal)
             if need < 0:
                 raise RuntimeError("prefix paged: arguments rejected")
             # Allocated for the stream that uses it, which then orders its reuse.
             with torch.cuda.stream(None if stream is None else torch.cuda.ExternalStream(stream)):
                 workspace = torch.empty(need, device=q.device, dtype=torch.uint8)
-        if stream is None:
-            stream = torch.cuda.current_stream().cuda_stream
-        status = self.serving.fav4_bshd_forward_prefix_paged(
-            C.byref(a), int(causal), workspace.data_ptr(), workspace.numel() * workspace.element_size(), stream)
+        assert workspace.get_device() == q.get_device() and workspace.is_contiguous()
+        status = self.serving.fav4_bshd_forward_prefix_paged(block, causal, workspace.data_ptr(), workspace.nbytes, raw)
         if status:
             raise RuntimeError(f"prefix paged: HIP status {status}")
         return workspace

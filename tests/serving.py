@@ -100,25 +100,26 @@ class Batch:
             seen = (sk - sq + torch.arange(sq, device=self.dev) if causal == 2
                     else torch.full((sq,), sk - 1, device=self.dev))
             hidden = (torch.arange(sk, device=self.dev)[None] > seen[:, None]).repeat_interleave(g, 0)
-            for j in range(self.kv_heads):
-                hs = slice(j * g, (j + 1) * g)
-                got = o[rows, hs].double().reshape(sq * g, D)
-                assert torch.isfinite(got).all(), (b, j)
-                x = q[rows, hs].double().reshape(sq * g, D)
-                s = (x @ k[:, j].T * SCALE).masked_fill(hidden, -np.inf)
-                want_lse = torch.logsumexp(s, 1) if sk else torch.full((sq * g,), -np.inf, device=self.dev)
-                w = torch.exp(s - torch.where(torch.isneginf(want_lse), 0.0, want_lse)[:, None])
-                ref = w @ v[:, j]
-                # sum_j w_j |v_j - o| <= sqrt(sum_j w_j (v_j - o)^2), the weights' sum being 1 (0 in empty rows).
-                spread = (w @ v[:, j].square() - ref.square()).clamp(min=0).sqrt()
-                tol = (1.01 * HALF_STEP + weight_err) * spread + 1.01 * HALF_STEP * ref.abs() + 1e-5
-                worst = ((got - ref).abs() / tol).max().item()
-                assert worst <= 1, (b, sq, sk, j, worst)
-                if lse is not None:
-                    l = lse[hs, rows].double().T.reshape(sq * g)
-                    assert torch.equal(torch.isneginf(l), torch.isneginf(want_lse)), (b, j)
-                    fin = torch.isfinite(want_lse)
-                    assert ((l - want_lse)[fin].abs() <= LSE_TOL).all(), (b, j, (l - want_lse)[fin].abs().max())
+            by_head = lambda x: x.double().reshape(sq, self.kv_heads, g, D).transpose(0, 1).reshape(
+                self.kv_heads, sq * g, D)
+            k, v = k.transpose(0, 1).contiguous(), v.transpose(0, 1).contiguous()
+            got, x = by_head(o[rows]), by_head(q[rows])
+            assert torch.isfinite(got).all(), b
+            s = torch.bmm(x, k.transpose(1, 2).contiguous()).mul_(SCALE).masked_fill_(hidden, -np.inf)
+            want_lse = (torch.logsumexp(s, 2) if sk else
+                        torch.full((self.kv_heads, sq * g), -np.inf, dtype=torch.float64, device=self.dev))
+            w = torch.exp(s - torch.where(torch.isneginf(want_lse), 0.0, want_lse)[..., None])
+            ref = torch.bmm(w, v)
+            # sum_j w_j |v_j - o| <= sqrt(sum_j w_j (v_j - o)^2), the weights' sum being 1 (0 in empty rows).
+            spread = (torch.bmm(w, v.square()) - ref.square()).clamp(min=0).sqrt()
+            tol = (1.01 * HALF_STEP + weight_err) * spread + 1.01 * HALF_STEP * ref.abs() + 1e-5
+            worst = ((got - ref).abs() / tol).max().item()
+            assert worst <= 1, (b, sq, sk, worst)
+            if lse is not None:
+                l = lse[:, rows].double().reshape(self.kv_heads, g, sq).transpose(1, 2).reshape(self.kv_heads, sq * g)
+                assert torch.equal(torch.isneginf(l), torch.isneginf(want_lse)), b
+                fin = torch.isfinite(want_lse)
+                assert ((l - want_lse)[fin].abs() <= LSE_TOL).all(), (b, (l - want_lse)[fin].abs().max())
 
 
 def angles(rows, rotary_dim, dev):

@@ -26,6 +26,8 @@ CASES = {
     "prefill_mqa": (8, 1, 32, [(96, [(130, 226), (61, 157)])], [], 2),
     "more_queries_than_keys": (4, 2, 64, [(64, [(90, 70), (3, 66)])], [(5, 2)], 2),
     "no_prefix_at_all": (8, 2, 64, [(0, [(1, 500), (2, 64)])], [(1, 1000)], 0),
+    "more_row_tiles_than_workgroups": (64, 64, 32, [(128, [(300, 428), (290, 420), (310, 450), (257, 400)])], [], 2),
+    "more_row_tiles_than_workgroups_decode": (128, 128, 32, [(96, [(1, 97 + i % 60) for i in range(300)])], [], 0),
     "wide_group": (64, 2, 32, [(1600, [(2, 1700), (3, 1605)])], [], 2),
 }
 

@@ -69,6 +69,18 @@ def test_ctypes_layout_matches_the_header(pkg, name, tmp_path):
     assert got == [C.sizeof(cls)] + [getattr(cls, f).offset for f in fields]
 
 
+def test_packed_blocks_match_the_structs(pkg):
+    """The blocks that Runner packs in one step lie as the ctypes structs do."""
+    b = pkg.fav4_bshd
+    for packer, block in ((b._APPEND, append_args(pkg, positions=0xc0000)), (b._PREFIX, prefix_args(pkg, lse=0xb0000))):
+        assert packer.size == C.sizeof(block)
+        flat = []
+        for name, *_ in block._fields_:
+            value = getattr(block, name)
+            flat += [getattr(value, n) for n, *_ in value._fields_] if isinstance(value, C.Structure) else [value]
+        assert packer.pack(*flat) == bytes(block)
+
+
 APPEND_BAD = [{n: None} for n in ("k", "v", "q", "q_out", "k_cache", "v_cache", "cos", "sin", "cu_seqlens_q",
                                   "seqlens_k", "block_table")]
 APPEND_BAD += [{n: 0x10008} for n in ("q", "k", "v", "q_out", "k_cache", "v_cache", "cos", "sin")]
