@@ -80,7 +80,7 @@ bool prefix_shape_ok(const Fav4PrefixArgs* args, int causal) {
 
 struct PrefixSizes {
     fav4::PrefixPlan plan;
-    int64_t part_rows, note_rows, bytes, prefix_segs, prefix_ranges;
+    int64_t part_rows, note_rows, bytes, prefix_segs, prefix_ranges, prefix_tiles;
     int waves, prefix_rows;    // of a workgroup, of a prefix block
     fav4::Cut cut;
     bool ok;
@@ -108,13 +108,18 @@ PrefixSizes prefix_sizes(const Fav4PrefixArgs& args, int causal) {
     const int64_t prefix_segs = s.prefix_segs = tiles(args.num_prefixes, rows, BM);
     const int64_t own_segs = tiles(a.batch, a.max_seqlen_q * group, own_bm);
     const int64_t prefix_keys = std::min<int64_t>(int64_t(args.max_pages_per_prefix) * a.page_size, a.max_seqlen_k);
-    const int64_t extra = 1 + fav4::SEG_TILES;
+    s.prefix_tiles = prefix_keys / 32;
+    s.plan.most_prefix_keys = int(prefix_keys);
+    const int64_t lead = 1 + fav4::SEG_TILES;
+    const int64_t units = prefix_segs * (prefix_keys / 32 + lead) + own_segs * (a.max_seqlen_k / 32 + lead);
+    // No more waves than ranges (starting the waves of a full GPU takes 2 us).
+    if (s.cut == fav4::FEWEST)
+        s.plan.ranges = int(std::min<int64_t>(s.plan.ranges, std::max<int64_t>(2, units / (fav4::MIN_OWN_TILES * WAVES) + 1)));
     s.prefix_ranges = s.plan.ranges * (s.cut == fav4::FEWEST ? WAVES : 1);
     const int64_t prefix_blocks = prefix_segs + s.prefix_ranges;
     const int64_t own_blocks = own_segs + s.plan.ranges * (own_waves ? WAVES : 1);
     s.part_rows = (a.kv_heads * (prefix_blocks * BM + own_blocks * own_rows) + 1) & ~int64_t(1);   // notes 16-byte aligned
-    s.ok = prefix_segs * (prefix_keys / 32 + extra) < (1 << 30) && own_segs * (a.max_seqlen_k / 32 + extra) < (1 << 30) &&
-           prefix_blocks * BM <= INT_MAX && own_blocks * own_rows <= INT_MAX;
+    s.ok = units < (1 << 30) && prefix_blocks * BM <= INT_MAX && own_blocks * own_rows <= INT_MAX;
     s.plan.prefix_blocks = int(prefix_blocks);
     s.plan.own_blocks = int(own_blocks);
     s.plan.own_rows = int(own_rows);
@@ -162,10 +167,12 @@ extern "C" __attribute__((visibility("default"))) int fav4_bshd_append_paged(con
     if (!append_ok(a)) return hipErrorInvalidValue;
     const int rows = (a->q ? a->heads : 0) + 2 * a->kv_heads, units = (rows + 7) / 8;
     const int64_t total = int64_t(units) * a->total_q, blocks = std::min((total + 3) / 4, MAX_GRID);
-    if (a->interleaved)
-        hipLaunchKernelGGL(fav4::append_kernel<true>, dim3(unsigned(blocks)), dim3(256), 0, stream, *a, units, total);
-    else
-        hipLaunchKernelGGL(fav4::append_kernel<false>, dim3(unsigned(blocks)), dim3(256), 0, stream, *a, units, total);
+    const fav4::FastDiv by_units = fav4::fast_div(units), by_page = fav4::fast_div(a->page_size);
+    auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(unsigned(blocks)), dim3(256), 0, stream, *a, units, total, by_units, by_page);
+    };
+    if (a->interleaved) go(fav4::append_kernel<true>);
+    else go(fav4::append_kernel<false>);
     return hipGetLastError();
 }
 
@@ -197,20 +204,17 @@ extern "C" __attribute__((visibility("default"))) int fav4_bshd_forward_prefix_p
     launch_prefix(*args, s, stream);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    // Lane groups per merged row, by the parts that a prefix's row tile has when the
-    // prefixes take every range, as long as the rows leave the GPU some for it.
-    const int64_t rows = int64_t(a.total_q) * a.heads, parts = s.prefix_ranges / std::max<int64_t>(1, s.prefix_segs);
-    const int per = rows <= 1024 || (parts > 16 && rows <= 2048) ? 8
-                    : rows <= 2048 || (parts > 8 && rows <= 4096) ? 4
-                    : rows <= 4096                                ? 2
-                                                                  : 1;
-    const unsigned blocks = unsigned(std::min((rows * per + 7) / 8, MAX_GRID));
+    // Teams per merged row, by the most parts that a prefix's row tile can have on
+    // average, as long as the rows leave the GPU some for it.
+    const int64_t rows = int64_t(a.total_q) * a.heads;
+    const int64_t parts = std::min(s.prefix_ranges / std::max<int64_t>(1, s.prefix_segs), s.prefix_tiles / 2);
+    const int per = parts > 64 && rows <= 1024 ? 16 : rows <= 4096 ? 4 : 1;
+    const unsigned blocks = unsigned(std::min((rows * per + 15) / 16, MAX_GRID));
     auto merge = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, dim3(blocks), dim3(256), 0, stream, *args, s.plan, s.prefix_rows);
     };
-    if (per == 8) merge(fav4::prefix_merge_kernel<8>);
+    if (per == 16) merge(fav4::prefix_merge_kernel<16>);
     else if (per == 4) merge(fav4::prefix_merge_kernel<4>);
-    else if (per == 2) merge(fav4::prefix_merge_kernel<2>);
     else merge(fav4::prefix_merge_kernel<1>);
     return hipGetLastError();
 }

@@ -50,22 +50,22 @@ __device__ __forceinline__ int wave_find(const int* cu, int n, int x, int lane) 
 // themselves are loaded ahead of it.
 // ---------------------------------------------------------------------------
 template <bool INTERLEAVED>
-__global__ __launch_bounds__(256) void append_kernel(Fav4AppendArgs a, int units, int64_t total) {
+__global__ __launch_bounds__(256) void append_kernel(Fav4AppendArgs a, int units, int64_t total, FastDiv by_units, FastDiv by_page) {
     const int lane = threadIdx.x & 63, j = lane & 7;
     const int64_t stride = int64_t(gridDim.x) * 4;
     const int qheads = a.q ? a.heads : 0, rows = qheads + 2 * a.kv_heads;
     const int half = a.rotary_dim >> 4;                    // granules of half the rotated dims
     for (int64_t id = int64_t(blockIdx.x) * 4 + uniform(threadIdx.x >> 6); id < total; id += stride) {
-        const int t = uniform(int(id / units)), unit = uniform(int(id - int64_t(t) * units));
+        const int t = uniform(by_units(int(id))), unit = uniform(int(id) - t * units);
         const int row = unit * 8 + (lane >> 3);
         const bool live = row < rows, is_q = row < qheads, is_v = row >= qheads + a.kv_heads;
         const int head = is_q ? row : is_v ? row - qheads - a.kv_heads : row - qheads;
         const char* src = static_cast<const char*>(is_q ? a.q : is_v ? a.v : a.k);
         src += (int64_t(t) * (is_q ? a.q_stride : is_v ? a.v_stride : a.k_stride) + int64_t(head) * D) * 2;
         // This lane's granules of the row.
-        const bool turn = INTERLEAVED ? j < half : j < half;
-        const int g0 = INTERLEAVED ? 2 * j : turn ? j : 2 * half + 2 * (j - half);
-        const int g1 = INTERLEAVED ? g0 + 1 : turn ? j + half : g0 + 1;
+        const bool turn = j < half;
+        const int g0 = INTERLEAVED || !turn ? 2 * j : j;
+        const int g1 = INTERLEAVED || !turn ? g0 + 1 : j + half;
         bf16x8 x{}, y{};
         if (live) {
             x = *reinterpret_cast<const bf16x8*>(src + g0 * 16);
@@ -74,15 +74,14 @@ __global__ __launch_bounds__(256) void append_kernel(Fav4AppendArgs a, int units
         const int b = wave_find(a.cu_seqlens_q, a.batch, t, lane);
         if (b >= a.batch || t < a.cu_seqlens_q[0]) continue;           // behind the last sequence
         const int64_t slot = int64_t(a.seqlens_k[b]) - a.cu_seqlens_q[b + 1] + t;
-        const int64_t slots = int64_t(a.max_pages_per_seq) * a.page_size;
         int page = -1, in_page = 0;
-        if (slot >= 0 && slot < slots) {
-            const int at = int(slot / a.page_size);
-            in_page = int(slot - int64_t(at) * a.page_size);
+        if (slot >= 0 && slot < int64_t(a.max_pages_per_seq) * a.page_size && slot <= INT_MAX) {
+            const int at = by_page(int(slot));
+            in_page = int(slot) - at * a.page_size;
             page = a.block_table[int64_t(b) * a.max_pages_per_seq + at];
         }
         const bool stored = page >= 0 && page < a.num_pages;
-        if (half > 0 && turn && !is_v && live) {
+        if (turn && !is_v && live) {
             const int64_t pos = a.positions ? int64_t(a.positions[t]) : slot;
             const int64_t r = min(max(pos, int64_t(0)), int64_t(a.rotary_rows - 1));
             const int64_t at = r * (half * 8) + j * 8;
@@ -155,6 +154,7 @@ struct PrefixPlan {
     FastDiv by_kv_heads, by_group, by_page, by_heads, by_bm, by_own_rows;
     int prefix_blocks, own_blocks;    // partial blocks of a K/V head
     int own_rows;                     // rows of an own block
+    int most_prefix_keys;             // of a prefix: its table's, and max_seqlen_k
     int br;                           // bottom-right causal
 };
 
@@ -163,11 +163,20 @@ constexpr int MIN_PREFIX_TILES = 2, MIN_OWN_TILES = 2;  // shortest ranges
 // What a prefix's key tile costs, in own key tiles of a wave (its share of the
 // workgroups follows): 32 keys by four waves, 64 keys by eight.
 constexpr float PREFIX_COST_4 = 1.5f, PREFIX_COST_8 = 4.f;
-// Sequences and prefixes whose lengths are kept in LDS (others are read again
-// from memory where they are needed).
-constexpr int PLAN_SEQS = 1024, PLAN_PREFIXES = 256;
+// A prefix or a sequence: its tokens and the keys [k0, k1) that they read here.
+// A sequence of no prefix has k0 = -1 for 0.
+struct Family {
+    int t0, tokens, k0, k1;
+};
+
+// The families of a batch of up to so many sequences and prefixes are worked out
+// once and kept in LDS; of larger ones they are read from memory where they are
+// needed.  (What comes before the first tile is some 300 instructions that every
+// workgroup runs once, at about 10 ns each: their code has to be fetched.)
+constexpr int PLAN_SEQS = 512, PLAN_PREFIXES = 256;
 struct PlanLds {
-    int cu[PLAN_SEQS + 1], keys[PLAN_SEQS], shared[PLAN_SEQS], first_seq[PLAN_PREFIXES + 1], prefix_keys[PLAN_PREFIXES];
+    int4 own[PLAN_SEQS + 1], prefix[PLAN_PREFIXES];
+    int first_seq[PLAN_PREFIXES + 1], prefix_keys[PLAN_PREFIXES];
 };
 
 // The batch as read on the device, clamped: tokens to [0, total_q], keys to
@@ -189,12 +198,10 @@ struct PrefixBatch {
         return min(max(a.cu_prefix_seqs[p], 0), a.paged.batch);
     }
     __device__ __forceinline__ int load_prefix_keys(int p) const {
-        const int page = a.paged.page_size;
-        const int most = int(min(int64_t(a.max_pages_per_prefix) * page, int64_t(a.paged.max_seqlen_k)));
-        return pl.by_page(min(max(a.prefix_lens[p], 0), most)) * page;
+        return pl.by_page(min(max(a.prefix_lens[p], 0), pl.most_prefix_keys)) * a.paged.page_size;
     }
-    __device__ __forceinline__ int cu(int b) const { return CACHED ? lds.cu[b] : load_cu(b); }
-    __device__ __forceinline__ int keys(int b) const { return CACHED ? lds.keys[b] : load_keys(b); }
+    __device__ __forceinline__ int cu(int b) const { return CACHED ? lds.own[b].x : load_cu(b); }
+    __device__ __forceinline__ int keys(int b) const { return CACHED ? lds.own[b].w : load_keys(b); }
     __device__ __forceinline__ int first_seq(int p) const { return CACHED ? lds.first_seq[p] : load_first_seq(p); }
     __device__ __forceinline__ int prefix_keys(int p) const { return CACHED ? lds.prefix_keys[p] : load_prefix_keys(p); }
     // Shared keys of sequence b: of the last prefix that starts at or before it.
@@ -207,23 +214,22 @@ struct PrefixBatch {
         }
         return first_seq(lo) <= b && b < first_seq(lo + 1) ? prefix_keys(lo) : 0;
     }
-    __device__ __forceinline__ int shared(int b) const { return CACHED ? lds.shared[b] : find_shared(b); }
+    __device__ __forceinline__ Family make_prefix(int p) const {
+        const int s0 = first_seq(p), s1 = max(first_seq(p + 1), s0), t0 = cu(s0), keys = prefix_keys(p);
+        return {t0, keys > 0 ? max(0, cu(s1) - t0) : 0, 0, keys};
+    }
+    __device__ __forceinline__ Family make_own(int t0, int t1, int sk, int shared) const {
+        return {t0, min(max(t1 - t0, 0), a.paged.max_seqlen_q), shared > 0 ? min(shared, sk) : -1, sk};
+    }
+    __device__ __forceinline__ Family prefix_family(int p) const {
+        if constexpr (CACHED) return __builtin_bit_cast(Family, lds.prefix[p]);
+        return make_prefix(p);
+    }
+    __device__ __forceinline__ Family own_family(int b) const {
+        if constexpr (CACHED) return __builtin_bit_cast(Family, lds.own[b]);
+        return make_own(load_cu(b), load_cu(b + 1), load_keys(b), find_shared(b));
+    }
 };
-
-// A prefix or a sequence: its tokens and the keys [k0, k1) that they read here.
-struct Family {
-    int t0, tokens, k0, k1;
-};
-template <class B>
-__device__ __forceinline__ Family prefix_family(const B& x, int p) {
-    const int s0 = x.first_seq(p), s1 = max(x.first_seq(p + 1), s0), t0 = x.cu(s0), keys = x.prefix_keys(p);
-    return {t0, keys > 0 ? max(0, x.cu(s1) - t0) : 0, 0, keys};
-}
-template <class B>
-__device__ __forceinline__ Family own_family(const B& x, int b) {
-    const int t0 = x.cu(b), sk = x.keys(b);
-    return {t0, min(max(x.cu(b + 1) - t0, 0), x.a.paged.max_seqlen_q), min(x.shared(b), sk), sk};
-}
 
 // A line of families' segments: row tiles of ROWS rows, key tiles of BN keys,
 // LEAD units before each segment's key tiles.
@@ -231,9 +237,9 @@ template <class B, bool OWN, int ROWS, int BN, int LEAD>
 struct Line {
     const B& x;
     int count, group;
-    __device__ __forceinline__ Family family(int i) const { return OWN ? own_family(x, i) : prefix_family(x, i); }
+    __device__ __forceinline__ Family family(int i) const { return OWN ? x.own_family(i) : x.prefix_family(i); }
     __device__ __forceinline__ int tiles(const Family& f) const { return int(uint32_t(f.tokens * group + ROWS - 1) / ROWS); }
-    __device__ __forceinline__ int key_tiles(const Family& f) const { return int(uint32_t(f.k1 - f.k0 + BN - 1) / BN); }
+    __device__ __forceinline__ int key_tiles(const Family& f) const { return int(uint32_t(f.k1 - max(f.k0, 0) + BN - 1) / BN); }
     __device__ __forceinline__ int seg_cost(const Family& f) const { return max(1, key_tiles(f)) + LEAD; }
 
     // Up to 64 families from i on in the wave's lanes: the units and segments up to and with each.
@@ -329,8 +335,9 @@ __device__ __forceinline__ Visible visible(const B& x, const PrefixPlan& pl, con
         if (!pl.br) return {f.k1 - 1, uniform(f.k1), uniform(f.k1)};
         const int shift = f.k1 - f.tokens;                             // last visible key of query 0
         const int i0 = pl.by_group(first), i1 = pl.by_group(last);
-        return {shift + tok - f.t0, uniform(max(f.k0, min(f.k1, shift + i0 + 1))),
-                uniform(max(f.k0, min(f.k1, shift + i1 + 1)))};
+        const int k0 = max(f.k0, 0);
+        return {shift + tok - f.t0, uniform(max(k0, min(f.k1, shift + i0 + 1))),
+                uniform(max(k0, min(f.k1, shift + i1 + 1)))};
     } else {
         if (!x.hidden) return {INT_MAX, uniform(f.k1), uniform(f.k1)};
         // The last of the prefix's sequences that starts at or before tok.
@@ -391,7 +398,7 @@ __device__ __forceinline__ void attend_shared(const B& x, const PrefixPlan& pl, 
     typename L::Place at = aligned ? typename L::Place{0, 0, 0} : line.find(g0, lane, head);
     for (; at.idx < line.count && at.base < g1; ++at.idx) {
         const Family f = line.family(at.idx);
-        const int t0 = uniform(f.t0), tokens = uniform(f.tokens), k0 = uniform(f.k0), k1 = uniform(f.k1);
+        const int t0 = uniform(f.t0), tokens = uniform(f.tokens), k0 = uniform(max(f.k0, 0)), k1 = uniform(f.k1);
         const int tiles = uniform(line.tiles(f)), ktiles = uniform(line.key_tiles(f)),
                   seg_cost = aligned ? aligned : uniform(line.seg_cost(f));
         const int rows = tokens * group;
@@ -475,7 +482,7 @@ __device__ __forceinline__ void attend_shared(const B& x, const PrefixPlan& pl, 
                 const int parts = ktiles > 0 ? (first + ktiles - 1) / per - first / per + 1 : 0;
                 int2* note = pl.notes + (int64_t(t0) * group + row) * 2;
                 note[OWN] = int2{block * stride + wave * 32 + lane, parts};
-                if (OWN && k0 == 0 && x.shared(at.idx) == 0) note[0] = int2{0, 0};
+                if (OWN && uniform(f.k0) < 0) note[0] = int2{0, 0};
             }
             // The staging has been read (its values were stored) before this wave's
             // next copy into its slots.
@@ -512,7 +519,7 @@ __device__ __forceinline__ void attend_wave(const B& x, const PrefixPlan& pl, co
     typename L::Place at = line.find(max(0, g0 - origin), lane, head);
     for (at.base += origin; at.idx < line.count && at.base < g1; ++at.idx) {
         const Family f = line.family(at.idx);
-        const int t0 = uniform(f.t0), tokens = uniform(f.tokens), k0 = uniform(f.k0), k1 = uniform(f.k1);
+        const int t0 = uniform(f.t0), tokens = uniform(f.tokens), k0 = uniform(max(f.k0, 0)), k1 = uniform(f.k1);
         const int tiles = uniform(line.tiles(f)), ktiles = uniform(line.key_tiles(f)), seg_cost = uniform(line.seg_cost(f));
         const int rows = tokens * group;
         const int kvh = uniform(turn + at.idx - pl.by_kv_heads(turn + at.idx) * pg.kv_heads);
@@ -570,7 +577,7 @@ __device__ __forceinline__ void attend_wave(const B& x, const PrefixPlan& pl, co
                 const int parts = ktiles > 0 ? (first + ktiles - 1) / per - first / per + 1 : 0;
                 int2* note = pl.notes + (int64_t(t0) * group + row) * 2;
                 note[OWN] = int2{block * stride + lane, parts};
-                if (OWN && k0 == 0 && x.shared(at.idx) == 0) note[0] = int2{0, 0};
+                if (OWN && uniform(f.k0) < 0) note[0] = int2{0, 0};
             }
             // The staging has been read (its values were stored) before the next copy.
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -605,20 +612,23 @@ void prefix_kernel(Fav4PrefixArgs a, PrefixPlan pl) {
     if constexpr (CACHED) {
         // One round of loads for as many sequences as the workgroup has lanes.
         for (int i = threadIdx.x; i <= max(pg.batch, a.num_prefixes); i += WAVES * 64) {
-            const int cu = x.load_cu(min(i, pg.batch)), keys = x.load_keys(min(i, pg.batch - 1));
+            const int t0 = x.load_cu(min(i, pg.batch)), t1 = x.load_cu(min(i + 1, pg.batch));
+            const int sk = x.load_keys(min(i, pg.batch - 1));
             const int first = x.load_first_seq(min(i, a.num_prefixes));
             const int prefix_keys = x.load_prefix_keys(min(i, a.num_prefixes - 1));
-            if (i <= pg.batch) lds.cu[i] = cu;
-            if (i < pg.batch) lds.keys[i] = keys;
+            if (i <= pg.batch) lds.own[i] = __builtin_bit_cast(int4, x.make_own(t0, t1, sk, 0));
             if (i <= a.num_prefixes) lds.first_seq[i] = first;
             if (i < a.num_prefixes) lds.prefix_keys[i] = prefix_keys;
         }
         __syncthreads();
         int hidden = 0;
-        for (int i = threadIdx.x; i < pg.batch; i += WAVES * 64) {
-            const int shared = x.find_shared(i), n = lds.cu[i + 1] - lds.cu[i];
-            lds.shared[i] = shared;
-            hidden |= n > 0 && lds.keys[i] - (pl.br ? n : 1) < shared - 1;
+        for (int i = threadIdx.x; i < max(pg.batch, a.num_prefixes); i += WAVES * 64) {
+            if (i < pg.batch) {
+                const int shared = x.find_shared(i), sk = lds.own[i].w, n = lds.own[i + 1].x - lds.own[i].x;
+                if (shared > 0) lds.own[i].z = min(shared, sk);
+                hidden |= n > 0 && sk - (pl.br ? n : 1) < shared - 1;
+            }
+            if (i < a.num_prefixes) lds.prefix[i] = __builtin_bit_cast(int4, x.make_prefix(i));
         }
         x.hidden = __syncthreads_or(hidden);
     }
@@ -675,17 +685,19 @@ void prefix_kernel(Fav4PrefixArgs a, PrefixPlan pl) {
     }
 }
 
-// Merge of a row's parts: PER groups of 32 lanes share one row of one head, 4
-// dims a lane; a group takes every PER-th part, NS at a time with all their
-// loads in flight, and keeps the running maximum and sums of a softmax over
-// the parts' log-sums.
+// Merge of a row's parts.  PER teams of 16 lanes share one row of one head, 8
+// dims a lane; a team takes every PER-th part, NS at a time with all their loads
+// in flight, and keeps the running maximum and sums of a softmax over the
+// parts' log-sums.  Bound by the chain notes -> parts -> output, and by the rate
+// at which waves start: few teams with many loads each, and rather than 32
+// lanes a row.
 template <int PER>
 __global__ __launch_bounds__(256) void prefix_merge_kernel(Fav4PrefixArgs a, PrefixPlan pl, int bm) {
-    constexpr int RPB = 8 / PER, NS = 4;
-    __shared__ float4 red[8];
-    __shared__ f32x4 red_o[8][32];
+    constexpr int RPB = 16 / PER, NS = PER == 1 ? 4 : 8;
+    __shared__ float4 red[16];
+    __shared__ f32x4 red_o[16][32];
     const Fav4PagedArgs& pg = a.paged;
-    const int grp = threadIdx.x >> 5, q4 = threadIdx.x & 31;
+    const int grp = threadIdx.x >> 4, l16 = threadIdx.x & 15;
     const int slot = grp / PER, part = grp - slot * PER;
     const int group = pl.group;
     const uint32_t rows = uint32_t(pg.total_q) * uint32_t(pg.heads), blocks = (rows + RPB - 1) / RPB;
@@ -699,9 +711,8 @@ __global__ __launch_bounds__(256) void prefix_merge_kernel(Fav4PrefixArgs a, Pre
             const int4 note = *reinterpret_cast<const int4*>(pl.notes + (int64_t(tok) * group + hg) * 2);
             live = tok >= pg.cu_seqlens_q[0] && tok < pg.cu_seqlens_q[pg.batch];
             // Clamped: bad offsets leave notes unwritten.
-            const int last_p = pl.prefix_blocks * bm - 1, last_o = pl.own_blocks * pl.own_rows - 1;
-            first[0] = min(max(note.x, 0), last_p);
-            first[1] = min(max(note.z, 0), last_o);
+            first[0] = min(max(note.x, 0), pl.prefix_blocks * bm - 1);
+            first[1] = min(max(note.z, 0), pl.own_blocks * pl.own_rows - 1);
             if (live) {
                 n[0] = min(max(note.y, 0), pl.prefix_blocks - pl.by_bm(first[0]));
                 n[1] = min(max(note.w, 0), pl.own_blocks - pl.by_own_rows(first[1]));
@@ -712,17 +723,18 @@ __global__ __launch_bounds__(256) void prefix_merge_kernel(Fav4PrefixArgs a, Pre
         const int64_t at_o = int64_t(pg.kv_heads) * pl.prefix_blocks * bm + int64_t(kvh) * pl.own_blocks * pl.own_rows +
                              first[1];
         float mb = -__builtin_inff(), ml = mb, den = 0.f, suml = 0.f;
-        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        f32x4 acc[2] = {};
         for (int c0 = part; c0 < total; c0 += PER * NS) {
             // Loads past the last part repeat it, with weight 0: no branch between the loads.
             float2 v[NS];
-            f32x4 xo[NS];
+            f32x4 xo[NS][2];
 #pragma unroll
             for (int i = 0; i < NS; ++i) {
                 const int c = min(c0 + i * PER, total - 1);
                 const int64_t row = c < n[0] ? at_p + int64_t(c) * bm : at_o + int64_t(c - n[0]) * pl.own_rows;
                 v[i] = reinterpret_cast<const float2*>(pl.lse_part)[row];
-                xo[i] = *reinterpret_cast<const f32x4*>(pl.o_part + row * D + q4 * 4);
+                const f32x4* o = reinterpret_cast<const f32x4*>(pl.o_part + row * D + l16 * 8);
+                xo[i][0] = o[0], xo[i][1] = o[1];
             }
 #pragma unroll
             for (int i = 0; i < NS; ++i)
@@ -732,26 +744,26 @@ __global__ __launch_bounds__(256) void prefix_merge_kernel(Fav4PrefixArgs a, Pre
             for (int i = 0; i < NS; ++i) nb = fmaxf(nb, v[i].x), nl = fmaxf(nl, v[i].y);
             if (nb == -__builtin_inff()) continue;             // parts without a visible key
             const float keep = exp2_native(mb - nb);
-            acc *= keep;
+            acc[0] *= keep, acc[1] *= keep;
             den *= keep;
             suml *= exp2_native(ml - nl);
             mb = nb, ml = nl;
 #pragma unroll
             for (int i = 0; i < NS; ++i) {
                 const float wgt = exp2_native(v[i].x - mb);
-                if (wgt > 0.f) acc += wgt * xo[i];
+                if (wgt > 0.f) acc[0] += wgt * xo[i][0], acc[1] += wgt * xo[i][1];
                 den += wgt;
                 suml += exp2_native(v[i].y - ml);
             }
         }
         if constexpr (PER > 1) {
-            if (q4 == 0) red[grp] = float4{mb, ml, den, suml};
-            red_o[grp][q4] = acc;
+            if (l16 == 0) red[grp] = float4{mb, ml, den, suml};
+            red_o[grp][l16 * 2] = acc[0], red_o[grp][l16 * 2 + 1] = acc[1];
             __syncthreads();
 #pragma unroll
             for (int p = 0; p < PER; ++p) mb = fmaxf(mb, red[slot * PER + p].x), ml = fmaxf(ml, red[slot * PER + p].y);
             den = suml = 0.f;
-            acc = f32x4{0.f, 0.f, 0.f, 0.f};
+            acc[0] = acc[1] = f32x4{};
 #pragma unroll
             for (int p = 0; p < PER; ++p) {
                 const float4 o = red[slot * PER + p];
@@ -759,19 +771,18 @@ __global__ __launch_bounds__(256) void prefix_merge_kernel(Fav4PrefixArgs a, Pre
                 const float wgt = exp2_native(o.x - mb);
                 den += wgt * o.z;
                 suml += exp2_native(o.y - ml) * o.w;
-                acc += wgt * red_o[slot * PER + p][q4];
+                acc[0] += wgt * red_o[slot * PER + p][l16 * 2], acc[1] += wgt * red_o[slot * PER + p][l16 * 2 + 1];
             }
             __syncthreads();
         }
         if (!live || part != 0) continue;
         // No key in any part: O = 0, LSE = -inf.
         const float rden = den > 0.f ? 1.f / den : 0.f;
-        const f32x4 y = acc * rden;
-        const f32x2 y0 = {y[0], y[1]}, y1 = {y[2], y[3]};
-        const bf16x2 b0 = __builtin_convertvector(y0, bf16x2), b1 = __builtin_convertvector(y1, bf16x2);
-        *reinterpret_cast<bf16x4*>(static_cast<char*>(pg.o) + int64_t(r) * ROW_BYTES + q4 * 8) =
-            bf16x4{b0[0], b0[1], b1[0], b1[1]};
-        if (pg.lse && q4 == 0) pg.lse[int64_t(head) * pg.total_q + tok] =
+        bf16x8 y;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = __bf16(acc[i >> 2][i & 3] * rden);
+        *reinterpret_cast<bf16x8*>(static_cast<char*>(pg.o) + int64_t(r) * ROW_BYTES + l16 * 16) = y;
+        if (pg.lse && l16 == 0) pg.lse[int64_t(head) * pg.total_q + tok] =
             den > 0.f ? (ml + __builtin_amdgcn_logf(suml)) * LN2 : -__builtin_inff();
     }
 }
