@@ -43,7 +43,7 @@ bool append_ok(const Fav4AppendArgs* a) {
         return false;
     if (a->rotary_dim > 0 ? !a->cos || !a->sin || a->rotary_rows < 1 : a->cos || a->sin) return false;
     const int64_t rows = (a->q ? int64_t(a->heads) : 0) + 2 * int64_t(a->kv_heads);
-    if (rows * a->total_q > INT_MAX) return false;
+    if (rows > INT_MAX || rows * a->total_q > INT_MAX) return false;
     auto stride_ok = [&](long long stride, int heads) {
         return stride >= int64_t(heads) * fav4::D && (stride & 7) == 0 &&
                static_cast<__int128>(stride) * a->total_q * 2 < MAX_BYTES;
@@ -62,6 +62,8 @@ constexpr int BOTTOM_RIGHT = 2;
 constexpr int PREFIX_WAVE_ROWS = 32;  // up to this many rows of a prefix (the mean): its keys are, too
 constexpr int WAVE_ROWS = 64;      // up to this many rows of a sequence: its own keys are read by single waves
 
+constexpr int MAX_HEADS = 1 << 15;    // the Q rows of a 256-row tile lie within 4 GiB
+
 bool prefix_shape_ok(const Fav4PrefixArgs* args, int causal) {
     if (!args) return false;
     const Fav4PagedArgs& a = args->paged;
@@ -71,7 +73,7 @@ bool prefix_shape_ok(const Fav4PrefixArgs* args, int causal) {
         (causal != 0 && causal != BOTTOM_RIGHT) || !std::isfinite(a.scale) || a.scale <= 0)
         return false;
     if (a.page_size % 32 || a.max_seqlen_k > int64_t(a.max_pages_per_seq) * a.page_size ||
-        a.heads > INT_MAX / fav4::D || int64_t(a.total_q) * a.heads > INT_MAX ||
+        a.heads > MAX_HEADS || int64_t(a.total_q) * a.heads > INT_MAX ||
         int64_t(a.kv_heads) * fav4::ROW_BYTES * 32 > INT_MAX ||
         static_cast<__int128>(a.num_pages) * a.page_size * a.kv_heads * fav4::ROW_BYTES >= MAX_BYTES)
         return false;
@@ -80,7 +82,7 @@ bool prefix_shape_ok(const Fav4PrefixArgs* args, int causal) {
 
 struct PrefixSizes {
     fav4::PrefixPlan plan;
-    int64_t part_rows, note_rows, bytes, prefix_segs, prefix_ranges, prefix_tiles;
+    int64_t part_rows, bytes, prefix_segs, prefix_ranges, prefix_tiles;
     int waves, prefix_rows;    // of a workgroup, of a prefix block
     fav4::Cut cut;
     bool ok;
@@ -88,6 +90,7 @@ struct PrefixSizes {
 PrefixSizes prefix_sizes(const Fav4PrefixArgs& args, int causal) {
     const Fav4PagedArgs& a = args.paged;
     const int64_t group = a.heads / a.kv_heads, rows = a.total_q * group;
+    const int64_t seq_rows = std::min<int64_t>(a.max_seqlen_q * group, rows);
     PrefixSizes s{};
     s.plan.br = causal == BOTTOM_RIGHT;
     s.cut = a.max_seqlen_q * group > WAVE_ROWS                     ? fav4::MANY
@@ -104,9 +107,9 @@ PrefixSizes prefix_sizes(const Fav4PrefixArgs& args, int causal) {
         return std::min(n * ((most + bm - 1) / bm), (rows + n * (bm - 1)) / bm);
     };
     const int own_bm = own_waves ? 32 : BM;
-    const int64_t own_rows = std::min<int64_t>(own_bm, a.max_seqlen_q * group);
+    const int64_t own_rows = std::min<int64_t>(own_bm, seq_rows);
     const int64_t prefix_segs = s.prefix_segs = tiles(args.num_prefixes, rows, BM);
-    const int64_t own_segs = tiles(a.batch, a.max_seqlen_q * group, own_bm);
+    const int64_t own_segs = tiles(a.batch, seq_rows, own_bm);
     const int64_t prefix_keys = std::min<int64_t>(int64_t(args.max_pages_per_prefix) * a.page_size, a.max_seqlen_k);
     s.prefix_tiles = prefix_keys / 32;
     s.plan.most_prefix_keys = int(prefix_keys);
@@ -130,8 +133,14 @@ PrefixSizes prefix_sizes(const Fav4PrefixArgs& args, int causal) {
     s.plan.by_heads = fav4::fast_div(a.heads);
     s.plan.by_bm = fav4::fast_div(BM);
     s.plan.by_own_rows = fav4::fast_div(int(own_rows));
-    s.note_rows = rows;
-    s.bytes = s.part_rows * (fav4::D * 4 + 8) + s.note_rows * 16;
+    // What a call of any cut needs at most: a larger batch, more queries or prefixes
+    // never need less, so that one workspace serves a serving loop's smaller steps.
+    const int64_t range_rows = std::max<int64_t>(512, int64_t(2) * device_cus() * 128 / a.kv_heads);
+    const int64_t own_pad = a.max_seqlen_q * group > WAVE_ROWS ? 255 : 31;
+    const int64_t most = a.kv_heads * (2 * (rows + range_rows) + int64_t(args.num_prefixes) * 255 + a.batch * own_pad);
+    s.ok = s.ok && s.part_rows <= most + 1 && most < (int64_t(1) << 40);
+    if (!s.ok) return s;
+    s.bytes = (most + 1) * (fav4::D * 4 + 8) + rows * 16;
     return s;
 }
 

@@ -519,9 +519,10 @@ class Runner:
     @staticmethod
     def _stream(torch, device, stream):
         """The stream to launch on (None: torch's current one), with `device`, the tensors', current."""
-        if device < 0 or device != torch.cuda.current_device():
-            raise ValueError(f"tensors on {'the host' if device < 0 else f'cuda:{device}'}, current device "
-                             f"cuda:{torch.cuda.current_device()}")
+        if device < 0:
+            raise ValueError("tensors on the host: the library works on GPU memory")
+        if device != torch.cuda.current_device():
+            raise ValueError(f"tensors on cuda:{device}, current device cuda:{torch.cuda.current_device()}")
         if stream is not None:
             return stream
         raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)       # without a Stream object

@@ -151,6 +151,40 @@ def test_prefix_in_a_graph(gpu_runner):
         assert torch.equal(o.view(torch.int16), eager.view(torch.int16)) and torch.equal(l, el)
 
 
+def test_prefix_far_pages(gpu_runner):
+    """Caches of more than 2^31 elements: shared and own pages past 4 GiB."""
+    x = Batch(8, 8, 128, [(256, [(1, 300), (2, 257)])], seed=3)
+    pool, far = x.k.shape[0], 17000
+    k = torch.zeros((far, 128, 8, 128), dtype=torch.bfloat16, device=x.dev)
+    v = torch.zeros_like(k)
+    k[far - pool:], v[far - pool:] = x.k, x.v
+    x.k, x.v = k, v
+    for t in (x.table, x.prefix_table):
+        t[(t >= 0) & (t < pool)] += far - pool
+        t[t == pool] = far
+    x.pages = [p + far - pool for p in x.pages]
+    x.table_d.copy_(torch.from_numpy(x.table))
+    x.prefix_table_d.copy_(torch.from_numpy(x.prefix_table))
+    o, l = x.outputs(True)
+    x.attend(gpu_runner, o, l, 2)
+    torch.cuda.synchronize()
+    x.check(o, l, 2)
+
+
+def test_prefix_bad_pages_stay_with_their_sequence(gpu_runner):
+    """Page numbers out of range are clamped: the sequence that has them gets some value, the others theirs."""
+    x = Batch(8, 2, 64, [(128, [(1, 200), (1, 400), (1, 300)])])
+    x.k.nan_to_num_(0.0)
+    x.v.nan_to_num_(0.0)
+    x.table_d[1, 2:] = torch.tensor([-7, 1 << 30, x.k.shape[0], -1, 5], dtype=torch.int32)[:x.table_d.shape[1] - 2]
+    o, l = x.outputs(True)
+    x.attend(gpu_runner, o, l, 0)
+    torch.cuda.synchronize()
+    assert torch.isfinite(o).all()
+    x.lens[1] = (0, 400)                    # not checked
+    x.check(o, l, 0)
+
+
 def test_prefix_on_two_streams(gpu_runner):
     """Two calls at once, each on a stream and with a workspace of its own."""
     xs = [Batch(16, 4, 64, [(1024, [(1, 1100 + 10 * i) for i in range(8)])], seed=s) for s in (1, 2)]

@@ -92,7 +92,8 @@ APPEND_BAD += [dict(q_stride=4088), dict(q_stride=4100), dict(k_stride=1016), di
                dict(q_out_stride=2048), dict(q_out=0x10000, q_out_stride=8192),
                dict(rotary_dim=0), dict(rotary_dim=0, cos=None), dict(total_q=1 << 27),
                dict(k_stride=1 << 50), dict(num_pages=1 << 30, page_size=1 << 20),
-               dict(kv_heads=1 << 30), dict(heads=(1 << 31) - 1)]
+               dict(kv_heads=1 << 30), dict(heads=(1 << 31) - 1),
+               dict(heads=(1 << 31) - 1, kv_heads=(1 << 31) - 1, total_q=(1 << 31) - 1)]
 
 
 @pytest.mark.parametrize("over", APPEND_BAD, ids=str)
@@ -109,9 +110,11 @@ PREFIX_SHAPES_BAD = [{n: v} for n in ("batch", "heads", "kv_heads", "max_seqlen_
                                       "max_pages_per_prefix") for v in (0, -1)]
 PREFIX_SHAPES_BAD += [dict(total_k=-1), dict(kv_heads=5), dict(kv_heads=64), dict(scale=0.0), dict(scale=-1.0),
                       dict(scale=float("nan")), dict(scale=float("inf")), dict(page_size=16), dict(page_size=33),
-                      dict(max_seqlen_k=1025), dict(total_q=1 << 27), dict(heads=1 << 25, kv_heads=1),
+                      dict(max_seqlen_k=1025), dict(total_q=1 << 27), dict(heads=1 << 25, kv_heads=1), dict(heads=(1 << 15) + 8),
                       dict(num_pages=1 << 30, page_size=1 << 20),
-                      dict(batch=1 << 20, max_seqlen_k=1 << 20, max_pages_per_seq=1 << 20)]
+                      dict(batch=1 << 20, max_seqlen_k=1 << 20, max_pages_per_seq=1 << 20),
+                      dict(batch=(1 << 31) - 1, num_prefixes=(1 << 31) - 1, max_seqlen_q=(1 << 31) - 1,
+                           heads=1 << 15, kv_heads=1 << 15, total_q=65535)]
 
 
 @pytest.mark.parametrize("over", PREFIX_SHAPES_BAD, ids=str)
@@ -145,11 +148,50 @@ def test_prefix_refuses_masks_and_workspaces(pkg, lib):
 
 
 def test_prefix_workspace_grows_with_the_batch(pkg, lib):
-    """One workspace, sized for a serving loop's largest batch, serves the smaller ones."""
+    """One workspace, sized for a serving loop's largest batch, serves the smaller ones, whatever way they are cut."""
     size = lambda **over: lib.fav4_bshd_prefix_paged_workspace_size(C.byref(prefix_args(pkg, **over)), 2)
     base = size()
-    for over in (dict(batch=9, total_q=9), dict(max_seqlen_q=5, total_q=20), dict(num_prefixes=4, total_q=64, batch=64),
-                 dict(batch=300, total_q=300)):
-        assert size(**over) >= base
+    assert base > 0
+    for kvh in (1, 2, 8, 32, 128):
+        heads = max(32, kvh)
+        last = 0
+        for batch, q, prefixes in ((1, 1, 1), (2, 1, 1), (40, 1, 1), (40, 1, 20), (100, 1, 20), (100, 4, 20),
+                                   (100, 30, 20), (300, 200, 64), (2000, 200, 64), (2000, 300, 300)):
+            for keys in (64, 1000):
+                n = size(batch=batch, max_seqlen_q=q, total_q=batch * q, num_prefixes=prefixes, max_seqlen_k=keys,
+                         heads=heads, kv_heads=kvh)
+                assert n >= last, (kvh, batch, q, prefixes, keys)
+            last = n
     # Keys do not count: the partials are as many as the ranges and the row tiles.
     assert size(max_seqlen_k=64) == base == size(max_pages_per_prefix=100)
+
+
+def test_runner_refuses_host_tensors(pkg):
+    import torch
+    r = pkg.Runner()
+    bf16 = lambda *s: torch.zeros(s, dtype=torch.bfloat16)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32)
+    kc, vc, table = bf16(2, 64, 1, 128), bf16(2, 64, 1, 128), torch.zeros((1, 2), dtype=torch.int32)
+    with pytest.raises(ValueError):
+        r.call_append_paged(bf16(1, 2, 128), bf16(1, 1, 128), bf16(1, 1, 128), bf16(1, 2, 128), kc, vc, i32(0, 1),
+                            i32(1), table)
+    with pytest.raises(ValueError):
+        r.call_prefix_paged(bf16(1, 2, 128), kc, vc, bf16(1, 2, 128), None, i32(0, 1), i32(1), table, table, i32(0),
+                            i32(0, 1), 1, 64)
+
+
+@pytest.mark.parametrize("wrong", ["dtype", "shape", "heads", "stride", "lens", "table", "angles", "q_out"])
+def test_runner_checks_append_tensors(pkg, wrong):
+    import torch
+    bf16 = lambda *s: torch.zeros(s, dtype=torch.bfloat16)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32)
+    x = dict(q=bf16(3, 4, 128), k=bf16(3, 2, 128), v=bf16(3, 2, 128), q_out=bf16(3, 4, 128), k_cache=bf16(2, 64, 2, 128),
+             v_cache=bf16(2, 64, 2, 128), cu_q=i32(0, 1, 3), seqlens_k=i32(1, 2),
+             block_table=torch.zeros((2, 1), dtype=torch.int32), cos=torch.zeros(9, 64), sin=torch.zeros(9, 64))
+    x.update(dict(dtype=dict(k=torch.zeros(3, 2, 128)), shape=dict(v=bf16(2, 2, 128)), heads=dict(k=bf16(3, 1, 128)),
+                  stride=dict(k=bf16(3, 128, 2).transpose(1, 2)), lens=dict(seqlens_k=i32(1)),
+                  table=dict(block_table=torch.zeros((2, 2), dtype=torch.int32).t()), angles=dict(sin=torch.zeros(9, 32)),
+                  q_out=dict(q_out=None))[wrong])
+    with pytest.raises((AssertionError, ValueError)) as e:
+        pkg.Runner().call_append_paged(**x)
+    assert "host" not in str(e.value)
