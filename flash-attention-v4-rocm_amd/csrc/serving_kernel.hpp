@@ -22,18 +22,9 @@ inline FastDiv fast_div(int d) {
     return {uint32_t((uint64_t(1) << (31 + l)) / uint32_t(d) + 1), l};
 }
 
-// floor(n / d) for 0 <= n <= 2^30, d >= 1 (larger ones, which only bad offsets make,
-// are cut to that, so that no product overflows and both loops end): the product
-// with the reciprocal is within a few of it (one, below 2^21), in a fifth of the
-// instructions of a division.
-__device__ __forceinline__ int quick_div(int num, int den) {
-    const uint32_t n = min(uint32_t(num), 1u << 30), d = min(uint32_t(den), 1u << 30);
-    uint32_t q = uint32_t(float(n) * __builtin_amdgcn_rcpf(float(d)));
-    while (q * d > n) --q;
-    while ((q + 1) * d <= n) ++q;
-    return uniform(int(q));
-}
-__device__ __forceinline__ int quick_div_up(int n, int d) { return quick_div(n + d - 1, d); }
+// Of values that are the same in every lane.
+__device__ __forceinline__ int udiv(int n, int d) { return uniform(int(uint32_t(n) / uint32_t(d))); }
+__device__ __forceinline__ int udiv_up(int n, int d) { return udiv(n + d - 1, d); }
 
 // How many of the non-decreasing cu[1..n] are <= x, found by the whole wave: 64
 // entries at a time, so two rounds of loads up to 4096 entries.  For x >=
@@ -389,7 +380,7 @@ __device__ __forceinline__ void attend_shared(const B& x, const PrefixPlan& pl, 
     constexpr int BM = WAVES * 32, AHEAD = STAGES - 1;         // prefetch distance in tiles
     constexpr int TILE_BYTES = BN * ROW_BYTES, STAGE_BYTES = 2 * TILE_BYTES;
     constexpr int DMA = BN / 4 / WAVES, SLAB = DMA * 4;        // this wave's key rows of a tile
-    static_assert(DMA == 2 && STAGES == 4, "a wave's slots hold 2 KiB per matrix and stage (O staging, Q)");
+    static_assert(DMA >= 2, "a wave's DMA slots hold 2 KiB per matrix (O staging)");
     static_assert(32 % SLAB == 0, "a wave's rows of a tile lie in one page");
     const Fav4PrefixArgs& a = x.a;
     const Fav4PagedArgs& pg = a.paged;
@@ -400,6 +391,7 @@ __device__ __forceinline__ void attend_shared(const B& x, const PrefixPlan& pl, 
     const uint32_t smem_base = lds_addr(smem);
     const int g0 = range * per, g1 = g0 + per;
 
+    const LdsOffsets off = lds_offsets(lane);
     DmaOffsets<DMA> dofs;
 #pragma unroll
     for (int i = 0; i < DMA; ++i) {
@@ -416,7 +408,7 @@ __device__ __forceinline__ void attend_shared(const B& x, const PrefixPlan& pl, 
         const int rows = tokens * group;
         // The first row tile whose units reach past g0 (bad offsets may overlap the
         // families and overflow the line: every index stays in bounds all the same).
-        for (int rt = at.base < g0 && tiles > 1 ? quick_div(max(0, g0 - at.base), seg_cost) : 0; rt < tiles; ++rt) {
+        for (int rt = at.base < g0 && tiles > 1 ? udiv(max(0, g0 - at.base), seg_cost) : 0; rt < tiles; ++rt) {
             const int first = at.base + (rt + 1) * seg_cost - max(ktiles, 1);     // unit of its first key tile
             if (first >= g1) break;
             if (first + max(ktiles, 1) <= g0) continue;
@@ -431,7 +423,7 @@ __device__ __forceinline__ void attend_shared(const B& x, const PrefixPlan& pl, 
             const int e1 = min(a1, (end - k0 + BN - 1) / BN);          // past what any row sees: nothing to do
 
             RowState st;
-            if (a0 >= e1) clear(st);
+            clear(st);
             if (a0 < e1) {
                 PageWalk walk{nullptr, 0, pg.page_size, pg.num_pages};
                 const int key0 = k0 + a0 * BN + wave * SLAB;           // this wave's first key row
@@ -441,8 +433,13 @@ __device__ __forceinline__ void attend_shared(const B& x, const PrefixPlan& pl, 
                 else
                     walk.start(a.prefix_table + int64_t(at.idx) * a.max_pages_per_prefix, a.max_pages_per_prefix,
                                key0, pl.by_page, lane);
-                // The pages have landed before the first tile is asked for, so that the
-                // loop's only outstanding loads are its tiles.
+                bf16x8 qr[8];
+                load_q(pg, tok, qhead, half, qr);
+                // Q and the pages have landed before the first tile is asked for, so that
+                // the loop's only outstanding loads are its tiles.  (Q through LDS, between
+                // the first two tiles, was 1.7% slower over 32 cases.)
+#pragma unroll
+                for (int c = 0; c < 8; ++c) asm volatile("" ::"v"(qr[c]));
                 asm volatile("" ::"v"(walk.pages));
                 // Tiles past the last one read nothing (the descriptors' bound is 0) and land
                 // in a stage that no later step reads, which keeps the vmcnt count uniform.
@@ -454,33 +451,8 @@ __device__ __forceinline__ void attend_shared(const B& x, const PrefixPlan& pl, 
                     const u32x4 rv = make_desc(static_cast<const char*>(pg.v_cache) + byte, bytes);
                     dma_tile<DMA, TILE_BYTES>(rk, rv, smem_base + stage * STAGE_BYTES, wave, dofs);
                 };
-                // Q goes through LDS, between the first two tiles: this wave's slots of the
-                // last two stages, operand c of lane l at 1 KiB c + 16 bytes l.
-                auto q_slot = [&](int c) {
-                    return uint32_t((2 + (c >> 2)) * STAGE_BYTES + ((c >> 1) & 1) * TILE_BYTES + wave * 2048 + (c & 1) * 1024);
-                };
-                issue(a0, 0);
-                {
-                    const int tok0 = t0 + pl.by_group(q0);
-                    const u32x4 rq = make_desc(static_cast<const char*>(pg.q) +
-                                                   (int64_t(tok0) * pg.heads + kvh * group) * ROW_BYTES, ~0u);
-                    const uint32_t at_q = uint32_t((tok - tok0) * pg.heads + qhead - kvh * group) * ROW_BYTES + half * 16;
 #pragma unroll
-                    for (int c = 0; c < 8; ++c) dma16(rq, smem_base + q_slot(c), at_q + c * 32);
-                }
-                issue(a0 + 1, 1);
-                // Beside the loads: what only the tiles need.  (Opaque, or it moves ahead of them.)
-                int late = lane;
-                asm volatile("" : "+v"(late));
-                const LdsOffsets off = lds_offsets(late);
-                clear(st);
-                wait_vmem_keep<2 * DMA>();
-                bf16x8 qr[8];
-#pragma unroll
-                for (int c = 0; c < 8; ++c) qr[c] = lds_read16(smem + q_slot(c) + lane * 16);
-#pragma unroll
-                for (int c = 0; c < 8; ++c) asm volatile("" ::"v"(qr[c]) : "memory");
-                issue(a0 + 2, 2);
+                for (int i = 0; i < AHEAD; ++i) issue(a0 + i, i);
                 const bool idle = qw >= rows;                          // all of this wave's rows are past the family's
                 int t = a0, stage = 0;
                 auto steps = [&](auto masked_c, int to) {
@@ -512,7 +484,7 @@ __device__ __forceinline__ void attend_shared(const B& x, const PrefixPlan& pl, 
                 store_parts<LSE, TILE_BYTES>(st, pl, prow, live, smem, wave * DMA * 1024, lane);
             }
             if (kvh == 0 && first >= g0 && lane < 32 && lane < live) {
-                const int parts = ktiles > 0 ? quick_div(first + ktiles - 1, per) - range + 1 : 0;
+                const int parts = ktiles > 0 ? udiv(first + ktiles - 1, per) - range + 1 : 0;
                 int2* note = pl.notes + (int64_t(t0) * group + row) * 2;
                 note[OWN] = int2{block * stride + wave * 32 + lane, parts};
                 if (OWN && uniform(f.k0) < 0) note[0] = int2{0, 0};
@@ -547,6 +519,7 @@ __device__ __forceinline__ void attend_wave(const B& x, const PrefixPlan& pl, co
     const uint32_t stage = lds_addr(smem) + slot;
     const int g0 = range * per, g1 = g0 + per;
 
+    const LdsOffsets off = lds_offsets(lane);
     const DmaOffsets<DMA> dofs = dma_offsets<DMA>(0, lane, kv_row_bytes, kv_row_bytes);
     typename L::Place at = line.find(max(0, g0 - origin), lane, head);
     for (at.base += origin; at.idx < line.count && at.base < g1; ++at.idx) {
@@ -555,7 +528,7 @@ __device__ __forceinline__ void attend_wave(const B& x, const PrefixPlan& pl, co
         const int tiles = uniform(line.tiles(f)), ktiles = uniform(line.key_tiles(f)), seg_cost = uniform(line.seg_cost(f));
         const int rows = tokens * group;
         const int kvh = uniform(turn + at.idx - pl.by_kv_heads(turn + at.idx) * pg.kv_heads);
-        for (int rt = at.base < g0 && tiles > 1 ? quick_div(max(0, g0 - at.base), seg_cost) : 0; rt < tiles; ++rt) {
+        for (int rt = at.base < g0 && tiles > 1 ? udiv(max(0, g0 - at.base), seg_cost) : 0; rt < tiles; ++rt) {
             const int first = at.base + (rt + 1) * seg_cost - max(ktiles, 1);
             if (first >= g1) break;
             if (first + max(ktiles, 1) <= g0) continue;
@@ -566,7 +539,7 @@ __device__ __forceinline__ void attend_wave(const B& x, const PrefixPlan& pl, co
             const int lim = see.lim, nfull = max(0, see.plain - k0) / BN, e1 = min(a1, (see.end - k0 + BN - 1) / BN);
 
             RowState st;
-            if (a0 >= e1) clear(st);
+            clear(st);
             if (a0 < e1) {
                 PageWalk walk{nullptr, 0, pg.page_size, pg.num_pages};
                 if constexpr (OWN)
@@ -575,6 +548,10 @@ __device__ __forceinline__ void attend_wave(const B& x, const PrefixPlan& pl, co
                 else
                     walk.start(x.a.prefix_table + int64_t(at.idx) * x.a.max_pages_per_prefix, x.a.max_pages_per_prefix,
                                a0 * BN, pl.by_page, lane);
+                bf16x8 qr[8];
+                load_q(pg, tok, qhead, half, qr);
+#pragma unroll
+                for (int c = 0; c < 8; ++c) asm volatile("" ::"v"(qr[c]));
                 auto issue = [&](int t) {
                     const int left = min(k1 - (k0 + t * BN), BN);
                     const uint32_t bytes = uint32_t(left - 1) * kv_row_bytes + ROW_BYTES;
@@ -584,16 +561,6 @@ __device__ __forceinline__ void attend_wave(const B& x, const PrefixPlan& pl, co
                     dma_tile<DMA, TILE_BYTES, true>(rk, rv, stage, 0, dofs);
                 };
                 issue(a0);
-                // Beside the tile's load: Q, and what only the tiles need (opaque, or it
-                // moves ahead of the load).
-                bf16x8 qr[8];
-                load_q(pg, tok, qhead, half, qr);
-                int late = lane;
-                asm volatile("" : "+v"(late));
-                const LdsOffsets off = lds_offsets(late);
-                clear(st);
-#pragma unroll
-                for (int c = 0; c < 8; ++c) asm volatile("" ::"v"(qr[c]));
                 const unsigned char* ks = smem + slot;
                 auto step = [&](auto masked_c, int t) {
                     wait_vmem();
@@ -606,13 +573,14 @@ __device__ __forceinline__ void attend_wave(const B& x, const PrefixPlan& pl, co
                 int t = a0;
                 for (; t < min(e1, nfull); ++t) step(std::integral_constant<bool, false>{}, t);
                 for (; t < e1; ++t) step(std::integral_constant<bool, true>{}, t);
+                wait_vmem();                                           // (the last step left none in flight)
             }
             const int block = at.seg + rt + range, live = min(min(32, stride), rows - q0);
             if (ktiles > 0 && uint32_t(block) < uint32_t(blocks))
                 store_parts<LSE, TILE_BYTES>(st, pl, part0 + (int64_t(kvh) * blocks + block) * stride, live, smem, slot,
                                              lane);
             if (kvh == 0 && first >= g0 && lane < 32 && lane < live) {
-                const int parts = ktiles > 0 ? quick_div(first + ktiles - 1, per) - range + 1 : 0;
+                const int parts = ktiles > 0 ? udiv(first + ktiles - 1, per) - range + 1 : 0;
                 int2* note = pl.notes + (int64_t(t0) * group + row) * 2;
                 note[OWN] = int2{block * stride + lane, parts};
                 if (OWN && uniform(f.k0) < 0) note[0] = int2{0, 0};
@@ -664,7 +632,7 @@ void prefix_kernel(Fav4PrefixArgs a, PrefixPlan pl) {
             if (i < pg.batch) {
                 const int shared = x.find_shared(i), sk = lds.own[i].w, n = lds.own[i + 1].x - lds.own[i].x;
                 if (shared > 0) lds.own[i].z = min(shared, sk);
-                hidden |= n > 0 && sk - (pl.br ? n : 1) < shared - 1;
+                hidden |= shared > 0 && n > 0 && sk - (pl.br ? n : 1) < shared - 1;
             }
             if (i < a.num_prefixes) lds.prefix[i] = __builtin_bit_cast(int4, x.make_prefix(i));
         }
@@ -681,7 +649,7 @@ void prefix_kernel(Fav4PrefixArgs a, PrefixPlan pl) {
     const int64_t own_part0 = int64_t(pg.kv_heads) * pl.prefix_blocks * BM;
     if constexpr (CUT == FEWEST) {
         const int ranges = pl.ranges * WAVES, range = w * WAVES + wave, total = prefix_units + own_units;
-        const int per = max(quick_div_up(total, ranges), MIN_OWN_TILES);
+        const int per = max(udiv_up(total, ranges), MIN_OWN_TILES);
         const uint32_t slot = wave * 64 * ROW_BYTES;
         if (range * per < prefix_units)
             attend_wave<LSE, false>(x, pl, prefixes, prefix_head, 0, range, per, kvh, smem, slot, 0, pl.prefix_blocks, BM);
@@ -689,37 +657,37 @@ void prefix_kernel(Fav4PrefixArgs a, PrefixPlan pl) {
             attend_wave<LSE, true>(x, pl, own, own_head, prefix_units, range, per, kvh, smem, slot, own_part0,
                                    pl.own_blocks, pl.own_rows);
         return;
-    } else {
+    }
     // The workgroups of either line, by what its tiles cost; the two kinds alternate,
-    // so that a CU has both.
+    // so that the XCDs have both.
     const float cost = prefix_units * (OWN_WAVES ? WAVES == 4 ? PREFIX_COST_4 : PREFIX_COST_8 : 1.f);
     int pw = min(max(int(cost / (cost + own_units) * pl.ranges + 0.5f), 1), pl.ranges - 1);
     if (prefix_units <= 0) pw = 0;
-    int per = max(quick_div_up(prefix_units, max(pw, 1)), MIN_PREFIX_TILES);
-    int aligned = 0;
-    if (a.num_prefixes == 1 && pw >= uniform(prefixes.tiles(prefixes.family(0)))) {
-        // One prefix, a range or more for each row tile: they are cut at the same keys (the lead units take up the
-        // rest), so that they read them at the same time and share them in L2.
-        const Family f = prefixes.family(0);
-        const int cost = uniform(prefixes.seg_cost(f)), cuts = quick_div(pw, uniform(max(prefixes.tiles(f), 1)));
-        per = max(quick_div_up(cost, max(cuts, 1)), MIN_PREFIX_TILES);
-        aligned = quick_div_up(cost, per) * per;
-    }
     // w pw / ranges, exact: both factors are at most 1024.
     const float step = 1.f / pl.ranges;
     const int before = int((w * pw + 0.5f) * step);
     if (int(((w + 1) * pw + 0.5f) * step) > before) {
-        attend_shared<LSE, WAVES, false, BN, STAGES>(x, pl, prefixes, prefix_head, before, per, aligned, kvh,
-                                                     smem);
+        int per = max(udiv_up(prefix_units, pw), MIN_PREFIX_TILES), aligned = 0;
+        const Family f = prefixes.family(0);
+        const int tiles = uniform(prefixes.tiles(f));
+        if (a.num_prefixes == 1 && tiles <= pw) {
+            // One prefix, a range or more for each row tile: they are cut at the same keys
+            // (the lead units take up the rest), so that they read them at the same time
+            // and share them in L2 (64 sequences behind 8192 keys H32 KVH8 on 128-row tiles
+            // 40.5 -> 39.0 us).
+            const int cost = uniform(prefixes.seg_cost(f));
+            per = max(udiv_up(cost, udiv(pw, tiles)), MIN_PREFIX_TILES);
+            aligned = udiv_up(cost, per) * per;
+        }
+        attend_shared<LSE, WAVES, false, BN, STAGES>(x, pl, prefixes, prefix_head, before, per, aligned, kvh, smem);
     } else {
         const int ranges = (pl.ranges - pw) * OWN_RANGES, range = w - before;
-        per = max(quick_div_up(own_units, ranges), MIN_OWN_TILES);
+        const int per = max(udiv_up(own_units, ranges), MIN_OWN_TILES);
         if constexpr (OWN_WAVES)
             attend_wave<LSE, true>(x, pl, own, own_head, 0, range * WAVES + wave, per, kvh, smem, wave * 64 * ROW_BYTES,
                                    own_part0, pl.own_blocks, pl.own_rows);
         else
             attend_shared<LSE, WAVES, true, BN, STAGES>(x, pl, own, own_head, range, per, 0, kvh, smem);
-    }
     }
 }
 
