@@ -82,7 +82,8 @@ bool prefix_shape_ok(const Fav4PrefixArgs* args, int causal) {
 
 struct PrefixSizes {
     fav4::PrefixPlan plan;
-    int64_t part_rows, bytes, prefix_segs, prefix_ranges, prefix_tiles;
+    int64_t part_rows, bytes;
+    int64_t parts;             // that a row can have of its prefix and of its own, on average
     int waves, prefix_rows;    // of a workgroup, of a prefix block
     fav4::Cut cut;
     bool ok;
@@ -108,19 +109,20 @@ PrefixSizes prefix_sizes(const Fav4PrefixArgs& args, int causal) {
     };
     const int own_bm = own_waves ? 32 : BM;
     const int64_t own_rows = std::min<int64_t>(own_bm, seq_rows);
-    const int64_t prefix_segs = s.prefix_segs = tiles(args.num_prefixes, rows, BM);
+    const int64_t prefix_segs = tiles(args.num_prefixes, rows, BM);
     const int64_t own_segs = tiles(a.batch, seq_rows, own_bm);
     const int64_t prefix_keys = std::min<int64_t>(int64_t(args.max_pages_per_prefix) * a.page_size, a.max_seqlen_k);
-    s.prefix_tiles = prefix_keys / 32;
     s.plan.most_prefix_keys = int(prefix_keys);
     const int64_t lead = 1 + fav4::SEG_TILES;
     const int64_t units = prefix_segs * (prefix_keys / 32 + lead) + own_segs * (a.max_seqlen_k / 32 + lead);
     // No more waves than ranges (starting the waves of a full GPU takes 2 us).
     if (s.cut == fav4::FEWEST)
         s.plan.ranges = int(std::min<int64_t>(s.plan.ranges, std::max<int64_t>(2, units / (fav4::MIN_OWN_TILES * WAVES) + 1)));
-    s.prefix_ranges = s.plan.ranges * (s.cut == fav4::FEWEST ? WAVES : 1);
-    const int64_t prefix_blocks = prefix_segs + s.prefix_ranges;
-    const int64_t own_blocks = own_segs + s.plan.ranges * (own_waves ? WAVES : 1);
+    const int64_t prefix_ranges = s.plan.ranges * (s.cut == fav4::FEWEST ? WAVES : 1);
+    const int64_t own_ranges = s.plan.ranges * (own_waves ? WAVES : 1);
+    const int64_t prefix_blocks = prefix_segs + prefix_ranges, own_blocks = own_segs + own_ranges;
+    s.parts = std::min(prefix_ranges / std::max<int64_t>(1, prefix_segs), prefix_keys / 32 / fav4::MIN_PREFIX_TILES) +
+              std::min(own_ranges / std::max<int64_t>(1, own_segs), std::max<int64_t>(0, a.max_seqlen_k - prefix_keys) / 32 / fav4::MIN_OWN_TILES);
     s.part_rows = (a.kv_heads * (prefix_blocks * BM + own_blocks * own_rows) + 1) & ~int64_t(1);   // notes 16-byte aligned
     s.ok = units < (1 << 30) && prefix_blocks * BM <= INT_MAX && own_blocks * own_rows <= INT_MAX;
     s.plan.prefix_blocks = int(prefix_blocks);
@@ -213,11 +215,13 @@ extern "C" __attribute__((visibility("default"))) int fav4_bshd_forward_prefix_p
     launch_prefix(*args, s, stream);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    // Teams per merged row, by the most parts that a prefix's row tile can have on
-    // average, as long as the rows leave the GPU some for it.
+    // Teams per merged row: many where a row can have many parts (16 sequences of
+    // 2000..6800 keys H16 KVH16: 28.0 us on 4, 25.3 on 16), one where it has few (106
+    // sequences H32 KVH32 35.4 on 4, 33.3 on one; 64 behind 8192 keys 36.5 and 38.5).
     const int64_t rows = int64_t(a.total_q) * a.heads;
-    const int64_t parts = std::min(s.prefix_ranges / std::max<int64_t>(1, s.prefix_segs), s.prefix_tiles / 2);
-    const int per = parts > 64 && rows <= 1024 ? 16 : rows <= 4096 ? 4 : 1;
+    const bool many = (s.parts > 44 && rows <= 256) || (s.parts > 96 && rows <= 1024);
+    const bool few = rows > 4096 || (s.cut != fav4::FEWEST && s.parts <= 18 && rows > 1024);
+    const int per = many ? 16 : few ? 1 : 4;
     const unsigned blocks = unsigned(std::min((rows * per + 15) / 16, MAX_GRID));
     auto merge = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, dim3(blocks), dim3(256), 0, stream, *args, s.plan, s.prefix_rows);
