@@ -529,59 +529,47 @@ class Runner:
         return raw(device) if raw is not None else torch.cuda.current_stream().cuda_stream
 
     @staticmethod
-    def _paged_batch(torch, device, cu_q, seqlens_k, block_table):
-        """Checks of a paged batch's index tensors; (batch, max_pages_per_seq)."""
-        i32 = torch.int32
-        for x in (cu_q, seqlens_k, block_table):
-            assert x.dtype is i32 and x.is_contiguous() and x.get_device() == device, "int32, contiguous, on one device"
-        batch, pages = block_table.shape
-        assert cu_q.shape == (batch + 1,) and seqlens_k.shape == (batch,)
-        return batch, pages
-
-    @staticmethod
-    def _caches(torch, device, k_cache, v_cache):
-        """Checks of the paged caches; their shape."""
-        shape = k_cache.shape
-        assert len(shape) == 4 and shape[3] == D and v_cache.shape == shape
-        assert k_cache.dtype is torch.bfloat16 and v_cache.dtype is torch.bfloat16
+    def _append_block(torch, q, k, v, q_out, k_cache, v_cache, cu_q, seqlens_k, block_table, cos, sin, interleaved,
+                      positions) -> bytes:
+        bf16, i32, dev = torch.bfloat16, torch.int32, k.get_device()
+        num_pages, page_size, kv_heads, d = caches = k_cache.shape
+        assert d == D and v_cache.shape == caches and k_cache.dtype is bf16 and v_cache.dtype is bf16
         assert k_cache.is_contiguous() and v_cache.is_contiguous()
-        assert k_cache.get_device() == device and v_cache.get_device() == device
-        return shape
-
-    @staticmethod
-    def _rows(torch, device, x, tokens):
-        """Checks of [tokens, heads, 128] BF16 rows with any stride between tokens; (heads, stride)."""
-        n, heads, d = x.shape
-        s0, s1, s2 = x.stride()
-        assert n == tokens and d == D and x.dtype is torch.bfloat16 and x.get_device() == device
-        assert s2 == 1 and (s1 == D or heads == 1)
-        return heads, s0 if n > 1 else heads * D          # a single token has no stride that counts
-
-    def _append_block(self, torch, q, k, v, q_out, k_cache, v_cache, cu_q, seqlens_k, block_table, cos, sin,
-                      interleaved, positions) -> bytes:
-        device = k.get_device()
-        num_pages, page_size, kv_heads, _ = self._caches(torch, device, k_cache, v_cache)
-        batch, pages = self._paged_batch(torch, device, cu_q, seqlens_k, block_table)
+        batch, pages = block_table.shape
+        assert cu_q.dtype is i32 and seqlens_k.dtype is i32 and block_table.dtype is i32
+        assert cu_q.shape == (batch + 1,) and seqlens_k.shape == (batch,)
+        assert cu_q.is_contiguous() and seqlens_k.is_contiguous() and block_table.is_contiguous()
+        assert dev == k_cache.get_device() == v_cache.get_device() == v.get_device() == cu_q.get_device() \
+            == seqlens_k.get_device() == block_table.get_device(), "all tensors on one device"
+        # Rows: any stride between tokens (a single token has none that counts), heads and dims contiguous.
         tokens = k.shape[0]
-        k_heads, k_stride = self._rows(torch, device, k, tokens)
-        v_heads, v_stride = self._rows(torch, device, v, tokens)
-        assert k_heads == v_heads == kv_heads and (q is None) == (q_out is None)
+        assert k.shape == v.shape == (tokens, kv_heads, D) and k.dtype is bf16 and v.dtype is bf16
+        k_stride, k1, k2 = k.stride()
+        v_stride, v1, v2 = v.stride()
+        assert k2 == v2 == 1 and (kv_heads == 1 or k1 == v1 == D)
         heads, q_stride, o_stride, q_ptr, o_ptr = 1, 0, 0, 0, 0
+        assert (q is None) == (q_out is None)
         if q is not None:
-            heads, q_stride = self._rows(torch, device, q, tokens)
-            o_heads, o_stride = self._rows(torch, device, q_out, tokens)
-            assert o_heads == heads
+            heads = q.shape[1]
+            assert q.shape == q_out.shape == (tokens, heads, D) and q.dtype is bf16 and q_out.dtype is bf16
+            assert q.get_device() == q_out.get_device() == dev, "all tensors on one device"
+            q_stride, q1, q2 = q.stride()
+            o_stride, o1, o2 = q_out.stride()
+            assert q2 == o2 == 1 and (heads == 1 or q1 == o1 == D)
             q_ptr, o_ptr = q.data_ptr(), q_out.data_ptr()
+        if tokens == 1:
+            k_stride = v_stride = kv_heads * D
+            q_stride = o_stride = heads * D
         rows = half = c_ptr = s_ptr = p_ptr = 0
         assert (cos is None) == (sin is None)
         if cos is not None:
             rows, half = cos.shape
-            assert sin.shape == (rows, half) and cos.dtype is sin.dtype is torch.float32
-            assert cos.is_contiguous() and sin.is_contiguous() and cos.get_device() == sin.get_device() == device
+            assert sin.shape == cos.shape and cos.dtype is sin.dtype is torch.float32
+            assert cos.is_contiguous() and sin.is_contiguous() and cos.get_device() == sin.get_device() == dev
             c_ptr, s_ptr = cos.data_ptr(), sin.data_ptr()
         if positions is not None:
-            assert positions.dtype is torch.int32 and positions.shape == (tokens,) and positions.is_contiguous()
-            assert positions.get_device() == device
+            assert positions.dtype is i32 and positions.shape == (tokens,) and positions.is_contiguous()
+            assert positions.get_device() == dev, "all tensors on one device"
             p_ptr = positions.data_ptr()
         return _APPEND.pack(q_ptr, k.data_ptr(), v.data_ptr(), o_ptr, k_cache.data_ptr(), v_cache.data_ptr(), c_ptr,
                             s_ptr, cu_q.data_ptr(), seqlens_k.data_ptr(), block_table.data_ptr(), p_ptr, q_stride,
@@ -602,23 +590,28 @@ class Runner:
         if status:
             raise RuntimeError(f"append paged: HIP status {status}")
 
-    def _prefix_block(self, torch, q, k_cache, v_cache, o, lse, cu_q, seqlens_k, block_table, prefix_table,
-                      prefix_lens, cu_prefix_seqs, max_q, max_k, total_k, scale) -> bytes:
-        device = q.get_device()
-        num_pages, page_size, kv_heads, _ = self._caches(torch, device, k_cache, v_cache)
-        batch, pages = self._paged_batch(torch, device, cu_q, seqlens_k, block_table)
+    @staticmethod
+    def _prefix_block(torch, q, k_cache, v_cache, o, lse, cu_q, seqlens_k, block_table, prefix_table, prefix_lens,
+                      cu_prefix_seqs, max_q, max_k, total_k, scale) -> bytes:
+        bf16, i32, dev = torch.bfloat16, torch.int32, q.get_device()
+        num_pages, page_size, kv_heads, d = caches = k_cache.shape
+        assert d == D and v_cache.shape == caches and k_cache.dtype is bf16 and v_cache.dtype is bf16
+        assert k_cache.is_contiguous() and v_cache.is_contiguous()
+        batch, pages = block_table.shape
+        prefixes, prefix_pages = prefix_table.shape
+        assert cu_q.shape == (batch + 1,) and seqlens_k.shape == (batch,)
+        assert prefix_lens.shape == (prefixes,) and cu_prefix_seqs.shape == (prefixes + 1,)
+        for x in (cu_q, seqlens_k, block_table, prefix_table, prefix_lens, cu_prefix_seqs):
+            assert x.dtype is i32 and x.is_contiguous() and x.get_device() == dev, "int32, contiguous, on one device"
         tokens, heads, d = q.shape
-        assert d == D and o.shape == q.shape and q.dtype is o.dtype is torch.bfloat16
-        assert q.is_contiguous() and o.is_contiguous() and o.get_device() == device
+        assert d == D and o.shape == q.shape and q.dtype is bf16 and o.dtype is bf16
+        assert q.is_contiguous() and o.is_contiguous()
+        assert dev == k_cache.get_device() == v_cache.get_device() == o.get_device(), "all tensors on one device"
         lse_ptr = 0
         if lse is not None:
             assert lse.shape == (heads, tokens) and lse.is_contiguous() and lse.dtype is torch.float32
-            assert lse.get_device() == device
+            assert lse.get_device() == dev, "all tensors on one device"
             lse_ptr = lse.data_ptr()
-        prefixes, prefix_pages = prefix_table.shape
-        assert prefix_lens.shape == (prefixes,) and cu_prefix_seqs.shape == (prefixes + 1,)
-        for x in (prefix_table, prefix_lens, cu_prefix_seqs):
-            assert x.dtype is torch.int32 and x.is_contiguous() and x.get_device() == device
         return _PREFIX.pack(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), o.data_ptr(), lse_ptr,
                             cu_q.data_ptr(), seqlens_k.data_ptr(), block_table.data_ptr(), batch, heads, kv_heads,
                             int(max_q), int(max_k), tokens, 0 if total_k is None else int(total_k), num_pages,

@@ -80,6 +80,37 @@ def test_prefix_many_sequences_and_prefixes(gpu_runner):
     x.check(o, l, 0)
 
 
+# (heads, kv_heads, prefixes, sequences of each, most queries of a sequence, causal)
+LARGE_BATCHES = {
+    "rows_of_many_sequences": (8, 1, 3, 230, 1, 0),
+    "few_rows_a_prefix": (4, 2, 290, 2, 1, 0),
+    "many_prefixes": (64, 2, 300, 2, 1, 0),
+    "many_prefixes_and_sequences": (16, 1, 300, 3, 2, 2),
+    "many_rows_a_sequence": (32, 2, 5, 104, 9, 2),
+    "many_rows_a_sequence_and_prefixes": (16, 1, 280, 2, 6, 2),
+}
+
+
+@pytest.mark.parametrize("name", LARGE_BATCHES)
+def test_prefix_large_batches(gpu_runner, name):
+    """More than 512 sequences or 256 prefixes: each workgroup reads their lengths from global memory."""
+    heads, kvh, n, members, most_q, causal = LARGE_BATCHES[name]
+    rng = np.random.default_rng(31)
+    prefixes = []
+    for i in range(n):
+        p = 32 * int(rng.integers(0, 8))
+        prefixes.append((p, [(int(rng.integers(min(most_q, j), most_q + 1)), p + int(rng.integers(0, 120)))
+                             for j in range(members)]))
+    print("prefix large", name, flush=True)
+    x = Batch(heads, kvh, 32, prefixes, [(1, 40)] * 3)
+    assert len(x.lens) > 512 or n > 256
+    o, l = x.outputs(True)
+    x.attend(gpu_runner, o, l, causal)
+    torch.cuda.synchronize()
+    x.check(o, l, causal)
+    assert torch.isnan(x.o_all[o.shape[0]:]).all()
+
+
 def test_prefix_long(gpu_runner):
     """Keys over many ranges: a prefix of 50000 keys, and one sequence's own 20000 behind a short prefix."""
     for prefixes in ([(49984, [(1, 50000), (1, 51000), (2, 50001)])], [(64, [(1, 20000), (1, 70)])]):
