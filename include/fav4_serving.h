@@ -69,6 +69,9 @@ extern "C" int fav4_bshd_append_paged(const Fav4AppendArgs* args, hipStream_t st
 //    attended over their own pages alone.  A sequence with fewer keys than its
 //    prefix sees those alone; one without keys gets O = 0 and LSE = -inf, one
 //    without queries writes nothing.
+//  * K and V of every key in [0, seqlens_k) and of every shared key must be
+//    finite, also for rows that do not see it: hidden keys have weight 0, and 0
+//    times a NaN is one.  Slots behind seqlens_k may hold anything.
 //  * Results meet the tolerances of the paged call (not bitwise its results:
 //    the parts are cut elsewhere), and are the same from call to call.
 struct Fav4PrefixArgs {
@@ -80,12 +83,13 @@ struct Fav4PrefixArgs {
 };
 // Checks: those of Fav4PagedArgs with causal 0 or 2, page_size a multiple of 32,
 // max_seqlen_k <= max_pages_per_seq * page_size, num_prefixes and
-// max_pages_per_prefix >= 1, heads <= 2^15, total_q * heads < 2^31, and a plan of fewer than
-// 2^30 key tiles.  The workspace is caller-owned device memory, 256-byte
-// aligned, of at least fav4_bshd_prefix_paged_workspace_size() bytes and not
-// shared with a concurrent call (two captured graphs that may run at once
-// included); its contents do not matter.  The size query reads only the sizes
-// (pointers may be NULL) and returns -1 for rejected arguments.
+// max_pages_per_prefix >= 1, heads <= 2^15, total_q * heads < 2^31, and a plan
+// of fewer than 2^30 key tiles.  The workspace is caller-owned device memory,
+// 256-byte aligned, of at least fav4_bshd_prefix_paged_workspace_size() bytes
+// and not shared with a concurrent call (two captured graphs that may run at
+// once included); its contents do not matter.  The size query reads only the
+// sizes (pointers may be NULL), returns -1 for rejected arguments, and never
+// less for a larger batch, more queries, prefixes or pages.
 extern "C" int fav4_bshd_forward_prefix_paged(const Fav4PrefixArgs* args, int causal, void* workspace,
                                               size_t workspace_bytes, hipStream_t stream);
 extern "C" long long fav4_bshd_prefix_paged_workspace_size(const Fav4PrefixArgs* args, int causal);
