@@ -59,8 +59,14 @@ bool append_ok(const Fav4AppendArgs* a) {
 
 // ---- attention behind shared prefixes ------------------------------------------
 constexpr int BOTTOM_RIGHT = 2;
-constexpr int PREFIX_WAVE_ROWS = 32;  // up to this many rows of a prefix (the mean): its keys are, too
-constexpr int WAVE_ROWS = 64;      // up to this many rows of a sequence: its own keys are read by single waves
+// Up to this many rows of a prefix (the mean) its keys are split over a workgroup's
+// waves (H32 KVH8, 16 prefixes of 4096 keys: at 24..32 rows 73 us split, 82 shared; at
+// 48 rows 122 and 84).
+constexpr int SPLIT_ROWS = 32;
+// Up to this many rows of a sequence its own keys are read by single waves (32 rows,
+// 64 sequences behind 4096 H32 KVH8: 60 us by waves, 70 by workgroups; 48 rows, 48
+// sequences of 1000..4000 own keys: 203, two row tiles each, and 151).
+constexpr int WAVE_ROWS = 32;
 
 constexpr int MAX_HEADS = 1 << 15;    // the Q rows of a 256-row tile lie within 4 GiB
 
@@ -84,7 +90,7 @@ struct PrefixSizes {
     fav4::PrefixPlan plan;
     int64_t part_rows, bytes;
     int64_t parts;             // that a row can have of its prefix and of its own, on average
-    int waves, prefix_rows;    // of a workgroup, of a prefix block
+    int prefix_rows;           // of a prefix block
     fav4::Cut cut;
     bool ok;
 };
@@ -95,14 +101,12 @@ PrefixSizes prefix_sizes(const Fav4PrefixArgs& args, int causal) {
     PrefixSizes s{};
     s.plan.br = causal == BOTTOM_RIGHT;
     s.cut = a.max_seqlen_q * group > WAVE_ROWS                     ? fav4::MANY
-            : rows <= int64_t(args.num_prefixes) * PREFIX_WAVE_ROWS ? fav4::FEWEST
+            : rows <= int64_t(args.num_prefixes) * SPLIT_ROWS ? fav4::FEWEST
                                                                     : fav4::FEW;
-    // 256-row tiles where the prefixes or the sequences have that many rows, else 128.
-    s.waves = s.cut == fav4::MANY || (s.cut == fav4::FEW && rows > int64_t(args.num_prefixes) * 128) ? 8 : 4;
-    const int WAVES = s.waves, BM = s.prefix_rows = s.cut == fav4::FEWEST ? 32 : WAVES * 32;
+    const int WAVES = 8, BM = s.prefix_rows = s.cut == fav4::FEWEST ? 32 : WAVES * 32;
     const bool own_waves = s.cut != fav4::MANY;
     // As many workgroups as are resident at once; at least one for each line.
-    s.plan.ranges = std::min(1024, std::max(2, (WAVES == 8 ? 1 : 2) * device_cus() / a.kv_heads));
+    s.plan.ranges = std::min(1024, std::max(2, device_cus() / a.kv_heads));
     // Row tiles that the rows of n families can have.
     auto tiles = [&](int64_t n, int64_t most, int bm) {
         return std::min(n * ((most + bm - 1) / bm), (rows + n * (bm - 1)) / bm);
@@ -115,14 +119,13 @@ PrefixSizes prefix_sizes(const Fav4PrefixArgs& args, int causal) {
     s.plan.most_prefix_keys = int(prefix_keys);
     const int64_t lead = 1 + fav4::SEG_TILES;
     const int64_t units = prefix_segs * (prefix_keys / 32 + lead) + own_segs * (a.max_seqlen_k / 32 + lead);
-    // No more waves than ranges (starting the waves of a full GPU takes 2 us).
-    if (s.cut == fav4::FEWEST)
-        s.plan.ranges = int(std::min<int64_t>(s.plan.ranges, std::max<int64_t>(2, units / (fav4::MIN_OWN_TILES * WAVES) + 1)));
-    const int64_t prefix_ranges = s.plan.ranges * (s.cut == fav4::FEWEST ? WAVES : 1);
+    const int64_t prefix_ranges = s.plan.ranges;
     const int64_t own_ranges = s.plan.ranges * (own_waves ? WAVES : 1);
     const int64_t prefix_blocks = prefix_segs + prefix_ranges, own_blocks = own_segs + own_ranges;
-    s.parts = std::min(prefix_ranges / std::max<int64_t>(1, prefix_segs), prefix_keys / 32 / fav4::MIN_PREFIX_TILES) +
-              std::min(own_ranges / std::max<int64_t>(1, own_segs), std::max<int64_t>(0, a.max_seqlen_k - prefix_keys) / 32 / fav4::MIN_OWN_TILES);
+    s.parts = std::min(prefix_ranges / std::max<int64_t>(1, prefix_segs),
+                       prefix_keys / (s.cut == fav4::FEWEST ? 32 * fav4::MIN_SPLIT_TILES : 64 * fav4::MIN_PREFIX_TILES)) +
+              std::min(own_ranges / std::max<int64_t>(1, own_segs), std::max<int64_t>(0, a.max_seqlen_k - prefix_keys) /
+                                                                        (own_waves ? 32 * fav4::MIN_OWN_TILES : 64 * fav4::MIN_PREFIX_TILES));
     s.part_rows = (a.kv_heads * (prefix_blocks * BM + own_blocks * own_rows) + 1) & ~int64_t(1);   // notes 16-byte aligned
     s.ok = units < (1 << 30) && prefix_blocks * BM <= INT_MAX && own_blocks * own_rows <= INT_MAX;
     s.plan.prefix_blocks = int(prefix_blocks);
@@ -148,27 +151,20 @@ PrefixSizes prefix_sizes(const Fav4PrefixArgs& args, int causal) {
 
 void launch_prefix(const Fav4PrefixArgs& args, const PrefixSizes& s, hipStream_t stream) {
     const dim3 grid(unsigned(args.paged.kv_heads) * unsigned(s.plan.ranges));
-    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(s.waves * 64), 0, stream, args, s.plan); };
-    auto with_lse = [&](auto waves, auto cut, auto cached) {
-        constexpr int W = decltype(waves)::value;
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(512), 0, stream, args, s.plan); };
+    auto with_lse = [&](auto cut, auto cached) {
         constexpr fav4::Cut CUT = decltype(cut)::value;
         constexpr bool C = decltype(cached)::value;
-        if (args.paged.lse) go(fav4::prefix_kernel<true, W, CUT, C>);
-        else go(fav4::prefix_kernel<false, W, CUT, C>);
+        if (args.paged.lse) go(fav4::prefix_kernel<true, CUT, C>);
+        else go(fav4::prefix_kernel<false, CUT, C>);
     };
-    auto with_waves = [&](auto cached) {
-        using Four = std::integral_constant<int, 4>;
-        using Eight = std::integral_constant<int, 8>;
-        using Many = std::integral_constant<fav4::Cut, fav4::MANY>;
-        using Few = std::integral_constant<fav4::Cut, fav4::FEW>;
-        using Fewest = std::integral_constant<fav4::Cut, fav4::FEWEST>;
-        if (s.cut == fav4::MANY) with_lse(Eight{}, Many{}, cached);
-        else if (s.cut == fav4::FEWEST) with_lse(Four{}, Fewest{}, cached);
-        else if (s.waves == 8) with_lse(Eight{}, Few{}, cached);
-        else with_lse(Four{}, Few{}, cached);
+    auto with_cut = [&](auto cached) {
+        if (s.cut == fav4::MANY) with_lse(std::integral_constant<fav4::Cut, fav4::MANY>{}, cached);
+        else if (s.cut == fav4::FEW) with_lse(std::integral_constant<fav4::Cut, fav4::FEW>{}, cached);
+        else with_lse(std::integral_constant<fav4::Cut, fav4::FEWEST>{}, cached);
     };
-    if (args.paged.batch <= fav4::PLAN_SEQS && args.num_prefixes <= fav4::PLAN_PREFIXES) with_waves(std::true_type{});
-    else with_waves(std::false_type{});
+    if (args.paged.batch <= fav4::PLAN_SEQS && args.num_prefixes <= fav4::PLAN_PREFIXES) with_cut(std::true_type{});
+    else with_cut(std::false_type{});
 }
 
 }  // namespace
@@ -215,12 +211,13 @@ extern "C" __attribute__((visibility("default"))) int fav4_bshd_forward_prefix_p
     launch_prefix(*args, s, stream);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    // Teams per merged row: many where a row can have many parts (16 sequences of
-    // 2000..6800 keys H16 KVH16: 28.0 us on 4, 25.3 on 16), one where it has few (106
-    // sequences H32 KVH32 35.4 on 4, 33.3 on one; 64 behind 8192 keys 36.5 and 38.5).
+    // Teams per merged row: many where a row can have many parts (24 sequences behind
+    // 16384 keys H8 KVH1, 132 parts: 24.6 us on 4, 21.6 on 16), one where it has few or
+    // the rows alone fill the GPU (384 sequences behind 1024 keys H32 KVH8: 66.5 on 4,
+    // 57.3 on one; 64 behind 8192, 36 parts: 35.8 and 37.7).
     const int64_t rows = int64_t(a.total_q) * a.heads;
     const bool many = (s.parts > 44 && rows <= 256) || (s.parts > 96 && rows <= 1024);
-    const bool few = rows > 4096 || (s.cut != fav4::FEWEST && s.parts <= 18 && rows > 1024);
+    const bool few = rows > 4096 || s.parts <= 5 || (s.parts <= 18 && rows > 2048);
     const int per = many ? 16 : few ? 1 : 4;
     const unsigned blocks = unsigned(std::min((rows * per + 15) / 16, MAX_GRID));
     auto merge = [&](auto kernel) {

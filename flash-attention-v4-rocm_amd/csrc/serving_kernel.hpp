@@ -135,10 +135,11 @@ __global__ __launch_bounds__(256) void append_kernel(Fav4AppendArgs a, int units
 // the sequences' own on another, and each line is cut into ranges of one
 // length, whatever segments they cross.
 //
-// A prefix range is a workgroup's: its WAVES waves take 32 rows each of the
-// row tile and share the K/V tiles.  An own range is a workgroup's too
-// (OWN_WAVES false: many rows per sequence), or a single wave's (up to 64 rows
-// of a sequence): the wave streams 32-key tiles through 16 KiB of LDS of its
+// A prefix range is a workgroup's: its eight waves take 32 rows each of the row
+// tile and share the K/V tiles (attend_shared), or, where the prefixes have few
+// rows, all take the same 32 rows, each every eighth key tile (attend_split).  An
+// own range is a workgroup's too, or a single wave's where the sequences have few
+// rows (attend_wave): the wave streams 32-key tiles through 16 KiB of LDS of its
 // own, with no barrier, and the eight such waves of a CU hide each other's
 // latency.
 //
@@ -162,11 +163,13 @@ struct PrefixPlan {
     int br;                           // bottom-right causal
 };
 
-constexpr int SEG_TILES = 4, OWN_SEG_TILES = 2;        // OWN_SEG_TILES: of a single wave's segment
-constexpr int MIN_PREFIX_TILES = 2, MIN_OWN_TILES = 2;  // shortest ranges
+constexpr int SEG_TILES = 4, OWN_SEG_TILES = 2, SPLIT_SEG_TILES = 8;
+constexpr int MIN_PREFIX_TILES = 2, MIN_OWN_TILES = 1, MIN_SPLIT_TILES = 4;  // shortest ranges
 // What a prefix's key tile costs, in own key tiles of a wave (its share of the
-// workgroups follows): 32 keys by four waves, 64 keys by eight.
-constexpr float PREFIX_COST_4 = 1.5f, PREFIX_COST_8 = 4.f;
+// workgroups follows): 64 keys against 256 rows, and 32 keys against 32 rows split
+// over the waves (at 2: 32.4 -> 33.6 us over 53 calls).
+constexpr float PREFIX_COST = 4.f, SPLIT_COST = 1.f;
+
 // A prefix or a sequence: its tokens and the keys [k0, k1) that they read here.
 // A sequence of no prefix has k0 = -1 for 0.
 struct Family {
@@ -498,31 +501,69 @@ __device__ __forceinline__ void attend_shared(const B& x, const PrefixPlan& pl, 
     }
 }
 
-// The segments of the range [g0, g0 + per) of a line by one wave: 32-row tiles,
-// 32-key tiles in the wave's own 16 KiB of LDS at `slot`.  The line starts at
-// unit `origin`; partial blocks of `stride` rows from row part0 on, `blocks` of
-// them per K/V head.  Neighbouring families are taken with neighbouring K/V
-// heads: a wave that stays with one head reads one eighth of the memory
-// channels, and some of them are slower (128 sequences of 64..4096 own keys
-// behind 32768, H32 KVH8: the slowest head's tiles took 3.48 us, the fastest's
-// 2.75; 159 -> 146 us for the call).
-template <bool LSE, bool OWN, class B, class L>
+// A part of a segment of up to 32 rows, by single waves: wave `turn` of every
+// `step` waves takes the part's key tiles a0 + turn, a0 + turn + step, ... below
+// e1, 32 keys each, through 16 KiB of LDS of its own at `slot`, with no barrier.
+template <bool LSE>
+__device__ __forceinline__ void attend_tiles(const Fav4PagedArgs& pg, const int* table, int entries,
+                                             const FastDiv& by_page, int t, int step, int e1, int nfull, int k0, int k1,
+                                             int lim, int tok, int qhead, int kvh, uint32_t kv_row_bytes, float scale2,
+                                             const LdsOffsets& off, const DmaOffsets<8>& dofs, unsigned char* smem,
+                                             uint32_t slot, RowState& st, int lane) {
+    constexpr int BN = 32, TILE_BYTES = BN * ROW_BYTES, DMA = BN / 4;
+    const int half = lane >> 5;
+    PageWalk walk{nullptr, 0, pg.page_size, pg.num_pages};
+    walk.start(table, entries, k0 + t * BN, by_page, lane);
+    bf16x8 qr[8];
+    load_q(pg, tok, qhead, half, qr);
+#pragma unroll
+    for (int c = 0; c < 8; ++c) asm volatile("" ::"v"(qr[c]));
+    const uint32_t stage = lds_addr(smem) + slot;
+    auto issue = [&](int at) {
+        const int left = min(k1 - (k0 + at * BN), BN);
+        const uint32_t bytes = uint32_t(left - 1) * kv_row_bytes + ROW_BYTES;
+        const int64_t byte = (walk.row(BN * step, lane) * pg.kv_heads + kvh) * ROW_BYTES;
+        const u32x4 rk = make_desc(static_cast<const char*>(pg.k_cache) + byte, bytes);
+        const u32x4 rv = make_desc(static_cast<const char*>(pg.v_cache) + byte, bytes);
+        dma_tile<DMA, TILE_BYTES, true>(rk, rv, stage, 0, dofs);
+    };
+    issue(t);
+    const unsigned char* ks = smem + slot;
+    bool first = true;
+    auto tile = [&](auto masked_c) {
+        wait_vmem();
+        attend_fused<BN, decltype(masked_c)::value, true, LSE, true>(ks, ks + TILE_BYTES, off, qr, st, first,
+                                                                     k0 + t * BN, k1, lim, half, scale2);
+        // The tile has been read: the next one may land in its place.
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        first = false;
+        t += step;
+        if (t < e1) issue(t);
+    };
+    while (t < min(e1, nfull)) tile(std::integral_constant<bool, false>{});
+    while (t < e1) tile(std::integral_constant<bool, true>{});
+    wait_vmem();                                                       // (the last tile left none in flight)
+}
+
+// The segments of the range [g0, g0 + per) of the sequences' line by one wave.
+// Neighbouring families are taken with neighbouring K/V heads: a wave that stays
+// with one head reads one eighth of the memory channels, and some of them are
+// slower (128 sequences of 64..4096 own keys behind 32768, H32 KVH8: the slowest
+// head's tiles took 3.48 us, the fastest's 2.75; 159 -> 146 us for the call).
+template <bool LSE, class B, class L>
 __device__ __forceinline__ void attend_wave(const B& x, const PrefixPlan& pl, const L& line,
-                                            const typename L::Sums& head, int origin, int range, int per, int turn,
-                                            unsigned char* smem, uint32_t slot, int64_t part0, int blocks,
-                                            int stride) {
-    constexpr int BN = 32, BM = 32, TILE_BYTES = BN * ROW_BYTES, DMA = BN / 4;
+                                            const typename L::Sums& head, int range, int per, int turn,
+                                            unsigned char* smem, uint32_t slot, int64_t part0) {
+    constexpr int BN = 32, BM = 32, TILE_BYTES = BN * ROW_BYTES;
     const Fav4PagedArgs& pg = x.a.paged;
-    const int lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5, group = line.group;
+    const int lane = threadIdx.x & 63, col = lane & 31, group = line.group;
     const uint32_t kv_row_bytes = uint32_t(pg.kv_heads) * ROW_BYTES;
     const float scale2 = pg.scale * LOG2E;
-    const uint32_t stage = lds_addr(smem) + slot;
-    const int g0 = range * per, g1 = g0 + per;
+    const int g0 = range * per, g1 = g0 + per, blocks = pl.own_blocks, stride = pl.own_rows;
 
     const LdsOffsets off = lds_offsets(lane);
-    const DmaOffsets<DMA> dofs = dma_offsets<DMA>(0, lane, kv_row_bytes, kv_row_bytes);
-    typename L::Place at = line.find(max(0, g0 - origin), lane, head);
-    for (at.base += origin; at.idx < line.count && at.base < g1; ++at.idx) {
+    const DmaOffsets<8> dofs = dma_offsets<8>(0, lane, kv_row_bytes, kv_row_bytes);
+    for (typename L::Place at = line.find(g0, lane, head); at.idx < line.count && at.base < g1; ++at.idx) {
         const Family f = line.family(at.idx);
         const int t0 = uniform(f.t0), tokens = uniform(f.tokens), k0 = uniform(max(f.k0, 0)), k1 = uniform(f.k1);
         const int tiles = uniform(line.tiles(f)), ktiles = uniform(line.key_tiles(f)), seg_cost = uniform(line.seg_cost(f));
@@ -535,46 +576,15 @@ __device__ __forceinline__ void attend_wave(const B& x, const PrefixPlan& pl, co
             const int a0 = max(0, g0 - first), a1 = min(ktiles, g1 - first);
             const int q0 = rt * BM, row = q0 + col, srow = min(row, rows - 1);
             const int trow = pl.by_group(srow), tok = t0 + trow, qhead = kvh * group + srow - trow * group;
-            const Visible see = visible<OWN>(x, pl, f, at.idx, q0, min(rows, q0 + BM) - 1, tok);
-            const int lim = see.lim, nfull = max(0, see.plain - k0) / BN, e1 = min(a1, (see.end - k0 + BN - 1) / BN);
+            const Visible see = visible<true>(x, pl, f, at.idx, q0, min(rows, q0 + BM) - 1, tok);
+            const int nfull = max(0, see.plain - k0) / BN, e1 = min(a1, (see.end - k0 + BN - 1) / BN);
 
             RowState st;
             clear(st);
-            if (a0 < e1) {
-                PageWalk walk{nullptr, 0, pg.page_size, pg.num_pages};
-                if constexpr (OWN)
-                    walk.start(pg.block_table + int64_t(at.idx) * pg.max_pages_per_seq, pg.max_pages_per_seq,
-                               k0 + a0 * BN, pl.by_page, lane);
-                else
-                    walk.start(x.a.prefix_table + int64_t(at.idx) * x.a.max_pages_per_prefix, x.a.max_pages_per_prefix,
-                               a0 * BN, pl.by_page, lane);
-                bf16x8 qr[8];
-                load_q(pg, tok, qhead, half, qr);
-#pragma unroll
-                for (int c = 0; c < 8; ++c) asm volatile("" ::"v"(qr[c]));
-                auto issue = [&](int t) {
-                    const int left = min(k1 - (k0 + t * BN), BN);
-                    const uint32_t bytes = uint32_t(left - 1) * kv_row_bytes + ROW_BYTES;
-                    const int64_t byte = (walk.row(BN, lane) * pg.kv_heads + kvh) * ROW_BYTES;
-                    const u32x4 rk = make_desc(static_cast<const char*>(pg.k_cache) + byte, bytes);
-                    const u32x4 rv = make_desc(static_cast<const char*>(pg.v_cache) + byte, bytes);
-                    dma_tile<DMA, TILE_BYTES, true>(rk, rv, stage, 0, dofs);
-                };
-                issue(a0);
-                const unsigned char* ks = smem + slot;
-                auto step = [&](auto masked_c, int t) {
-                    wait_vmem();
-                    attend_fused<BN, decltype(masked_c)::value, true, LSE, true>(ks, ks + TILE_BYTES, off, qr, st, t == a0,
-                                                                                 k0 + t * BN, k1, lim, half, scale2);
-                    // The tile has been read: the next one may land in its place.
-                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-                    if (t + 1 < e1) issue(t + 1);
-                };
-                int t = a0;
-                for (; t < min(e1, nfull); ++t) step(std::integral_constant<bool, false>{}, t);
-                for (; t < e1; ++t) step(std::integral_constant<bool, true>{}, t);
-                wait_vmem();                                           // (the last step left none in flight)
-            }
+            if (a0 < e1)
+                attend_tiles<LSE>(pg, pg.block_table + int64_t(at.idx) * pg.max_pages_per_seq, pg.max_pages_per_seq,
+                                  pl.by_page, a0, 1, e1, nfull, k0, k1, see.lim, tok, qhead, kvh, kv_row_bytes, scale2,
+                                  off, dofs, smem, slot, st, lane);
             const int block = at.seg + rt + range, live = min(min(32, stride), rows - q0);
             if (ktiles > 0 && uint32_t(block) < uint32_t(blocks))
                 store_parts<LSE, TILE_BYTES>(st, pl, part0 + (int64_t(kvh) * blocks + block) * stride, live, smem, slot,
@@ -582,8 +592,8 @@ __device__ __forceinline__ void attend_wave(const B& x, const PrefixPlan& pl, co
             if (kvh == 0 && first >= g0 && lane < 32 && lane < live) {
                 const int parts = ktiles > 0 ? udiv(first + ktiles - 1, per) - range + 1 : 0;
                 int2* note = pl.notes + (int64_t(t0) * group + row) * 2;
-                note[OWN] = int2{block * stride + lane, parts};
-                if (OWN && uniform(f.k0) < 0) note[0] = int2{0, 0};
+                note[1] = int2{block * stride + lane, parts};
+                if (uniform(f.k0) < 0) note[0] = int2{0, 0};
             }
             // The staging has been read (its values were stored) before the next copy.
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -593,22 +603,121 @@ __device__ __forceinline__ void attend_wave(const B& x, const PrefixPlan& pl, co
     }
 }
 
+// The segments of the range [g0, g0 + per) of the prefixes' line where they have
+// 32 rows: the workgroup's eight waves take the range's key tiles in turn, and join
+// their parts in LDS (by the largest maximum of each row) before one is written.
+// One wave a range writes eight times the parts, and a 64-key tile shared by
+// eight waves, seven of them idle, takes 1.9 us where eight 32-key tiles take
+// 2.7 (H32 KVH8, 4 rows a prefix: 64 sequences each behind its own 2048 keys
+// 103 us by single waves, 132 shared, 97 split; 2 behind 8192 21.3, 18.8, 17.5).
+template <bool LSE, class B, class L>
+__device__ __forceinline__ void attend_split(const B& x, const PrefixPlan& pl, const L& line,
+                                             const typename L::Sums& head, int range, int per, int turn,
+                                             unsigned char* smem, float4 (&stats)[8][32]) {
+    constexpr int WAVES = 8, BN = 32, BM = 32, SLOT = 2 * BN * ROW_BYTES;
+    const Fav4PrefixArgs& a = x.a;
+    const Fav4PagedArgs& pg = a.paged;
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), col = lane & 31, half = lane >> 5;
+    const int group = line.group;
+    const uint32_t kv_row_bytes = uint32_t(pg.kv_heads) * ROW_BYTES;
+    const float scale2 = pg.scale * LOG2E;
+    const int g0 = range * per, g1 = g0 + per, blocks = pl.prefix_blocks;
+
+    const LdsOffsets off = lds_offsets(lane);
+    const DmaOffsets<8> dofs = dma_offsets<8>(0, lane, kv_row_bytes, kv_row_bytes);
+    for (typename L::Place at = line.find(g0, lane, head); at.idx < line.count && at.base < g1; ++at.idx) {
+        const Family f = line.family(at.idx);
+        const int t0 = uniform(f.t0), tokens = uniform(f.tokens), k1 = uniform(f.k1);
+        const int tiles = uniform(line.tiles(f)), ktiles = uniform(line.key_tiles(f)), seg_cost = uniform(line.seg_cost(f));
+        const int rows = tokens * group;
+        const int kvh = uniform(turn + at.idx - pl.by_kv_heads(turn + at.idx) * pg.kv_heads);
+        for (int rt = at.base < g0 && tiles > 1 ? udiv(max(0, g0 - at.base), seg_cost) : 0; rt < tiles; ++rt) {
+            const int first = at.base + (rt + 1) * seg_cost - max(ktiles, 1);
+            if (first >= g1) break;
+            if (first + max(ktiles, 1) <= g0) continue;
+            const int a0 = max(0, g0 - first), a1 = min(ktiles, g1 - first);
+            const int q0 = rt * BM, row = q0 + col, srow = min(row, rows - 1);
+            const int trow = pl.by_group(srow), tok = t0 + trow, qhead = kvh * group + srow - trow * group;
+            const Visible see = visible<false>(x, pl, f, at.idx, q0, min(rows, q0 + BM) - 1, tok);
+            const int block = at.seg + rt + range, live = min(32, rows - q0);
+
+            RowState st;
+            clear(st);
+            if (a0 + wave < a1)
+                attend_tiles<LSE>(pg, a.prefix_table + int64_t(at.idx) * a.max_pages_per_prefix, a.max_pages_per_prefix,
+                                  pl.by_page, a0 + wave, WAVES, a1, see.plain / BN, 0, k1, see.lim, tok, qhead, kvh,
+                                  kv_row_bytes, scale2, off, dofs, smem, wave * SLOT, st, lane);
+            // O by quads of 4 dims: quad q of a lane holds dims 32 (q / 4) + 8 (q % 4) +
+            // 4 half of row col.  Wave w sums quads 2w and 2w + 1 of all waves.
+            if (half == 0) stats[wave][col] = float4{st.m, st.lb, st.l, 0.f};
+#pragma unroll
+            for (int q = 0; q < 16; ++q) {
+                const f32x16& o = st.o[q >> 2];
+                const int i = (q & 3) * 4;
+                *reinterpret_cast<FAV4_LDS f32x4*>((FAV4_LDS void*)(smem + wave * SLOT + q * 1024 + lane * 16)) =
+                    f32x4{o[i], o[i + 1], o[i + 2], o[i + 3]};
+            }
+            __syncthreads();
+            float m = -__builtin_inff(), lb = 0.f, l = 0.f, weight[WAVES];
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) m = fmaxf(m, weight[w] = stats[w][col].x);
+            const float base = m == -__builtin_inff() ? 0.f : m;       // rows that see no key of the part
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) {
+                weight[w] = exp2_native(weight[w] - base);
+                lb += weight[w] * stats[w][col].y;
+                if constexpr (LSE) l += weight[w] * stats[w][col].z;
+            }
+            const float inv = lb > 0.f ? 1.f / lb : 0.f;
+            if (ktiles > 0 && uint32_t(block) < uint32_t(blocks)) {
+                const int64_t prow = (int64_t(kvh) * blocks + block) * BM;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int q = wave * 2 + i;
+                    f32x4 sum{};
+#pragma unroll
+                    for (int w = 0; w < WAVES; ++w)
+                        sum += weight[w] * *reinterpret_cast<const FAV4_LDS f32x4*>(
+                                               (FAV4_LDS const void*)(smem + w * SLOT + q * 1024 + lane * 16));
+                    if (col < live)
+                        *reinterpret_cast<f32x4*>(pl.o_part + (prow + col) * D + (q >> 2) * 32 + (q & 3) * 8 + half * 4) =
+                            sum * inv;
+                }
+                if (wave == 0 && lane < live) {
+                    const float sb = base + __builtin_amdgcn_logf(lb);
+                    reinterpret_cast<float2*>(pl.lse_part)[prow + lane] =
+                        float2{sb, LSE ? base + __builtin_amdgcn_logf(l) : sb};
+                }
+            }
+            if (wave == 0 && kvh == 0 && first >= g0 && lane < live) {
+                const int parts = ktiles > 0 ? udiv(first + ktiles - 1, per) - range + 1 : 0;
+                pl.notes[(int64_t(t0) * group + row) * 2] = int2{block * BM + lane, parts};
+            }
+            // Every wave has read the sums before the next segment's copies and statistics.
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            __syncthreads();
+        }
+        at.base += tiles * seg_cost;
+        at.seg += tiles;
+    }
+}
+
 // How a call's lines are cut (by the host, from the sizes): MANY rows per
 // sequence, both lines by whole workgroups; FEW, the prefixes' by workgroups
-// and the sequences' own by waves; FEWEST (a prefix's rows, too, few), both
-// by waves, as one line.
+// and the sequences' own by waves; FEWEST (a prefix's rows, too, few), the same,
+// with a prefix's keys split over the workgroup's waves.
 enum Cut { MANY, FEW, FEWEST };
 
-template <bool LSE, int WAVES, Cut CUT, bool CACHED>
-__global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
+template <bool LSE, Cut CUT, bool CACHED>
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void prefix_kernel(Fav4PrefixArgs a, PrefixPlan pl) {
-    constexpr bool OWN_WAVES = CUT != MANY;
-    constexpr int BN = WAVES == 4 ? 32 : 64, STAGES = 4;               // three tiles in flight
-    constexpr int BM = CUT == FEWEST ? 32 : WAVES * 32;                // rows of a prefix segment
+    constexpr int WAVES = 8, BN = 64, STAGES = 4;                      // three tiles in flight
+    constexpr bool OWN_WAVES = CUT != MANY, SPLIT = CUT == FEWEST;
+    constexpr int BM = SPLIT ? 32 : WAVES * 32;                        // rows of a prefix segment
     constexpr int OWN_RANGES = OWN_WAVES ? WAVES : 1;                  // of a workgroup
     __shared__ __attribute__((aligned(1024))) unsigned char smem[STAGES * 2 * BN * ROW_BYTES];
     __shared__ PlanLds lds;
-    static_assert(!OWN_WAVES || sizeof(smem) >= WAVES * 64 * ROW_BYTES, "a 32-key tile of K and V for each wave");
+    static_assert(sizeof(smem) >= WAVES * 64 * ROW_BYTES, "a 32-key tile of K and V for each wave");
     const Fav4PagedArgs& pg = a.paged;
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
     const int w = uniform(pl.by_kv_heads(blockIdx.x)), kvh = uniform(int(blockIdx.x) - w * pg.kv_heads);
@@ -639,53 +748,51 @@ void prefix_kernel(Fav4PrefixArgs a, PrefixPlan pl) {
         x.hidden = __syncthreads_or(hidden);
     }
     using B = PrefixBatch<CACHED>;
-    const Line<B, false, BM, BN, CUT == FEWEST ? OWN_SEG_TILES : SEG_TILES> prefixes{x, a.num_prefixes, group};
+    const Line<B, false, BM, SPLIT ? 32 : BN, SPLIT ? SPLIT_SEG_TILES : SEG_TILES> prefixes{x, a.num_prefixes, group};
     const Line<B, true, OWN_WAVES ? 32 : BM, OWN_WAVES ? 32 : BN, OWN_WAVES ? OWN_SEG_TILES : SEG_TILES> own{
         x, pg.batch, group};
     typename decltype(prefixes)::Sums prefix_head;
     typename decltype(own)::Sums own_head;
     const int prefix_units = prefixes.length(lane, prefix_head), own_units = own.length(lane, own_head);
 
-    const int64_t own_part0 = int64_t(pg.kv_heads) * pl.prefix_blocks * BM;
-    if constexpr (CUT == FEWEST) {
-        const int ranges = pl.ranges * WAVES, range = w * WAVES + wave, total = prefix_units + own_units;
-        const int per = max(udiv_up(total, ranges), MIN_OWN_TILES);
-        const uint32_t slot = wave * 64 * ROW_BYTES;
-        if (range * per < prefix_units)
-            attend_wave<LSE, false>(x, pl, prefixes, prefix_head, 0, range, per, kvh, smem, slot, 0, pl.prefix_blocks, BM);
-        if ((range + 1) * per > prefix_units)
-            attend_wave<LSE, true>(x, pl, own, own_head, prefix_units, range, per, kvh, smem, slot, own_part0,
-                                   pl.own_blocks, pl.own_rows);
-        return;
-    }
     // The workgroups of either line, by what its tiles cost; the two kinds alternate,
     // so that the XCDs have both.
-    const float cost = prefix_units * (OWN_WAVES ? WAVES == 4 ? PREFIX_COST_4 : PREFIX_COST_8 : 1.f);
+    const float cost = prefix_units * (SPLIT ? SPLIT_COST : OWN_WAVES ? PREFIX_COST : 1.f);
     int pw = min(max(int(cost / (cost + own_units) * pl.ranges + 0.5f), 1), pl.ranges - 1);
     if (prefix_units <= 0) pw = 0;
+    // One prefix, a range or more for each row tile: the tiles are cut at the same
+    // keys (the lead units take up the rest), so that they read them at the same time
+    // and share them in L2, where that takes about as many workgroups.
+    int tiles = 0;
+    if (a.num_prefixes == 1 && pw > 0) {
+        tiles = uniform(prefixes.tiles(prefixes.family(0)));
+        const int even = udiv(2 * pw + tiles, 2 * tiles) * tiles;      // the nearest multiple
+        if (tiles <= pw && even < pl.ranges && abs(even - pw) * 4 <= pw) pw = even;
+        else tiles = 0;
+    }
     // w pw / ranges, exact: both factors are at most 1024.
     const float step = 1.f / pl.ranges;
     const int before = int((w * pw + 0.5f) * step);
     if (int(((w + 1) * pw + 0.5f) * step) > before) {
-        int per = max(udiv_up(prefix_units, pw), MIN_PREFIX_TILES), aligned = 0;
-        const Family f = prefixes.family(0);
-        const int tiles = uniform(prefixes.tiles(f));
-        if (a.num_prefixes == 1 && tiles <= pw) {
-            // One prefix, a range or more for each row tile: they are cut at the same keys
-            // (the lead units take up the rest), so that they read them at the same time
-            // and share them in L2 (64 sequences behind 8192 keys H32 KVH8 on 128-row tiles
-            // 40.5 -> 39.0 us).
-            const int cost = uniform(prefixes.seg_cost(f));
-            per = max(udiv_up(cost, udiv(pw, tiles)), MIN_PREFIX_TILES);
-            aligned = udiv_up(cost, per) * per;
+        if constexpr (SPLIT) {
+            __shared__ float4 stats[WAVES][32];
+            const int per = max(udiv_up(prefix_units, pw), MIN_SPLIT_TILES);
+            attend_split<LSE>(x, pl, prefixes, prefix_head, before, per, kvh, smem, stats);
+        } else {
+            int per = max(udiv_up(prefix_units, pw), MIN_PREFIX_TILES), aligned = 0;
+            if (tiles) {
+                const int cost = uniform(prefixes.seg_cost(prefixes.family(0)));
+                per = max(udiv_up(cost, udiv(pw, tiles)), MIN_PREFIX_TILES);
+                aligned = udiv_up(cost, per) * per;
+            }
+            attend_shared<LSE, WAVES, false, BN, STAGES>(x, pl, prefixes, prefix_head, before, per, aligned, kvh, smem);
         }
-        attend_shared<LSE, WAVES, false, BN, STAGES>(x, pl, prefixes, prefix_head, before, per, aligned, kvh, smem);
     } else {
         const int ranges = (pl.ranges - pw) * OWN_RANGES, range = w - before;
         const int per = max(udiv_up(own_units, ranges), MIN_OWN_TILES);
         if constexpr (OWN_WAVES)
-            attend_wave<LSE, true>(x, pl, own, own_head, 0, range * WAVES + wave, per, kvh, smem, wave * 64 * ROW_BYTES,
-                                   own_part0, pl.own_blocks, pl.own_rows);
+            attend_wave<LSE>(x, pl, own, own_head, range * WAVES + wave, per, kvh, smem, wave * 64 * ROW_BYTES,
+                             int64_t(pg.kv_heads) * pl.prefix_blocks * BM);
         else
             attend_shared<LSE, WAVES, true, BN, STAGES>(x, pl, own, own_head, range, per, 0, kvh, smem);
     }
