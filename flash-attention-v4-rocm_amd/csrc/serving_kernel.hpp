@@ -163,6 +163,7 @@ struct PrefixPlan {
     int br;                           // bottom-right causal
 };
 
+// Of a shared segment (the eight waves' key tiles), a wave's, and a split one.
 constexpr int SEG_TILES = 4, OWN_SEG_TILES = 2, SPLIT_SEG_TILES = 8;
 constexpr int MIN_PREFIX_TILES = 2, MIN_OWN_TILES = 1, MIN_SPLIT_TILES = 4;  // shortest ranges
 // What a prefix's key tile costs, in own key tiles of a wave (its share of the
@@ -762,13 +763,13 @@ void prefix_kernel(Fav4PrefixArgs a, PrefixPlan pl) {
     if (prefix_units <= 0) pw = 0;
     // One prefix, a range or more for each row tile: the tiles are cut at the same
     // keys (the lead units take up the rest), so that they read them at the same time
-    // and share them in L2, where that takes about as many workgroups.
+    // and share them in L2, unless that leaves over a quarter of the workgroups idle
+    // (H32 KVH8: 256 sequences behind 1024 keys 42.6 us alike, 45.8 not; 40 x 16 queries
+    // behind 8192 114 not alike, 130 alike).
     int tiles = 0;
     if (a.num_prefixes == 1 && pw > 0) {
         tiles = uniform(prefixes.tiles(prefixes.family(0)));
-        const int even = udiv(2 * pw + tiles, 2 * tiles) * tiles;      // the nearest multiple
-        if (tiles <= pw && even < pl.ranges && abs(even - pw) * 4 <= pw) pw = even;
-        else tiles = 0;
+        if (udiv(pw, tiles) * tiles * 4 < pw * 3) tiles = 0;
     }
     // w pw / ranges, exact: both factors are at most 1024.
     const float step = 1.f / pl.ranges;

@@ -28,6 +28,10 @@ CASES = {
     "no_prefix_at_all": (8, 2, 64, [(0, [(1, 500), (2, 64)])], [(1, 1000)], 0),
     "more_row_tiles_than_workgroups": (64, 64, 32, [(128, [(300, 428), (290, 420), (310, 450), (257, 400)])], [], 2),
     "more_row_tiles_than_workgroups_decode": (128, 128, 32, [(96, [(1, 97 + i % 60) for i in range(300)])], [], 0),
+    "rows_of_prefixes_uneven": (8, 2, 64, [(1024, [(1, 1025 + 9 * i) for i in range(30)])] +
+                                [(64 * i, [(1, 64 * i + 30)]) for i in range(6)], [], 0),
+    "rows_of_prefixes_uneven_causal": (16, 2, 32, [(416, [(3, 400 + 7 * i) for i in range(5)])] +
+                                       [(32 * i, [(1, 32 * i + 1)]) for i in range(9)], [(2, 70)], 2),
     "wide_group": (64, 2, 32, [(1600, [(2, 1700), (3, 1605)])], [], 2),
 }
 
