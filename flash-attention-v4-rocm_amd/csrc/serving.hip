@@ -117,7 +117,7 @@ PrefixSizes prefix_sizes(const Fav4PrefixArgs& args, int causal) {
     const int64_t own_segs = tiles(a.batch, seq_rows, own_bm);
     const int64_t prefix_keys = std::min<int64_t>(int64_t(args.max_pages_per_prefix) * a.page_size, a.max_seqlen_k);
     s.plan.most_prefix_keys = int(prefix_keys);
-    const int64_t lead = 1 + fav4::SEG_TILES;
+    const int64_t lead = 1 + std::max(fav4::SEG_TILES, fav4::SPLIT_SEG_TILES);
     const int64_t units = prefix_segs * (prefix_keys / 32 + lead) + own_segs * (a.max_seqlen_k / 32 + lead);
     const int64_t prefix_ranges = s.plan.ranges;
     const int64_t own_ranges = s.plan.ranges * (own_waves ? WAVES : 1);

@@ -129,7 +129,7 @@ __global__ __launch_bounds__(256) void append_kernel(Fav4AppendArgs a, int units
 // head's group), r = token * group + head: the rows of all sequences of a
 // prefix are neighbours, and so are those of one sequence.  A segment is a row
 // tile of one prefix against the prefix's keys (BM rows), or of one sequence
-// against the sequence's own keys; it costs its key tiles and SEG_TILES more,
+// against the sequence's own keys; it costs its key tiles and some more (SEG_TILES),
 // laid before them, for what its start and end cost (without keys, one tile).
 // The segments of a K/V head are laid end to end, the prefixes' on one line,
 // the sequences' own on another, and each line is cut into ranges of one

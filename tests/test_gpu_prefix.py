@@ -186,6 +186,26 @@ def test_prefix_in_a_graph(gpu_runner):
         assert torch.equal(o.view(torch.int16), eager.view(torch.int16)) and torch.equal(l, el)
 
 
+@pytest.mark.parametrize("heads,kvh,queries,causal", [(64, 2, 1, 0), (32, 2, 2, 2), (16, 4, 9, 2), (8, 1, 40, 2)])
+def test_prefix_in_a_graph_of_more_rows(gpu_runner, heads, kvh, queries, causal):
+    """More rows than one wave's for each prefix, and for each sequence: replayed with other lengths and prefixes."""
+    x = Batch(heads, kvh, 64, [(256, [(queries, 500), (queries, 400), (queries, 300)]), (128, [(queries, 600), (queries, 222)])])
+    o, l = x.outputs(True)
+    ws = x.attend(gpu_runner, o, l, causal)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        x.attend(gpu_runner, o, l, causal, workspace=ws)
+    for keys in ([500, 400, 300, 600, 222], [257, 310, 256, 129, 128], [499, 0, 300, 128, 100], [300, 300, 300, 300, 222]):
+        x.lens = [(queries, k) for k in keys]
+        x.seqlens.copy_(torch.tensor(keys, dtype=torch.int32))
+        x.q.copy_(torch.randn(x.q.shape, device=x.dev).to(torch.bfloat16))
+        o.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        x.check(o, l, causal)
+
+
 def test_prefix_far_pages(gpu_runner):
     """Caches of more than 2^31 elements: shared and own pages past 4 GiB."""
     x = Batch(8, 8, 128, [(256, [(1, 300), (2, 257)])], seed=3)
