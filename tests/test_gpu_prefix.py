@@ -32,6 +32,10 @@ CASES = {
                                 [(64 * i, [(1, 64 * i + 30)]) for i in range(6)], [], 0),
     "rows_of_prefixes_uneven_causal": (16, 2, 32, [(416, [(3, 400 + 7 * i) for i in range(5)])] +
                                        [(32 * i, [(1, 32 * i + 1)]) for i in range(9)], [(2, 70)], 2),
+    "more_kv_heads_than_cus": (300, 300, 32, [(64, [(1, 100), (2, 70)])], [(1, 9)], 0),
+    "more_kv_heads_than_cus_prefill": (300, 300, 32, [(64, [(40, 140), (33, 70)])], [], 2),
+    "large_pages": (8, 2, 1024, [(2048, [(1, 3000), (1, 2049)])], [(1, 10)], 0),
+    "widest_group": (256, 1, 64, [(320, [(1, 321), (2, 700)])], [(1, 65)], 2),
     "wide_group": (64, 2, 32, [(1600, [(2, 1700), (3, 1605)])], [], 2),
 }
 
