@@ -115,7 +115,10 @@ PrefixSizes prefix_sizes(const Fav4PrefixArgs& args, int causal) {
     const int64_t own_rows = std::min<int64_t>(own_bm, seq_rows);
     const int64_t prefix_segs = tiles(args.num_prefixes, rows, BM);
     const int64_t own_segs = tiles(a.batch, seq_rows, own_bm);
-    const int64_t prefix_keys = std::min<int64_t>(int64_t(args.max_pages_per_prefix) * a.page_size, a.max_seqlen_k);
+    // Whole pages of a prefix, the one too that the longest sequence ends in (a sequence
+    // may have fewer keys than its prefix, and reads none of those in its own table).
+    const int64_t page = a.page_size, most_pages = (a.max_seqlen_k + page - 1) / page;
+    const int64_t prefix_keys = std::min({int64_t(args.max_pages_per_prefix), most_pages, INT_MAX / page}) * page;
     s.plan.most_prefix_keys = int(prefix_keys);
     const int64_t lead = 1 + std::max(fav4::SEG_TILES, fav4::SPLIT_SEG_TILES);
     const int64_t units = prefix_segs * (prefix_keys / 32 + lead) + own_segs * (a.max_seqlen_k / 32 + lead);

@@ -159,7 +159,7 @@ struct PrefixPlan {
     FastDiv by_kv_heads, by_group, by_page, by_heads, by_bm, by_own_rows;
     int prefix_blocks, own_blocks;    // partial blocks of a K/V head
     int own_rows;                     // rows of an own block
-    int most_prefix_keys;             // of a prefix: its table's, and max_seqlen_k
+    int most_prefix_keys;             // of a prefix, whole pages: its table's, and those that max_seqlen_k reaches into
     int br;                           // bottom-right causal
 };
 
@@ -188,7 +188,8 @@ struct PlanLds {
 };
 
 // The batch as read on the device, clamped: tokens to [0, total_q], keys to
-// [0, max_seqlen_k], a prefix's keys to whole pages of its table.
+// [0, max_seqlen_k], a prefix's keys to whole pages of its table (of those that a
+// sequence of max_seqlen_k keys reaches into).
 template <bool CACHED>
 struct PrefixBatch {
     const Fav4PrefixArgs& a;

@@ -67,7 +67,8 @@ extern "C" int fav4_bshd_append_paged(const Fav4AppendArgs* args, hipStream_t st
 //  * Any number of new queries per sequence, dense (causal 0) or bottom-right
 //    causal (2).  Sequences in no prefix, or of a prefix without keys, are
 //    attended over their own pages alone.  A sequence with fewer keys than its
-//    prefix sees those alone; one without keys gets O = 0 and LSE = -inf, one
+//    prefix sees those alone (max_seqlen_k bounds the sequences' keys, and may
+//    lie inside a prefix); one without keys gets O = 0 and LSE = -inf, one
 //    without queries writes nothing.
 //  * K and V of every key in [0, seqlens_k) and of every shared key must be
 //    finite, also for rows that do not see it: hidden keys have weight 0, and 0
