@@ -50,8 +50,9 @@ __device__ __forceinline__ int wave_find(const int* cu, int n, int x, int lane) 
 // then V): 8 lanes a row, each with the two 16-byte granules whose dims are
 // rotated together (both lie in this lane: granules j and j + rotary_dim / 16,
 // or neighbours).  Bound by memory, for few tokens by the chain of dependent
-// loads: offsets -> key count and table entry -> angles -> store; the rows
-// themselves are loaded ahead of it.
+// loads: offsets -> sequence and rows -> key count, table entry and angles ->
+// store.  Rows are loaded behind the check that a sequence has them, for a
+// caller's buffers may end with the last sequence.
 // ---------------------------------------------------------------------------
 template <bool INTERLEAVED>
 __global__ __launch_bounds__(256) void append_kernel(Fav4AppendArgs a, int units, int64_t total, FastDiv by_units, FastDiv by_page) {
@@ -59,8 +60,10 @@ __global__ __launch_bounds__(256) void append_kernel(Fav4AppendArgs a, int units
     const int64_t stride = int64_t(gridDim.x) * 4;
     const int qheads = a.q ? a.heads : 0, rows = qheads + 2 * a.kv_heads;
     const int half = a.rotary_dim >> 4;                    // granules of half the rotated dims
+    const int first = a.cu_seqlens_q[0], end = a.cu_seqlens_q[a.batch];
     for (int64_t id = int64_t(blockIdx.x) * 4 + uniform(threadIdx.x >> 6); id < total; id += stride) {
         const int t = uniform(by_units(int(id))), unit = uniform(int(id) - t * units);
+        if (t < first || t >= end) continue;               // in no sequence
         const int row = unit * 8 + (lane >> 3);
         const bool live = row < rows, is_q = row < qheads, is_v = row >= qheads + a.kv_heads;
         const int head = is_q ? row : is_v ? row - qheads - a.kv_heads : row - qheads;
@@ -75,8 +78,7 @@ __global__ __launch_bounds__(256) void append_kernel(Fav4AppendArgs a, int units
             x = *reinterpret_cast<const bf16x8*>(src + g0 * 16);
             y = *reinterpret_cast<const bf16x8*>(src + g1 * 16);
         }
-        const int b = wave_find(a.cu_seqlens_q, a.batch, t, lane);
-        if (b >= a.batch || t < a.cu_seqlens_q[0]) continue;           // behind the last sequence
+        const int b = wave_find(a.cu_seqlens_q, a.batch, t, lane);     // below batch: the last offset is above t
         const int64_t slot = int64_t(a.seqlens_k[b]) - a.cu_seqlens_q[b + 1] + t;
         int page = -1, in_page = 0;
         if (slot >= 0 && slot < int64_t(a.max_pages_per_seq) * a.page_size && slot <= INT_MAX) {
