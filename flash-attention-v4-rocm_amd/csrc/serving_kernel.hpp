@@ -859,7 +859,14 @@ __global__ __launch_bounds__(256) void prefix_merge_kernel(Fav4PrefixArgs a, Pre
             float nb = mb, nl = ml;
 #pragma unroll
             for (int i = 0; i < NS; ++i) nb = fmaxf(nb, v[i].x), nl = fmaxf(nl, v[i].y);
-            if (nb == -__builtin_inff()) continue;             // parts without a visible key
+            if (nb == -__builtin_inff()) {
+                // Parts without a visible key, or of a query that is no number: its log-sums
+                // are none either (maxima pass over them), and so are then O and the LSE.
+#pragma unroll
+                for (int i = 0; i < NS; ++i)
+                    if (v[i].x != v[i].x) den = suml = __builtin_nanf("");
+                continue;
+            }
             const float keep = exp2_native(mb - nb);
             acc[0] *= keep, acc[1] *= keep;
             den *= keep;
@@ -868,7 +875,7 @@ __global__ __launch_bounds__(256) void prefix_merge_kernel(Fav4PrefixArgs a, Pre
 #pragma unroll
             for (int i = 0; i < NS; ++i) {
                 const float wgt = exp2_native(v[i].x - mb);
-                if (wgt > 0.f) acc[0] += wgt * xo[i][0], acc[1] += wgt * xo[i][1];
+                if (wgt != 0.f) acc[0] += wgt * xo[i][0], acc[1] += wgt * xo[i][1];
                 den += wgt;
                 suml += exp2_native(v[i].y - ml);
             }
@@ -884,7 +891,7 @@ __global__ __launch_bounds__(256) void prefix_merge_kernel(Fav4PrefixArgs a, Pre
 #pragma unroll
             for (int p = 0; p < PER; ++p) {
                 const float4 o = red[slot * PER + p];
-                if (o.x == -__builtin_inff()) continue;
+                if (o.z == 0.f) continue;                      // no part with a visible key
                 const float wgt = exp2_native(o.x - mb);
                 den += wgt * o.z;
                 suml += exp2_native(o.y - ml) * o.w;
@@ -894,13 +901,13 @@ __global__ __launch_bounds__(256) void prefix_merge_kernel(Fav4PrefixArgs a, Pre
         }
         if (!live || part != 0) continue;
         // No key in any part: O = 0, LSE = -inf.
-        const float rden = den > 0.f ? 1.f / den : 0.f;
+        const float rden = den == 0.f ? 0.f : 1.f / den;
         bf16x8 y;
 #pragma unroll
         for (int i = 0; i < 8; ++i) y[i] = __bf16(acc[i >> 2][i & 3] * rden);
         *reinterpret_cast<bf16x8*>(static_cast<char*>(pg.o) + int64_t(r) * ROW_BYTES + l16 * 16) = y;
         if (pg.lse && l16 == 0) pg.lse[int64_t(head) * pg.total_q + tok] =
-            den > 0.f ? (ml + __builtin_amdgcn_logf(suml)) * LN2 : -__builtin_inff();
+            den == 0.f ? -__builtin_inff() : (ml + __builtin_amdgcn_logf(suml)) * LN2;
     }
 }
 
