@@ -529,6 +529,14 @@ class Runner:
         return raw(device) if raw is not None else torch.cuda.current_stream().cuda_stream
 
     @staticmethod
+    def _allocation_stream(torch, stream):
+        """torch's stream for a raw handle (None: its current one), to allocate on; 0 is the default stream, for which
+        ExternalStream would make a stream of its own."""
+        if stream is None:
+            return None
+        return torch.cuda.ExternalStream(stream) if stream else torch.cuda.default_stream()
+
+    @staticmethod
     def _append_block(torch, q, k, v, q_out, k_cache, v_cache, cu_q, seqlens_k, block_table, cos, sin, interleaved,
                       positions) -> bytes:
         bf16, i32, dev = torch.bfloat16, torch.int32, k.get_device()
@@ -642,7 +650,7 @@ class Runner:
             if need < 0:
                 raise RuntimeError("prefix paged: arguments rejected")
             # Allocated for the stream that uses it, which then orders its reuse.
-            with torch.cuda.stream(None if stream is None else torch.cuda.ExternalStream(stream)):
+            with torch.cuda.stream(self._allocation_stream(torch, stream)):
                 workspace = torch.empty(need, device=q.device, dtype=torch.uint8)
         assert workspace.get_device() == q.get_device() and workspace.is_contiguous()
         status = self.serving.fav4_bshd_forward_prefix_paged(block, causal, workspace.data_ptr(), workspace.nbytes, raw)
