@@ -68,7 +68,12 @@ constexpr int SPLIT_ROWS = 32;
 // sequences of 1000..4000 own keys: 203, two row tiles each, and 151).
 constexpr int WAVE_ROWS = 32;
 
+// Keys of a sequence and of a prefix, whole pages: a position and a tile's width fit an int.
+constexpr int MAX_KEYS = INT_MAX - 255;
 constexpr int MAX_HEADS = 1 << 15;    // the Q rows of a 256-row tile lie within 4 GiB
+
+// Pages that max_seqlen_k keys take.
+int64_t whole_pages(const Fav4PagedArgs& a) { return (int64_t(a.max_seqlen_k) + a.page_size - 1) / a.page_size; }
 
 bool prefix_shape_ok(const Fav4PrefixArgs* args, int causal) {
     if (!args) return false;
@@ -79,7 +84,7 @@ bool prefix_shape_ok(const Fav4PrefixArgs* args, int causal) {
         (causal != 0 && causal != BOTTOM_RIGHT) || !std::isfinite(a.scale) || a.scale <= 0)
         return false;
     if (a.page_size % 32 || a.max_seqlen_k > int64_t(a.max_pages_per_seq) * a.page_size ||
-        a.heads > MAX_HEADS || int64_t(a.total_q) * a.heads > INT_MAX ||
+        whole_pages(a) > MAX_KEYS / a.page_size || a.heads > MAX_HEADS || int64_t(a.total_q) * a.heads > INT_MAX ||
         int64_t(a.kv_heads) * fav4::ROW_BYTES * 32 > INT_MAX ||
         static_cast<__int128>(a.num_pages) * a.page_size * a.kv_heads * fav4::ROW_BYTES >= MAX_BYTES)
         return false;
@@ -117,8 +122,7 @@ PrefixSizes prefix_sizes(const Fav4PrefixArgs& args, int causal) {
     const int64_t own_segs = tiles(a.batch, seq_rows, own_bm);
     // Whole pages of a prefix, the one too that the longest sequence ends in (a sequence
     // may have fewer keys than its prefix, and reads none of those in its own table).
-    const int64_t page = a.page_size, most_pages = (a.max_seqlen_k + page - 1) / page;
-    const int64_t prefix_keys = std::min({int64_t(args.max_pages_per_prefix), most_pages, INT_MAX / page}) * page;
+    const int64_t prefix_keys = std::min<int64_t>(args.max_pages_per_prefix, whole_pages(a)) * a.page_size;
     s.plan.most_prefix_keys = int(prefix_keys);
     const int64_t lead = 1 + std::max(fav4::SEG_TILES, fav4::SPLIT_SEG_TILES);
     const int64_t units = prefix_segs * (prefix_keys / 32 + lead) + own_segs * (a.max_seqlen_k / 32 + lead);

@@ -84,8 +84,8 @@ struct Fav4PrefixArgs {
     int num_prefixes, max_pages_per_prefix;
 };
 // Checks: those of Fav4PagedArgs with causal 0 or 2, page_size a multiple of 32,
-// max_seqlen_k <= max_pages_per_seq * page_size, num_prefixes and
-// max_pages_per_prefix >= 1, heads <= 2^15, total_q * heads < 2^31, and a plan
+// max_seqlen_k <= max_pages_per_seq * page_size and in whole pages < 2^31 - 255,
+// num_prefixes and max_pages_per_prefix >= 1, heads <= 2^15, total_q * heads < 2^31, and a plan
 // of fewer than 2^30 key tiles.  The workspace is caller-owned device memory,
 // 256-byte aligned, of at least fav4_bshd_prefix_paged_workspace_size() bytes
 // and not shared with a concurrent call (two captured graphs that may run at
