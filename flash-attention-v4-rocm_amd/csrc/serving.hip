@@ -131,8 +131,8 @@ PrefixSizes prefix_sizes(const Fav4PrefixArgs& args, int causal) {
     const int64_t prefix_blocks = prefix_segs + prefix_ranges, own_blocks = own_segs + own_ranges;
     s.parts = std::min(prefix_ranges / std::max<int64_t>(1, prefix_segs),
                        prefix_keys / (s.cut == fav4::FEWEST ? 32 * fav4::MIN_SPLIT_TILES : 64 * fav4::MIN_PREFIX_TILES)) +
-              std::min(own_ranges / std::max<int64_t>(1, own_segs), std::max<int64_t>(0, a.max_seqlen_k - prefix_keys) /
-                                                                        (own_waves ? 32 * fav4::MIN_OWN_TILES : 64 * fav4::MIN_PREFIX_TILES));
+              std::min(own_ranges / std::max<int64_t>(1, own_segs),
+                       std::max<int64_t>(0, a.max_seqlen_k - prefix_keys) / ((own_waves ? 32 : 64) * fav4::MIN_OWN_TILES));
     s.part_rows = (a.kv_heads * (prefix_blocks * BM + own_blocks * own_rows) + 1) & ~int64_t(1);   // notes 16-byte aligned
     s.ok = units < (1 << 30) && prefix_blocks * BM <= INT_MAX && own_blocks * own_rows <= INT_MAX;
     s.plan.prefix_blocks = int(prefix_blocks);

@@ -171,3 +171,14 @@ def test_calls_repeat_bitwise(gpu_runner, name):
         x.attend(gpu_runner, again, al, causal, workspace=ws)
         torch.cuda.synchronize()
         assert torch.equal(again.view(torch.int16), o.view(torch.int16)) and torch.equal(al, l)
+
+
+@pytest.mark.parametrize("prefix", [0, 1024])
+@pytest.mark.parametrize("heads,kvh,queries,own", [(8, 1, 9, 4000), (8, 1, 33, 2000), (16, 2, 9, 6000), (32, 8, 40, 9000)])
+def test_many_own_parts_of_a_row(gpu_runner, heads, kvh, queries, own, prefix):
+    """More than 32 rows a sequence, and long keys of its own: as many parts as there are key tiles, or workgroups."""
+    x = Batch(heads, kvh, 64, [(prefix, [(queries, prefix + own), (queries, prefix + own - 1000)])])
+    o, l = x.outputs(True)
+    x.attend(gpu_runner, o, l, 2)
+    torch.cuda.synchronize()
+    x.check(o, l, 2)
