@@ -33,13 +33,14 @@ bool aligned(uintptr_t to, P... p) {
 }
 
 // ---- append ------------------------------------------------------------------
+constexpr int MAX_BATCH = INT_MAX - 63;      // wave_find's 64 steps through the offsets fit an int
 bool append_ok(const Fav4AppendArgs* a) {
     if (!a || !a->k || !a->v || !a->k_cache || !a->v_cache || !a->cu_seqlens_q || !a->seqlens_k || !a->block_table ||
         !a->q != !a->q_out)
         return false;
-    if (a->batch < 1 || a->heads < 1 || a->kv_heads < 1 || a->total_q < 1 || a->num_pages < 1 || a->page_size < 1 ||
-        a->max_pages_per_seq < 1 || a->rotary_dim < 0 || a->rotary_dim > fav4::D || a->rotary_dim % 16 ||
-        (a->interleaved != 0 && a->interleaved != 1))
+    if (a->batch < 1 || a->batch > MAX_BATCH || a->heads < 1 || a->kv_heads < 1 || a->total_q < 1 ||
+        a->num_pages < 1 || a->page_size < 1 || a->max_pages_per_seq < 1 || a->rotary_dim < 0 ||
+        a->rotary_dim > fav4::D || a->rotary_dim % 16 || (a->interleaved != 0 && a->interleaved != 1))
         return false;
     if (a->rotary_dim > 0 ? !a->cos || !a->sin || a->rotary_rows < 1 : a->cos || a->sin) return false;
     const int64_t rows = (a->q ? int64_t(a->heads) : 0) + 2 * int64_t(a->kv_heads);
@@ -70,7 +71,7 @@ constexpr int WAVE_ROWS = 32;
 
 // Keys of a sequence and of a prefix, whole pages: a position and a tile's width fit an int.
 constexpr int MAX_KEYS = INT_MAX - 255;
-constexpr int MAX_HEADS = 1 << 15;    // the Q rows of a 256-row tile lie within 4 GiB
+constexpr int MAX_HEADS = 1 << 15;    // the documented limit; indexes need total_q * heads < 2^31 alone
 
 // Pages that max_seqlen_k keys take.
 int64_t whole_pages(const Fav4PagedArgs& a) { return (int64_t(a.max_seqlen_k) + a.page_size - 1) / a.page_size; }

@@ -49,8 +49,8 @@ struct Fav4AppendArgs {
 // rotary_rows >= 1 where it is not 0, interleaved 0 or 1, strides of at least
 // heads * 128 (kv_heads * 128) elements that are multiples of 8, q_out_stride =
 // q_stride where q_out is q, 16-byte aligned rows and tables of angles, 4-byte
-// aligned int arrays, (heads + 2 kv_heads) * total_q < 2^31 and tensors of less
-// than 2^48 bytes.
+// aligned int arrays, (heads + 2 kv_heads) * total_q < 2^31, batch <= 2^31 - 64
+// and tensors of less than 2^48 bytes.
 extern "C" int fav4_bshd_append_paged(const Fav4AppendArgs* args, hipStream_t stream);
 
 // ---- Attention behind shared prefixes ----------------------------------------

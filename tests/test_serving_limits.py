@@ -3,7 +3,7 @@ import ctypes as C
 
 import pytest
 
-from tests.test_serving_abi import INVALID, lib, pkg, prefix_args  # noqa: F401
+from tests.test_serving_abi import INVALID, append_args, lib, pkg, prefix_args  # noqa: F401
 
 TOP = (1 << 31) - 1
 
@@ -21,3 +21,9 @@ def test_prefix_refuses_key_counts_near_2_31(pkg, lib, page):
         assert (lib.fav4_bshd_prefix_paged_workspace_size(C.byref(a), 0) > 0) == ok, keys
         if not ok:
             assert lib.fav4_bshd_forward_prefix_paged(C.byref(a), 0, 0x1000000, 1 << 40, None) == INVALID
+
+
+@pytest.mark.parametrize("batch", [TOP, TOP - 62])
+def test_append_refuses_batches_near_2_31(pkg, lib, batch):
+    """A wave's search for a token's sequence takes 64 equal steps through the offsets, which are ints."""
+    assert lib.fav4_bshd_append_paged(C.byref(append_args(pkg, batch=batch)), None) == INVALID
