@@ -54,3 +54,13 @@ def test_sequences_shorter_than_their_prefixes(gpu_runner, name, seed):
     torch.cuda.synchronize()
     x.check(o, l, causal)
     assert torch.isnan(x.o_all[o.shape[0]:]).all()
+
+
+@pytest.mark.parametrize("causal", [0, 2])
+def test_more_keys_than_the_paged_call_takes(gpu_runner, causal):
+    """Over 2^19 keys, most of them shared."""
+    x = Batch(4, 1, 128, [(600064, [(1, 600200), (2, 660000)])])
+    o, l = x.outputs(True)
+    x.attend(gpu_runner, o, l, causal)
+    torch.cuda.synchronize()
+    x.check(o, l, causal)
