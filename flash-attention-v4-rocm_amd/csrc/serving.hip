@@ -222,7 +222,8 @@ extern "C" __attribute__((visibility("default"))) int fav4_bshd_forward_prefix_p
     // Teams per merged row: many where a row can have many parts (24 sequences behind
     // 16384 keys H8 KVH1, 132 parts: 24.6 us on 4, 21.6 on 16), one where it has few or
     // the rows alone fill the GPU (384 sequences behind 1024 keys H32 KVH8: 66.5 on 4,
-    // 57.3 on one; 64 behind 8192, 36 parts: 35.8 and 37.7).
+    // 57.3 on one; 64 behind 8192, 36 parts: 35.8 and 37.7).  The steps lie where 44 such
+    // calls changed sides; between those points they are a guess.
     const int64_t rows = int64_t(a.total_q) * a.heads;
     const bool many = (s.parts > 44 && rows <= 256) || (s.parts > 96 && rows <= 1024);
     const bool few = rows > 4096 || s.parts <= 5 || (s.parts <= 18 && rows > 2048);

@@ -85,13 +85,22 @@ struct Fav4PrefixArgs {
 };
 // Checks: those of Fav4PagedArgs with causal 0 or 2, page_size a multiple of 32,
 // max_seqlen_k <= max_pages_per_seq * page_size and in whole pages < 2^31 - 255,
-// num_prefixes and max_pages_per_prefix >= 1, heads <= 2^15, total_q * heads < 2^31, and a plan
-// of fewer than 2^30 key tiles.  The workspace is caller-owned device memory,
-// 256-byte aligned, of at least fav4_bshd_prefix_paged_workspace_size() bytes
-// and not shared with a concurrent call (two captured graphs that may run at
-// once included); its contents do not matter.  The size query reads only the
-// sizes (pointers may be NULL), returns -1 for rejected arguments, and never
-// less for a larger batch, more queries, prefixes or pages.
+// num_prefixes and max_pages_per_prefix >= 1, heads <= 2^15, total_q * heads <
+// 2^31, and a plan of fewer than 2^30 key tiles.  The workspace is caller-owned
+// device memory, 256-byte aligned, of at least
+// fav4_bshd_prefix_paged_workspace_size() bytes and not shared with a concurrent
+// call (two captured graphs that may run at once included); its contents do not
+// matter.  The size query reads only the sizes (pointers may be NULL), returns
+// -1 for rejected arguments, and never less for a larger batch, more queries,
+// prefixes or pages: it counts what any cut of the call could need, about twice
+// what a decode step lays out (80 MB for 64 sequences, 32 heads on 8).
+//
+// Sizes that steer the speed: up to 32 * num_prefixes rows (total_q * heads /
+// kv_heads) are taken for few rows a prefix, slots without sequences counted, so
+// num_prefixes should be near the number in use.  A sequence with fewer keys
+// than its prefix (an idle slot inside its range) makes the prefix tiles of the
+// whole call masked ones, as more than 512 sequences or 256 prefixes do: idle
+// slots are better behind the last prefix.
 extern "C" int fav4_bshd_forward_prefix_paged(const Fav4PrefixArgs* args, int causal, void* workspace,
                                               size_t workspace_bytes, hipStream_t stream);
 extern "C" long long fav4_bshd_prefix_paged_workspace_size(const Fav4PrefixArgs* args, int causal);
