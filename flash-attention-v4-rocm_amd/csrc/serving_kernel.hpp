@@ -149,6 +149,9 @@ __global__ __launch_bounds__(256) void append_kernel(Fav4AppendArgs a, int units
 // log-sums (log2: of the BF16 weights, and of the FP32 ones) to partial block
 // (segment + w) of its line: segments and ranges both only grow along the line,
 // so no two parts have the same sum, and the blocks number segments + ranges.
+// Weights are rounded to BF16 for the product with V, whose matrix instruction
+// takes no wider operand beside a BF16 V, and summed as rounded, as in the forward:
+// 0.0023 of O against 64 bits, 0.0017 with FP32 weights; everything else is FP32.
 // The part that holds a segment's first key tile also notes for each of its rows
 // where its partials start and how many there are; prefix_merge_kernel goes by
 // those notes.

@@ -72,8 +72,9 @@ extern "C" int fav4_bshd_append_paged(const Fav4AppendArgs* args, hipStream_t st
 //    without queries writes nothing.
 //  * K and V of every key in [0, seqlens_k) and of every shared key must be
 //    finite, also for rows that do not see it: hidden keys have weight 0, and 0
-//    times a NaN is one.  Slots behind seqlens_k may hold anything.  A query row
-//    that is not finite gets O and LSE of NaN, and changes no other row.
+//    times a NaN is one.  Slots behind seqlens_k may hold anything.  A row whose
+//    query holds a NaN and that sees a key gets O and LSE of NaN; no query changes
+//    another row.
 //  * Results meet the tolerances of the paged call (not bitwise its results:
 //    the parts are cut elsewhere), and are the same from call to call.
 struct Fav4PrefixArgs {
