@@ -1,0 +1,232 @@
+// C-ABI host dispatch of the operators of 4-bit paged K/V caches
+// (include/fav4_mx4.h): the argument checks, before any HIP call, and the launches.
+#include "fav4_mx4.h"
+#include "mx4_kernel.hpp"
+
+#include <algorithm>
+#include <atomic>
+#include <climits>
+#include <cmath>
+#include <cstdint>
+
+namespace {
+
+constexpr int64_t MAX_GRID = int64_t(1) << 22;
+constexpr int64_t MAX_BYTES = int64_t(1) << 48;
+constexpr int MAX_BATCH = INT_MAX - 63;       // wave_find's 64 steps through the offsets fit an int
+constexpr int BOTTOM_RIGHT = 2;
+constexpr int MAX_KEYS = INT_MAX - 255;       // in whole pages: a position and a tile's width fit an int
+constexpr int MAX_HEADS = 1 << 15;            // the documented limit; indexes need total_q * heads < 2^31 alone
+constexpr int MAX_ROW_TILES = 1 << 22;
+
+// CU count of the current device (256 if it cannot be read), cached per
+// device after the first query.
+int device_cus() {
+    static std::atomic<int> cache[64];
+    int dev = 0, cus = 0;
+    if (hipGetDevice(&dev) != hipSuccess) return 256;
+    const bool slot = dev >= 0 && dev < 64;
+    if (slot && (cus = cache[dev].load(std::memory_order_relaxed)) > 0) return cus;
+    if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus <= 0) cus = 256;
+    if (slot) cache[dev].store(cus, std::memory_order_relaxed);
+    return cus;
+}
+
+template <class... P>
+bool aligned(uintptr_t to, P... p) {
+    return ((... | reinterpret_cast<uintptr_t>(p)) & (to - 1)) == 0;
+}
+
+bool caches_fit(int num_pages, int page_size, int kv_heads) {
+    return static_cast<__int128>(num_pages) * page_size * kv_heads * fav4::MX4_CODES < MAX_BYTES;
+}
+bool stride_ok(long long stride, int heads, int rows) {
+    return stride >= int64_t(heads) * fav4::D && (stride & 7) == 0 && static_cast<__int128>(stride) * rows * 2 < MAX_BYTES;
+}
+
+bool append_ok(const Fav4Mx4AppendArgs* args) {
+    if (!args || !args->k_scales || !args->v_scales || !aligned(16, args->k_scales, args->v_scales)) return false;
+    const Fav4AppendArgs* a = &args->append;
+    if (!a->k || !a->v || !a->k_cache || !a->v_cache || !a->cu_seqlens_q || !a->seqlens_k || !a->block_table ||
+        !a->q != !a->q_out)
+        return false;
+    if (a->batch < 1 || a->batch > MAX_BATCH || a->heads < 1 || a->kv_heads < 1 || a->total_q < 1 ||
+        a->num_pages < 1 || a->page_size < 1 || a->max_pages_per_seq < 1 || a->rotary_dim < 0 ||
+        a->rotary_dim > fav4::D || a->rotary_dim % 16 || (a->interleaved != 0 && a->interleaved != 1))
+        return false;
+    if (a->rotary_dim > 0 ? !a->cos || !a->sin || a->rotary_rows < 1 : a->cos || a->sin) return false;
+    const int64_t rows = (a->q ? int64_t(a->heads) : 0) + 2 * int64_t(a->kv_heads);
+    if (rows > INT_MAX || rows * a->total_q > INT_MAX) return false;
+    if (!stride_ok(a->k_stride, a->kv_heads, a->total_q) || !stride_ok(a->v_stride, a->kv_heads, a->total_q)) return false;
+    if (a->q && (!stride_ok(a->q_stride, a->heads, a->total_q) || !stride_ok(a->q_out_stride, a->heads, a->total_q) ||
+                 (a->q == a->q_out && a->q_stride != a->q_out_stride)))
+        return false;
+    return caches_fit(a->num_pages, a->page_size, a->kv_heads) &&
+           aligned(16, a->q, a->k, a->v, a->q_out, a->k_cache, a->v_cache, a->cos, a->sin) &&
+           aligned(4, a->cu_seqlens_q, a->seqlens_k, a->block_table, a->positions);
+}
+
+bool gather_ok(const Fav4Mx4GatherArgs* a) {
+    if (!a || !a->k_cache || !a->k_scales || !a->v_cache || !a->v_scales || !a->k || !a->v || !a->cu_seqlens_k ||
+        !a->block_table)
+        return false;
+    if (a->batch < 1 || a->batch > MAX_BATCH || a->kv_heads < 1 || a->total_k < 1 || a->num_pages < 1 ||
+        a->page_size < 1 || a->max_pages_per_seq < 1 || 2 * int64_t(a->kv_heads) * a->total_k > INT_MAX)
+        return false;
+    return stride_ok(a->k_stride, a->kv_heads, a->total_k) && stride_ok(a->v_stride, a->kv_heads, a->total_k) &&
+           caches_fit(a->num_pages, a->page_size, a->kv_heads) &&
+           aligned(16, a->k_cache, a->k_scales, a->v_cache, a->v_scales, a->k, a->v) &&
+           aligned(4, a->cu_seqlens_k, a->starts, a->block_table);
+}
+
+// ---- attention -------------------------------------------------------------------
+bool paged_shape_ok(const Fav4Mx4PagedArgs* args, int causal) {
+    if (!args) return false;
+    const Fav4PagedArgs& a = args->paged;
+    if (a.batch < 1 || a.heads < 1 || a.kv_heads < 1 || a.heads % a.kv_heads || a.max_seqlen_q < 1 ||
+        a.max_seqlen_k < 1 || a.total_q < 1 || a.total_k < 0 || a.num_pages < 1 || a.page_size < 1 ||
+        a.max_pages_per_seq < 1 || (causal != 0 && causal != BOTTOM_RIGHT) || !std::isfinite(a.scale) || a.scale <= 0)
+        return false;
+    return a.page_size % 16 == 0 && a.max_seqlen_k <= int64_t(a.max_pages_per_seq) * a.page_size &&
+           (int64_t(a.max_seqlen_k) + a.page_size - 1) / a.page_size <= MAX_KEYS / a.page_size && a.heads <= MAX_HEADS &&
+           int64_t(a.total_q) * a.heads <= INT_MAX && caches_fit(a.num_pages, a.page_size, a.kv_heads);
+}
+
+// Up to this many rows a sequence go by the decode kernel.
+constexpr int FEW_ROWS = 64;
+// Most parts' rows of a prefill call over all heads: parts are made where the row tiles
+// are fewer than two for each CU, up to that many.
+constexpr int64_t PREFILL_PART_TILES = 1024;
+
+struct Sizes {
+    fav4::Mx4Plan plan;
+    int64_t bytes, grid;
+    bool few, split;
+    bool ok;
+};
+Sizes paged_sizes(const Fav4Mx4PagedArgs& args, int causal) {
+    const Fav4PagedArgs& a = args.paged;
+    const int64_t group = a.heads / a.kv_heads, rows = a.total_q * group;
+    const int64_t seq_rows = std::min<int64_t>(a.max_seqlen_q * group, rows);
+    const int cus = device_cus();
+    Sizes s{};
+    fav4::Mx4Plan& p = s.plan;
+    p.group = int(group);
+    p.br = causal == BOTTOM_RIGHT;
+    s.few = seq_rows <= FEW_ROWS;
+    const int64_t ranges = std::max<int64_t>(1, 2 * cus / a.kv_heads);
+    if (s.few) {
+        p.stride = seq_rows <= 16 ? 16 : 32;
+        p.tiles = int((seq_rows + p.stride - 1) / p.stride);
+        const int64_t segs = int64_t(a.batch) * p.tiles;
+        s.split = segs * a.kv_heads < 4 * cus && a.max_seqlen_k > 2048;
+        p.ranges = s.split ? int(ranges) : 1;
+        p.blocks = int(std::min<int64_t>(std::min(segs, (rows + int64_t(a.batch) * (p.stride - 1)) / p.stride) + ranges, INT_MAX));
+        s.grid = a.kv_heads * (s.split ? ranges : segs);
+        s.ok = segs * (int64_t(a.max_seqlen_k) / 64 + 1 + fav4::MX4_LEAD) < (1 << 30) && s.grid < (int64_t(1) << 30) &&
+               int64_t(p.blocks) * p.stride <= INT_MAX;
+    } else {
+        const int64_t tiles = std::min<int64_t>(a.batch * ((seq_rows + fav4::MX4_BM - 1) / fav4::MX4_BM),
+                                                (rows + int64_t(a.batch) * (fav4::MX4_BM - 1)) / fav4::MX4_BM);
+        const int64_t all = tiles * a.kv_heads;
+        const int64_t parts = std::min<int64_t>(std::max<int64_t>(1, 2 * cus / all), std::max(1, a.max_seqlen_k / 256));
+        p.tiles = int(std::min<int64_t>(tiles, INT_MAX));
+        p.ranges = int(parts);
+        s.split = parts > 1;
+        p.stride = fav4::MX4_BM;
+        p.blocks = int(std::min<int64_t>(tiles * parts, INT_MAX));
+        s.grid = all * parts;
+        s.ok = tiles <= MAX_ROW_TILES && all <= MAX_ROW_TILES && (!s.split || s.grid <= PREFILL_PART_TILES);
+    }
+    p.by_kv_heads = fav4::fast_div(a.kv_heads);
+    p.by_group = fav4::fast_div(int(group));
+    p.by_page = fav4::fast_div(a.page_size);
+    p.by_heads = fav4::fast_div(a.heads);
+    p.by_stride = fav4::fast_div(p.stride);
+    // What a call of either kind could need: more queries or sequences never need less.
+    const int64_t few_rows = a.kv_heads * (std::min<int64_t>(rows, int64_t(a.batch) * FEW_ROWS) + (int64_t(a.batch) + ranges) * 32);
+    const int64_t many_rows = s.few ? 0 : PREFILL_PART_TILES * fav4::MX4_BM;
+    const int64_t part_rows = (few_rows + many_rows + 1) & ~int64_t(1);
+    s.ok = s.ok && (!s.split || int64_t(a.kv_heads) * p.blocks * p.stride <= part_rows) && part_rows < (int64_t(1) << 40);
+    s.bytes = part_rows * (fav4::D * 4 + 8) + rows * 8;
+    return s;
+}
+
+template <int NT>
+void launch_few(const Fav4Mx4PagedArgs& a, const Sizes& s, hipStream_t stream) {
+    auto go = [&](auto kernel, int waves) {
+        hipLaunchKernelGGL(kernel, dim3(unsigned(s.grid)), dim3(waves * 64), 0, stream, a, s.plan);
+    };
+    if (s.split) go(fav4::mx4_decode_kernel<NT, 4, true>, 4);
+    else go(fav4::mx4_decode_kernel<NT, 8, false>, 8);
+}
+
+}  // namespace
+
+extern "C" __attribute__((visibility("default"))) int fav4_bshd_append_paged_mx4(const Fav4Mx4AppendArgs* args,
+                                                                                hipStream_t stream) {
+    if (!append_ok(args)) return hipErrorInvalidValue;
+    const Fav4AppendArgs& a = args->append;
+    const int rows = (a.q ? a.heads : 0) + 2 * a.kv_heads, units = (rows + 7) / 8;
+    const int64_t total = int64_t(units) * a.total_q, blocks = std::min((total + 3) / 4, MAX_GRID);
+    const fav4::FastDiv by_units = fav4::fast_div(units), by_page = fav4::fast_div(a.page_size);
+    auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(unsigned(blocks)), dim3(256), 0, stream, *args, units, total, by_units, by_page);
+    };
+    if (a.interleaved) go(fav4::mx4_store_kernel<true>);
+    else go(fav4::mx4_store_kernel<false>);
+    return hipGetLastError();
+}
+
+extern "C" __attribute__((visibility("default"))) int fav4_bshd_gather_paged_mx4(const Fav4Mx4GatherArgs* a,
+                                                                                hipStream_t stream) {
+    if (!gather_ok(a)) return hipErrorInvalidValue;
+    const int64_t per = 4 * fav4::MX4_READ_ROWS, blocks = std::min((a->total_k + per - 1) / per, MAX_GRID);
+    hipLaunchKernelGGL(fav4::mx4_read_kernel, dim3(unsigned(blocks)), dim3(256), 0, stream, *a, fav4::fast_div(a->page_size));
+    return hipGetLastError();
+}
+
+extern "C" __attribute__((visibility("default"))) long long fav4_bshd_paged_mx4_workspace_size(
+    const Fav4Mx4PagedArgs* args, int causal) {
+    if (!paged_shape_ok(args, causal)) return -1;
+    const Sizes s = paged_sizes(*args, causal);
+    return s.ok ? s.bytes : -1;
+}
+
+extern "C" __attribute__((visibility("default"))) int fav4_bshd_forward_paged_mx4(const Fav4Mx4PagedArgs* args,
+                                                                                 int causal, void* workspace,
+                                                                                 size_t workspace_bytes,
+                                                                                 hipStream_t stream) {
+    if (!paged_shape_ok(args, causal)) return hipErrorInvalidValue;
+    const Fav4PagedArgs& a = args->paged;
+    if (!a.q || !a.k_cache || !a.v_cache || !a.o || !a.cu_seqlens_q || !a.seqlens_k || !a.block_table ||
+        !args->k_scales || !args->v_scales ||
+        !aligned(16, a.q, a.k_cache, a.v_cache, a.o, args->k_scales, args->v_scales) ||
+        !aligned(4, a.lse, a.cu_seqlens_q, a.seqlens_k, a.block_table))
+        return hipErrorInvalidValue;
+    Sizes s = paged_sizes(*args, causal);
+    if (!s.ok || !workspace || !aligned(256, workspace) || uint64_t(s.bytes) > workspace_bytes)
+        return hipErrorInvalidValue;
+    fav4::Mx4Plan& p = s.plan;
+    const int64_t part_rows = s.split ? (int64_t(a.kv_heads) * p.blocks * p.stride + 1) & ~int64_t(1) : 0;
+    p.o_part = static_cast<float*>(workspace);
+    p.lse_part = p.o_part + part_rows * fav4::D;
+    p.notes = reinterpret_cast<int2*>(p.lse_part + part_rows * 2);
+    if (s.few) {
+        if (p.stride == 16) launch_few<1>(*args, s, stream);
+        else launch_few<2>(*args, s, stream);
+    } else {
+        auto go = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3(unsigned(s.grid)), dim3(512), 0, stream, *args, p);
+        };
+        if (a.lse) s.split ? go(fav4::mx4_prefill_kernel<true, true>) : go(fav4::mx4_prefill_kernel<true, false>);
+        else s.split ? go(fav4::mx4_prefill_kernel<false, true>) : go(fav4::mx4_prefill_kernel<false, false>);
+    }
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || !s.split) return e;
+    const int64_t rows = int64_t(a.total_q) * a.heads;
+    constexpr int per = 4;
+    hipLaunchKernelGGL(fav4::mx4_merge_kernel<per>, dim3(unsigned(std::min((rows * per + 15) / 16, MAX_GRID))), dim3(256), 0,
+                       stream, *args, p);
+    return hipGetLastError();
+}

@@ -1,0 +1,853 @@
+// Kernels of the operators of 4-bit (MXFP4) paged K/V caches: storing new tokens,
+// reading rows back, and attention.
+#pragma once
+#include "fav4_mx4.h"
+#include "serving_kernel.hpp"
+
+namespace fav4 {
+
+constexpr int MX4_CODES = D / 2, MX4_SCALES = D / 32;      // bytes of a cache row
+
+__device__ __forceinline__ float mx4_scale(uint32_t byte) { return __uint_as_float(byte << 23); }
+
+// Eight numbers (one dword of codes) times their block's scale: exact in BF16.
+__device__ __forceinline__ bf16x8 mx4_values(uint32_t codes, float scale) {
+    const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 0);
+    const bf16x2 b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 1);
+    const bf16x2 c = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 2);
+    const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, 3);
+    return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+// Whether one of four bytes is 255.
+__device__ __forceinline__ bool mx4_has_255(uint32_t x) { return ((~x - 0x01010101u) & x & 0x80808080u) != 0; }
+
+// ---------------------------------------------------------------------------
+// Append.  The layout of append_kernel: one wave takes 8 of a token's heads + 2 *
+// kv_heads rows (Q, then K, then V), 8 lanes a row, each with the two 16-byte
+// granules whose dims are rotated together.  The four granules of a block of 32 dims
+// then lie in up to four lanes, so the granules' largest magnitudes go through LDS
+// (as bits, whose order is that of the magnitudes, infinities and NaN above them) and
+// each lane reads its blocks' four.  Bound by memory, for few tokens by the chain of
+// dependent loads.
+// ---------------------------------------------------------------------------
+// The block's scale byte (255: not all numbers are finite) from its largest
+// magnitude's bits: the smallest e with max <= 1.75 * 2^(e + 2), i.e. the exponent,
+// one more where the mantissa is above 0.75.
+__device__ __forceinline__ int mx4_block_scale(u32x4 most) {
+    const uint32_t m = max(max(most[0], most[1]), max(most[2], most[3]));
+    return m >= 0x7f800000u ? 255 : min(max(int((m + 0x1fffffu) >> 23) - 2, 2), 252);
+}
+__device__ __forceinline__ uint32_t mx4_codes(const float (&x)[8], int scale) {
+    const float inv = __uint_as_float(uint32_t(254 - scale) << 23);
+    uint32_t c = 0;
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[0] * inv, x[1] * inv, 1.f, 0);
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[2] * inv, x[3] * inv, 1.f, 1);
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[4] * inv, x[5] * inv, 1.f, 2);
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[6] * inv, x[7] * inv, 1.f, 3);
+    return scale == 255 ? 0 : c;
+}
+
+// Products and sums rounded one by one: what is quantised does not depend on which of
+// them the compiler would fuse.
+__device__ __forceinline__ void mx4_turn(float& p, float& q, float c, float s) {
+#pragma clang fp contract(off)
+    const float u = p * c - q * s, w = q * c + p * s;
+    p = u;
+    q = w;
+}
+
+template <bool INTERLEAVED>
+__global__ __launch_bounds__(256) void mx4_store_kernel(Fav4Mx4AppendArgs args, int units, int64_t total,
+                                                        FastDiv by_units, FastDiv by_page) {
+    __shared__ __attribute__((aligned(16))) uint32_t most[4][8][16];
+    const Fav4AppendArgs& a = args.append;
+    const int lane = threadIdx.x & 63, j = lane & 7, wave = uniform(threadIdx.x >> 6);
+    const int64_t stride = int64_t(gridDim.x) * 4;
+    const int qheads = a.q ? a.heads : 0, rows = qheads + 2 * a.kv_heads;
+    const int half = a.rotary_dim >> 4;                    // granules of half the rotated dims
+    const int first = a.cu_seqlens_q[0], end = a.cu_seqlens_q[a.batch];
+    for (int64_t id = int64_t(blockIdx.x) * 4 + wave; id < total; id += stride) {
+        const int t = uniform(by_units(int(id))), unit = uniform(int(id) - t * units);
+        if (t < first || t >= end) continue;               // in no sequence
+        const int row = unit * 8 + (lane >> 3);
+        const bool live = row < rows, is_q = row < qheads, is_v = row >= qheads + a.kv_heads;
+        const int head = is_q ? row : is_v ? row - qheads - a.kv_heads : row - qheads;
+        const char* src = static_cast<const char*>(is_q ? a.q : is_v ? a.v : a.k);
+        src += (int64_t(t) * (is_q ? a.q_stride : is_v ? a.v_stride : a.k_stride) + int64_t(head) * D) * 2;
+        // This lane's granules of the row.
+        const bool turn = j < half && !is_v;
+        const int g0 = INTERLEAVED || !turn ? 2 * j : j;
+        const int g1 = INTERLEAVED || !turn ? g0 + 1 : j + half;
+        bf16x8 bx{}, by{};
+        if (live) {
+            bx = *reinterpret_cast<const bf16x8*>(src + g0 * 16);
+            by = *reinterpret_cast<const bf16x8*>(src + g1 * 16);
+        }
+        const int b = wave_find(a.cu_seqlens_q, a.batch, t, lane);     // below batch: the last offset is above t
+        const int64_t slot = int64_t(a.seqlens_k[b]) - a.cu_seqlens_q[b + 1] + t;
+        int page = -1, in_page = 0;
+        if (slot >= 0 && slot < int64_t(a.max_pages_per_seq) * a.page_size && slot <= INT_MAX) {
+            const int at = by_page(int(slot));
+            in_page = int(slot) - at * a.page_size;
+            page = a.block_table[int64_t(b) * a.max_pages_per_seq + at];
+        }
+        const bool stored = page >= 0 && page < a.num_pages;
+        float x[8], y[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = float(bx[i]), y[i] = float(by[i]);
+        if (turn && live) {
+            const int64_t pos = a.positions ? int64_t(a.positions[t]) : slot;
+            const int64_t r = min(max(pos, int64_t(0)), int64_t(a.rotary_rows - 1));
+            const int64_t at = r * (half * 8) + j * 8;
+            const f32x4* cp = reinterpret_cast<const f32x4*>(a.cos + at);
+            const f32x4* sp = reinterpret_cast<const f32x4*>(a.sin + at);
+            const f32x4 c[2] = {cp[0], cp[1]}, s[2] = {sp[0], sp[1]};
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float ci = c[i >> 2][i & 3], si = s[i >> 2][i & 3];
+                float& p = INTERLEAVED ? (i < 4 ? x : y)[2 * (i & 3)] : x[i];
+                float& q = INTERLEAVED ? (i < 4 ? x : y)[2 * (i & 3) + 1] : y[i];
+                mx4_turn(p, q, ci, si);
+            }
+        }
+        if (is_q && live) {
+            char* dst = static_cast<char*>(a.q_out) + (int64_t(t) * a.q_out_stride + int64_t(head) * D) * 2;
+            bf16x8 u, w;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) u[i] = __bf16(x[i]), w[i] = __bf16(y[i]);
+            *reinterpret_cast<bf16x8*>(dst + g0 * 16) = u;
+            *reinterpret_cast<bf16x8*>(dst + g1 * 16) = w;
+        }
+        if (is_q || !live || !stored) continue;
+        // The granules' largest magnitudes; the blocks' scales.  (A row's eight lanes
+        // are here together; LDS takes a wave's accesses in order.)
+        uint32_t m0 = 0, m1 = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            m0 = max(m0, __float_as_uint(x[i]) & 0x7fffffffu);
+            m1 = max(m1, __float_as_uint(y[i]) & 0x7fffffffu);
+        }
+        uint32_t* mine = most[wave][lane >> 3];
+        mine[g0] = m0;
+        mine[g1] = m1;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        const u32x4* blocks = reinterpret_cast<const u32x4*>(mine);
+        const int s0 = mx4_block_scale(blocks[g0 >> 2]), s1 = mx4_block_scale(blocks[g1 >> 2]);
+        const int own = mx4_block_scale(blocks[j & 3]);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        const int64_t at = (int64_t(page) * a.kv_heads + head) * a.page_size + in_page;
+        char* codes = static_cast<char*>(is_v ? a.v_cache : a.k_cache) + at * MX4_CODES;
+        *reinterpret_cast<uint32_t*>(codes + g0 * 4) = mx4_codes(x, s0);
+        *reinterpret_cast<uint32_t*>(codes + g1 * 4) = mx4_codes(y, s1);
+        if (j < 4) static_cast<uint8_t*>(is_v ? args.v_scales : args.k_scales)[at * MX4_SCALES + j] = uint8_t(own);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Reading back.  One wave takes 8 neighbouring rows (tokens): their sequences by one
+// search and one look at the offsets behind it, their places in the caches in the
+// wave's lanes, then K and V, 16 lanes a head's row (4 bytes of codes, 16 of BF16).
+// Bound by memory: 256 of 324 bytes are written.
+// ---------------------------------------------------------------------------
+constexpr int MX4_READ_ROWS = 8;
+__global__ __launch_bounds__(256) void mx4_read_kernel(Fav4Mx4GatherArgs a, FastDiv by_page) {
+    const int lane = threadIdx.x & 63, sub = lane >> 4, l16 = lane & 15;
+    const int first = max(a.cu_seqlens_k[0], 0), end = min(a.cu_seqlens_k[a.batch], a.total_k);
+    const int64_t step = int64_t(gridDim.x) * 4 * MX4_READ_ROWS;
+    for (int64_t at = (int64_t(blockIdx.x) * 4 + uniform(threadIdx.x >> 6)) * MX4_READ_ROWS; at < end; at += step) {
+        const int t0 = max(int(at), first), n = uniform(min(int(at) + MX4_READ_ROWS, end) - t0);
+        if (n <= 0) continue;
+        // Lane i: the sequence of row t0 + i, and its row of the caches (-1: in no page).
+        const int b0 = wave_find(a.cu_seqlens_k, a.batch, t0, lane);
+        const int next = a.cu_seqlens_k[min(b0 + 1 + lane, a.batch)];
+        int b = b0;
+        for (int i = 0; i < n; ++i) {
+            const uint64_t past = __builtin_amdgcn_ballot_w64(b0 + 1 + lane <= a.batch && next <= t0 + i);
+            const int here = past == ~0ull ? wave_find(a.cu_seqlens_k, a.batch, t0 + i, lane)
+                                           : b0 + __builtin_popcountll(past);
+            if (lane == i) b = here;
+        }
+        int64_t place = -1;
+        if (lane < n && b < a.batch) {
+            const int64_t slot = int64_t(t0) + lane - a.cu_seqlens_k[b] + (a.starts ? a.starts[b] : 0);
+            if (slot >= 0 && slot < int64_t(a.max_pages_per_seq) * a.page_size && slot <= INT_MAX) {
+                const int entry = by_page(int(slot));
+                const int page = a.block_table[int64_t(b) * a.max_pages_per_seq + entry];
+                if (page >= 0 && page < a.num_pages)
+                    place = int64_t(page) * a.kv_heads * a.page_size + (int(slot) - entry * a.page_size);
+            }
+        }
+        const int lo = int(place), hi = int(place >> 32);
+        const int rows = 2 * a.kv_heads, per = (rows + 3) >> 2;        // groups of four rows a token
+        for (int i = 0; i < n; ++i) {
+            const int64_t base = int64_t(uint32_t(__builtin_amdgcn_readlane(lo, i))) |
+                                 int64_t(__builtin_amdgcn_readlane(hi, i)) << 32;
+#pragma unroll 4
+            for (int u = 0; u < per; ++u) {
+                const int row = u * 4 + sub;
+                if (row >= rows) continue;
+                const bool is_v = row >= a.kv_heads;
+                const int head = is_v ? row - a.kv_heads : row;
+                bf16x8 x{};
+                if (base >= 0) {
+                    const int64_t r = base + int64_t(head) * a.page_size;
+                    const uint32_t codes = reinterpret_cast<const uint32_t*>(
+                        static_cast<const char*>(is_v ? a.v_cache : a.k_cache) + r * MX4_CODES)[l16];
+                    const uint32_t s = static_cast<const uint8_t*>(is_v ? a.v_scales : a.k_scales)[r * MX4_SCALES + (l16 >> 2)];
+                    x = mx4_values(codes, mx4_scale(s));
+                }
+                char* dst = static_cast<char*>(is_v ? a.v : a.k) +
+                            (int64_t(t0 + i) * (is_v ? a.v_stride : a.k_stride) + int64_t(head) * D) * 2;
+                *reinterpret_cast<bf16x8*>(dst + l16 * 16) = x;
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Attention.  Rows are (token, query head of the K/V head's group), r = token *
+// group + head.  Sequences of up to 64 rows (decode, drafts) go by mx4_decode_kernel,
+// longer ones by mx4_prefill_kernel.
+// ---------------------------------------------------------------------------
+struct Mx4Plan {
+    float *o_part, *lse_part;         // partial blocks of all K/V heads: `blocks` of `stride` rows each
+    int2* notes;                      // [total_q * group]: first partial row of a head's row, and parts
+    int group;                        // query heads of a K/V head
+    int ranges;                       // decode: workgroups of a K/V head; prefill: parts of a row tile's keys
+    FastDiv by_kv_heads, by_group, by_page, by_heads, by_stride;
+    int blocks, stride;
+    int tiles;                        // prefill: row tiles that the batch can have
+    int br;                           // bottom-right causal
+};
+
+// A sequence as read on the device, clamped.
+struct Mx4Seq {
+    int t0, tokens, keys;
+};
+__device__ __forceinline__ Mx4Seq mx4_seq(const Fav4PagedArgs& pg, int b) {
+    const int t0 = min(max(pg.cu_seqlens_q[b], 0), pg.total_q), t1 = min(max(pg.cu_seqlens_q[b + 1], 0), pg.total_q);
+    return {t0, min(max(t1 - t0, 0), pg.max_seqlen_q), min(max(pg.seqlens_k[b], 0), pg.max_seqlen_k)};
+}
+
+// A sequence's pages, 64 entries of the table in the wave's lanes.
+struct Mx4Pages {
+    const int* table;
+    int entries, num_pages, page_size, slot0, pages;
+    int64_t page_rows, head_row;      // cache rows of a page, and of the head within it
+    __device__ __forceinline__ void load(int slot, int lane) {
+        slot0 = slot;
+        pages = min(max(table[min(slot + lane, entries - 1)], 0), num_pages - 1);
+    }
+    // The cache row of a key (keys in ascending order).
+    __device__ __forceinline__ int64_t row(int key, const FastDiv& by_page, int lane) {
+        const int slot = uniform(by_page(key));
+        if (slot - slot0 >= 64) load(slot, lane);
+        const int page = __builtin_amdgcn_readlane(pages, slot - slot0);
+        return page * page_rows + head_row + (key - slot * page_size);
+    }
+};
+__device__ __forceinline__ Mx4Pages mx4_pages(const Fav4PagedArgs& pg, int b, int kvh, int key, const FastDiv& by_page,
+                                              int lane) {
+    Mx4Pages p{pg.block_table + int64_t(b) * pg.max_pages_per_seq, pg.max_pages_per_seq, pg.num_pages, pg.page_size};
+    p.page_rows = int64_t(pg.kv_heads) * pg.page_size;
+    p.head_row = int64_t(kvh) * pg.page_size;
+    p.load(uniform(by_page(key)), lane);
+    return p;
+}
+
+__device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+// Over the four lanes that hold one row (l, l ^ 16, l ^ 32, l ^ 48).
+__device__ __forceinline__ float quad_max(float x) {
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return xhalf_max(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+__device__ __forceinline__ float quad_sum(float x) {
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return xhalf_sum(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+
+// ---- Few rows ---------------------------------------------------------------------
+// A workgroup's waves all take the same NT * 16 rows, and every WAVES-th tile of 64
+// keys of a part of the keys; they join in LDS.  Per tile a wave loads 4 KiB of codes of
+// K and of V and 256 bytes of scales of each, straight into registers and a tile ahead.
+//  * S^T = K Q^T on 16x16x32 MFMAs: lane l has key l % 16 of a subtile and the block
+//    of 32 dims l / 16, 16 bytes of codes and one scale; the four dwords of codes are
+//    the four k-steps, whose order over the dims is free as long as Q's is the same.
+//  * O^T += V^T P^T: P leaves the accumulators as the B operand, lane l / 16 = g
+//    holding keys 4g + e of both subtiles of 32 keys.  V is converted as K is and goes
+//    through 8 KiB of LDS of the wave's own, from where ds_read_b64_tr_b16 reads it
+//    turned.  Keys are masked by their scores, so V needs no other care than to be
+//    finite: a block without numbers becomes 0 there, and its key's scores NaN by way of
+//    its K scale.
+template <int NT>
+struct Mx4State {
+    f32x4 o[NT][8];
+    float m[NT], lb[NT], l[NT];       // base (log2), sums of the BF16 and the FP32 weights of this lane's keys
+};
+struct Mx4Tile {
+    u32x4 k[4], v[4];
+    uint32_t ks[4], vs[4];
+};
+
+template <int NT, int WAVES>
+struct Mx4Decode {
+    static constexpr int SLOT = 32 * ROW_BYTES, BM = NT * 16;
+    const Fav4Mx4PagedArgs& a;
+    const Mx4Plan& pl;
+    unsigned char* smem;              // WAVES slots
+    float4 (*stats)[16];              // [WAVES][16]
+    int lane, wave;
+
+    // The cache rows of a tile's subtiles; those past the keys repeat the last one, and are masked.
+    __device__ __forceinline__ void rows(int64_t (&row)[4], int t, int keys, Mx4Pages& pages) const {
+        const int last = (keys - 1) & ~15;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) row[i] = pages.row(min(t * 64 + i * 16, last), pl.by_page, lane);
+    }
+    __device__ __forceinline__ void load_k(Mx4Tile& x, int i, int64_t row) const {
+        const char* k = static_cast<const char*>(a.paged.k_cache) + row * MX4_CODES;
+        const char* ks = static_cast<const char*>(a.k_scales) + row * MX4_SCALES;
+        const char* vs = static_cast<const char*>(a.v_scales) + row * MX4_SCALES;
+        const uint32_t at = uint32_t(lane & 15), g = uint32_t(lane >> 4);
+        x.k[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(k + at * MX4_CODES + g * 16));
+        x.ks[i] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(ks + at * MX4_SCALES));
+        x.vs[i] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(vs + at * MX4_SCALES));
+    }
+    __device__ __forceinline__ void load_v(Mx4Tile& x, int i, int64_t row) const {
+        const char* v = static_cast<const char*>(a.paged.v_cache) + row * MX4_CODES;
+        x.v[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(v + (lane & 15) * MX4_CODES + (lane >> 4) * 16));
+    }
+
+    // Tile t, in x; the tile at `next` (if any) is loaded in its place, each register as soon as it has been used.
+    __device__ __forceinline__ void tile(Mx4Tile& x, const bf16x8 (&q)[NT][4], Mx4State<NT>& st, bool first, int t,
+                                         int next, bool masked, int keys, const int (&lim)[NT], float scale2,
+                                         Mx4Pages& pages) const {
+        const int col = lane & 15, g = lane >> 4, start = t * 64;
+        uint32_t vb[4];
+        f32x4 s[NT][4];
+        int64_t row[4];
+        if (next >= 0) rows(row, next, keys, pages);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uint32_t ks = x.ks[i], vs = x.vs[i];
+            if (masked) {
+                const bool in = start + i * 16 + col < keys;
+                ks = in ? ks : 0, vs = in ? vs : 0;
+            }
+            const uint32_t kb = mx4_has_255(vs) ? 255u : ks >> (8 * g) & 255u;
+            vb[i] = vs >> (8 * g) & 255u;
+            const float scale = mx4_scale(kb);
+            bf16x8 kop[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) kop[c] = mx4_values(x.k[i][c], scale);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                s[n][i] = f32x4{};
+#pragma unroll
+                for (int c = 0; c < 4; ++c) s[n][i] = mfma16(kop[c], q[n][c], s[n][i]);
+            }
+        }
+        if (next >= 0) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) load_k(x, i, row[i]);
+        }
+        bf16x8 p[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            if (masked) {
+                const int d = lim[n] - start - 4 * g;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[n][i][e] = i * 16 + e > d ? -__builtin_inff() : s[n][i][e];
+            }
+            float mx = -__builtin_inff();
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) mx = fmaxf(mx, s[n][i][e]);
+            // The base moves where a maximum passes it by more than the threshold.
+            const float cand = fmaxf(st.m[n], quad_max(mx) * scale2);
+            const bool update = first || cand > st.m[n] + RESCALE_THRESHOLD;
+            const float now = update ? cand : st.m[n];
+            const float base = now == -__builtin_inff() ? 0.f : now;        // rows that have seen no key
+            const float alpha = exp2_native(st.m[n] - base);
+            const bool rescale = !first && __builtin_amdgcn_ballot_w64(update) != 0;
+            st.m[n] = now;
+            float lb = 0.f, l = 0.f;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float w = exp2_native(fmaf(s[n][2 * h + (j >> 2)][j & 3], scale2, -base));
+                    l += w;
+                    p[n][h][j] = __bf16(w);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) lb = bf16_pair_sum(bf16x2{p[n][h][2 * j], p[n][h][2 * j + 1]}, lb);
+            }
+            if (rescale) {
+#pragma unroll
+                for (int db = 0; db < 8; ++db) st.o[n][db] *= alpha;
+            }
+            st.lb[n] = first ? lb : st.lb[n] * alpha + lb;
+            st.l[n] = first ? l : st.l[n] * alpha + l;
+        }
+        // V, 32 keys at a time: row r's granule c at c ^ v_swz(r).
+        unsigned char* slot = smem + wave * SLOT;
+        const int r = lane >> 2 & 3;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint32_t byte = vb[2 * h + i];
+                const float scale = mx4_scale(byte == 255u ? 0u : byte);
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const uint32_t codes = byte == 255u ? 0u : x.v[2 * h + i][c];
+                    *reinterpret_cast<FAV4_LDS bf16x8*>((FAV4_LDS void*)(
+                        slot + (i * 16 + col) * ROW_BYTES + (((4 * g + c) ^ v_swz(col)) << 4))) = mx4_values(codes, scale);
+                }
+            }
+            if (next >= 0) load_v(x, 2 * h, row[2 * h]), load_v(x, 2 * h + 1, row[2 * h + 1]);
+#pragma unroll
+            for (int db = 0; db < 8; ++db) {
+                const int vr = 4 * g + r, c = 2 * db + (lane >> 1 & 1);
+                const unsigned char* at = slot + vr * ROW_BYTES + ((c ^ v_swz(vr)) << 4) + ((lane & 1) << 3);
+                const bf16x4 lo = lds_read_tr(at), hi = lds_read_tr(at + 16 * ROW_BYTES);
+                const bf16x8 vop{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+#pragma unroll
+                for (int n = 0; n < NT; ++n) st.o[n][db] = mfma16(vop, p[n][h], st.o[n][db]);
+            }
+        }
+    }
+
+    // Key tiles [a0, a1) of the rows from r0 on of sequence b with head kvh.  split: the part is not all of the
+    // sequence's keys, and goes to partial block `block`.
+    __device__ __forceinline__ void attend(int b, const Mx4Seq& f, int r0, int kvh, int a0, int a1, bool split,
+                                           int block) const {
+        const Fav4PagedArgs& pg = a.paged;
+        const int col = lane & 15, g = lane >> 4, group = pl.group, rows = f.tokens * group;
+        const float scale2 = pg.scale * LOG2E;
+        int lim[NT];
+        bf16x8 q[NT][4];
+        Mx4State<NT> st;
+        const int shift = f.keys - f.tokens;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const int row = min(r0 + n * 16 + col, rows - 1), token = pl.by_group(row), head = kvh * group + row - token * group;
+            lim[n] = pl.br ? min(shift + token, f.keys - 1) : f.keys - 1;
+            const char* qp = static_cast<const char*>(pg.q) + (int64_t(f.t0 + token) * pg.heads + head) * ROW_BYTES + g * 64;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) q[n][c] = *reinterpret_cast<const bf16x8*>(qp + c * 16);
+#pragma unroll
+            for (int db = 0; db < 8; ++db) st.o[n][db] = f32x4{};
+            st.m[n] = -__builtin_inff();
+            st.lb[n] = st.l[n] = 0.f;
+        }
+        // Tiles whose keys all rows see, and the end of those that some row sees.
+        const int i0 = pl.by_group(r0), i1 = pl.by_group(min(rows, r0 + BM) - 1);
+        const int plain = pl.br ? max(0, min(f.keys, shift + i0 + 1)) : f.keys;
+        const int seen = pl.br ? max(0, min(f.keys, shift + i1 + 1)) : f.keys;
+        const int nfull = uniform(plain >> 6), e1 = uniform(min(a1, (seen + 63) >> 6));
+        int t = a0 + wave;
+        if (t < e1) {
+            Mx4Pages pages = mx4_pages(pg, b, kvh, min(t * 64, (f.keys - 1) & ~15), pl.by_page, lane);
+            Mx4Tile x;
+            int64_t row[4];
+            this->rows(row, t, f.keys, pages);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) load_k(x, i, row[i]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) load_v(x, i, row[i]);
+            for (bool first = true; t < e1; t += WAVES, first = false)
+                tile(x, q, st, first, t, t + WAVES < e1 ? t + WAVES : -1, t >= nfull, f.keys, lim, scale2, pages);
+        }
+        // Join: row n's quad of dims 4u at u ^ n of its 512 bytes.
+        unsigned char* slot = smem + wave * SLOT;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const float lb = quad_sum(st.lb[n]), l = quad_sum(st.l[n]);
+            if (n > 0) __syncthreads();
+#pragma unroll
+            for (int db = 0; db < 8; ++db)
+                *reinterpret_cast<FAV4_LDS f32x4*>((FAV4_LDS void*)(slot + col * 512 + (((db * 4 + g) ^ col) << 4))) = st.o[n][db];
+            if (g == 0) stats[wave][col] = float4{st.m[n], lb, l, 0.f};
+            __syncthreads();
+            for (int id = threadIdx.x; id < 512; id += WAVES * 64) {
+                const int r = id >> 5, u = id & 31, row = r0 + n * 16 + r;
+                if (row >= rows) continue;
+                float m = -__builtin_inff(), sb = 0.f, sl = 0.f;
+#pragma unroll
+                for (int w = 0; w < WAVES; ++w) m = fmaxf(m, stats[w][r].x);
+                const float base = m == -__builtin_inff() ? 0.f : m;
+                f32x4 o{};
+#pragma unroll
+                for (int w = 0; w < WAVES; ++w) {
+                    const float4 v = stats[w][r];
+                    const float weight = exp2_native(v.x - base);
+                    sb += weight * v.y;
+                    sl += weight * v.z;
+                    o += weight * *reinterpret_cast<const FAV4_LDS f32x4*>((FAV4_LDS const void*)(smem + w * SLOT + r * 512 + ((u ^ r) << 4)));
+                }
+                // (No key: 0; sums that are no numbers stay so.)
+                o *= sb == 0.f ? 0.f : 1.f / sb;
+                const int token = pl.by_group(row), head = kvh * group + row - token * group;
+                if (!split) {
+                    const bf16x4 y{__bf16(o[0]), __bf16(o[1]), __bf16(o[2]), __bf16(o[3])};
+                    *reinterpret_cast<bf16x4*>(static_cast<char*>(pg.o) + (int64_t(f.t0 + token) * pg.heads + head) * ROW_BYTES + u * 8) = y;
+                    if (pg.lse && u == 0)
+                        pg.lse[int64_t(head) * pg.total_q + f.t0 + token] = (base + __builtin_amdgcn_logf(sl)) * LN2;
+                } else if (uint32_t(block) < uint32_t(pl.blocks)) {
+                    const int64_t prow = (int64_t(kvh) * pl.blocks + block) * BM + n * 16 + r;
+                    *reinterpret_cast<f32x4*>(pl.o_part + prow * D + u * 4) = o;
+                    if (u == 0)
+                        reinterpret_cast<float2*>(pl.lse_part)[prow] =
+                            float2{base + __builtin_amdgcn_logf(sb), base + __builtin_amdgcn_logf(sl)};
+                }
+            }
+        }
+        __syncthreads();               // read: the next part may use the slots
+    }
+};
+
+// One row tile of a sequence and one K/V head a workgroup (SPLIT false), or the row
+// tiles' key tiles end to end on a line, MX4_LEAD units before each, cut into equal
+// ranges, one a workgroup: row tiles whole in a range are finished there, parts of
+// others go to partial block (row tile + range), unique because both only grow along
+// the line, and are merged by mx4_merge_kernel.
+constexpr int MX4_LEAD = 2;
+template <int NT, int WAVES, bool SPLIT>
+__global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void mx4_decode_kernel(Fav4Mx4PagedArgs a, Mx4Plan pl) {
+    constexpr int BM = NT * 16;
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[WAVES * 32 * ROW_BYTES];
+    __shared__ float4 stats[WAVES][16];
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+    const Fav4PagedArgs& pg = a.paged;
+    const Mx4Decode<NT, WAVES> decode{a, pl, smem, stats, lane, wave};
+    const int w = uniform(pl.by_kv_heads(blockIdx.x)), turn = uniform(int(blockIdx.x) - w * pg.kv_heads);
+    auto uniform_seq = [&](int b) {
+        const Mx4Seq f = mx4_seq(pg, b);
+        return Mx4Seq{uniform(f.t0), uniform(f.tokens), uniform(f.keys)};
+    };
+    if constexpr (!SPLIT) {
+        const int b = pl.tiles > 1 ? udiv(w, pl.tiles) : w, r0 = (w - b * pl.tiles) * BM;
+        const Mx4Seq f = uniform_seq(b);
+        if (r0 < f.tokens * pl.group) decode.attend(b, f, r0, turn, 0, (f.keys + 63) >> 6, false, 0);
+    } else {
+        auto tiles_of = [&](const Mx4Seq& f) { return int(uint32_t(f.tokens * pl.group + BM - 1) / BM); };
+        auto cost_of = [&](const Mx4Seq& f) { return max(1, (f.keys + 63) >> 6) + MX4_LEAD; };
+        // Row tiles and units of 64 sequences from i on, in the lanes.
+        struct Sums {
+            int tiles, cost, tiles_end, cost_end;
+        };
+        auto sums = [&](int i) {
+            Mx4Seq f{};
+            if (i + lane < pg.batch) f = mx4_seq(pg, i + lane);
+            const int n = tiles_of(f), c = n * cost_of(f);
+            return Sums{n, c, wave_scan(n), wave_scan(c)};
+        };
+        const Sums head = sums(0);
+        int units = __builtin_amdgcn_readlane(head.cost_end, 63);
+        for (int i = 64; i < pg.batch; i += 64) units += __builtin_amdgcn_readlane(sums(i).cost_end, 63);
+        const int per = max(udiv_up(units, pl.ranges), 1), g0 = w * per, g1 = g0 + per;
+        // The sequence that holds unit g0, the unit where it starts and the row tiles before it.
+        int idx = 0, base = 0, seg = 0;
+        for (Sums v = head;; v = sums(idx)) {
+            const uint64_t hit = __builtin_amdgcn_ballot_w64(base + v.cost_end > g0);
+            if (hit) {
+                const int l = __builtin_ctzll(hit);
+                idx = uniform(idx + l);
+                base = uniform(base + __builtin_amdgcn_readlane(v.cost_end - v.cost, l));
+                seg = uniform(seg + __builtin_amdgcn_readlane(v.tiles_end - v.tiles, l));
+                break;
+            }
+            base += __builtin_amdgcn_readlane(v.cost_end, 63);
+            seg += __builtin_amdgcn_readlane(v.tiles_end, 63);
+            idx += 64;
+            if (idx >= pg.batch) return;
+        }
+        for (; idx < pg.batch && base < g1; ++idx) {
+            const Mx4Seq f = uniform_seq(idx);
+            const int n = tiles_of(f), cost = cost_of(f), tiles = (f.keys + 63) >> 6;
+            // Neighbouring sequences are taken with neighbouring heads, as in attend_wave.
+            const int kvh = uniform(turn + idx - pl.by_kv_heads(turn + idx) * pg.kv_heads);
+            for (int rt = 0; rt < n; ++rt, ++seg, base += cost) {
+                const int end = base + cost, first = end - max(tiles, 1);      // unit of the first key tile
+                if (first >= g1 || end <= g0) continue;
+                const bool split = first < g0 || end > g1;
+                decode.attend(idx, f, rt * BM, kvh, max(0, g0 - first), min(tiles, g1 - first), split, seg + w);
+                const int row = rt * BM + int(threadIdx.x);
+                if (kvh == 0 && first >= g0 && int(threadIdx.x) < BM && row < f.tokens * pl.group)
+                    pl.notes[int64_t(f.t0) * pl.group + row] =
+                        int2{(seg + w) * BM + int(threadIdx.x), split ? udiv(end - 1, per) - w + 1 : 0};
+            }
+        }
+    }
+}
+
+// ---- Many rows --------------------------------------------------------------------
+// Eight waves of 32 rows each share 64-key tiles of K and V, which they convert to BF16
+// on the way into LDS (two stages): the loop of the forward, attend_fused, behind another
+// source.  A thread has 16 dims of one key: 8 bytes of codes and the key's four scales,
+// loaded two tiles ahead.
+constexpr int MX4_BM = 256;
+template <bool LSE, bool SPLIT>
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void mx4_prefill_kernel(Fav4Mx4PagedArgs a, Mx4Plan pl) {
+    constexpr int BN = 64, TILE_BYTES = BN * ROW_BYTES;
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * TILE_BYTES];
+    const Fav4PagedArgs& pg = a.paged;
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), col = lane & 31, half = lane >> 5;
+    const int group = pl.group;
+    int id = uniform(pl.by_kv_heads(blockIdx.x));
+    const int kvh = uniform(int(blockIdx.x) - id * pg.kv_heads);
+    int part = 0;
+    if constexpr (SPLIT) {
+        part = id / pl.tiles;
+        id -= part * pl.tiles;
+    }
+    // Row tile `id` of the batch: of which sequence.
+    auto tiles_of = [&](const Mx4Seq& f) { return int(uint32_t(f.tokens * group + MX4_BM - 1) / MX4_BM); };
+    int b = 0, before = 0;
+    for (;;) {
+        const int n = b + lane < pg.batch ? tiles_of(mx4_seq(pg, b + lane)) : 0, end = wave_scan(n);
+        const uint64_t hit = __builtin_amdgcn_ballot_w64(before + end > id);
+        if (hit) {
+            const int l = __builtin_ctzll(hit);
+            before = uniform(before + __builtin_amdgcn_readlane(end - n, l));
+            b = uniform(b + l);
+            break;
+        }
+        before += __builtin_amdgcn_readlane(end, 63);
+        b += 64;
+        if (b >= pg.batch) return;
+    }
+    Mx4Seq f = mx4_seq(pg, b);
+    f = {uniform(f.t0), uniform(f.tokens), uniform(f.keys)};
+    const int rows = f.tokens * group, rt = uniform(tiles_of(f)) - 1 - (id - before);      // the longest first
+    const int q0 = rt * MX4_BM, qw = q0 + wave * 32, row = qw + col, srow = min(row, rows - 1);
+    const int token = pl.by_group(srow), head = kvh * group + srow - token * group;
+    const int shift = f.keys - f.tokens, i0 = pl.by_group(q0), i1 = pl.by_group(min(rows, q0 + MX4_BM) - 1);
+    const int plain = uniform(pl.br ? max(0, min(f.keys, shift + i0 + 1)) : f.keys);
+    const int seen = uniform(pl.br ? max(0, min(f.keys, shift + i1 + 1)) : f.keys);
+    const int lim = pl.br ? shift + token : f.keys - 1;
+    const float scale2 = pg.scale * LOG2E;
+    int t = 0, e1 = (seen + BN - 1) / BN;
+    if constexpr (SPLIT) {
+        const int n = e1;
+        t = uniform(int(int64_t(n) * part / pl.ranges));
+        e1 = uniform(int(int64_t(n) * (part + 1) / pl.ranges));
+    }
+    RowState st;
+    clear(st);
+    if (t < e1) {
+        const LdsOffsets off = lds_offsets(lane);
+        bf16x8 qr[8];
+        load_q(pg, f.t0 + token, head, half, qr);
+        const int kr = wave * 8 + (lane >> 3), j = lane & 7;           // this thread's key and 16 dims
+        const int last = (f.keys - 1) & ~7;
+        Mx4Pages pages = mx4_pages(pg, b, kvh, min(t * BN + wave * 8, last), pl.by_page, lane);
+        u32x2 ck, cv;
+        uint32_t ks, vs;
+        auto load = [&](int at) {
+            if (at >= e1) return;
+            const int64_t r = pages.row(min(at * BN + wave * 8, last), pl.by_page, lane);
+            ck = *reinterpret_cast<const u32x2*>(static_cast<const char*>(pg.k_cache) + r * MX4_CODES + lane * 8);
+            cv = *reinterpret_cast<const u32x2*>(static_cast<const char*>(pg.v_cache) + r * MX4_CODES + lane * 8);
+            ks = *reinterpret_cast<const uint32_t*>(static_cast<const char*>(a.k_scales) + r * MX4_SCALES + (lane >> 3) * 4);
+            vs = *reinterpret_cast<const uint32_t*>(static_cast<const char*>(a.v_scales) + r * MX4_SCALES + (lane >> 3) * 4);
+        };
+        const uint32_t k0 = kr * ROW_BYTES + (((2 * j) ^ k_swz(kr)) << 4), k1 = kr * ROW_BYTES + (((2 * j + 1) ^ k_swz(kr)) << 4);
+        const uint32_t v0 = kr * ROW_BYTES + (((2 * j) ^ v_swz(kr)) << 4), v1 = kr * ROW_BYTES + (((2 * j + 1) ^ v_swz(kr)) << 4);
+        auto store = [&](int at, int stage) {
+            if (at >= e1) return;
+            const bool in = at * BN + kr < f.keys;
+            const uint32_t ksc = in ? ks : 0u, vsc = in ? vs : 0u;
+            const uint32_t kb = mx4_has_255(vsc) ? 255u : ksc >> (8 * (j >> 1)) & 255u;
+            const uint32_t byte = vsc >> (8 * (j >> 1)) & 255u;
+            const bool none = !in || byte == 255u;
+            const float sk = mx4_scale(kb), sv = mx4_scale(none ? 0u : byte);
+            unsigned char* k = smem + stage * 2 * TILE_BYTES;
+            unsigned char* v = k + TILE_BYTES;
+            auto put = [](unsigned char* p, bf16x8 x) { *reinterpret_cast<FAV4_LDS bf16x8*>((FAV4_LDS void*)p) = x; };
+            put(k + k0, mx4_values(ck[0], sk));
+            put(k + k1, mx4_values(ck[1], sk));
+            put(v + v0, mx4_values(none ? 0u : cv[0], sv));
+            put(v + v1, mx4_values(none ? 0u : cv[1], sv));
+        };
+        const bool idle = qw >= rows;
+        const int t0 = t;
+        load(t);
+        store(t, 0);
+        load(t + 1);
+        int stage = 0;
+        auto steps = [&](auto masked, int to) {
+            for (; t < to; ++t) {
+                __syncthreads();
+                store(t + 1, stage ^ 1);
+                load(t + 2);
+                const unsigned char* cur = smem + stage * 2 * TILE_BYTES;
+                if (!idle)
+                    attend_fused<BN, decltype(masked)::value, true, LSE, true>(cur, cur + TILE_BYTES, off, qr, st, t == t0,
+                                                                               t * BN, f.keys, lim, half, scale2);
+                stage ^= 1;
+            }
+        };
+        steps(std::integral_constant<bool, false>{}, min(e1, plain / BN));
+        steps(std::integral_constant<bool, true>{}, e1);
+        __syncthreads();               // every wave has read its last tile: the stages may hold O
+    }
+    const int live = min(32, rows - qw);
+    if (live <= 0) return;
+    const float inv = st.lb == 0.f ? 0.f : 1.f / st.lb;
+    const uint32_t slot = wave * 2048;
+    if constexpr (SPLIT) {
+        const int block = id * pl.ranges + part;
+        const int64_t prow = (int64_t(kvh) * pl.blocks + block) * MX4_BM + wave * 32;
+        if (block >= pl.blocks) return;
+        store_part_rows<TILE_BYTES, true>(st, inv, smem, slot, make_rsrc(pl.o_part + prow * D, uint32_t(live) * D * 4), 0,
+                                          live, lane);
+        if (lane < live) {
+            const float sb = st.m + __builtin_amdgcn_logf(st.lb);
+            reinterpret_cast<float2*>(pl.lse_part)[prow + lane] = float2{sb, LSE ? st.m + __builtin_amdgcn_logf(st.l) : sb};
+            if (kvh == 0 && part == 0)
+                pl.notes[int64_t(f.t0) * group + row] = int2{block * MX4_BM + wave * 32 + lane, pl.ranges};
+        }
+    } else {
+        // Through LDS, 32 rows x 128 bytes at a time, so that a store writes whole lines: as store_o_rows, for rows
+        // that lie at any multiple of 256 bytes.
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int dl = 0; dl < 2; ++dl)
+#pragma unroll
+                for (int vg = 0; vg < 4; ++vg) {
+                    const f32x16& o = st.o[2 * h + dl];
+                    const bf16x4 y{__bf16(o[vg * 4] * inv), __bf16(o[vg * 4 + 1] * inv), __bf16(o[vg * 4 + 2] * inv),
+                                   __bf16(o[vg * 4 + 3] * inv)};
+                    const uint32_t at = slot + (col >> 4) * TILE_BYTES + (col & 15) * 128 +
+                                        (((4 * dl + vg) ^ (col & 7)) << 4) + half * 8;
+                    *reinterpret_cast<FAV4_LDS bf16x4*>((FAV4_LDS void*)(smem + at)) = y;
+                }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int r = 8 * i + (lane >> 3), c = lane & 7;
+                const uint32_t at = slot + (r >> 4) * TILE_BYTES + (r & 15) * 128 + ((c ^ (r & 7)) << 4);
+                const bf16x8 y = *reinterpret_cast<const FAV4_LDS bf16x8*>((FAV4_LDS const void*)(smem + at));
+                if (r < live) {
+                    const int tk = pl.by_group(qw + r), hd = kvh * group + qw + r - tk * group;
+                    *reinterpret_cast<bf16x8*>(static_cast<char*>(pg.o) + (int64_t(f.t0 + tk) * pg.heads + hd) * ROW_BYTES +
+                                               h * 128 + c * 16) = y;
+                }
+            }
+        }
+        if (LSE && lane < live)
+            pg.lse[int64_t(head) * pg.total_q + f.t0 + token] =
+                st.lb == 0.f ? -__builtin_inff() : (st.m + __builtin_amdgcn_logf(st.l)) * LN2;
+    }
+}
+
+// ---- Merge --------------------------------------------------------------------------
+// Rows whose keys were split.  PER teams of 16 lanes share one row of one head, 8 dims a
+// lane; a team takes every PER-th part, eight at a time with all their loads in flight,
+// with the running maximum and sums of a softmax over the parts' log-sums.
+template <int PER>
+__global__ __launch_bounds__(256) void mx4_merge_kernel(Fav4Mx4PagedArgs a, Mx4Plan pl) {
+    constexpr int RPB = 16 / PER, NS = PER == 1 ? 4 : 8;
+    __shared__ float4 red[16];
+    __shared__ f32x4 red_o[16][32];
+    const Fav4PagedArgs& pg = a.paged;
+    const int grp = threadIdx.x >> 4, l16 = threadIdx.x & 15;
+    const int slot = grp / PER, part = grp - slot * PER;
+    const uint32_t rows = uint32_t(pg.total_q) * uint32_t(pg.heads), blocks = (rows + RPB - 1) / RPB;
+    for (uint32_t blk = blockIdx.x; blk < blocks; blk += gridDim.x) {
+        const uint32_t r = blk * RPB + slot;                   // token * heads + head
+        const int tok = pl.by_heads(int(min(r, rows - 1))), head = int(min(r, rows - 1) - uint32_t(tok) * uint32_t(pg.heads));
+        const int kvh = pl.by_group(head), hg = head - kvh * pl.group;
+        // Rows in no sequence have no note.  Clamped: bad offsets leave notes unwritten.
+        const bool live = r < rows && tok >= pg.cu_seqlens_q[0] && tok < pg.cu_seqlens_q[pg.batch];
+        int first = 0, total = 0;
+        if (live) {
+            const int2 note = pl.notes[int64_t(tok) * pl.group + hg];
+            first = min(max(note.x, 0), pl.blocks * pl.stride - 1);
+            total = min(max(note.y, 0), pl.blocks - pl.by_stride(first));
+        }
+        const int64_t at = int64_t(kvh) * pl.blocks * pl.stride + first;
+        float mb = -__builtin_inff(), ml = mb, den = 0.f, suml = 0.f;
+        f32x4 acc[2] = {};
+        for (int c0 = part; c0 < total; c0 += PER * NS) {
+            // Loads past the last part repeat it, with weight 0: no branch between the loads.
+            float2 v[NS];
+            f32x4 xo[NS][2];
+#pragma unroll
+            for (int i = 0; i < NS; ++i) {
+                const int64_t row = at + int64_t(min(c0 + i * PER, total - 1)) * pl.stride;
+                v[i] = reinterpret_cast<const float2*>(pl.lse_part)[row];
+                const f32x4* o = reinterpret_cast<const f32x4*>(pl.o_part + row * D + l16 * 8);
+                xo[i][0] = o[0], xo[i][1] = o[1];
+            }
+#pragma unroll
+            for (int i = 0; i < NS; ++i)
+                if (c0 + i * PER >= total) v[i] = float2{-__builtin_inff(), -__builtin_inff()};
+            float nb = mb, nl = ml;
+#pragma unroll
+            for (int i = 0; i < NS; ++i) nb = fmaxf(nb, v[i].x), nl = fmaxf(nl, v[i].y);
+            if (nb == -__builtin_inff()) {
+                // Parts without a visible key, or with sums that are no numbers (which maxima
+                // pass over): so are then O and the LSE.
+#pragma unroll
+                for (int i = 0; i < NS; ++i)
+                    if (v[i].x != v[i].x) den = suml = __builtin_nanf("");
+                continue;
+            }
+            const float keep = exp2_native(mb - nb);
+            acc[0] *= keep, acc[1] *= keep;
+            den *= keep;
+            suml *= exp2_native(ml - nl);
+            mb = nb, ml = nl;
+#pragma unroll
+            for (int i = 0; i < NS; ++i) {
+                const float wgt = exp2_native(v[i].x - mb);
+                if (wgt != 0.f) acc[0] += wgt * xo[i][0], acc[1] += wgt * xo[i][1];
+                den += wgt;
+                suml += exp2_native(v[i].y - ml);
+            }
+        }
+        if constexpr (PER > 1) {
+            if (l16 == 0) red[grp] = float4{mb, ml, den, suml};
+            red_o[grp][l16 * 2] = acc[0], red_o[grp][l16 * 2 + 1] = acc[1];
+            __syncthreads();
+#pragma unroll
+            for (int p = 0; p < PER; ++p) mb = fmaxf(mb, red[slot * PER + p].x), ml = fmaxf(ml, red[slot * PER + p].y);
+            den = suml = 0.f;
+            acc[0] = acc[1] = f32x4{};
+#pragma unroll
+            for (int p = 0; p < PER; ++p) {
+                const float4 o = red[slot * PER + p];
+                if (o.z == 0.f) continue;                      // no part with a visible key
+                const float wgt = exp2_native(o.x - mb);
+                den += wgt * o.z;
+                suml += exp2_native(o.y - ml) * o.w;
+                acc[0] += wgt * red_o[slot * PER + p][l16 * 2], acc[1] += wgt * red_o[slot * PER + p][l16 * 2 + 1];
+            }
+            __syncthreads();
+        }
+        if (!live || part != 0 || total == 0) continue;        // (no parts: finished where it was attended)
+        const float rden = den == 0.f ? 0.f : 1.f / den;
+        bf16x8 y;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = __bf16(acc[i >> 2][i & 3] * rden);
+        *reinterpret_cast<bf16x8*>(static_cast<char*>(pg.o) + int64_t(r) * ROW_BYTES + l16 * 16) = y;
+        if (pg.lse && l16 == 0) pg.lse[int64_t(head) * pg.total_q + tok] =
+            den == 0.f ? -__builtin_inff() : (ml + __builtin_amdgcn_logf(suml)) * LN2;
+    }
+}
+
+}  // namespace fav4

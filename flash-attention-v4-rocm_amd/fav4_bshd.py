@@ -37,6 +37,7 @@ HIPCC_FLAGS = [
 KAT_LIB_PATH = ROOT / "build" / "libfav4_loader_kat.so"
 CEILING_LIB_PATH = ROOT / "build" / "libfav4_mfma_ceiling.so"
 SERVING_LIB_PATH = ROOT / "build" / "libfav4_serving.so"
+MX4_LIB_PATH = ROOT / "build" / "libfav4_mx4.so"
 RESOURCE_LOG = ROOT / "build" / "resource-usage.txt"
 MANIFEST = ROOT / "build" / "build-manifest.json"
 
@@ -82,6 +83,29 @@ _APPEND = struct.Struct("@12P4q10i")
 _PREFIX = struct.Struct("@8P10if3P2i0P")
 
 
+class Mx4AppendArgs(C.Structure):
+    """``struct Fav4Mx4AppendArgs`` (include/fav4_mx4.h): AppendArgs, 2 pointers."""
+    _fields_ = [("append", AppendArgs)] + [(n, C.c_void_p) for n in ("k_scales", "v_scales")]
+
+
+class Mx4GatherArgs(C.Structure):
+    """``struct Fav4Mx4GatherArgs`` (include/fav4_mx4.h): 9 pointers, 2 long longs, 6 ints."""
+    _fields_ = [(n, C.c_void_p) for n in ("k_cache", "k_scales", "v_cache", "v_scales", "k", "v", "cu_seqlens_k",
+                                          "starts", "block_table")] + [
+        (n, C.c_longlong) for n in ("k_stride", "v_stride")] + [
+        (n, C.c_int) for n in ("batch", "kv_heads", "total_k", "num_pages", "page_size", "max_pages_per_seq")]
+
+
+class Mx4PagedArgs(C.Structure):
+    """``struct Fav4Mx4PagedArgs`` (include/fav4_mx4.h): PagedArgs, 2 pointers."""
+    _fields_ = [("paged", PagedArgs)] + [(n, C.c_void_p) for n in ("k_scales", "v_scales")]
+
+
+_MX4_APPEND = struct.Struct("@12P4q10i2P")
+_MX4_GATHER = struct.Struct("@9P2q6i")
+_MX4_PAGED = struct.Struct("@8P10if2P")
+
+
 class Strides(C.Structure):
     """``struct Fav4Strides`` (include/fav4_bshd.h): element strides of a [B, S, H, 128] view."""
     _fields_ = [(n, C.c_longlong) for n in ("batch", "seq", "head")]
@@ -106,8 +130,8 @@ def parse_resource_usage(text: str) -> dict:
 
 def build_library(out: Path = LIB_PATH, verbose: bool = False) -> Path:
     """Compile ``csrc/bshd.hip`` for gfx950 into ``build/libfav4_bshd.so``, the
-    serving operators ``csrc/serving.hip`` into ``build/libfav4_serving.so``, the
-    loader probe ``csrc/loader_kat.hip`` into ``build/libfav4_loader_kat.so``
+    serving operators ``csrc/serving.hip`` into ``build/libfav4_serving.so``, those of
+    4-bit caches ``csrc/mx4.hip`` into ``build/libfav4_mx4.so``, the loader probe ``csrc/loader_kat.hip`` into ``build/libfav4_loader_kat.so``
     (a test library) and the MFMA-only probe ``csrc/mfma_ceiling.hip`` into
     ``build/libfav4_mfma_ceiling.so`` (a measurement library, read by
     ``bench.py --mfma-ceiling``), keep the compiler's kernel-resource-usage remarks in
@@ -119,8 +143,8 @@ def build_library(out: Path = LIB_PATH, verbose: bool = False) -> Path:
     import time
     out.parent.mkdir(parents=True, exist_ok=True)
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
-    jobs = {out: CSRC / "bshd.hip", SERVING_LIB_PATH: CSRC / "serving.hip", KAT_LIB_PATH: CSRC / "loader_kat.hip",
-            CEILING_LIB_PATH: CSRC / "mfma_ceiling.hip"}
+    jobs = {out: CSRC / "bshd.hip", SERVING_LIB_PATH: CSRC / "serving.hip", MX4_LIB_PATH: CSRC / "mx4.hip",
+            KAT_LIB_PATH: CSRC / "loader_kat.hip", CEILING_LIB_PATH: CSRC / "mfma_ceiling.hip"}
     procs = {}
     for lib, src in jobs.items():
         tmp = lib.with_suffix(".so.tmp")
@@ -246,6 +270,34 @@ def load_serving_library(path: Path = SERVING_LIB_PATH) -> C.CDLL:
         lib.fav4_bshd_prefix_paged_workspace_size.restype = C.c_longlong
         _SERVING = lib
     return _SERVING
+
+
+_MX4 = None
+
+
+def load_mx4_library(path: Path = MX4_LIB_PATH) -> C.CDLL:
+    """Load the library of the 4-bit caches' operators (raises OSError if it is missing); torch first, as load_library
+    says."""
+    global _MX4
+    if _MX4 is None or Path(_MX4._name) != Path(path):
+        if not Path(path).exists():
+            raise OSError(f"{path} not built; run __graft_entry__.build() first")
+        try:
+            import torch  # noqa: F401
+        except ImportError:
+            pass
+        lib = C.CDLL(str(path))
+        # The argument blocks are passed as packed bytes or by reference.
+        lib.fav4_bshd_append_paged_mx4.argtypes = [C.c_void_p, C.c_void_p]
+        lib.fav4_bshd_append_paged_mx4.restype = C.c_int
+        lib.fav4_bshd_gather_paged_mx4.argtypes = [C.c_void_p, C.c_void_p]
+        lib.fav4_bshd_gather_paged_mx4.restype = C.c_int
+        lib.fav4_bshd_forward_paged_mx4.argtypes = [C.c_void_p, C.c_int, C.c_void_p, C.c_size_t, C.c_void_p]
+        lib.fav4_bshd_forward_paged_mx4.restype = C.c_int
+        lib.fav4_bshd_paged_mx4_workspace_size.argtypes = [C.c_void_p, C.c_int]
+        lib.fav4_bshd_paged_mx4_workspace_size.restype = C.c_longlong
+        _MX4 = lib
+    return _MX4
 
 
 class Runner:
@@ -656,6 +708,166 @@ class Runner:
         status = self.serving.fav4_bshd_forward_prefix_paged(block, causal, workspace.data_ptr(), workspace.nbytes, raw)
         if status:
             raise RuntimeError(f"prefix paged: HIP status {status}")
+        return workspace
+
+    # ---- 4-bit paged K/V caches (include/fav4_mx4.h; no reference counterpart) ----
+    # Caches as pairs of uint8 tensors, contiguous: codes [num_pages, kv_heads, page_size, 64] and scales
+    # [num_pages, kv_heads, page_size, 4].
+    @property
+    def mx4(self) -> C.CDLL:
+        lib = self.__dict__.get("_mx4")
+        if lib is None:
+            lib = self._mx4 = load_mx4_library()
+        return lib
+
+    @staticmethod
+    def mx4_caches(num_pages, kv_heads, page_size, device="cuda"):
+        """(k_cache, k_scales, v_cache, v_scales) of zeros."""
+        import torch
+        shape = (num_pages, kv_heads, page_size)
+        return tuple(torch.zeros((*shape, n), dtype=torch.uint8, device=device)
+                     for n in (D // 2, D // 32, D // 2, D // 32))
+
+    @staticmethod
+    def _mx4_cache_shape(torch, dev, k_cache, k_scales, v_cache, v_scales):
+        num_pages, kv_heads, page_size, d = shape = k_cache.shape
+        scales = (num_pages, kv_heads, page_size, D // 32)
+        assert d == D // 2 and v_cache.shape == shape and k_scales.shape == v_scales.shape == scales
+        for x in (k_cache, k_scales, v_cache, v_scales):
+            assert x.dtype is torch.uint8 and x.is_contiguous() and x.get_device() == dev, \
+                "uint8, contiguous, all tensors on one device"
+        return num_pages, kv_heads, page_size
+
+    @staticmethod
+    def _mx4_rows(torch, x, tokens, heads, dev):
+        """The stride between the tokens of BF16 rows [tokens, heads, 128] (a single one has none that counts)."""
+        assert x.shape == (tokens, heads, D) and x.dtype is torch.bfloat16 and x.get_device() == dev, \
+            "BF16 rows [tokens, heads, 128] on one device"
+        stride, s1, s2 = x.stride()
+        assert s2 == 1 and (heads == 1 or s1 == D)
+        return stride if tokens > 1 else heads * D
+
+    @staticmethod
+    def _mx4_ints(torch, dev, *arrays):
+        for x, shape in arrays:
+            assert x.dtype is torch.int32 and x.shape == shape and x.is_contiguous() and x.get_device() == dev, \
+                "int32, contiguous, on one device"
+
+    @classmethod
+    def _mx4_append_block(cls, torch, q, k, v, q_out, k_cache, k_scales, v_cache, v_scales, cu_q, seqlens_k,
+                          block_table, cos, sin, interleaved, positions) -> bytes:
+        dev = k.get_device()
+        num_pages, kv_heads, page_size = cls._mx4_cache_shape(torch, dev, k_cache, k_scales, v_cache, v_scales)
+        batch, pages = block_table.shape
+        cls._mx4_ints(torch, dev, (cu_q, (batch + 1,)), (seqlens_k, (batch,)), (block_table, (batch, pages)))
+        tokens, heads = k.shape[0], 1
+        k_stride, v_stride = cls._mx4_rows(torch, k, tokens, kv_heads, dev), cls._mx4_rows(torch, v, tokens, kv_heads, dev)
+        q_stride = o_stride = q_ptr = o_ptr = rows = half = c_ptr = s_ptr = p_ptr = 0
+        assert (q is None) == (q_out is None) and (cos is None) == (sin is None)
+        if q is not None:
+            heads = q.shape[1]
+            q_stride, o_stride = cls._mx4_rows(torch, q, tokens, heads, dev), cls._mx4_rows(torch, q_out, tokens, heads, dev)
+            q_ptr, o_ptr = q.data_ptr(), q_out.data_ptr()
+        if cos is not None:
+            rows, half = cos.shape
+            assert sin.shape == cos.shape and cos.dtype is sin.dtype is torch.float32
+            assert cos.is_contiguous() and sin.is_contiguous() and cos.get_device() == sin.get_device() == dev
+            c_ptr, s_ptr = cos.data_ptr(), sin.data_ptr()
+        if positions is not None:
+            cls._mx4_ints(torch, dev, (positions, (tokens,)))
+            p_ptr = positions.data_ptr()
+        return _MX4_APPEND.pack(q_ptr, k.data_ptr(), v.data_ptr(), o_ptr, k_cache.data_ptr(), v_cache.data_ptr(),
+                                c_ptr, s_ptr, cu_q.data_ptr(), seqlens_k.data_ptr(), block_table.data_ptr(), p_ptr,
+                                q_stride, k_stride, v_stride, o_stride, batch, heads, kv_heads, tokens, num_pages,
+                                page_size, pages, 2 * half, rows, 1 if interleaved else 0, k_scales.data_ptr(),
+                                v_scales.data_ptr())
+
+    def call_append_paged_mx4(self, q, k, v, q_out, k_cache, k_scales, v_cache, v_scales, cu_q, seqlens_k, block_table,
+                              cos=None, sin=None, interleaved=False, positions=None, stream=None):
+        """fav4_bshd_append_paged_mx4: call_append_paged into 4-bit caches (see mx4_caches); the other tensors as
+        there."""
+        import torch
+        block = self._mx4_append_block(torch, q, k, v, q_out, k_cache, k_scales, v_cache, v_scales, cu_q, seqlens_k,
+                                       block_table, cos, sin, interleaved, positions)
+        status = self.mx4.fav4_bshd_append_paged_mx4(block, self._stream(torch, k.get_device(), stream))
+        if status:
+            raise RuntimeError(f"append paged mx4: HIP status {status}")
+
+    @classmethod
+    def _mx4_gather_block(cls, torch, k_cache, k_scales, v_cache, v_scales, k, v, cu_k, block_table, starts) -> bytes:
+        dev = k.get_device()
+        num_pages, kv_heads, page_size = cls._mx4_cache_shape(torch, dev, k_cache, k_scales, v_cache, v_scales)
+        batch, pages = block_table.shape
+        cls._mx4_ints(torch, dev, (cu_k, (batch + 1,)), (block_table, (batch, pages)))
+        if starts is not None:
+            cls._mx4_ints(torch, dev, (starts, (batch,)))
+        rows = k.shape[0]
+        k_stride, v_stride = cls._mx4_rows(torch, k, rows, kv_heads, dev), cls._mx4_rows(torch, v, rows, kv_heads, dev)
+        return _MX4_GATHER.pack(k_cache.data_ptr(), k_scales.data_ptr(), v_cache.data_ptr(), v_scales.data_ptr(),
+                                k.data_ptr(), v.data_ptr(), cu_k.data_ptr(), 0 if starts is None else starts.data_ptr(),
+                                block_table.data_ptr(), k_stride, v_stride, batch, kv_heads, rows, num_pages, page_size,
+                                pages)
+
+    def call_gather_paged_mx4(self, k_cache, k_scales, v_cache, v_scales, k, v, cu_k, block_table, starts=None,
+                              stream=None):
+        """fav4_bshd_gather_paged_mx4: the numbers that 4-bit caches (see mx4_caches) hold, as BF16 rows.  k/v:
+        [total_k, kv_heads, 128] (any stride between rows), of which [cu_k[b], cu_k[b + 1]) get keys starts[b], ... of
+        sequence b; cu_k: int32 [batch+1]; block_table: int32 [batch, max_pages]; starts: int32 [batch] or None (0)."""
+        import torch
+        block = self._mx4_gather_block(torch, k_cache, k_scales, v_cache, v_scales, k, v, cu_k, block_table, starts)
+        status = self.mx4.fav4_bshd_gather_paged_mx4(block, self._stream(torch, k.get_device(), stream))
+        if status:
+            raise RuntimeError(f"gather paged mx4: HIP status {status}")
+
+    @classmethod
+    def _mx4_paged_block(cls, torch, q, k_cache, k_scales, v_cache, v_scales, o, lse, cu_q, seqlens_k, block_table,
+                         max_q, max_k, total_k, scale) -> bytes:
+        dev = q.get_device()
+        num_pages, kv_heads, page_size = cls._mx4_cache_shape(torch, dev, k_cache, k_scales, v_cache, v_scales)
+        batch, pages = block_table.shape
+        cls._mx4_ints(torch, dev, (cu_q, (batch + 1,)), (seqlens_k, (batch,)), (block_table, (batch, pages)))
+        tokens, heads, d = q.shape
+        assert d == D and o.shape == q.shape and q.dtype is torch.bfloat16 and o.dtype is torch.bfloat16
+        assert q.is_contiguous() and o.is_contiguous() and o.get_device() == dev, "all tensors on one device"
+        lse_ptr = 0
+        if lse is not None:
+            assert lse.shape == (heads, tokens) and lse.is_contiguous() and lse.dtype is torch.float32
+            assert lse.get_device() == dev, "all tensors on one device"
+            lse_ptr = lse.data_ptr()
+        return _MX4_PAGED.pack(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), o.data_ptr(), lse_ptr,
+                               cu_q.data_ptr(), seqlens_k.data_ptr(), block_table.data_ptr(), batch, heads, kv_heads,
+                               int(max_q), int(max_k), tokens, 0 if total_k is None else int(total_k), num_pages,
+                               page_size, pages, SCALE if scale is None else scale, k_scales.data_ptr(),
+                               v_scales.data_ptr())
+
+    def paged_mx4_workspace_size(self, batch, heads, kv_heads, max_q, max_k, total_q, page_size, max_pages, num_pages,
+                                 causal=0) -> int:
+        """Workspace bytes of call_paged_mx4 for a batch of this shape (-1: rejected)."""
+        a = Mx4PagedArgs(self.paged_shape_args(batch, heads, kv_heads, max_q, max_k, total_q, 0, page_size, max_pages,
+                                               num_pages), None, None)
+        return self.mx4.fav4_bshd_paged_mx4_workspace_size(C.byref(a), int(causal))
+
+    def call_paged_mx4(self, q, k_cache, k_scales, v_cache, v_scales, o, lse, cu_q, seqlens_k, block_table, max_q,
+                       max_k, workspace=None, total_k=None, scale=None, stream=None, causal=0):
+        """fav4_bshd_forward_paged_mx4: attention over 4-bit caches (see mx4_caches); the other tensors as for
+        paged_args.  causal 0 dense, 2 bottom-right.  `workspace` as for call_splitkv (None: allocated here); returned
+        for the next call."""
+        import torch
+        block = self._mx4_paged_block(torch, q, k_cache, k_scales, v_cache, v_scales, o, lse, cu_q, seqlens_k,
+                                      block_table, max_q, max_k, total_k, scale)
+        raw = self._stream(torch, q.get_device(), stream)
+        causal = int(causal)
+        if workspace is None:
+            need = self.mx4.fav4_bshd_paged_mx4_workspace_size(block, causal)
+            if need < 0:
+                raise RuntimeError("paged mx4: arguments rejected")
+            # Allocated for the stream that uses it, which then orders its reuse.
+            with torch.cuda.stream(self._allocation_stream(torch, stream)):
+                workspace = torch.empty(need, device=q.device, dtype=torch.uint8)
+        assert workspace.get_device() == q.get_device() and workspace.is_contiguous()
+        status = self.mx4.fav4_bshd_forward_paged_mx4(block, causal, workspace.data_ptr(), workspace.nbytes, raw)
+        if status:
+            raise RuntimeError(f"paged mx4: HIP status {status}")
         return workspace
 
 
