@@ -94,13 +94,11 @@ bool paged_shape_ok(const Fav4Mx4PagedArgs* args, int causal) {
 
 // Up to this many rows a sequence go by the decode kernel.
 constexpr int FEW_ROWS = 64;
-// Most parts' rows of a prefill call over all heads: parts are made where the row tiles
-// are fewer than two for each CU, up to that many.
-constexpr int64_t PREFILL_PART_TILES = 1024;
 
 struct Sizes {
     fav4::Mx4Plan plan;
-    int64_t bytes, grid;
+    int64_t bytes, part_rows, grid, merge_grid;
+    int merge_teams;
     bool few, split;
     bool ok;
 };
@@ -114,41 +112,37 @@ Sizes paged_sizes(const Fav4Mx4PagedArgs& args, int causal) {
     p.group = int(group);
     p.br = causal == BOTTOM_RIGHT;
     s.few = seq_rows <= FEW_ROWS;
-    const int64_t ranges = std::max<int64_t>(1, 2 * cus / a.kv_heads);
+    // Workgroups of a K/V head that are resident at once: two of four waves a CU, or one of eight.
+    const int few_ranges = std::max(1, 2 * cus / a.kv_heads), many_ranges = std::max(1, cus / a.kv_heads);
+    int64_t segs;
     if (s.few) {
         p.stride = seq_rows <= 16 ? 16 : 32;
         p.tiles = int((seq_rows + p.stride - 1) / p.stride);
-        const int64_t segs = int64_t(a.batch) * p.tiles;
+        segs = int64_t(a.batch) * p.tiles;
         s.split = segs * a.kv_heads < 4 * cus && a.max_seqlen_k > 2048;
-        p.ranges = s.split ? int(ranges) : 1;
-        p.blocks = int(std::min<int64_t>(std::min(segs, (rows + int64_t(a.batch) * (p.stride - 1)) / p.stride) + ranges, INT_MAX));
-        s.grid = a.kv_heads * (s.split ? ranges : segs);
-        s.ok = segs * (int64_t(a.max_seqlen_k) / 64 + 1 + fav4::MX4_LEAD) < (1 << 30) && s.grid < (int64_t(1) << 30) &&
-               int64_t(p.blocks) * p.stride <= INT_MAX;
+        p.ranges = s.split ? few_ranges : 1;
     } else {
-        const int64_t tiles = std::min<int64_t>(a.batch * ((seq_rows + fav4::MX4_BM - 1) / fav4::MX4_BM),
-                                                (rows + int64_t(a.batch) * (fav4::MX4_BM - 1)) / fav4::MX4_BM);
-        const int64_t all = tiles * a.kv_heads;
-        const int64_t parts = std::min<int64_t>(std::max<int64_t>(1, 2 * cus / all), std::max(1, a.max_seqlen_k / 256));
-        p.tiles = int(std::min<int64_t>(tiles, INT_MAX));
-        p.ranges = int(parts);
-        s.split = parts > 1;
+        segs = std::min<int64_t>(a.batch * ((seq_rows + fav4::MX4_BM - 1) / fav4::MX4_BM),
+                                 (rows + int64_t(a.batch) * (fav4::MX4_BM - 1)) / fav4::MX4_BM);
         p.stride = fav4::MX4_BM;
-        p.blocks = int(std::min<int64_t>(tiles * parts, INT_MAX));
-        s.grid = all * parts;
-        s.ok = tiles <= MAX_ROW_TILES && all <= MAX_ROW_TILES && (!s.split || s.grid <= PREFILL_PART_TILES);
+        p.tiles = int(std::min<int64_t>(segs, INT_MAX));
+        s.split = segs <= fav4::MX4_LINE_TILES && a.batch <= fav4::MX4_LINE_SEQS && segs * a.kv_heads < 8 * cus;
+        p.ranges = s.split ? many_ranges : 1;
+        s.ok = segs <= MAX_ROW_TILES;
     }
+    s.grid = a.kv_heads * (s.split ? int64_t(p.ranges) : segs);
+    s.ok = segs <= MAX_ROW_TILES && s.grid < (int64_t(1) << 30) &&
+           segs * (int64_t(a.max_seqlen_k) / 64 + 1 + std::max(fav4::MX4_LEAD, fav4::MX4_MANY_LEAD)) < (1 << 30);
     p.by_kv_heads = fav4::fast_div(a.kv_heads);
     p.by_group = fav4::fast_div(int(group));
     p.by_page = fav4::fast_div(a.page_size);
-    p.by_heads = fav4::fast_div(a.heads);
-    p.by_stride = fav4::fast_div(p.stride);
+    // Teams per merged row: many where the row tiles are few and cut into many parts.
+    s.merge_teams = s.few ? 4 : 1;
+    s.merge_grid = int64_t(p.ranges) * a.kv_heads * (p.stride * s.merge_teams / 16);
+    p.by_merge = fav4::fast_div(p.stride * s.merge_teams / 16);
     // What a call of either kind could need: more queries or sequences never need less.
-    const int64_t few_rows = a.kv_heads * (std::min<int64_t>(rows, int64_t(a.batch) * FEW_ROWS) + (int64_t(a.batch) + ranges) * 32);
-    const int64_t many_rows = s.few ? 0 : PREFILL_PART_TILES * fav4::MX4_BM;
-    const int64_t part_rows = (few_rows + many_rows + 1) & ~int64_t(1);
-    s.ok = s.ok && (!s.split || int64_t(a.kv_heads) * p.blocks * p.stride <= part_rows) && part_rows < (int64_t(1) << 40);
-    s.bytes = part_rows * (fav4::D * 4 + 8) + rows * 8;
+    s.part_rows = int64_t(a.kv_heads) * 2 * (s.few ? few_ranges * 32 : std::max(few_ranges * 32, many_ranges * fav4::MX4_BM));
+    s.bytes = s.part_rows * (fav4::D * 4 + 8) + int64_t(few_ranges) * 16;
     return s;
 }
 
@@ -168,10 +162,10 @@ extern "C" __attribute__((visibility("default"))) int fav4_bshd_append_paged_mx4
     if (!append_ok(args)) return hipErrorInvalidValue;
     const Fav4AppendArgs& a = args->append;
     const int rows = (a.q ? a.heads : 0) + 2 * a.kv_heads, units = (rows + 7) / 8;
-    const int64_t total = int64_t(units) * a.total_q, blocks = std::min((total + 3) / 4, MAX_GRID);
+    const int64_t total = int64_t(units) * ((int64_t(a.total_q) + 3) / 4), blocks = std::min(total, MAX_GRID);
     const fav4::FastDiv by_units = fav4::fast_div(units), by_page = fav4::fast_div(a.page_size);
     auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3(unsigned(blocks)), dim3(256), 0, stream, *args, units, total, by_units, by_page);
+        hipLaunchKernelGGL(kernel, dim3(unsigned(blocks)), dim3(256), 0, stream, *args, units, int(total), by_units, by_page);
     };
     if (a.interleaved) go(fav4::mx4_store_kernel<true>);
     else go(fav4::mx4_store_kernel<false>);
@@ -181,8 +175,11 @@ extern "C" __attribute__((visibility("default"))) int fav4_bshd_append_paged_mx4
 extern "C" __attribute__((visibility("default"))) int fav4_bshd_gather_paged_mx4(const Fav4Mx4GatherArgs* a,
                                                                                 hipStream_t stream) {
     if (!gather_ok(a)) return hipErrorInvalidValue;
-    const int64_t per = 4 * fav4::MX4_READ_ROWS, blocks = std::min((a->total_k + per - 1) / per, MAX_GRID);
-    hipLaunchKernelGGL(fav4::mx4_read_kernel, dim3(unsigned(blocks)), dim3(256), 0, stream, *a, fav4::fast_div(a->page_size));
+    // Rows a wave: one each until the waves fill the GPU.
+    const int each = int(std::min<int64_t>(std::max<int64_t>(a->total_k / (int64_t(16) * device_cus()), 1), fav4::MX4_READ_ROWS));
+    const int64_t per = 4 * each, blocks = std::min((a->total_k + per - 1) / per, MAX_GRID);
+    hipLaunchKernelGGL(fav4::mx4_read_kernel, dim3(unsigned(blocks)), dim3(256), 0, stream, *a, fav4::fast_div(a->page_size),
+                       each);
     return hipGetLastError();
 }
 
@@ -208,10 +205,9 @@ extern "C" __attribute__((visibility("default"))) int fav4_bshd_forward_paged_mx
     if (!s.ok || !workspace || !aligned(256, workspace) || uint64_t(s.bytes) > workspace_bytes)
         return hipErrorInvalidValue;
     fav4::Mx4Plan& p = s.plan;
-    const int64_t part_rows = s.split ? (int64_t(a.kv_heads) * p.blocks * p.stride + 1) & ~int64_t(1) : 0;
     p.o_part = static_cast<float*>(workspace);
-    p.lse_part = p.o_part + part_rows * fav4::D;
-    p.notes = reinterpret_cast<int2*>(p.lse_part + part_rows * 2);
+    p.lse_part = p.o_part + s.part_rows * fav4::D;
+    p.notes = reinterpret_cast<int4*>(p.lse_part + s.part_rows * 2);
     if (s.few) {
         if (p.stride == 16) launch_few<1>(*args, s, stream);
         else launch_few<2>(*args, s, stream);
@@ -219,14 +215,15 @@ extern "C" __attribute__((visibility("default"))) int fav4_bshd_forward_paged_mx
         auto go = [&](auto kernel) {
             hipLaunchKernelGGL(kernel, dim3(unsigned(s.grid)), dim3(512), 0, stream, *args, p);
         };
-        if (a.lse) s.split ? go(fav4::mx4_prefill_kernel<true, true>) : go(fav4::mx4_prefill_kernel<true, false>);
-        else s.split ? go(fav4::mx4_prefill_kernel<false, true>) : go(fav4::mx4_prefill_kernel<false, false>);
+        if (a.lse) s.split ? go(fav4::mx4_prefill_line_kernel<true>) : go(fav4::mx4_prefill_kernel<true>);
+        else s.split ? go(fav4::mx4_prefill_line_kernel<false>) : go(fav4::mx4_prefill_kernel<false>);
     }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || !s.split) return e;
-    const int64_t rows = int64_t(a.total_q) * a.heads;
-    constexpr int per = 4;
-    hipLaunchKernelGGL(fav4::mx4_merge_kernel<per>, dim3(unsigned(std::min((rows * per + 15) / 16, MAX_GRID))), dim3(256), 0,
-                       stream, *args, p);
+    auto merge = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(unsigned(s.merge_grid)), dim3(256), 0, stream, *args, p);
+    };
+    if (s.merge_teams == 4) merge(fav4::mx4_merge_kernel<4>);
+    else merge(fav4::mx4_merge_kernel<1>);
     return hipGetLastError();
 }

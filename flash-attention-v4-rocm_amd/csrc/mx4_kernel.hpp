@@ -58,17 +58,16 @@ __device__ __forceinline__ void mx4_turn(float& p, float& q, float c, float s) {
 }
 
 template <bool INTERLEAVED>
-__global__ __launch_bounds__(256) void mx4_store_kernel(Fav4Mx4AppendArgs args, int units, int64_t total,
+__global__ __launch_bounds__(256) void mx4_store_kernel(Fav4Mx4AppendArgs args, int units, int total,
                                                         FastDiv by_units, FastDiv by_page) {
     __shared__ __attribute__((aligned(16))) uint32_t most[4][8][16];
     const Fav4AppendArgs& a = args.append;
     const int lane = threadIdx.x & 63, j = lane & 7, wave = uniform(threadIdx.x >> 6);
-    const int64_t stride = int64_t(gridDim.x) * 4;
     const int qheads = a.q ? a.heads : 0, rows = qheads + 2 * a.kv_heads;
     const int half = a.rotary_dim >> 4;                    // granules of half the rotated dims
-    const int first = a.cu_seqlens_q[0], end = a.cu_seqlens_q[a.batch];
-    for (int64_t id = int64_t(blockIdx.x) * 4 + wave; id < total; id += stride) {
-        const int t = uniform(by_units(int(id))), unit = uniform(int(id) - t * units);
+    const int first = a.cu_seqlens_q[0], end = min(a.cu_seqlens_q[a.batch], a.total_q);
+    for (int id = blockIdx.x; id < total; id += gridDim.x) {
+        const int four = uniform(by_units(id)), unit = uniform(id - four * units), t = four * 4 + wave;
         if (t < first || t >= end) continue;               // in no sequence
         const int row = unit * 8 + (lane >> 3);
         const bool live = row < rows, is_q = row < qheads, is_v = row >= qheads + a.kv_heads;
@@ -147,24 +146,29 @@ __global__ __launch_bounds__(256) void mx4_store_kernel(Fav4Mx4AppendArgs args, 
 }
 
 // ---------------------------------------------------------------------------
-// Reading back.  One wave takes 8 neighbouring rows (tokens): their sequences by one
-// search and one look at the offsets behind it, their places in the caches in the
-// wave's lanes, then K and V, 16 lanes a head's row (4 bytes of codes, 16 of BF16).
-// Bound by memory: 256 of 324 bytes are written.
+// Reading back.  One wave takes two neighbouring rows (tokens), or one where there are
+// few: their sequences by one search and one look at the offsets behind it, their places
+// in the caches in the wave's lanes, then K and V, 16 lanes a head's row (4 bytes of
+// codes, 16 of BF16), 16 heads' rows with all their loads in flight.  Bound by memory:
+// 256 of 324 bytes are written, past the caches (12 histories of up to 16384 keys H32/8,
+// 268 MB: 44.4 us, 6.0 TB/s; 73.5 with ordinary stores; 45.1 with one row a wave, 45.3
+// with four, 48.0 with eight); for few rows by the chain offsets -> table -> codes ->
+// store (4 rows 3.1 us).
 // ---------------------------------------------------------------------------
-constexpr int MX4_READ_ROWS = 8;
-__global__ __launch_bounds__(256) void mx4_read_kernel(Fav4Mx4GatherArgs a, FastDiv by_page) {
+constexpr int MX4_READ_ROWS = 2;
+__global__ __launch_bounds__(256) void mx4_read_kernel(Fav4Mx4GatherArgs a, FastDiv by_page, int each) {
+    constexpr int U = 4;
     const int lane = threadIdx.x & 63, sub = lane >> 4, l16 = lane & 15;
     const int first = max(a.cu_seqlens_k[0], 0), end = min(a.cu_seqlens_k[a.batch], a.total_k);
-    const int64_t step = int64_t(gridDim.x) * 4 * MX4_READ_ROWS;
-    for (int64_t at = (int64_t(blockIdx.x) * 4 + uniform(threadIdx.x >> 6)) * MX4_READ_ROWS; at < end; at += step) {
-        const int t0 = max(int(at), first), n = uniform(min(int(at) + MX4_READ_ROWS, end) - t0);
+    const int64_t step = int64_t(gridDim.x) * 4 * each;
+    for (int64_t at = (int64_t(blockIdx.x) * 4 + uniform(threadIdx.x >> 6)) * each; at < end; at += step) {
+        const int t0 = max(int(at), first), n = uniform(min(int(at) + each, end) - t0);
         if (n <= 0) continue;
         // Lane i: the sequence of row t0 + i, and its row of the caches (-1: in no page).
         const int b0 = wave_find(a.cu_seqlens_k, a.batch, t0, lane);
         const int next = a.cu_seqlens_k[min(b0 + 1 + lane, a.batch)];
         int b = b0;
-        for (int i = 0; i < n; ++i) {
+        for (int i = 1; i < n; ++i) {
             const uint64_t past = __builtin_amdgcn_ballot_w64(b0 + 1 + lane <= a.batch && next <= t0 + i);
             const int here = past == ~0ull ? wave_find(a.cu_seqlens_k, a.batch, t0 + i, lane)
                                            : b0 + __builtin_popcountll(past);
@@ -181,27 +185,34 @@ __global__ __launch_bounds__(256) void mx4_read_kernel(Fav4Mx4GatherArgs a, Fast
             }
         }
         const int lo = int(place), hi = int(place >> 32);
-        const int rows = 2 * a.kv_heads, per = (rows + 3) >> 2;        // groups of four rows a token
+        const int rows = 2 * a.kv_heads;
         for (int i = 0; i < n; ++i) {
             const int64_t base = int64_t(uint32_t(__builtin_amdgcn_readlane(lo, i))) |
                                  int64_t(__builtin_amdgcn_readlane(hi, i)) << 32;
-#pragma unroll 4
-            for (int u = 0; u < per; ++u) {
-                const int row = u * 4 + sub;
-                if (row >= rows) continue;
-                const bool is_v = row >= a.kv_heads;
-                const int head = is_v ? row - a.kv_heads : row;
-                bf16x8 x{};
+            for (int row0 = 0; row0 < rows; row0 += 4 * U) {
+                uint32_t codes[U] = {}, scale[U] = {};
                 if (base >= 0) {
-                    const int64_t r = base + int64_t(head) * a.page_size;
-                    const uint32_t codes = reinterpret_cast<const uint32_t*>(
-                        static_cast<const char*>(is_v ? a.v_cache : a.k_cache) + r * MX4_CODES)[l16];
-                    const uint32_t s = static_cast<const uint8_t*>(is_v ? a.v_scales : a.k_scales)[r * MX4_SCALES + (l16 >> 2)];
-                    x = mx4_values(codes, mx4_scale(s));
+#pragma unroll
+                    for (int u = 0; u < U; ++u) {
+                        const int row = min(row0 + u * 4 + sub, rows - 1);         // past the last: it again
+                        const bool is_v = row >= a.kv_heads;
+                        const int64_t r = base + int64_t(is_v ? row - a.kv_heads : row) * a.page_size;
+                        codes[u] = reinterpret_cast<const uint32_t*>(
+                            static_cast<const char*>(is_v ? a.v_cache : a.k_cache) + r * MX4_CODES)[l16];
+                        scale[u] = static_cast<const uint8_t*>(is_v ? a.v_scales : a.k_scales)[r * MX4_SCALES + (l16 >> 2)];
+                    }
                 }
-                char* dst = static_cast<char*>(is_v ? a.v : a.k) +
-                            (int64_t(t0 + i) * (is_v ? a.v_stride : a.k_stride) + int64_t(head) * D) * 2;
-                *reinterpret_cast<bf16x8*>(dst + l16 * 16) = x;
+#pragma unroll
+                for (int u = 0; u < U; ++u) {
+                    const int row = row0 + u * 4 + sub;
+                    if (row >= rows) continue;
+                    const bool is_v = row >= a.kv_heads;
+                    char* dst = static_cast<char*>(is_v ? a.v : a.k) +
+                                (int64_t(t0 + i) * (is_v ? a.v_stride : a.k_stride) +
+                                 int64_t(is_v ? row - a.kv_heads : row) * D) * 2;
+                    __builtin_nontemporal_store(__builtin_bit_cast(u32x4, mx4_values(codes[u], mx4_scale(scale[u]))),
+                                                reinterpret_cast<u32x4*>(dst + l16 * 16));
+                }
             }
         }
     }
@@ -212,16 +223,27 @@ __global__ __launch_bounds__(256) void mx4_read_kernel(Fav4Mx4GatherArgs a, Fast
 // group + head.  Sequences of up to 64 rows (decode, drafts) go by mx4_decode_kernel,
 // longer ones by mx4_prefill_kernel.
 // ---------------------------------------------------------------------------
+// Sequences' row tiles and their key tiles lie end to end on a line, a few units more
+// before each row tile for what its start and end cost, and the line is cut into equal
+// ranges, one a workgroup of each K/V head.  A row tile whole in a range is finished
+// there.  Of the others a range has at most two: one that began before it, whose part
+// goes to the range's partial block 0, and one that ends behind it (block 1); they are
+// merged by mx4_merge_kernel.
 struct Mx4Plan {
-    float *o_part, *lse_part;         // partial blocks of all K/V heads: `blocks` of `stride` rows each
-    int2* notes;                      // [total_q * group]: first partial row of a head's row, and parts
+    float *o_part, *lse_part;         // partial blocks of all K/V heads: two a range, of `stride` rows each
+    int4* notes;                      // [ranges]: first row (token * group + head), rows and parts of the row tile whose
+                                      // first part is the range's block 1 (no parts: there is none)
     int group;                        // query heads of a K/V head
-    int ranges;                       // decode: workgroups of a K/V head; prefill: parts of a row tile's keys
-    FastDiv by_kv_heads, by_group, by_page, by_heads, by_stride;
-    int blocks, stride;
-    int tiles;                        // prefill: row tiles that the batch can have
+    int ranges;                       // of a K/V head
+    FastDiv by_kv_heads, by_group, by_page, by_merge;
+    int stride;
+    int tiles;                        // row tiles that a sequence (few rows) or the batch (many) can have
     int br;                           // bottom-right causal
 };
+// The partial block of a row tile's part in range w.
+__device__ __forceinline__ int mx4_block(int w, bool began_before) { return 2 * w + (began_before ? 0 : 1); }
+// How far behind a row's first partial block its part c lies.
+__device__ __forceinline__ int mx4_part(int c) { return c > 0 ? 2 * c - 1 : 0; }
 
 // A sequence as read on the device, clamped.
 struct Mx4Seq {
@@ -503,8 +525,8 @@ struct Mx4Decode {
                     *reinterpret_cast<bf16x4*>(static_cast<char*>(pg.o) + (int64_t(f.t0 + token) * pg.heads + head) * ROW_BYTES + u * 8) = y;
                     if (pg.lse && u == 0)
                         pg.lse[int64_t(head) * pg.total_q + f.t0 + token] = (base + __builtin_amdgcn_logf(sl)) * LN2;
-                } else if (uint32_t(block) < uint32_t(pl.blocks)) {
-                    const int64_t prow = (int64_t(kvh) * pl.blocks + block) * BM + n * 16 + r;
+                } else {
+                    const int64_t prow = (int64_t(kvh) * 2 * pl.ranges + block) * BM + n * 16 + r;
                     *reinterpret_cast<f32x4*>(pl.o_part + prow * D + u * 4) = o;
                     if (u == 0)
                         reinterpret_cast<float2*>(pl.lse_part)[prow] =
@@ -516,11 +538,8 @@ struct Mx4Decode {
     }
 };
 
-// One row tile of a sequence and one K/V head a workgroup (SPLIT false), or the row
-// tiles' key tiles end to end on a line, MX4_LEAD units before each, cut into equal
-// ranges, one a workgroup: row tiles whole in a range are finished there, parts of
-// others go to partial block (row tile + range), unique because both only grow along
-// the line, and are merged by mx4_merge_kernel.
+// One row tile of a sequence and one K/V head a workgroup (SPLIT false), or a range of
+// the line.
 constexpr int MX4_LEAD = 2;
 template <int NT, int WAVES, bool SPLIT>
 __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
@@ -543,52 +562,49 @@ void mx4_decode_kernel(Fav4Mx4PagedArgs a, Mx4Plan pl) {
     } else {
         auto tiles_of = [&](const Mx4Seq& f) { return int(uint32_t(f.tokens * pl.group + BM - 1) / BM); };
         auto cost_of = [&](const Mx4Seq& f) { return max(1, (f.keys + 63) >> 6) + MX4_LEAD; };
-        // Row tiles and units of 64 sequences from i on, in the lanes.
-        struct Sums {
-            int tiles, cost, tiles_end, cost_end;
-        };
+        // Units of 64 sequences from i on, in the lanes: of each, and up to and with it.
         auto sums = [&](int i) {
             Mx4Seq f{};
             if (i + lane < pg.batch) f = mx4_seq(pg, i + lane);
-            const int n = tiles_of(f), c = n * cost_of(f);
-            return Sums{n, c, wave_scan(n), wave_scan(c)};
+            const int c = tiles_of(f) * cost_of(f);
+            return int2{c, wave_scan(c)};
         };
-        const Sums head = sums(0);
-        int units = __builtin_amdgcn_readlane(head.cost_end, 63);
-        for (int i = 64; i < pg.batch; i += 64) units += __builtin_amdgcn_readlane(sums(i).cost_end, 63);
+        const int2 head = sums(0);
+        int units = __builtin_amdgcn_readlane(head.y, 63);
+        for (int i = 64; i < pg.batch; i += 64) units += __builtin_amdgcn_readlane(sums(i).y, 63);
         const int per = max(udiv_up(units, pl.ranges), 1), g0 = w * per, g1 = g0 + per;
-        // The sequence that holds unit g0, the unit where it starts and the row tiles before it.
-        int idx = 0, base = 0, seg = 0;
-        for (Sums v = head;; v = sums(idx)) {
-            const uint64_t hit = __builtin_amdgcn_ballot_w64(base + v.cost_end > g0);
+        // The sequence that holds unit g0, and the unit where it starts.
+        int idx = 0, base = 0;
+        for (int2 v = head;; v = sums(idx)) {
+            const uint64_t hit = __builtin_amdgcn_ballot_w64(base + v.y > g0);
             if (hit) {
                 const int l = __builtin_ctzll(hit);
                 idx = uniform(idx + l);
-                base = uniform(base + __builtin_amdgcn_readlane(v.cost_end - v.cost, l));
-                seg = uniform(seg + __builtin_amdgcn_readlane(v.tiles_end - v.tiles, l));
+                base = uniform(base + __builtin_amdgcn_readlane(v.y - v.x, l));
                 break;
             }
-            base += __builtin_amdgcn_readlane(v.cost_end, 63);
-            seg += __builtin_amdgcn_readlane(v.tiles_end, 63);
+            base += __builtin_amdgcn_readlane(v.y, 63);
             idx += 64;
-            if (idx >= pg.batch) return;
+            if (idx >= pg.batch) break;
         }
+        int4 note{};
         for (; idx < pg.batch && base < g1; ++idx) {
             const Mx4Seq f = uniform_seq(idx);
             const int n = tiles_of(f), cost = cost_of(f), tiles = (f.keys + 63) >> 6;
             // Neighbouring sequences are taken with neighbouring heads, as in attend_wave.
             const int kvh = uniform(turn + idx - pl.by_kv_heads(turn + idx) * pg.kv_heads);
-            for (int rt = 0; rt < n; ++rt, ++seg, base += cost) {
+            for (int rt = 0; rt < n; ++rt, base += cost) {
                 const int end = base + cost, first = end - max(tiles, 1);      // unit of the first key tile
                 if (first >= g1 || end <= g0) continue;
-                const bool split = first < g0 || end > g1;
-                decode.attend(idx, f, rt * BM, kvh, max(0, g0 - first), min(tiles, g1 - first), split, seg + w);
-                const int row = rt * BM + int(threadIdx.x);
-                if (kvh == 0 && first >= g0 && int(threadIdx.x) < BM && row < f.tokens * pl.group)
-                    pl.notes[int64_t(f.t0) * pl.group + row] =
-                        int2{(seg + w) * BM + int(threadIdx.x), split ? udiv(end - 1, per) - w + 1 : 0};
+                const bool before = first < g0, split = before || end > g1;
+                const int block = mx4_block(w, before);
+                decode.attend(idx, f, rt * BM, kvh, max(0, g0 - first), min(tiles, g1 - first), split, block);
+                if (split && !before)
+                    note = int4{f.t0 * pl.group + rt * BM, min(BM, f.tokens * pl.group - rt * BM),
+                                udiv(end - 1, per) - w + 1, 0};
             }
         }
+        if (turn == 0 && threadIdx.x == 0) pl.notes[w] = note;
     }
 }
 
@@ -596,131 +612,121 @@ void mx4_decode_kernel(Fav4Mx4PagedArgs a, Mx4Plan pl) {
 // Eight waves of 32 rows each share 64-key tiles of K and V, which they convert to BF16
 // on the way into LDS (two stages): the loop of the forward, attend_fused, behind another
 // source.  A thread has 16 dims of one key: 8 bytes of codes and the key's four scales,
-// loaded two tiles ahead.
-constexpr int MX4_BM = 256;
-template <bool LSE, bool SPLIT>
-__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2)))
-void mx4_prefill_kernel(Fav4Mx4PagedArgs a, Mx4Plan pl) {
-    constexpr int BN = 64, TILE_BYTES = BN * ROW_BYTES;
-    __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * TILE_BYTES];
-    const Fav4PagedArgs& pg = a.paged;
-    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), col = lane & 31, half = lane >> 5;
-    const int group = pl.group;
-    int id = uniform(pl.by_kv_heads(blockIdx.x));
-    const int kvh = uniform(int(blockIdx.x) - id * pg.kv_heads);
-    int part = 0;
-    if constexpr (SPLIT) {
-        part = id / pl.tiles;
-        id -= part * pl.tiles;
+// loaded two tiles ahead.  Of the two waves of a SIMD one converts the next tile before
+// its products and the other behind them, so that one's conversion runs beside the
+// other's products.
+constexpr int MX4_BM = 256, MX4_MANY_LEAD = 2;
+constexpr int MX4_LINE_TILES = 1024, MX4_LINE_SEQS = 512;      // of a batch that is cut into ranges
+
+template <bool LSE>
+struct Mx4Prefill {
+    static constexpr int BN = 64, TILE_BYTES = BN * ROW_BYTES;
+    const Fav4Mx4PagedArgs& a;
+    const Mx4Plan& pl;
+    unsigned char* smem;              // two stages of a K and a V tile
+    int lane, wave;
+
+    __device__ __forceinline__ int tiles_of(const Mx4Seq& f) const {
+        return int(uint32_t(f.tokens * pl.group + MX4_BM - 1) / MX4_BM);
     }
-    // Row tile `id` of the batch: of which sequence.
-    auto tiles_of = [&](const Mx4Seq& f) { return int(uint32_t(f.tokens * group + MX4_BM - 1) / MX4_BM); };
-    int b = 0, before = 0;
-    for (;;) {
-        const int n = b + lane < pg.batch ? tiles_of(mx4_seq(pg, b + lane)) : 0, end = wave_scan(n);
-        const uint64_t hit = __builtin_amdgcn_ballot_w64(before + end > id);
-        if (hit) {
-            const int l = __builtin_ctzll(hit);
-            before = uniform(before + __builtin_amdgcn_readlane(end - n, l));
-            b = uniform(b + l);
-            break;
+    // Key tiles that some row of row tile rt sees.
+    __device__ __forceinline__ int key_tiles(const Mx4Seq& f, int rt) const {
+        const int last = pl.by_group(min(f.tokens * pl.group, (rt + 1) * MX4_BM) - 1);
+        const int seen = pl.br ? max(0, min(f.keys, f.keys - f.tokens + last + 1)) : f.keys;
+        return (seen + BN - 1) / BN;
+    }
+
+    // Key tiles [t, e1) of row tile rt of sequence b with head kvh; split as in Mx4Decode::attend.
+    __device__ __forceinline__ void attend(int b, const Mx4Seq& f, int rt, int kvh, int t, int e1, bool split,
+                                           int block) const {
+        const Fav4PagedArgs& pg = a.paged;
+        const int col = lane & 31, half = lane >> 5, group = pl.group, rows = f.tokens * group;
+        const int q0 = rt * MX4_BM, qw = q0 + wave * 32, row = qw + col, srow = min(row, rows - 1);
+        const int token = pl.by_group(srow), head = kvh * group + srow - token * group;
+        const int shift = f.keys - f.tokens;
+        const int plain = uniform(pl.br ? max(0, min(f.keys, shift + pl.by_group(q0) + 1)) : f.keys);
+        const int lim = pl.br ? shift + token : f.keys - 1;
+        const float scale2 = pg.scale * LOG2E;
+        RowState st;
+        clear(st);
+        if (t < e1) {
+            const LdsOffsets off = lds_offsets(lane);
+            bf16x8 qr[8];
+            load_q(pg, f.t0 + token, head, half, qr);
+            const int kr = wave * 8 + (lane >> 3), j = lane & 7;           // this thread's key and 16 dims
+            const int last = (f.keys - 1) & ~7;
+            Mx4Pages pages = mx4_pages(pg, b, kvh, min(t * BN + wave * 8, last), pl.by_page, lane);
+            u32x2 ck, cv;
+            uint32_t ks, vs;
+            auto load = [&](int at) {
+                if (at >= e1) return;
+                const int64_t r = pages.row(min(at * BN + wave * 8, last), pl.by_page, lane);
+                ck = *reinterpret_cast<const u32x2*>(static_cast<const char*>(pg.k_cache) + r * MX4_CODES + lane * 8);
+                cv = *reinterpret_cast<const u32x2*>(static_cast<const char*>(pg.v_cache) + r * MX4_CODES + lane * 8);
+                ks = *reinterpret_cast<const uint32_t*>(static_cast<const char*>(a.k_scales) + r * MX4_SCALES + (lane >> 3) * 4);
+                vs = *reinterpret_cast<const uint32_t*>(static_cast<const char*>(a.v_scales) + r * MX4_SCALES + (lane >> 3) * 4);
+            };
+            const uint32_t k0 = kr * ROW_BYTES + (((2 * j) ^ k_swz(kr)) << 4), k1 = kr * ROW_BYTES + (((2 * j + 1) ^ k_swz(kr)) << 4);
+            const uint32_t v0 = kr * ROW_BYTES + (((2 * j) ^ v_swz(kr)) << 4), v1 = kr * ROW_BYTES + (((2 * j + 1) ^ v_swz(kr)) << 4);
+            auto store = [&](int at, int stage) {
+                if (at >= e1) return;
+                const bool in = at * BN + kr < f.keys;
+                const uint32_t ksc = in ? ks : 0u, vsc = in ? vs : 0u;
+                const uint32_t kb = mx4_has_255(vsc) ? 255u : ksc >> (8 * (j >> 1)) & 255u;
+                const uint32_t byte = vsc >> (8 * (j >> 1)) & 255u;
+                const bool none = !in || byte == 255u;
+                const float sk = mx4_scale(kb), sv = mx4_scale(none ? 0u : byte);
+                unsigned char* k = smem + stage * 2 * TILE_BYTES;
+                unsigned char* v = k + TILE_BYTES;
+                auto put = [](unsigned char* p, bf16x8 x) { *reinterpret_cast<FAV4_LDS bf16x8*>((FAV4_LDS void*)p) = x; };
+                put(k + k0, mx4_values(ck[0], sk));
+                put(k + k1, mx4_values(ck[1], sk));
+                put(v + v0, mx4_values(none ? 0u : cv[0], sv));
+                put(v + v1, mx4_values(none ? 0u : cv[1], sv));
+            };
+            const bool idle = qw >= rows, early = wave < 4;
+            const int t0 = t;
+            load(t);
+            store(t, 0);
+            load(t + 1);
+            int stage = 0;
+            auto steps = [&](auto masked, int to) {
+                for (; t < to; ++t) {
+                    __syncthreads();
+                    if (early) {
+                        store(t + 1, stage ^ 1);
+                        load(t + 2);
+                    }
+                    const unsigned char* cur = smem + stage * 2 * TILE_BYTES;
+                    if (!idle)
+                        attend_fused<BN, decltype(masked)::value, true, LSE, true>(cur, cur + TILE_BYTES, off, qr, st, t == t0,
+                                                                                   t * BN, f.keys, lim, half, scale2);
+                    if (!early) {
+                        store(t + 1, stage ^ 1);
+                        load(t + 2);
+                    }
+                    stage ^= 1;
+                }
+            };
+            steps(std::integral_constant<bool, false>{}, min(e1, plain / BN));
+            steps(std::integral_constant<bool, true>{}, e1);
+            __syncthreads();               // every wave has read its last tile: the stages may hold O
         }
-        before += __builtin_amdgcn_readlane(end, 63);
-        b += 64;
-        if (b >= pg.batch) return;
-    }
-    Mx4Seq f = mx4_seq(pg, b);
-    f = {uniform(f.t0), uniform(f.tokens), uniform(f.keys)};
-    const int rows = f.tokens * group, rt = uniform(tiles_of(f)) - 1 - (id - before);      // the longest first
-    const int q0 = rt * MX4_BM, qw = q0 + wave * 32, row = qw + col, srow = min(row, rows - 1);
-    const int token = pl.by_group(srow), head = kvh * group + srow - token * group;
-    const int shift = f.keys - f.tokens, i0 = pl.by_group(q0), i1 = pl.by_group(min(rows, q0 + MX4_BM) - 1);
-    const int plain = uniform(pl.br ? max(0, min(f.keys, shift + i0 + 1)) : f.keys);
-    const int seen = uniform(pl.br ? max(0, min(f.keys, shift + i1 + 1)) : f.keys);
-    const int lim = pl.br ? shift + token : f.keys - 1;
-    const float scale2 = pg.scale * LOG2E;
-    int t = 0, e1 = (seen + BN - 1) / BN;
-    if constexpr (SPLIT) {
-        const int n = e1;
-        t = uniform(int(int64_t(n) * part / pl.ranges));
-        e1 = uniform(int(int64_t(n) * (part + 1) / pl.ranges));
-    }
-    RowState st;
-    clear(st);
-    if (t < e1) {
-        const LdsOffsets off = lds_offsets(lane);
-        bf16x8 qr[8];
-        load_q(pg, f.t0 + token, head, half, qr);
-        const int kr = wave * 8 + (lane >> 3), j = lane & 7;           // this thread's key and 16 dims
-        const int last = (f.keys - 1) & ~7;
-        Mx4Pages pages = mx4_pages(pg, b, kvh, min(t * BN + wave * 8, last), pl.by_page, lane);
-        u32x2 ck, cv;
-        uint32_t ks, vs;
-        auto load = [&](int at) {
-            if (at >= e1) return;
-            const int64_t r = pages.row(min(at * BN + wave * 8, last), pl.by_page, lane);
-            ck = *reinterpret_cast<const u32x2*>(static_cast<const char*>(pg.k_cache) + r * MX4_CODES + lane * 8);
-            cv = *reinterpret_cast<const u32x2*>(static_cast<const char*>(pg.v_cache) + r * MX4_CODES + lane * 8);
-            ks = *reinterpret_cast<const uint32_t*>(static_cast<const char*>(a.k_scales) + r * MX4_SCALES + (lane >> 3) * 4);
-            vs = *reinterpret_cast<const uint32_t*>(static_cast<const char*>(a.v_scales) + r * MX4_SCALES + (lane >> 3) * 4);
-        };
-        const uint32_t k0 = kr * ROW_BYTES + (((2 * j) ^ k_swz(kr)) << 4), k1 = kr * ROW_BYTES + (((2 * j + 1) ^ k_swz(kr)) << 4);
-        const uint32_t v0 = kr * ROW_BYTES + (((2 * j) ^ v_swz(kr)) << 4), v1 = kr * ROW_BYTES + (((2 * j + 1) ^ v_swz(kr)) << 4);
-        auto store = [&](int at, int stage) {
-            if (at >= e1) return;
-            const bool in = at * BN + kr < f.keys;
-            const uint32_t ksc = in ? ks : 0u, vsc = in ? vs : 0u;
-            const uint32_t kb = mx4_has_255(vsc) ? 255u : ksc >> (8 * (j >> 1)) & 255u;
-            const uint32_t byte = vsc >> (8 * (j >> 1)) & 255u;
-            const bool none = !in || byte == 255u;
-            const float sk = mx4_scale(kb), sv = mx4_scale(none ? 0u : byte);
-            unsigned char* k = smem + stage * 2 * TILE_BYTES;
-            unsigned char* v = k + TILE_BYTES;
-            auto put = [](unsigned char* p, bf16x8 x) { *reinterpret_cast<FAV4_LDS bf16x8*>((FAV4_LDS void*)p) = x; };
-            put(k + k0, mx4_values(ck[0], sk));
-            put(k + k1, mx4_values(ck[1], sk));
-            put(v + v0, mx4_values(none ? 0u : cv[0], sv));
-            put(v + v1, mx4_values(none ? 0u : cv[1], sv));
-        };
-        const bool idle = qw >= rows;
-        const int t0 = t;
-        load(t);
-        store(t, 0);
-        load(t + 1);
-        int stage = 0;
-        auto steps = [&](auto masked, int to) {
-            for (; t < to; ++t) {
-                __syncthreads();
-                store(t + 1, stage ^ 1);
-                load(t + 2);
-                const unsigned char* cur = smem + stage * 2 * TILE_BYTES;
-                if (!idle)
-                    attend_fused<BN, decltype(masked)::value, true, LSE, true>(cur, cur + TILE_BYTES, off, qr, st, t == t0,
-                                                                               t * BN, f.keys, lim, half, scale2);
-                stage ^= 1;
+        const int live = min(32, rows - qw);
+        const float inv = st.lb == 0.f ? 0.f : 1.f / st.lb;
+        const uint32_t slot = wave * 2048;
+        if (live <= 0) return;
+        if (split) {
+            const int64_t prow = (int64_t(kvh) * 2 * pl.ranges + block) * MX4_BM + wave * 32;
+            store_part_rows<TILE_BYTES, true>(st, inv, smem, slot, make_rsrc(pl.o_part + prow * D, uint32_t(live) * D * 4),
+                                              0, live, lane);
+            if (lane < live) {
+                const float sb = st.m + __builtin_amdgcn_logf(st.lb);
+                reinterpret_cast<float2*>(pl.lse_part)[prow + lane] =
+                    float2{sb, LSE ? st.m + __builtin_amdgcn_logf(st.l) : sb};
             }
-        };
-        steps(std::integral_constant<bool, false>{}, min(e1, plain / BN));
-        steps(std::integral_constant<bool, true>{}, e1);
-        __syncthreads();               // every wave has read its last tile: the stages may hold O
-    }
-    const int live = min(32, rows - qw);
-    if (live <= 0) return;
-    const float inv = st.lb == 0.f ? 0.f : 1.f / st.lb;
-    const uint32_t slot = wave * 2048;
-    if constexpr (SPLIT) {
-        const int block = id * pl.ranges + part;
-        const int64_t prow = (int64_t(kvh) * pl.blocks + block) * MX4_BM + wave * 32;
-        if (block >= pl.blocks) return;
-        store_part_rows<TILE_BYTES, true>(st, inv, smem, slot, make_rsrc(pl.o_part + prow * D, uint32_t(live) * D * 4), 0,
-                                          live, lane);
-        if (lane < live) {
-            const float sb = st.m + __builtin_amdgcn_logf(st.lb);
-            reinterpret_cast<float2*>(pl.lse_part)[prow + lane] = float2{sb, LSE ? st.m + __builtin_amdgcn_logf(st.l) : sb};
-            if (kvh == 0 && part == 0)
-                pl.notes[int64_t(f.t0) * group + row] = int2{block * MX4_BM + wave * 32 + lane, pl.ranges};
+            return;
         }
-    } else {
         // Through LDS, 32 rows x 128 bytes at a time, so that a store writes whole lines: as store_o_rows, for rows
         // that lie at any multiple of 256 bytes.
 #pragma unroll
@@ -752,12 +758,123 @@ void mx4_prefill_kernel(Fav4Mx4PagedArgs a, Mx4Plan pl) {
             pg.lse[int64_t(head) * pg.total_q + f.t0 + token] =
                 st.lb == 0.f ? -__builtin_inff() : (st.m + __builtin_amdgcn_logf(st.l)) * LN2;
     }
+};
+
+// One row tile of the batch and one K/V head a workgroup, a sequence's longest first.
+template <bool LSE>
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void mx4_prefill_kernel(Fav4Mx4PagedArgs a, Mx4Plan pl) {
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * Mx4Prefill<LSE>::TILE_BYTES];
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+    const Mx4Prefill<LSE> x{a, pl, smem, lane, wave};
+    const Fav4PagedArgs& pg = a.paged;
+    const int id = uniform(pl.by_kv_heads(blockIdx.x)), kvh = uniform(int(blockIdx.x) - id * pg.kv_heads);
+    int b = 0, before = 0;
+    for (;;) {
+        const int n = b + lane < pg.batch ? x.tiles_of(mx4_seq(pg, b + lane)) : 0, end = wave_scan(n);
+        const uint64_t hit = __builtin_amdgcn_ballot_w64(before + end > id);
+        if (hit) {
+            const int l = __builtin_ctzll(hit);
+            before = uniform(before + __builtin_amdgcn_readlane(end - n, l));
+            b = uniform(b + l);
+            break;
+        }
+        before += __builtin_amdgcn_readlane(end, 63);
+        b += 64;
+        if (b >= pg.batch) return;
+    }
+    Mx4Seq f = mx4_seq(pg, b);
+    f = {uniform(f.t0), uniform(f.tokens), uniform(f.keys)};
+    const int rt = uniform(x.tiles_of(f)) - 1 - (id - before);
+    x.attend(b, f, rt, kvh, 0, uniform(x.key_tiles(f, rt)), false, 0);
+}
+
+// A range of the line.  The workgroup first lays out the line in LDS: the sequences'
+// row tiles by a sum over the sequences, then each row tile's units by one over those.
+// (Of tiles past MX4_LINE_TILES, which only bad offsets can make, nothing is attended.)
+template <bool LSE>
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2)))
+void mx4_prefill_line_kernel(Fav4Mx4PagedArgs a, Mx4Plan pl) {
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * Mx4Prefill<LSE>::TILE_BYTES];
+    __shared__ int seq_end[MX4_LINE_SEQS], unit_end[MX4_LINE_TILES], waves[8];
+    __shared__ uint16_t seq_of[MX4_LINE_TILES];
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
+    const Mx4Prefill<LSE> x{a, pl, smem, lane, wave};
+    const Fav4PagedArgs& pg = a.paged;
+    const int w = uniform(pl.by_kv_heads(blockIdx.x)), kvh = uniform(int(blockIdx.x) - w * pg.kv_heads);
+    // The sum of x over threads 0..tid; `all` gets that over the workgroup.
+    auto scan = [&](int v, int& all) {
+        const int mine = wave_scan(v);
+        __syncthreads();
+        if (lane == 63) waves[wave] = mine;
+        __syncthreads();
+        int before = 0;
+        all = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (i < wave) before += waves[i];
+            all += waves[i];
+        }
+        return before + mine;
+    };
+    Mx4Seq f{};
+    if (tid < pg.batch) f = mx4_seq(pg, tid);
+    int tiles;
+    const int end_tile = scan(x.tiles_of(f), tiles);
+    if (tid < pg.batch) {
+        seq_end[tid] = end_tile;
+        for (int i = end_tile - x.tiles_of(f); i < min(end_tile, MX4_LINE_TILES); ++i) seq_of[i] = uint16_t(tid);
+    }
+    tiles = min(uniform(tiles), MX4_LINE_TILES);
+    __syncthreads();
+    int units = 0;
+    for (int i0 = 0; i0 < tiles; i0 += 512) {
+        const int i = i0 + tid;
+        int c = 0;
+        if (i < tiles) {
+            const int b = seq_of[i];
+            c = max(1, x.key_tiles(mx4_seq(pg, b), i - (b > 0 ? seq_end[b - 1] : 0))) + MX4_MANY_LEAD;
+        }
+        int all;
+        const int end = units + scan(c, all);
+        if (i < tiles) unit_end[i] = end;
+        units += all;
+    }
+    __syncthreads();
+    units = uniform(units);
+    const int per = max(udiv_up(units, pl.ranges), 1), g0 = w * per, g1 = min(g0 + per, units);
+    // The first row tile that ends behind unit g0.
+    int lo = 0, hi = tiles;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (unit_end[mid] > g0) hi = mid;
+        else lo = mid + 1;
+    }
+    int4 note{};
+    for (int i = uniform(lo); i < tiles; ++i) {
+        const int base = uniform(i > 0 ? unit_end[i - 1] : 0), end = uniform(unit_end[i]);
+        if (base >= g1) break;
+        const int b = uniform(seq_of[i]), rt = i - uniform(b > 0 ? seq_end[b - 1] : 0);
+        Mx4Seq f = mx4_seq(pg, b);
+        f = {uniform(f.t0), uniform(f.tokens), uniform(f.keys)};
+        const int n = uniform(x.key_tiles(f, rt)), first = end - max(n, 1);
+        if (first >= g1) break;
+        const bool before = first < g0, split = before || end > g1;
+        const int block = mx4_block(w, before);
+        x.attend(b, f, rt, kvh, max(0, g0 - first), min(n, g1 - first), split, block);
+        if (split && !before)
+            note = int4{f.t0 * pl.group + rt * MX4_BM, min(MX4_BM, f.tokens * pl.group - rt * MX4_BM),
+                        udiv(end - 1, per) - w + 1, 0};
+        __syncthreads();               // O has left the stages
+    }
+    if (kvh == 0 && tid == 0) pl.notes[w] = note;
 }
 
 // ---- Merge --------------------------------------------------------------------------
-// Rows whose keys were split.  PER teams of 16 lanes share one row of one head, 8 dims a
-// lane; a team takes every PER-th part, eight at a time with all their loads in flight,
-// with the running maximum and sums of a softmax over the parts' log-sums.
+// The row tiles that were cut: workgroup by workgroup 16 / PER rows of a range's, with one
+// K/V head.  PER teams of 16 lanes share a row, 8 dims a lane; a team takes every PER-th
+// part, eight at a time with all their loads in flight, with the running maximum and sums
+// of a softmax over the parts' log-sums.
 template <int PER>
 __global__ __launch_bounds__(256) void mx4_merge_kernel(Fav4Mx4PagedArgs a, Mx4Plan pl) {
     constexpr int RPB = 16 / PER, NS = PER == 1 ? 4 : 8;
@@ -766,88 +883,81 @@ __global__ __launch_bounds__(256) void mx4_merge_kernel(Fav4Mx4PagedArgs a, Mx4P
     const Fav4PagedArgs& pg = a.paged;
     const int grp = threadIdx.x >> 4, l16 = threadIdx.x & 15;
     const int slot = grp / PER, part = grp - slot * PER;
-    const uint32_t rows = uint32_t(pg.total_q) * uint32_t(pg.heads), blocks = (rows + RPB - 1) / RPB;
-    for (uint32_t blk = blockIdx.x; blk < blocks; blk += gridDim.x) {
-        const uint32_t r = blk * RPB + slot;                   // token * heads + head
-        const int tok = pl.by_heads(int(min(r, rows - 1))), head = int(min(r, rows - 1) - uint32_t(tok) * uint32_t(pg.heads));
-        const int kvh = pl.by_group(head), hg = head - kvh * pl.group;
-        // Rows in no sequence have no note.  Clamped: bad offsets leave notes unwritten.
-        const bool live = r < rows && tok >= pg.cu_seqlens_q[0] && tok < pg.cu_seqlens_q[pg.batch];
-        int first = 0, total = 0;
-        if (live) {
-            const int2 note = pl.notes[int64_t(tok) * pl.group + hg];
-            first = min(max(note.x, 0), pl.blocks * pl.stride - 1);
-            total = min(max(note.y, 0), pl.blocks - pl.by_stride(first));
-        }
-        const int64_t at = int64_t(kvh) * pl.blocks * pl.stride + first;
-        float mb = -__builtin_inff(), ml = mb, den = 0.f, suml = 0.f;
-        f32x4 acc[2] = {};
-        for (int c0 = part; c0 < total; c0 += PER * NS) {
-            // Loads past the last part repeat it, with weight 0: no branch between the loads.
-            float2 v[NS];
-            f32x4 xo[NS][2];
+    const int chunks = pl.stride / RPB, piece = pl.by_merge(blockIdx.x), r0 = (int(blockIdx.x) - piece * chunks) * RPB;
+    const int w = pl.by_kv_heads(piece), kvh = piece - w * pg.kv_heads;
+    const int4 note = pl.notes[w];
+    if (r0 >= note.y || note.z <= 0) return;
+    const int r = r0 + slot, total = min(note.z, pl.ranges - w);
+    const bool live = r < note.y;
+    const int tok = pl.by_group(note.x + min(r, note.y - 1)), head = kvh * pl.group + note.x + r - tok * pl.group;
+    const int64_t at = (int64_t(kvh) * 2 * pl.ranges + mx4_block(w, false)) * pl.stride + min(r, note.y - 1);
+    float mb = -__builtin_inff(), ml = mb, den = 0.f, suml = 0.f;
+    f32x4 acc[2] = {};
+    for (int c0 = part; c0 < total; c0 += PER * NS) {
+        // Loads past the last part repeat it, with weight 0: no branch between the loads.
+        float2 v[NS];
+        f32x4 xo[NS][2];
 #pragma unroll
-            for (int i = 0; i < NS; ++i) {
-                const int64_t row = at + int64_t(min(c0 + i * PER, total - 1)) * pl.stride;
-                v[i] = reinterpret_cast<const float2*>(pl.lse_part)[row];
-                const f32x4* o = reinterpret_cast<const f32x4*>(pl.o_part + row * D + l16 * 8);
-                xo[i][0] = o[0], xo[i][1] = o[1];
-            }
+        for (int i = 0; i < NS; ++i) {
+            const int64_t row = at + int64_t(mx4_part(min(c0 + i * PER, total - 1))) * pl.stride;
+            v[i] = reinterpret_cast<const float2*>(pl.lse_part)[row];
+            const f32x4* o = reinterpret_cast<const f32x4*>(pl.o_part + row * D + l16 * 8);
+            xo[i][0] = o[0], xo[i][1] = o[1];
+        }
+#pragma unroll
+        for (int i = 0; i < NS; ++i)
+            if (c0 + i * PER >= total) v[i] = float2{-__builtin_inff(), -__builtin_inff()};
+        float nb = mb, nl = ml;
+#pragma unroll
+        for (int i = 0; i < NS; ++i) nb = fmaxf(nb, v[i].x), nl = fmaxf(nl, v[i].y);
+        if (nb == -__builtin_inff()) {
+            // Parts without a visible key, or with sums that are no numbers (which maxima
+            // pass over): so are then O and the LSE.
 #pragma unroll
             for (int i = 0; i < NS; ++i)
-                if (c0 + i * PER >= total) v[i] = float2{-__builtin_inff(), -__builtin_inff()};
-            float nb = mb, nl = ml;
-#pragma unroll
-            for (int i = 0; i < NS; ++i) nb = fmaxf(nb, v[i].x), nl = fmaxf(nl, v[i].y);
-            if (nb == -__builtin_inff()) {
-                // Parts without a visible key, or with sums that are no numbers (which maxima
-                // pass over): so are then O and the LSE.
-#pragma unroll
-                for (int i = 0; i < NS; ++i)
-                    if (v[i].x != v[i].x) den = suml = __builtin_nanf("");
-                continue;
-            }
-            const float keep = exp2_native(mb - nb);
-            acc[0] *= keep, acc[1] *= keep;
-            den *= keep;
-            suml *= exp2_native(ml - nl);
-            mb = nb, ml = nl;
-#pragma unroll
-            for (int i = 0; i < NS; ++i) {
-                const float wgt = exp2_native(v[i].x - mb);
-                if (wgt != 0.f) acc[0] += wgt * xo[i][0], acc[1] += wgt * xo[i][1];
-                den += wgt;
-                suml += exp2_native(v[i].y - ml);
-            }
+                if (v[i].x != v[i].x) den = suml = __builtin_nanf("");
+            continue;
         }
-        if constexpr (PER > 1) {
-            if (l16 == 0) red[grp] = float4{mb, ml, den, suml};
-            red_o[grp][l16 * 2] = acc[0], red_o[grp][l16 * 2 + 1] = acc[1];
-            __syncthreads();
+        const float keep = exp2_native(mb - nb);
+        acc[0] *= keep, acc[1] *= keep;
+        den *= keep;
+        suml *= exp2_native(ml - nl);
+        mb = nb, ml = nl;
 #pragma unroll
-            for (int p = 0; p < PER; ++p) mb = fmaxf(mb, red[slot * PER + p].x), ml = fmaxf(ml, red[slot * PER + p].y);
-            den = suml = 0.f;
-            acc[0] = acc[1] = f32x4{};
-#pragma unroll
-            for (int p = 0; p < PER; ++p) {
-                const float4 o = red[slot * PER + p];
-                if (o.z == 0.f) continue;                      // no part with a visible key
-                const float wgt = exp2_native(o.x - mb);
-                den += wgt * o.z;
-                suml += exp2_native(o.y - ml) * o.w;
-                acc[0] += wgt * red_o[slot * PER + p][l16 * 2], acc[1] += wgt * red_o[slot * PER + p][l16 * 2 + 1];
-            }
-            __syncthreads();
+        for (int i = 0; i < NS; ++i) {
+            const float wgt = exp2_native(v[i].x - mb);
+            if (wgt != 0.f) acc[0] += wgt * xo[i][0], acc[1] += wgt * xo[i][1];
+            den += wgt;
+            suml += exp2_native(v[i].y - ml);
         }
-        if (!live || part != 0 || total == 0) continue;        // (no parts: finished where it was attended)
-        const float rden = den == 0.f ? 0.f : 1.f / den;
-        bf16x8 y;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = __bf16(acc[i >> 2][i & 3] * rden);
-        *reinterpret_cast<bf16x8*>(static_cast<char*>(pg.o) + int64_t(r) * ROW_BYTES + l16 * 16) = y;
-        if (pg.lse && l16 == 0) pg.lse[int64_t(head) * pg.total_q + tok] =
-            den == 0.f ? -__builtin_inff() : (ml + __builtin_amdgcn_logf(suml)) * LN2;
     }
+    if constexpr (PER > 1) {
+        if (l16 == 0) red[grp] = float4{mb, ml, den, suml};
+        red_o[grp][l16 * 2] = acc[0], red_o[grp][l16 * 2 + 1] = acc[1];
+        __syncthreads();
+#pragma unroll
+        for (int p = 0; p < PER; ++p) mb = fmaxf(mb, red[slot * PER + p].x), ml = fmaxf(ml, red[slot * PER + p].y);
+        den = suml = 0.f;
+        acc[0] = acc[1] = f32x4{};
+#pragma unroll
+        for (int p = 0; p < PER; ++p) {
+            const float4 o = red[slot * PER + p];
+            if (o.z == 0.f) continue;                      // no part with a visible key
+            const float wgt = exp2_native(o.x - mb);
+            den += wgt * o.z;
+            suml += exp2_native(o.y - ml) * o.w;
+            acc[0] += wgt * red_o[slot * PER + p][l16 * 2], acc[1] += wgt * red_o[slot * PER + p][l16 * 2 + 1];
+        }
+        __syncthreads();
+    }
+    if (!live || part != 0) return;
+    const float rden = den == 0.f ? 0.f : 1.f / den;
+    bf16x8 y;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = __bf16(acc[i >> 2][i & 3] * rden);
+    *reinterpret_cast<bf16x8*>(static_cast<char*>(pg.o) + (int64_t(tok) * pg.heads + head) * ROW_BYTES + l16 * 16) = y;
+    if (pg.lse && l16 == 0) pg.lse[int64_t(head) * pg.total_q + tok] =
+        den == 0.f ? -__builtin_inff() : (ml + __builtin_amdgcn_logf(suml)) * LN2;
 }
 
 }  // namespace fav4
