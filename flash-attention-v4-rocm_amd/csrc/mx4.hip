@@ -92,6 +92,8 @@ bool paged_shape_ok(const Fav4Mx4PagedArgs* args, int causal) {
            int64_t(a.total_q) * a.heads <= INT_MAX && caches_fit(a.num_pages, a.page_size, a.kv_heads);
 }
 
+constexpr int SUB1 = 2, DEP1 = 1, EU1 = 3, PER1 = 3, SUB2 = 4, DEP2 = 1, EU2 = 2, PER2 = 2, SW = 4, UW = 8, USUB1 = 4, UEU1 = 2;
+constexpr int FEW_PER_CU = 3, MIN_KEYS = 384, USPLIT = 2048, SEG_CU = 4;
 // Up to this many rows a sequence go by the decode kernel.
 constexpr int FEW_ROWS = 64;
 
@@ -112,15 +114,17 @@ Sizes paged_sizes(const Fav4Mx4PagedArgs& args, int causal) {
     p.group = int(group);
     p.br = causal == BOTTOM_RIGHT;
     s.few = seq_rows <= FEW_ROWS;
-    // Workgroups of a K/V head that are resident at once: two of four waves a CU, or one of eight.
-    const int few_ranges = std::max(1, 2 * cus / a.kv_heads), many_ranges = std::max(1, cus / a.kv_heads);
+    // Workgroups of a K/V head that are resident at once: FEW_PER_CU a CU with few rows, one of eight waves with many.
+    const int few_ranges = std::max(1, FEW_PER_CU * cus / a.kv_heads), many_ranges = std::max(1, cus / a.kv_heads);
     int64_t segs;
     if (s.few) {
         p.stride = seq_rows <= 16 ? 16 : 32;
         p.tiles = int((seq_rows + p.stride - 1) / p.stride);
         segs = int64_t(a.batch) * p.tiles;
-        s.split = segs * a.kv_heads < 4 * cus && a.max_seqlen_k > 2048;
-        p.ranges = s.split ? few_ranges : 1;
+        const int resident = std::max(1, (p.stride == 16 ? PER1 : PER2) * cus / a.kv_heads);
+        const int64_t keys = a.total_k > 0 ? a.total_k : int64_t(a.batch) * a.max_seqlen_k;
+        s.split = segs * a.kv_heads < SEG_CU * cus && a.max_seqlen_k > USPLIT;
+        p.ranges = s.split ? int(std::min<int64_t>(resident, keys * p.tiles / MIN_KEYS + 1)) : 1;
     } else {
         segs = std::min<int64_t>(a.batch * ((seq_rows + fav4::MX4_BM - 1) / fav4::MX4_BM),
                                  (rows + int64_t(a.batch) * (fav4::MX4_BM - 1)) / fav4::MX4_BM);
@@ -138,8 +142,9 @@ Sizes paged_sizes(const Fav4Mx4PagedArgs& args, int causal) {
     p.by_page = fav4::fast_div(a.page_size);
     // Teams per merged row: many where the row tiles are few and cut into many parts.
     s.merge_teams = s.few ? 4 : 1;
-    s.merge_grid = int64_t(p.ranges) * a.kv_heads * (p.stride * s.merge_teams / 16);
-    p.by_merge = fav4::fast_div(p.stride * s.merge_teams / 16);
+    p.merge_chunks = int((std::min<int64_t>(p.stride, seq_rows) * s.merge_teams + 15) / 16);
+    s.merge_grid = int64_t(p.ranges) * a.kv_heads * p.merge_chunks;
+    p.by_merge = fav4::fast_div(p.merge_chunks);
     // What a call of either kind could need: more queries or sequences never need less.
     s.part_rows = int64_t(a.kv_heads) * 2 * (s.few ? few_ranges * 32 : std::max(few_ranges * 32, many_ranges * fav4::MX4_BM));
     s.bytes = s.part_rows * (fav4::D * 4 + 8) + int64_t(few_ranges) * 16;
@@ -151,8 +156,15 @@ void launch_few(const Fav4Mx4PagedArgs& a, const Sizes& s, hipStream_t stream) {
     auto go = [&](auto kernel, int waves) {
         hipLaunchKernelGGL(kernel, dim3(unsigned(s.grid)), dim3(waves * 64), 0, stream, a, s.plan);
     };
-    if (s.split) go(fav4::mx4_decode_kernel<NT, 4, true>, 4);
-    else go(fav4::mx4_decode_kernel<NT, 8, false>, 8);
+    auto with = [&](auto lse, auto p64) {
+        constexpr bool L = decltype(lse)::value, P = decltype(p64)::value;
+        constexpr int SUB = NT == 1 ? SUB1 : SUB2, DEP = NT == 1 ? DEP1 : DEP2, EU = NT == 1 ? EU1 : EU2, USUB = NT == 1 ? USUB1 : SUB2, UEU = NT == 1 ? UEU1 : EU2;
+        if (s.split) go(fav4::mx4_decode_kernel<NT, SW, SUB, DEP, EU, true, L, P>, SW);
+        else go(fav4::mx4_decode_kernel<NT, UW, USUB, DEP, UEU, false, L, P>, UW);
+    };
+    const bool p64 = a.paged.page_size % 64 == 0;
+    if (a.paged.lse) p64 ? with(std::true_type{}, std::true_type{}) : with(std::true_type{}, std::false_type{});
+    else p64 ? with(std::false_type{}, std::true_type{}) : with(std::false_type{}, std::false_type{});
 }
 
 }  // namespace

@@ -6,6 +6,7 @@
 
 namespace fav4 {
 
+constexpr int MX4_VPAD = 16;
 constexpr int MX4_CODES = D / 2, MX4_SCALES = D / 32;      // bytes of a cache row
 
 __device__ __forceinline__ float mx4_scale(uint32_t byte) { return __uint_as_float(byte << 23); }
@@ -19,8 +20,11 @@ __device__ __forceinline__ bf16x8 mx4_values(uint32_t codes, float scale) {
     return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// Whether one of four bytes is 255.
-__device__ __forceinline__ bool mx4_has_255(uint32_t x) { return ((~x - 0x01010101u) & x & 0x80808080u) != 0; }
+// Whether one of four scales is above 252.  (Adding 3 to a byte's low seven bits carries
+// into its top bit from 125 on.)
+__device__ __forceinline__ bool mx4_no_numbers(uint32_t x) {
+    return (((x & 0x7f7f7f7fu) + 0x03030303u) & x & 0x80808080u) != 0;
+}
 
 // ---------------------------------------------------------------------------
 // Append.  The layout of append_kernel: one wave takes 8 of a token's heads + 2 *
@@ -236,7 +240,7 @@ struct Mx4Plan {
     int group;                        // query heads of a K/V head
     int ranges;                       // of a K/V head
     FastDiv by_kv_heads, by_group, by_page, by_merge;
-    int stride;
+    int stride, merge_chunks;         // rows of a partial block; workgroups of the merge for those that can be live
     int tiles;                        // row tiles that a sequence (few rows) or the batch (many) can have
     int br;                           // bottom-right causal
 };
@@ -294,154 +298,190 @@ __device__ __forceinline__ float quad_sum(float x) {
 }
 
 // ---- Few rows ---------------------------------------------------------------------
-// A workgroup's waves all take the same NT * 16 rows, and every WAVES-th tile of 64
-// keys of a part of the keys; they join in LDS.  Per tile a wave loads 4 KiB of codes of
-// K and of V and 256 bytes of scales of each, straight into registers and a tile ahead.
+// A workgroup's waves all take the same NT * 16 rows, and every WAVES-th tile of SUB * 16
+// keys of a part of the keys; they join in LDS.  Codes and scales are loaded straight into
+// registers, each as soon as the one before has been used.
 //  * S^T = K Q^T on 16x16x32 MFMAs: lane l has key l % 16 of a subtile and the block
 //    of 32 dims l / 16, 16 bytes of codes and one scale; the four dwords of codes are
 //    the four k-steps, whose order over the dims is free as long as Q's is the same.
 //  * O^T += V^T P^T: P leaves the accumulators as the B operand, lane l / 16 = g
 //    holding keys 4g + e of both subtiles of 32 keys.  V is converted as K is and goes
-//    through 8 KiB of LDS of the wave's own, from where ds_read_b64_tr_b16 reads it
-//    turned.  Keys are masked by their scores, so V needs no other care than to be
-//    finite: a block without numbers becomes 0 there, and its key's scores NaN by way of
-//    its K scale.
+//    through LDS of the wave's own, from where ds_read_b64_tr_b16 reads it turned.  The
+//    sums of the weights come from one more MFMA, against ones.
+//  * Keys are hidden by their scores, so V needs no other care than to be finite: a block
+//    with a scale above 252 becomes 0 there, and its key's scores NaN by way of its K
+//    scale.
 template <int NT>
 struct Mx4State {
-    f32x4 o[NT][8];
-    float m[NT], lb[NT], l[NT];       // base (log2), sums of the BF16 and the FP32 weights of this lane's keys
+    f32x4 o[NT][8], lb[NT];           // lb: sums of the BF16 weights, over all lanes
+    float m[NT], l[NT];               // base (log2), sums of the FP32 weights of this lane's keys
 };
+template <int SUB>
 struct Mx4Tile {
-    u32x4 k[4], v[4];
-    uint32_t ks[4], vs[4];
+    u32x4 k[SUB], v[SUB];
+    uint32_t ks[SUB], vs[SUB];
 };
 
-template <int NT, int WAVES>
+// P64: pages of a multiple of 64 keys, so that a tile lies in one.
+template <int NT, int WAVES, int SUB, int DEPTH, bool LSE, bool P64>
 struct Mx4Decode {
-    static constexpr int SLOT = 32 * ROW_BYTES, BM = NT * 16;
+    static constexpr int VROW = ROW_BYTES + MX4_VPAD, SLOT = 32 * VROW, BM = NT * 16, BN = SUB * 16;
+    static_assert(BN == 64 || BN == 32, "tiles lie in a page of a multiple of 64 keys");
     const Fav4Mx4PagedArgs& a;
     const Mx4Plan& pl;
     unsigned char* smem;              // WAVES slots
     float4 (*stats)[16];              // [WAVES][16]
     int lane, wave;
 
-    // The cache rows of a tile's subtiles; those past the keys repeat the last one, and are masked.
-    __device__ __forceinline__ void rows(int64_t (&row)[4], int t, int keys, Mx4Pages& pages) const {
-        const int last = (keys - 1) & ~15;
+    // Where this wave's tiles lie: the cache rows of the next 64 (with small pages: of the
+    // subtiles of the next 64 / SUB) in the lanes.
+    static constexpr int PIECES = P64 ? 1 : SUB, HELD = 64 / PIECES;
+    struct Places {
+        const int* table;
+        int64_t head_row;             // of the head within a page
+        int first, lo, hi;            // tile of lane 0; this lane's cache row
+    };
+    __device__ __forceinline__ void hold(Places& p, int t) const {
+        const Fav4PagedArgs& pg = a.paged;
+        p.first = t;
+        const int key = min(t + lane / PIECES * WAVES, pg.max_seqlen_k / BN) * BN + lane % PIECES * 16;
+        const int slot = pl.by_page(key), entry = p.table[min(slot, pg.max_pages_per_seq - 1)];
+        const int page = min(max(entry, 0), pg.num_pages - 1);
+        const int64_t row = int64_t(page) * pg.kv_heads * pg.page_size + p.head_row + (key - slot * pg.page_size);
+        p.lo = int(row), p.hi = int(row >> 32);
+    }
+    // Of sequence b with head kvh, this wave's tiles from t on.
+    __device__ __forceinline__ Places places(int b, int kvh, int t) const {
+        Places p{a.paged.block_table + int64_t(b) * a.paged.max_pages_per_seq, int64_t(kvh) * a.paged.page_size, t};
+        hold(p, t);
+        return p;
+    }
+    struct Rows {
+        int64_t at[PIECES];
+    };
+    __device__ __forceinline__ Rows rows(int t, Places& p) const {
+        int e = uniform((t - p.first) / WAVES);
+        if (e >= HELD) hold(p, t), e = 0;
+        Rows r;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) row[i] = pages.row(min(t * 64 + i * 16, last), pl.by_page, lane);
+        for (int i = 0; i < PIECES; ++i)
+            r.at[i] = int64_t(uint32_t(__builtin_amdgcn_readlane(p.lo, e * PIECES + i))) |
+                      int64_t(__builtin_amdgcn_readlane(p.hi, e * PIECES + i)) << 32;
+        return r;
     }
-    __device__ __forceinline__ void load_k(Mx4Tile& x, int i, int64_t row) const {
-        const char* k = static_cast<const char*>(a.paged.k_cache) + row * MX4_CODES;
-        const char* ks = static_cast<const char*>(a.k_scales) + row * MX4_SCALES;
-        const char* vs = static_cast<const char*>(a.v_scales) + row * MX4_SCALES;
-        const uint32_t at = uint32_t(lane & 15), g = uint32_t(lane >> 4);
-        x.k[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(k + at * MX4_CODES + g * 16));
-        x.ks[i] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(ks + at * MX4_SCALES));
-        x.vs[i] = __builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(vs + at * MX4_SCALES));
+    // Subtile i's first byte of a cache with `bytes` a row.
+    __device__ __forceinline__ const char* at(const void* cache, const Rows& r, int i, int bytes) const {
+        return static_cast<const char*>(cache) + (P64 ? r.at[0] * bytes + i * 16 * bytes : r.at[P64 ? 0 : i] * bytes);
     }
-    __device__ __forceinline__ void load_v(Mx4Tile& x, int i, int64_t row) const {
-        const char* v = static_cast<const char*>(a.paged.v_cache) + row * MX4_CODES;
-        x.v[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(v + (lane & 15) * MX4_CODES + (lane >> 4) * 16));
+    __device__ __forceinline__ void load_k(Mx4Tile<SUB>& x, const Rows& r) const {
+        const uint32_t code = uint32_t(lane & 15) * MX4_CODES + uint32_t(lane >> 4) * 16;
+        const uint32_t scale = uint32_t(lane & 15) * MX4_SCALES + uint32_t(lane >> 4);
+#pragma unroll
+        for (int i = 0; i < SUB; ++i) {
+            x.k[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(at(a.paged.k_cache, r, i, MX4_CODES) + code));
+            x.ks[i] = *reinterpret_cast<const uint8_t*>(at(a.k_scales, r, i, MX4_SCALES) + scale);
+            x.vs[i] = *reinterpret_cast<const uint8_t*>(at(a.v_scales, r, i, MX4_SCALES) + scale);
+        }
+    }
+    __device__ __forceinline__ void load_v(Mx4Tile<SUB>& x, const Rows& r, int i) const {
+        const uint32_t code = uint32_t(lane & 15) * MX4_CODES + uint32_t(lane >> 4) * 16;
+        x.v[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(at(a.paged.v_cache, r, i, MX4_CODES) + code));
     }
 
-    // Tile t, in x; the tile at `next` (if any) is loaded in its place, each register as soon as it has been used.
-    __device__ __forceinline__ void tile(Mx4Tile& x, const bf16x8 (&q)[NT][4], Mx4State<NT>& st, bool first, int t,
-                                         int next, bool masked, int keys, const int (&lim)[NT], float scale2,
-                                         Mx4Pages& pages) const {
-        const int col = lane & 15, g = lane >> 4, start = t * 64;
-        uint32_t vb[4];
-        f32x4 s[NT][4];
-        int64_t row[4];
-        if (next >= 0) rows(row, next, keys, pages);
+    // Tile t, in x; this wave's tile DEPTH tiles on is loaded in its place (behind the last
+    // one that again: with the loads behind a branch the compiler could no longer tell how
+    // many are under way, and would wait for the newest where it needs the oldest).
+    __device__ __forceinline__ void tile(Mx4Tile<SUB>& x, const bf16x8 (&q)[NT][4], Mx4State<NT>& st, int t, int last, bool masked,
+                                         const int (&lim)[NT], float scale2, Places& where) const {
+        const int col = lane & 15, g = lane >> 4;
+        const Rows r = rows(min(t + DEPTH * WAVES, last), where);
+        uint32_t most = x.vs[0];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            uint32_t ks = x.ks[i], vs = x.vs[i];
-            if (masked) {
-                const bool in = start + i * 16 + col < keys;
-                ks = in ? ks : 0, vs = in ? vs : 0;
-            }
-            const uint32_t kb = mx4_has_255(vs) ? 255u : ks >> (8 * g) & 255u;
-            vb[i] = vs >> (8 * g) & 255u;
-            const float scale = mx4_scale(kb);
-            bf16x8 kop[4];
+        for (int i = 1; i < SUB; ++i) most = max(most, x.vs[i]);
+        if (__builtin_amdgcn_ballot_w64(most > 252u)) {
 #pragma unroll
-            for (int c = 0; c < 4; ++c) kop[c] = mx4_values(x.k[i][c], scale);
-#pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                s[n][i] = f32x4{};
-#pragma unroll
-                for (int c = 0; c < 4; ++c) s[n][i] = mfma16(kop[c], q[n][c], s[n][i]);
+            for (int i = 0; i < SUB; ++i) {
+                const bool none = x.vs[i] > 252u;
+                uint64_t keys_of = __builtin_amdgcn_ballot_w64(none);
+                keys_of |= keys_of >> 32;
+                keys_of |= keys_of >> 16;
+                x.ks[i] = keys_of >> col & 1 ? 255u : x.ks[i];
+                x.vs[i] = none ? 127u : x.vs[i];
+                x.v[i] = none ? u32x4{} : x.v[i];
             }
         }
-        if (next >= 0) {
+        uint32_t vb[SUB];
+        f32x4 s[NT][SUB];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) load_k(x, i, row[i]);
-        }
-        bf16x8 p[NT][2];
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int i = 0; i < SUB; ++i) {
+                const bf16x8 kop = mx4_values(x.k[i][c], mx4_scale(x.ks[i]));
+#pragma unroll
+                for (int n = 0; n < NT; ++n) s[n][i] = mfma16(kop, q[n][c], c ? s[n][i] : f32x4{});
+            }
+#pragma unroll
+        for (int i = 0; i < SUB; ++i) vb[i] = x.vs[i];
+        load_k(x, r);
+        bf16x8 p[NT][SUB / 2];
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             if (masked) {
-                const int d = lim[n] - start - 4 * g;
+                const int d = lim[n] - t * BN - 4 * g;
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
+                for (int i = 0; i < SUB; ++i)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) s[n][i][e] = i * 16 + e > d ? -__builtin_inff() : s[n][i][e];
             }
             float mx = -__builtin_inff();
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
+            for (int i = 0; i < SUB; ++i)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) mx = fmaxf(mx, s[n][i][e]);
             // The base moves where a maximum passes it by more than the threshold.
             const float cand = fmaxf(st.m[n], quad_max(mx) * scale2);
-            const bool update = first || cand > st.m[n] + RESCALE_THRESHOLD;
-            const float now = update ? cand : st.m[n];
-            const float base = now == -__builtin_inff() ? 0.f : now;        // rows that have seen no key
-            const float alpha = exp2_native(st.m[n] - base);
-            const bool rescale = !first && __builtin_amdgcn_ballot_w64(update) != 0;
-            st.m[n] = now;
-            float lb = 0.f, l = 0.f;
+            const bool update = cand > st.m[n] + RESCALE_THRESHOLD;
+            if (__builtin_amdgcn_ballot_w64(update)) {
+                const float now = update ? cand : st.m[n], alpha = update ? exp2_native(st.m[n] - now) : 1.f;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
+                for (int db = 0; db < 8; ++db) st.o[n][db] *= alpha;
+                st.lb[n] *= alpha;
+                st.l[n] *= alpha;
+                st.m[n] = now;
+            }
+            const float base = st.m[n] == -__builtin_inff() ? 0.f : st.m[n];        // rows that have seen no key
+#pragma unroll
+            for (int h = 0; h < SUB / 2; ++h)
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const float w = exp2_native(fmaf(s[n][2 * h + (j >> 2)][j & 3], scale2, -base));
-                    l += w;
+                    if constexpr (LSE) st.l[n] += w;
                     p[n][h][j] = __bf16(w);
                 }
-#pragma unroll
-                for (int j = 0; j < 4; ++j) lb = bf16_pair_sum(bf16x2{p[n][h][2 * j], p[n][h][2 * j + 1]}, lb);
-            }
-            if (rescale) {
-#pragma unroll
-                for (int db = 0; db < 8; ++db) st.o[n][db] *= alpha;
-            }
-            st.lb[n] = first ? lb : st.lb[n] * alpha + lb;
-            st.l[n] = first ? l : st.l[n] * alpha + l;
         }
-        // V, 32 keys at a time: row r's granule c at c ^ v_swz(r).
+        // V, 32 keys at a time.  Rows lie further apart than they are long: the 16 rows that
+        // an access touches then start in different banks, and the offsets within a row are
+        // constants.
         unsigned char* slot = smem + wave * SLOT;
-        const int r = lane >> 2 & 3;
+        const __bf16 one(1.f);
+        const bf16x8 ones{one, one, one, one, one, one, one, one};
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < SUB / 2; ++h) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                const uint32_t byte = vb[2 * h + i];
-                const float scale = mx4_scale(byte == 255u ? 0u : byte);
+                const float scale = mx4_scale(vb[2 * h + i]);
 #pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                    const uint32_t codes = byte == 255u ? 0u : x.v[2 * h + i][c];
-                    *reinterpret_cast<FAV4_LDS bf16x8*>((FAV4_LDS void*)(
-                        slot + (i * 16 + col) * ROW_BYTES + (((4 * g + c) ^ v_swz(col)) << 4))) = mx4_values(codes, scale);
-                }
+                for (int c = 0; c < 4; ++c)
+                    *reinterpret_cast<FAV4_LDS bf16x8*>((FAV4_LDS void*)(slot + (i * 16 + col) * VROW + (4 * g + c) * 16)) =
+                        mx4_values(x.v[2 * h + i][c], scale);
             }
-            if (next >= 0) load_v(x, 2 * h, row[2 * h]), load_v(x, 2 * h + 1, row[2 * h + 1]);
+            load_v(x, r, 2 * h), load_v(x, r, 2 * h + 1);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) st.lb[n] = mfma16(ones, p[n][h], st.lb[n]);
 #pragma unroll
             for (int db = 0; db < 8; ++db) {
-                const int vr = 4 * g + r, c = 2 * db + (lane >> 1 & 1);
-                const unsigned char* at = slot + vr * ROW_BYTES + ((c ^ v_swz(vr)) << 4) + ((lane & 1) << 3);
-                const bf16x4 lo = lds_read_tr(at), hi = lds_read_tr(at + 16 * ROW_BYTES);
+                const unsigned char* from = slot + (4 * g + (lane >> 2 & 3)) * VROW + (lane & 3) * 8 + db * 32;
+                const bf16x4 lo = lds_read_tr(from), hi = lds_read_tr(from + 16 * VROW);
                 const bf16x8 vop{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
 #pragma unroll
                 for (int n = 0; n < NT; ++n) st.o[n][db] = mfma16(vop, p[n][h], st.o[n][db]);
@@ -449,12 +489,12 @@ struct Mx4Decode {
         }
     }
 
-    // Key tiles [a0, a1) of the rows from r0 on of sequence b with head kvh.  split: the part is not all of the
-    // sequence's keys, and goes to partial block `block`.
-    __device__ __forceinline__ void attend(int b, const Mx4Seq& f, int r0, int kvh, int a0, int a1, bool split,
+    // Key tiles [a0, a1) of the rows from r0 on of sequence f with head kvh; this wave's, from a0 + wave on, lie
+    // `where`.  split: the part is not all of the sequence's keys, and goes to partial block `block`.
+    __device__ __forceinline__ void attend(const Mx4Seq& f, int r0, int kvh, Places& where, int a0, int a1, bool split,
                                            int block) const {
         const Fav4PagedArgs& pg = a.paged;
-        const int col = lane & 15, g = lane >> 4, group = pl.group, rows = f.tokens * group;
+        const int col = lane & 15, g = lane >> 4, group = pl.group, live = f.tokens * group;
         const float scale2 = pg.scale * LOG2E;
         int lim[NT];
         bf16x8 q[NT][4];
@@ -462,39 +502,47 @@ struct Mx4Decode {
         const int shift = f.keys - f.tokens;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            const int row = min(r0 + n * 16 + col, rows - 1), token = pl.by_group(row), head = kvh * group + row - token * group;
+            const int row = min(r0 + n * 16 + col, live - 1), token = pl.by_group(row), head = kvh * group + row - token * group;
             lim[n] = pl.br ? min(shift + token, f.keys - 1) : f.keys - 1;
             const char* qp = static_cast<const char*>(pg.q) + (int64_t(f.t0 + token) * pg.heads + head) * ROW_BYTES + g * 64;
 #pragma unroll
             for (int c = 0; c < 4; ++c) q[n][c] = *reinterpret_cast<const bf16x8*>(qp + c * 16);
 #pragma unroll
             for (int db = 0; db < 8; ++db) st.o[n][db] = f32x4{};
+            st.lb[n] = f32x4{};
             st.m[n] = -__builtin_inff();
-            st.lb[n] = st.l[n] = 0.f;
+            st.l[n] = 0.f;
         }
         // Tiles whose keys all rows see, and the end of those that some row sees.
-        const int i0 = pl.by_group(r0), i1 = pl.by_group(min(rows, r0 + BM) - 1);
+        const int i0 = pl.by_group(r0), i1 = pl.by_group(min(live, r0 + BM) - 1);
         const int plain = pl.br ? max(0, min(f.keys, shift + i0 + 1)) : f.keys;
         const int seen = pl.br ? max(0, min(f.keys, shift + i1 + 1)) : f.keys;
-        const int nfull = uniform(plain >> 6), e1 = uniform(min(a1, (seen + 63) >> 6));
+        const int nfull = uniform(plain / BN), e1 = uniform(min(a1, (seen + BN - 1) / BN));
         int t = a0 + wave;
         if (t < e1) {
-            Mx4Pages pages = mx4_pages(pg, b, kvh, min(t * 64, (f.keys - 1) & ~15), pl.by_page, lane);
-            Mx4Tile x;
-            int64_t row[4];
-            this->rows(row, t, f.keys, pages);
+            const int last = t + (e1 - 1 - t) / WAVES * WAVES;             // of this wave
+            Mx4Tile<SUB> x[DEPTH];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) load_k(x, i, row[i]);
+            for (int d = 0; d < DEPTH; ++d) {
+                const Rows r = rows(min(t + d * WAVES, last), where);
+                load_k(x[d], r);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) load_v(x, i, row[i]);
-            for (bool first = true; t < e1; t += WAVES, first = false)
-                tile(x, q, st, first, t, t + WAVES < e1 ? t + WAVES : -1, t >= nfull, f.keys, lim, scale2, pages);
+                for (int i = 0; i < SUB; ++i) load_v(x[d], r, i);
+            }
+            while (t < e1) {
+#pragma unroll
+                for (int d = 0; d < DEPTH; ++d) {
+                    if (t >= e1) break;
+                    tile(x[d], q, st, t, last, t >= nfull, lim, scale2, where);
+                    t += WAVES;
+                }
+            }
         }
         // Join: row n's quad of dims 4u at u ^ n of its 512 bytes.
         unsigned char* slot = smem + wave * SLOT;
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            const float lb = quad_sum(st.lb[n]), l = quad_sum(st.l[n]);
+            const float lb = st.lb[n][0], l = LSE ? quad_sum(st.l[n]) : 0.f;
             if (n > 0) __syncthreads();
 #pragma unroll
             for (int db = 0; db < 8; ++db)
@@ -503,7 +551,7 @@ struct Mx4Decode {
             __syncthreads();
             for (int id = threadIdx.x; id < 512; id += WAVES * 64) {
                 const int r = id >> 5, u = id & 31, row = r0 + n * 16 + r;
-                if (row >= rows) continue;
+                if (row >= live) continue;
                 float m = -__builtin_inff(), sb = 0.f, sl = 0.f;
 #pragma unroll
                 for (int w = 0; w < WAVES; ++w) m = fmaxf(m, stats[w][r].x);
@@ -523,14 +571,14 @@ struct Mx4Decode {
                 if (!split) {
                     const bf16x4 y{__bf16(o[0]), __bf16(o[1]), __bf16(o[2]), __bf16(o[3])};
                     *reinterpret_cast<bf16x4*>(static_cast<char*>(pg.o) + (int64_t(f.t0 + token) * pg.heads + head) * ROW_BYTES + u * 8) = y;
-                    if (pg.lse && u == 0)
+                    if (LSE && u == 0)
                         pg.lse[int64_t(head) * pg.total_q + f.t0 + token] = (base + __builtin_amdgcn_logf(sl)) * LN2;
                 } else {
                     const int64_t prow = (int64_t(kvh) * 2 * pl.ranges + block) * BM + n * 16 + r;
                     *reinterpret_cast<f32x4*>(pl.o_part + prow * D + u * 4) = o;
                     if (u == 0)
                         reinterpret_cast<float2*>(pl.lse_part)[prow] =
-                            float2{base + __builtin_amdgcn_logf(sb), base + __builtin_amdgcn_logf(sl)};
+                            float2{base + __builtin_amdgcn_logf(sb), base + __builtin_amdgcn_logf(LSE ? sl : sb)};
                 }
             }
         }
@@ -541,28 +589,27 @@ struct Mx4Decode {
 // One row tile of a sequence and one K/V head a workgroup (SPLIT false), or a range of
 // the line.
 constexpr int MX4_LEAD = 2;
-template <int NT, int WAVES, bool SPLIT>
-__global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
+template <int NT, int WAVES, int SUB, int DEPTH, int EU, bool SPLIT, bool LSE, bool P64>
+__global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(EU, EU)))
 void mx4_decode_kernel(Fav4Mx4PagedArgs a, Mx4Plan pl) {
-    constexpr int BM = NT * 16;
-    __shared__ __attribute__((aligned(1024))) unsigned char smem[WAVES * 32 * ROW_BYTES];
+    constexpr int BM = NT * 16, BN = SUB * 16;
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[WAVES * Mx4Decode<NT, WAVES, SUB, DEPTH, LSE, P64>::SLOT];
     __shared__ float4 stats[WAVES][16];
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
     const Fav4PagedArgs& pg = a.paged;
-    const Mx4Decode<NT, WAVES> decode{a, pl, smem, stats, lane, wave};
     const int w = uniform(pl.by_kv_heads(blockIdx.x)), turn = uniform(int(blockIdx.x) - w * pg.kv_heads);
-    auto uniform_seq = [&](int b) {
-        const Mx4Seq f = mx4_seq(pg, b);
-        return Mx4Seq{uniform(f.t0), uniform(f.tokens), uniform(f.keys)};
-    };
     if constexpr (!SPLIT) {
         const int b = pl.tiles > 1 ? udiv(w, pl.tiles) : w, r0 = (w - b * pl.tiles) * BM;
-        const Mx4Seq f = uniform_seq(b);
-        if (r0 < f.tokens * pl.group) decode.attend(b, f, r0, turn, 0, (f.keys + 63) >> 6, false, 0);
+        const Mx4Decode<NT, WAVES, SUB, DEPTH, LSE, P64> decode{a, pl, smem, stats, lane, wave};
+        // (The table and the lengths load side by side.)
+        auto where = decode.places(b, turn, wave);
+        Mx4Seq f = mx4_seq(pg, b);
+        f = {uniform(f.t0), uniform(f.tokens), uniform(f.keys)};
+        if (r0 < f.tokens * pl.group) decode.attend(f, r0, turn, where, 0, (f.keys + BN - 1) / BN, false, 0);
     } else {
         auto tiles_of = [&](const Mx4Seq& f) { return int(uint32_t(f.tokens * pl.group + BM - 1) / BM); };
-        auto cost_of = [&](const Mx4Seq& f) { return max(1, (f.keys + 63) >> 6) + MX4_LEAD; };
-        // Units of 64 sequences from i on, in the lanes: of each, and up to and with it.
+        auto cost_of = [&](const Mx4Seq& f) { return max(1, (f.keys + BN - 1) / BN) + MX4_LEAD; };
+        // The units of 64 sequences from i on, in the lanes: of each, and up to and with it.
         auto sums = [&](int i) {
             Mx4Seq f{};
             if (i + lane < pg.batch) f = mx4_seq(pg, i + lane);
@@ -589,8 +636,9 @@ void mx4_decode_kernel(Fav4Mx4PagedArgs a, Mx4Plan pl) {
         }
         int4 note{};
         for (; idx < pg.batch && base < g1; ++idx) {
-            const Mx4Seq f = uniform_seq(idx);
-            const int n = tiles_of(f), cost = cost_of(f), tiles = (f.keys + 63) >> 6;
+            Mx4Seq f = mx4_seq(pg, idx);
+            f = {uniform(f.t0), uniform(f.tokens), uniform(f.keys)};
+            const int n = tiles_of(f), cost = cost_of(f), tiles = (f.keys + BN - 1) / BN;
             // Neighbouring sequences are taken with neighbouring heads, as in attend_wave.
             const int kvh = uniform(turn + idx - pl.by_kv_heads(turn + idx) * pg.kv_heads);
             for (int rt = 0; rt < n; ++rt, base += cost) {
@@ -598,7 +646,13 @@ void mx4_decode_kernel(Fav4Mx4PagedArgs a, Mx4Plan pl) {
                 if (first >= g1 || end <= g0) continue;
                 const bool before = first < g0, split = before || end > g1;
                 const int block = mx4_block(w, before);
-                decode.attend(idx, f, rt * BM, kvh, max(0, g0 - first), min(tiles, g1 - first), split, block);
+                const int a0 = max(0, g0 - first);
+                // An opaque lane number, so that what follows from it is not kept from one row tile to the next.
+                int own_lane = lane;
+                asm volatile("" : "+v"(own_lane));
+                const Mx4Decode<NT, WAVES, SUB, DEPTH, LSE, P64> decode{a, pl, smem, stats, own_lane, wave};
+                auto where = decode.places(idx, kvh, a0 + wave);
+                decode.attend(f, rt * BM, kvh, where, a0, min(tiles, g1 - first), split, block);
                 if (split && !before)
                     note = int4{f.t0 * pl.group + rt * BM, min(BM, f.tokens * pl.group - rt * BM),
                                 udiv(end - 1, per) - w + 1, 0};
@@ -672,9 +726,9 @@ struct Mx4Prefill {
                 if (at >= e1) return;
                 const bool in = at * BN + kr < f.keys;
                 const uint32_t ksc = in ? ks : 0u, vsc = in ? vs : 0u;
-                const uint32_t kb = mx4_has_255(vsc) ? 255u : ksc >> (8 * (j >> 1)) & 255u;
+                const uint32_t kb = mx4_no_numbers(vsc) ? 255u : ksc >> (8 * (j >> 1)) & 255u;
                 const uint32_t byte = vsc >> (8 * (j >> 1)) & 255u;
-                const bool none = !in || byte == 255u;
+                const bool none = !in || byte > 252u;
                 const float sk = mx4_scale(kb), sv = mx4_scale(none ? 0u : byte);
                 unsigned char* k = smem + stage * 2 * TILE_BYTES;
                 unsigned char* v = k + TILE_BYTES;
@@ -873,8 +927,9 @@ void mx4_prefill_line_kernel(Fav4Mx4PagedArgs a, Mx4Plan pl) {
 // ---- Merge --------------------------------------------------------------------------
 // The row tiles that were cut: workgroup by workgroup 16 / PER rows of a range's, with one
 // K/V head.  PER teams of 16 lanes share a row, 8 dims a lane; a team takes every PER-th
-// part, eight at a time with all their loads in flight, with the running maximum and sums
-// of a softmax over the parts' log-sums.
+// part, NS at a time with all their loads in flight, with the running maximum and sums of a
+// softmax over the parts' log-sums.  Bound by latency: the first parts are loaded beside the
+// note that says how many there are.
 template <int PER>
 __global__ __launch_bounds__(256) void mx4_merge_kernel(Fav4Mx4PagedArgs a, Mx4Plan pl) {
     constexpr int RPB = 16 / PER, NS = PER == 1 ? 4 : 8;
@@ -883,27 +938,32 @@ __global__ __launch_bounds__(256) void mx4_merge_kernel(Fav4Mx4PagedArgs a, Mx4P
     const Fav4PagedArgs& pg = a.paged;
     const int grp = threadIdx.x >> 4, l16 = threadIdx.x & 15;
     const int slot = grp / PER, part = grp - slot * PER;
-    const int chunks = pl.stride / RPB, piece = pl.by_merge(blockIdx.x), r0 = (int(blockIdx.x) - piece * chunks) * RPB;
+    const int piece = pl.by_merge(blockIdx.x), r = (int(blockIdx.x) - piece * pl.merge_chunks) * RPB + slot;
     const int w = pl.by_kv_heads(piece), kvh = piece - w * pg.kv_heads;
-    const int4 note = pl.notes[w];
-    if (r0 >= note.y || note.z <= 0) return;
-    const int r = r0 + slot, total = min(note.z, pl.ranges - w);
-    const bool live = r < note.y;
-    const int tok = pl.by_group(note.x + min(r, note.y - 1)), head = kvh * pl.group + note.x + r - tok * pl.group;
-    const int64_t at = (int64_t(kvh) * 2 * pl.ranges + mx4_block(w, false)) * pl.stride + min(r, note.y - 1);
-    float mb = -__builtin_inff(), ml = mb, den = 0.f, suml = 0.f;
-    f32x4 acc[2] = {};
-    for (int c0 = part; c0 < total; c0 += PER * NS) {
-        // Loads past the last part repeat it, with weight 0: no branch between the loads.
-        float2 v[NS];
-        f32x4 xo[NS][2];
+    const int64_t at = int64_t(kvh) * 2 * pl.ranges * pl.stride + r;
+    const int block = mx4_block(w, false), last = 2 * pl.ranges - 1;
+    float2 v[NS];
+    f32x4 xo[NS][2];
+    // Parts c0, c0 + PER, ...; blocks past the last are it again, and get weight 0.
+    auto load = [&](int c0) {
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
-            const int64_t row = at + int64_t(mx4_part(min(c0 + i * PER, total - 1))) * pl.stride;
+            const int64_t row = at + int64_t(min(block + mx4_part(c0 + i * PER), last)) * pl.stride;
             v[i] = reinterpret_cast<const float2*>(pl.lse_part)[row];
             const f32x4* o = reinterpret_cast<const f32x4*>(pl.o_part + row * D + l16 * 8);
             xo[i][0] = o[0], xo[i][1] = o[1];
         }
+    };
+    load(part);
+    const int4 note = pl.notes[w];
+    if (r - slot >= note.y || note.z <= 0) return;
+    const int total = min(note.z, pl.ranges - w);
+    const bool live = r < note.y;
+    const int tok = pl.by_group(note.x + min(r, note.y - 1)), head = kvh * pl.group + note.x + r - tok * pl.group;
+    float mb = -__builtin_inff(), ml = mb, den = 0.f, suml = 0.f;
+    f32x4 acc[2] = {};
+    for (int c0 = part; c0 < total; c0 += PER * NS) {
+        if (c0 != part) load(c0);
 #pragma unroll
         for (int i = 0; i < NS; ++i)
             if (c0 + i * PER >= total) v[i] = float2{-__builtin_inff(), -__builtin_inff()};
