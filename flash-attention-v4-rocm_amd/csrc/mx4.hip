@@ -92,10 +92,28 @@ bool paged_shape_ok(const Fav4Mx4PagedArgs* args, int causal) {
            int64_t(a.total_q) * a.heads <= INT_MAX && caches_fit(a.num_pages, a.page_size, a.kv_heads);
 }
 
-constexpr int SUB1 = 2, DEP1 = 1, EU1 = 3, PER1 = 3, SUB2 = 4, DEP2 = 1, EU2 = 2, PER2 = 2, SW = 4, UW = 8, USUB1 = 4, UEU1 = 2;
-constexpr int FEW_PER_CU = 3, MIN_KEYS = 384, USPLIT = 2048, SEG_CU = 4;
+// The decode kernel's workgroups on a line (cut): four waves of 32-key tiles, three a CU,
+// with up to 16 rows; of 64-key tiles, two a CU, with 32.  Whole sequences: eight waves of
+// 64-key tiles, one a CU.
+constexpr int LINE_WAVES = 4, WHOLE_WAVES = 8;
+constexpr int line_per_cu(int row_tiles) { return row_tiles == 1 ? 3 : 2; }
+constexpr int line_subtiles(int row_tiles) { return row_tiles == 1 ? 2 : 4; }
+// Keys that a workgroup of a line should have at least: 24 sequences of 1000..16384, H8
+// KVH1, 17.1 us with 384, 18.3 with 128; 32 x 4 queries behind 200..4096, H32 KVH8, 24.6
+// with 384, 25.5 with 768, 30.1 with 1536.
+constexpr int LINE_KEYS = 384;
 // Up to this many rows a sequence go by the decode kernel.
 constexpr int FEW_ROWS = 64;
+
+// Whether every sequence and K/V head (`pairs`) has a workgroup of its own, and no merge.
+// Measured (H32 KVH8 where not said): such a workgroup reads 264 keys a us and starts and
+// ends in 4.5; a line takes 13 and its bytes at 6.3 TB/s.  32 x 4 queries behind 200..4096
+// keys 20.3 us whole, 24.6 cut; 4 sequences of up to 2000 10.8 and 13; 4 of up to 3096,
+// KVH4, 15.1 and 13.1.  With more pairs than CUs whole sequences wait for one another: 48 of
+// 100..4096 23.3 whole, 21.7 cut; 64 of 500..8192 55.8 and 46.0.
+bool whole_sequences(int64_t pairs, int64_t max_keys, double all_keys, int cus) {
+    return pairs <= cus && double(max_keys) < 264 * (8.5 + all_keys * 136 / 6.3e6);
+}
 
 struct Sizes {
     fav4::Mx4Plan plan;
@@ -114,17 +132,17 @@ Sizes paged_sizes(const Fav4Mx4PagedArgs& args, int causal) {
     p.group = int(group);
     p.br = causal == BOTTOM_RIGHT;
     s.few = seq_rows <= FEW_ROWS;
-    // Workgroups of a K/V head that are resident at once: FEW_PER_CU a CU with few rows, one of eight waves with many.
-    const int few_ranges = std::max(1, FEW_PER_CU * cus / a.kv_heads), many_ranges = std::max(1, cus / a.kv_heads);
+    // Workgroups of a K/V head that are resident at once, at most: with few rows, and with many.
+    const int few_ranges = std::max(1, line_per_cu(1) * cus / a.kv_heads), many_ranges = std::max(1, cus / a.kv_heads);
     int64_t segs;
     if (s.few) {
         p.stride = seq_rows <= 16 ? 16 : 32;
         p.tiles = int((seq_rows + p.stride - 1) / p.stride);
         segs = int64_t(a.batch) * p.tiles;
-        const int resident = std::max(1, (p.stride == 16 ? PER1 : PER2) * cus / a.kv_heads);
+        const int resident = std::max(1, line_per_cu(p.stride / 16) * cus / a.kv_heads);
         const int64_t keys = a.total_k > 0 ? a.total_k : int64_t(a.batch) * a.max_seqlen_k;
-        s.split = segs * a.kv_heads < SEG_CU * cus && a.max_seqlen_k > USPLIT;
-        p.ranges = s.split ? int(std::min<int64_t>(resident, keys * p.tiles / MIN_KEYS + 1)) : 1;
+        s.split = !whole_sequences(segs * a.kv_heads, a.max_seqlen_k, double(keys) * p.tiles * a.kv_heads, cus);
+        p.ranges = s.split ? int(std::min<int64_t>(resident, keys * p.tiles / LINE_KEYS + 1)) : 1;
     } else {
         segs = std::min<int64_t>(a.batch * ((seq_rows + fav4::MX4_BM - 1) / fav4::MX4_BM),
                                  (rows + int64_t(a.batch) * (fav4::MX4_BM - 1)) / fav4::MX4_BM);
@@ -158,9 +176,10 @@ void launch_few(const Fav4Mx4PagedArgs& a, const Sizes& s, hipStream_t stream) {
     };
     auto with = [&](auto lse, auto p64) {
         constexpr bool L = decltype(lse)::value, P = decltype(p64)::value;
-        constexpr int SUB = NT == 1 ? SUB1 : SUB2, DEP = NT == 1 ? DEP1 : DEP2, EU = NT == 1 ? EU1 : EU2, USUB = NT == 1 ? USUB1 : SUB2, UEU = NT == 1 ? UEU1 : EU2;
-        if (s.split) go(fav4::mx4_decode_kernel<NT, SW, SUB, DEP, EU, true, L, P>, SW);
-        else go(fav4::mx4_decode_kernel<NT, UW, USUB, DEP, UEU, false, L, P>, UW);
+        if (s.split)
+            go(fav4::mx4_decode_kernel<NT, LINE_WAVES, line_subtiles(NT), line_per_cu(NT), true, L, P>, LINE_WAVES);
+        else
+            go(fav4::mx4_decode_kernel<NT, WHOLE_WAVES, 4, 2, false, L, P>, WHOLE_WAVES);
     };
     const bool p64 = a.paged.page_size % 64 == 0;
     if (a.paged.lse) p64 ? with(std::true_type{}, std::true_type{}) : with(std::true_type{}, std::false_type{});

@@ -6,7 +6,6 @@
 
 namespace fav4 {
 
-constexpr int MX4_VPAD = 16;
 constexpr int MX4_CODES = D / 2, MX4_SCALES = D / 32;      // bytes of a cache row
 
 __device__ __forceinline__ float mx4_scale(uint32_t byte) { return __uint_as_float(byte << 23); }
@@ -323,9 +322,9 @@ struct Mx4Tile {
 };
 
 // P64: pages of a multiple of 64 keys, so that a tile lies in one.
-template <int NT, int WAVES, int SUB, int DEPTH, bool LSE, bool P64>
+template <int NT, int WAVES, int SUB, bool LSE, bool P64>
 struct Mx4Decode {
-    static constexpr int VROW = ROW_BYTES + MX4_VPAD, SLOT = 32 * VROW, BM = NT * 16, BN = SUB * 16;
+    static constexpr int VROW = ROW_BYTES + 16, SLOT = 32 * VROW, BM = NT * 16, BN = SUB * 16;
     static_assert(BN == 64 || BN == 32, "tiles lie in a page of a multiple of 64 keys");
     const Fav4Mx4PagedArgs& a;
     const Mx4Plan& pl;
@@ -388,13 +387,13 @@ struct Mx4Decode {
         x.v[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(at(a.paged.v_cache, r, i, MX4_CODES) + code));
     }
 
-    // Tile t, in x; this wave's tile DEPTH tiles on is loaded in its place (behind the last
-    // one that again: with the loads behind a branch the compiler could no longer tell how
+    // Tile t, in x; this wave's next tile is loaded in its place (behind the last one that
+    // again: with the loads behind a branch the compiler could no longer tell how
     // many are under way, and would wait for the newest where it needs the oldest).
     __device__ __forceinline__ void tile(Mx4Tile<SUB>& x, const bf16x8 (&q)[NT][4], Mx4State<NT>& st, int t, int last, bool masked,
                                          const int (&lim)[NT], float scale2, Places& where) const {
         const int col = lane & 15, g = lane >> 4;
-        const Rows r = rows(min(t + DEPTH * WAVES, last), where);
+        const Rows r = rows(min(t + WAVES, last), where);
         uint32_t most = x.vs[0];
 #pragma unroll
         for (int i = 1; i < SUB; ++i) most = max(most, x.vs[i]);
@@ -521,22 +520,12 @@ struct Mx4Decode {
         int t = a0 + wave;
         if (t < e1) {
             const int last = t + (e1 - 1 - t) / WAVES * WAVES;             // of this wave
-            Mx4Tile<SUB> x[DEPTH];
+            Mx4Tile<SUB> x;
+            const Rows r = rows(t, where);
+            load_k(x, r);
 #pragma unroll
-            for (int d = 0; d < DEPTH; ++d) {
-                const Rows r = rows(min(t + d * WAVES, last), where);
-                load_k(x[d], r);
-#pragma unroll
-                for (int i = 0; i < SUB; ++i) load_v(x[d], r, i);
-            }
-            while (t < e1) {
-#pragma unroll
-                for (int d = 0; d < DEPTH; ++d) {
-                    if (t >= e1) break;
-                    tile(x[d], q, st, t, last, t >= nfull, lim, scale2, where);
-                    t += WAVES;
-                }
-            }
+            for (int i = 0; i < SUB; ++i) load_v(x, r, i);
+            for (; t < e1; t += WAVES) tile(x, q, st, t, last, t >= nfull, lim, scale2, where);
         }
         // Join: row n's quad of dims 4u at u ^ n of its 512 bytes.
         unsigned char* slot = smem + wave * SLOT;
@@ -589,18 +578,18 @@ struct Mx4Decode {
 // One row tile of a sequence and one K/V head a workgroup (SPLIT false), or a range of
 // the line.
 constexpr int MX4_LEAD = 2;
-template <int NT, int WAVES, int SUB, int DEPTH, int EU, bool SPLIT, bool LSE, bool P64>
+template <int NT, int WAVES, int SUB, int EU, bool SPLIT, bool LSE, bool P64>
 __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(EU, EU)))
 void mx4_decode_kernel(Fav4Mx4PagedArgs a, Mx4Plan pl) {
     constexpr int BM = NT * 16, BN = SUB * 16;
-    __shared__ __attribute__((aligned(1024))) unsigned char smem[WAVES * Mx4Decode<NT, WAVES, SUB, DEPTH, LSE, P64>::SLOT];
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[WAVES * Mx4Decode<NT, WAVES, SUB, LSE, P64>::SLOT];
     __shared__ float4 stats[WAVES][16];
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
     const Fav4PagedArgs& pg = a.paged;
     const int w = uniform(pl.by_kv_heads(blockIdx.x)), turn = uniform(int(blockIdx.x) - w * pg.kv_heads);
     if constexpr (!SPLIT) {
         const int b = pl.tiles > 1 ? udiv(w, pl.tiles) : w, r0 = (w - b * pl.tiles) * BM;
-        const Mx4Decode<NT, WAVES, SUB, DEPTH, LSE, P64> decode{a, pl, smem, stats, lane, wave};
+        const Mx4Decode<NT, WAVES, SUB, LSE, P64> decode{a, pl, smem, stats, lane, wave};
         // (The table and the lengths load side by side.)
         auto where = decode.places(b, turn, wave);
         Mx4Seq f = mx4_seq(pg, b);
@@ -650,7 +639,7 @@ void mx4_decode_kernel(Fav4Mx4PagedArgs a, Mx4Plan pl) {
                 // An opaque lane number, so that what follows from it is not kept from one row tile to the next.
                 int own_lane = lane;
                 asm volatile("" : "+v"(own_lane));
-                const Mx4Decode<NT, WAVES, SUB, DEPTH, LSE, P64> decode{a, pl, smem, stats, own_lane, wave};
+                const Mx4Decode<NT, WAVES, SUB, LSE, P64> decode{a, pl, smem, stats, own_lane, wave};
                 auto where = decode.places(idx, kvh, a0 + wave);
                 decode.attend(f, rt * BM, kvh, where, a0, min(tiles, g1 - first), split, block);
                 if (split && !before)
