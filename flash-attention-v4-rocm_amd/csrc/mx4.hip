@@ -115,10 +115,43 @@ bool whole_sequences(int64_t pairs, int64_t max_keys, double all_keys, int cus) 
     return pairs <= cus && double(max_keys) < 264 * (8.5 + all_keys * 136 / 6.3e6);
 }
 
+// Sequences of many rows: row tiles of eight waves (256 rows, one workgroup a CU) or four
+// (128, two), each whole, the longest of a sequence first, or on a line.  By an estimate in
+// us of each, from the sizes (of unequal lengths their means and the longest): a 64-key tile
+// takes a workgroup of eight waves 1.95, one of four 1.7 beside another, 2.15 in a full GPU
+// and 1.3 alone; a row tile on a line starts and ends in 4.5 more, and its merge takes 18
+// with the launch.  Measured, H32 KVH8 where not said, whole 8 / whole 4 / line 8 / line 4:
+// 8 x 64..512 queries behind 1024..8192 keys 246 / 296 / 162 / 182; prompts of 500..2500
+// 147 / 151 / 149 / 163; 3 prompts of 396..782 29.1 / 26.2 / 33.9 / 35.4; 2 prompts of
+// 1673 and 2078, KVH32, 86.7 / 90.2 / 106 / 106; 6 x 6..23 queries behind 241..1524, H8
+// KVH2, 35.0 / 36.8 / 18.0 / 17.1.
+struct Cut {
+    int waves;
+    bool line;
+};
+template <class F>
+Cut many_rows_cut(const Fav4PagedArgs& a, int causal, int cus, F&& row_tiles) {
+    const double mean_q = double(a.total_q) / a.batch;
+    const double mean_k = a.total_k > 0 ? double(a.total_k) / a.batch : double(a.max_seqlen_k);
+    const double units = std::max(1.0, (mean_k - (causal == BOTTOM_RIGHT ? 0.5 * mean_q : 0.0)) / 64);
+    const double most = std::max(units, a.max_seqlen_k / 64.0);
+    Cut best{8, false};
+    double least = 1e30;
+    for (int waves : {8, 4}) {
+        const double n = row_tiles(waves) * a.kv_heads, slots = double(cus) * (8 / waves);
+        const double unit = waves == 8 ? 1.95 : n <= cus ? 1.3 : n <= slots ? 1.7 : 2.15;
+        const double whole = 5 + unit * (n <= slots ? most : n * units / slots + 0.3 * most);
+        const double line = 18 + (waves == 8 ? 1.95 : 2.15) * n * units / slots + 4.5 * (n / slots + 1);
+        if (whole < least) least = whole, best = {waves, false};
+        if (line < least) least = line, best = {waves, true};
+    }
+    return best;
+}
+
 struct Sizes {
     fav4::Mx4Plan plan;
     int64_t bytes, part_rows, grid, merge_grid;
-    int merge_teams;
+    int merge_teams, waves;
     bool few, split;
     bool ok;
 };
@@ -133,7 +166,7 @@ Sizes paged_sizes(const Fav4Mx4PagedArgs& args, int causal) {
     p.br = causal == BOTTOM_RIGHT;
     s.few = seq_rows <= FEW_ROWS;
     // Workgroups of a K/V head that are resident at once, at most: with few rows, and with many.
-    const int few_ranges = std::max(1, line_per_cu(1) * cus / a.kv_heads), many_ranges = std::max(1, cus / a.kv_heads);
+    const int few_ranges = std::max(1, line_per_cu(1) * cus / a.kv_heads), many_ranges = std::max(1, 2 * cus / a.kv_heads);
     int64_t segs;
     if (s.few) {
         p.stride = seq_rows <= 16 ? 16 : 32;
@@ -144,13 +177,18 @@ Sizes paged_sizes(const Fav4Mx4PagedArgs& args, int causal) {
         s.split = !whole_sequences(segs * a.kv_heads, a.max_seqlen_k, double(keys) * p.tiles * a.kv_heads, cus);
         p.ranges = s.split ? int(std::min<int64_t>(resident, keys * p.tiles / LINE_KEYS + 1)) : 1;
     } else {
-        segs = std::min<int64_t>(a.batch * ((seq_rows + fav4::MX4_BM - 1) / fav4::MX4_BM),
-                                 (rows + int64_t(a.batch) * (fav4::MX4_BM - 1)) / fav4::MX4_BM);
-        p.stride = fav4::MX4_BM;
+        auto row_tiles = [&](int bm) {
+            return std::min<int64_t>(a.batch * ((seq_rows + bm - 1) / bm), (rows + int64_t(a.batch) * (bm - 1)) / bm);
+        };
+        const Cut cut = many_rows_cut(a, causal, cus, [&](int waves) {
+            return std::min(double(row_tiles(waves * 32)), double(rows) / (waves * 32) + 0.5 * a.batch);
+        });
+        s.waves = cut.waves;
+        p.stride = s.waves * 32;
+        segs = row_tiles(p.stride);
         p.tiles = int(std::min<int64_t>(segs, INT_MAX));
-        s.split = segs <= fav4::MX4_LINE_TILES && a.batch <= fav4::MX4_LINE_SEQS && segs * a.kv_heads < 8 * cus;
-        p.ranges = s.split ? many_ranges : 1;
-        s.ok = segs <= MAX_ROW_TILES;
+        s.split = cut.line && segs <= fav4::MX4_LINE_TILES && a.batch <= fav4::MX4_LINE_SEQS;
+        p.ranges = s.split ? std::max(1, 8 / s.waves * cus / a.kv_heads) : 1;
     }
     s.grid = a.kv_heads * (s.split ? int64_t(p.ranges) : segs);
     s.ok = segs <= MAX_ROW_TILES && s.grid < (int64_t(1) << 30) &&
@@ -164,7 +202,7 @@ Sizes paged_sizes(const Fav4Mx4PagedArgs& args, int causal) {
     s.merge_grid = int64_t(p.ranges) * a.kv_heads * p.merge_chunks;
     p.by_merge = fav4::fast_div(p.merge_chunks);
     // What a call of either kind could need: more queries or sequences never need less.
-    s.part_rows = int64_t(a.kv_heads) * 2 * (s.few ? few_ranges * 32 : std::max(few_ranges * 32, many_ranges * fav4::MX4_BM));
+    s.part_rows = int64_t(a.kv_heads) * 2 * (s.few ? few_ranges * 32 : std::max(few_ranges * 32, many_ranges * 128));
     s.bytes = s.part_rows * (fav4::D * 4 + 8) + int64_t(few_ranges) * 16;
     return s;
 }
@@ -184,6 +222,15 @@ void launch_few(const Fav4Mx4PagedArgs& a, const Sizes& s, hipStream_t stream) {
     const bool p64 = a.paged.page_size % 64 == 0;
     if (a.paged.lse) p64 ? with(std::true_type{}, std::true_type{}) : with(std::true_type{}, std::false_type{});
     else p64 ? with(std::false_type{}, std::true_type{}) : with(std::false_type{}, std::false_type{});
+}
+
+template <int WAVES, bool LSE>
+void launch_many(const Fav4Mx4PagedArgs& a, const Sizes& s, hipStream_t stream) {
+    auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(unsigned(s.grid)), dim3(WAVES * 64), 0, stream, a, s.plan);
+    };
+    if (s.split) go(fav4::mx4_prefill_line_kernel<WAVES, LSE>);
+    else go(fav4::mx4_prefill_kernel<WAVES, LSE>);
 }
 
 }  // namespace
@@ -243,11 +290,8 @@ extern "C" __attribute__((visibility("default"))) int fav4_bshd_forward_paged_mx
         if (p.stride == 16) launch_few<1>(*args, s, stream);
         else launch_few<2>(*args, s, stream);
     } else {
-        auto go = [&](auto kernel) {
-            hipLaunchKernelGGL(kernel, dim3(unsigned(s.grid)), dim3(512), 0, stream, *args, p);
-        };
-        if (a.lse) s.split ? go(fav4::mx4_prefill_line_kernel<true>) : go(fav4::mx4_prefill_kernel<true>);
-        else s.split ? go(fav4::mx4_prefill_line_kernel<false>) : go(fav4::mx4_prefill_kernel<false>);
+        if (a.lse) s.waves == 4 ? launch_many<4, true>(*args, s, stream) : launch_many<8, true>(*args, s, stream);
+        else s.waves == 4 ? launch_many<4, false>(*args, s, stream) : launch_many<8, false>(*args, s, stream);
     }
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess || !s.split) return e;

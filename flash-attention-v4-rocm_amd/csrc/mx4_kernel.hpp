@@ -652,29 +652,30 @@ void mx4_decode_kernel(Fav4Mx4PagedArgs a, Mx4Plan pl) {
 }
 
 // ---- Many rows --------------------------------------------------------------------
-// Eight waves of 32 rows each share 64-key tiles of K and V, which they convert to BF16
-// on the way into LDS (two stages): the loop of the forward, attend_fused, behind another
-// source.  A thread has 16 dims of one key: 8 bytes of codes and the key's four scales,
-// loaded two tiles ahead.  Of the two waves of a SIMD one converts the next tile before
-// its products and the other behind them, so that one's conversion runs beside the
-// other's products.
-constexpr int MX4_BM = 256, MX4_MANY_LEAD = 2;
+// Eight waves (or four) of 32 rows each share 64-key tiles of K and V, which they convert
+// to BF16 on the way into LDS (two stages): the loop of the forward, attend_fused, behind
+// another source.  A thread has 16 (32) dims of one key: 8 (16) bytes of codes and the key's
+// four scales, loaded two tiles ahead.  Of the two waves of a SIMD that eight make one
+// converts the next tile before its products and the other behind them, so that one's
+// conversion runs beside the other's products; two workgroups of four do that unasked.
+constexpr int MX4_MANY_LEAD = 2;
 constexpr int MX4_LINE_TILES = 1024, MX4_LINE_SEQS = 512;      // of a batch that is cut into ranges
 
-template <bool LSE>
+template <int WAVES, bool LSE>
 struct Mx4Prefill {
-    static constexpr int BN = 64, TILE_BYTES = BN * ROW_BYTES;
+    static constexpr int BM = WAVES * 32, BN = 64, TILE_BYTES = BN * ROW_BYTES;
+    static constexpr int DWORDS = 16 / WAVES, KEYS = 64 / WAVES;       // of codes a thread, and of a wave
     const Fav4Mx4PagedArgs& a;
     const Mx4Plan& pl;
     unsigned char* smem;              // two stages of a K and a V tile
     int lane, wave;
 
     __device__ __forceinline__ int tiles_of(const Mx4Seq& f) const {
-        return int(uint32_t(f.tokens * pl.group + MX4_BM - 1) / MX4_BM);
+        return int(uint32_t(f.tokens * pl.group + BM - 1) / BM);
     }
     // Key tiles that some row of row tile rt sees.
     __device__ __forceinline__ int key_tiles(const Mx4Seq& f, int rt) const {
-        const int last = pl.by_group(min(f.tokens * pl.group, (rt + 1) * MX4_BM) - 1);
+        const int last = pl.by_group(min(f.tokens * pl.group, (rt + 1) * BM) - 1);
         const int seen = pl.br ? max(0, min(f.keys, f.keys - f.tokens + last + 1)) : f.keys;
         return (seen + BN - 1) / BN;
     }
@@ -684,7 +685,7 @@ struct Mx4Prefill {
                                            int block) const {
         const Fav4PagedArgs& pg = a.paged;
         const int col = lane & 31, half = lane >> 5, group = pl.group, rows = f.tokens * group;
-        const int q0 = rt * MX4_BM, qw = q0 + wave * 32, row = qw + col, srow = min(row, rows - 1);
+        const int q0 = rt * BM, qw = q0 + wave * 32, row = qw + col, srow = min(row, rows - 1);
         const int token = pl.by_group(srow), head = kvh * group + srow - token * group;
         const int shift = f.keys - f.tokens;
         const int plain = uniform(pl.br ? max(0, min(f.keys, shift + pl.by_group(q0) + 1)) : f.keys);
@@ -696,38 +697,40 @@ struct Mx4Prefill {
             const LdsOffsets off = lds_offsets(lane);
             bf16x8 qr[8];
             load_q(pg, f.t0 + token, head, half, qr);
-            const int kr = wave * 8 + (lane >> 3), j = lane & 7;           // this thread's key and 16 dims
-            const int last = (f.keys - 1) & ~7;
-            Mx4Pages pages = mx4_pages(pg, b, kvh, min(t * BN + wave * 8, last), pl.by_page, lane);
-            u32x2 ck, cv;
+            // This thread's key, and which of its stretches of DWORDS * 8 dims.
+            const int kr = wave * KEYS + lane / WAVES, j = lane % WAVES, block = j * DWORDS / 4;
+            const int last = (f.keys - 1) & ~(KEYS - 1);
+            Mx4Pages pages = mx4_pages(pg, b, kvh, min(t * BN + wave * KEYS, last), pl.by_page, lane);
+            typedef uint32_t codes_t __attribute__((ext_vector_type(DWORDS)));
+            codes_t ck, cv;
             uint32_t ks, vs;
             auto load = [&](int at) {
                 if (at >= e1) return;
-                const int64_t r = pages.row(min(at * BN + wave * 8, last), pl.by_page, lane);
-                ck = *reinterpret_cast<const u32x2*>(static_cast<const char*>(pg.k_cache) + r * MX4_CODES + lane * 8);
-                cv = *reinterpret_cast<const u32x2*>(static_cast<const char*>(pg.v_cache) + r * MX4_CODES + lane * 8);
-                ks = *reinterpret_cast<const uint32_t*>(static_cast<const char*>(a.k_scales) + r * MX4_SCALES + (lane >> 3) * 4);
-                vs = *reinterpret_cast<const uint32_t*>(static_cast<const char*>(a.v_scales) + r * MX4_SCALES + (lane >> 3) * 4);
+                const int64_t r = pages.row(min(at * BN + wave * KEYS, last), pl.by_page, lane);
+                const uint32_t code = lane * DWORDS * 4, scale = lane / WAVES * MX4_SCALES;
+                ck = *reinterpret_cast<const codes_t*>(static_cast<const char*>(pg.k_cache) + r * MX4_CODES + code);
+                cv = *reinterpret_cast<const codes_t*>(static_cast<const char*>(pg.v_cache) + r * MX4_CODES + code);
+                ks = *reinterpret_cast<const uint32_t*>(static_cast<const char*>(a.k_scales) + r * MX4_SCALES + scale);
+                vs = *reinterpret_cast<const uint32_t*>(static_cast<const char*>(a.v_scales) + r * MX4_SCALES + scale);
             };
-            const uint32_t k0 = kr * ROW_BYTES + (((2 * j) ^ k_swz(kr)) << 4), k1 = kr * ROW_BYTES + (((2 * j + 1) ^ k_swz(kr)) << 4);
-            const uint32_t v0 = kr * ROW_BYTES + (((2 * j) ^ v_swz(kr)) << 4), v1 = kr * ROW_BYTES + (((2 * j + 1) ^ v_swz(kr)) << 4);
             auto store = [&](int at, int stage) {
                 if (at >= e1) return;
                 const bool in = at * BN + kr < f.keys;
                 const uint32_t ksc = in ? ks : 0u, vsc = in ? vs : 0u;
-                const uint32_t kb = mx4_no_numbers(vsc) ? 255u : ksc >> (8 * (j >> 1)) & 255u;
-                const uint32_t byte = vsc >> (8 * (j >> 1)) & 255u;
+                const uint32_t kb = mx4_no_numbers(vsc) ? 255u : ksc >> (8 * block) & 255u;
+                const uint32_t byte = vsc >> (8 * block) & 255u;
                 const bool none = !in || byte > 252u;
                 const float sk = mx4_scale(kb), sv = mx4_scale(none ? 0u : byte);
-                unsigned char* k = smem + stage * 2 * TILE_BYTES;
+                unsigned char* k = smem + stage * 2 * TILE_BYTES + kr * ROW_BYTES;
                 unsigned char* v = k + TILE_BYTES;
                 auto put = [](unsigned char* p, bf16x8 x) { *reinterpret_cast<FAV4_LDS bf16x8*>((FAV4_LDS void*)p) = x; };
-                put(k + k0, mx4_values(ck[0], sk));
-                put(k + k1, mx4_values(ck[1], sk));
-                put(v + v0, mx4_values(none ? 0u : cv[0], sv));
-                put(v + v1, mx4_values(none ? 0u : cv[1], sv));
+#pragma unroll
+                for (int i = 0; i < DWORDS; ++i) {
+                    put(k + (((DWORDS * j + i) ^ k_swz(kr)) << 4), mx4_values(ck[i], sk));
+                    put(v + (((DWORDS * j + i) ^ v_swz(kr)) << 4), mx4_values(none ? 0u : cv[i], sv));
+                }
             };
-            const bool idle = qw >= rows, early = wave < 4;
+            const bool idle = qw >= rows, early = WAVES == 4 || wave < 4;
             const int t0 = t;
             load(t);
             store(t, 0);
@@ -760,7 +763,7 @@ struct Mx4Prefill {
         const uint32_t slot = wave * 2048;
         if (live <= 0) return;
         if (split) {
-            const int64_t prow = (int64_t(kvh) * 2 * pl.ranges + block) * MX4_BM + wave * 32;
+            const int64_t prow = (int64_t(kvh) * 2 * pl.ranges + block) * BM + wave * 32;
             store_part_rows<TILE_BYTES, true>(st, inv, smem, slot, make_rsrc(pl.o_part + prow * D, uint32_t(live) * D * 4),
                                               0, live, lane);
             if (lane < live) {
@@ -804,12 +807,12 @@ struct Mx4Prefill {
 };
 
 // One row tile of the batch and one K/V head a workgroup, a sequence's longest first.
-template <bool LSE>
-__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2)))
+template <int WAVES, bool LSE>
+__global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void mx4_prefill_kernel(Fav4Mx4PagedArgs a, Mx4Plan pl) {
-    __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * Mx4Prefill<LSE>::TILE_BYTES];
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * Mx4Prefill<WAVES, LSE>::TILE_BYTES];
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
-    const Mx4Prefill<LSE> x{a, pl, smem, lane, wave};
+    const Mx4Prefill<WAVES, LSE> x{a, pl, smem, lane, wave};
     const Fav4PagedArgs& pg = a.paged;
     const int id = uniform(pl.by_kv_heads(blockIdx.x)), kvh = uniform(int(blockIdx.x) - id * pg.kv_heads);
     int b = 0, before = 0;
@@ -835,14 +838,15 @@ void mx4_prefill_kernel(Fav4Mx4PagedArgs a, Mx4Plan pl) {
 // A range of the line.  The workgroup first lays out the line in LDS: the sequences'
 // row tiles by a sum over the sequences, then each row tile's units by one over those.
 // (Of tiles past MX4_LINE_TILES, which only bad offsets can make, nothing is attended.)
-template <bool LSE>
-__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2, 2)))
+template <int WAVES, bool LSE>
+__global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void mx4_prefill_line_kernel(Fav4Mx4PagedArgs a, Mx4Plan pl) {
-    __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * Mx4Prefill<LSE>::TILE_BYTES];
-    __shared__ int seq_end[MX4_LINE_SEQS], unit_end[MX4_LINE_TILES], waves[8];
+    __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * Mx4Prefill<WAVES, LSE>::TILE_BYTES];
+    constexpr int BM = WAVES * 32, THREADS = WAVES * 64;
+    __shared__ int seq_end[MX4_LINE_SEQS], unit_end[MX4_LINE_TILES], waves[WAVES];
     __shared__ uint16_t seq_of[MX4_LINE_TILES];
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
-    const Mx4Prefill<LSE> x{a, pl, smem, lane, wave};
+    const Mx4Prefill<WAVES, LSE> x{a, pl, smem, lane, wave};
     const Fav4PagedArgs& pg = a.paged;
     const int w = uniform(pl.by_kv_heads(blockIdx.x)), kvh = uniform(int(blockIdx.x) - w * pg.kv_heads);
     // The sum of x over threads 0..tid; `all` gets that over the workgroup.
@@ -854,24 +858,25 @@ void mx4_prefill_line_kernel(Fav4Mx4PagedArgs a, Mx4Plan pl) {
         int before = 0;
         all = 0;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int i = 0; i < WAVES; ++i) {
             if (i < wave) before += waves[i];
             all += waves[i];
         }
         return before + mine;
     };
-    Mx4Seq f{};
-    if (tid < pg.batch) f = mx4_seq(pg, tid);
-    int tiles;
-    const int end_tile = scan(x.tiles_of(f), tiles);
-    if (tid < pg.batch) {
-        seq_end[tid] = end_tile;
-        for (int i = end_tile - x.tiles_of(f); i < min(end_tile, MX4_LINE_TILES); ++i) seq_of[i] = uint16_t(tid);
+    int tiles = 0;
+    for (int b0 = 0; b0 < pg.batch; b0 += THREADS) {
+        const int b = b0 + tid, n = b < pg.batch ? x.tiles_of(mx4_seq(pg, b)) : 0;
+        int all;
+        const int end = tiles + scan(n, all);
+        if (b < pg.batch) seq_end[b] = end;
+        for (int i = end - n; i < min(end, MX4_LINE_TILES); ++i) seq_of[i] = uint16_t(b);
+        tiles += all;
     }
     tiles = min(uniform(tiles), MX4_LINE_TILES);
     __syncthreads();
     int units = 0;
-    for (int i0 = 0; i0 < tiles; i0 += 512) {
+    for (int i0 = 0; i0 < tiles; i0 += THREADS) {
         const int i = i0 + tid;
         int c = 0;
         if (i < tiles) {
@@ -906,7 +911,7 @@ void mx4_prefill_line_kernel(Fav4Mx4PagedArgs a, Mx4Plan pl) {
         const int block = mx4_block(w, before);
         x.attend(b, f, rt, kvh, max(0, g0 - first), min(n, g1 - first), split, block);
         if (split && !before)
-            note = int4{f.t0 * pl.group + rt * MX4_BM, min(MX4_BM, f.tokens * pl.group - rt * MX4_BM),
+            note = int4{f.t0 * pl.group + rt * BM, min(BM, f.tokens * pl.group - rt * BM),
                         udiv(end - 1, per) - w + 1, 0};
         __syncthreads();               // O has left the stages
     }
