@@ -8,7 +8,9 @@ namespace fav4 {
 
 constexpr int MX4_CODES = D / 2, MX4_SCALES = D / 32;      // bytes of a cache row
 
+// A scale byte's power of two; 255 makes NaN of whatever it scales.
 __device__ __forceinline__ float mx4_scale(uint32_t byte) { return __uint_as_float(byte << 23); }
+constexpr uint32_t MX4_MOST = 252;                         // the largest scale of numbers
 
 // Eight numbers (one dword of codes) times their block's scale: exact in BF16.
 __device__ __forceinline__ bf16x8 mx4_values(uint32_t codes, float scale) {
@@ -213,7 +215,7 @@ __global__ __launch_bounds__(256) void mx4_read_kernel(Fav4Mx4GatherArgs a, Fast
                     char* dst = static_cast<char*>(is_v ? a.v : a.k) +
                                 (int64_t(t0 + i) * (is_v ? a.v_stride : a.k_stride) +
                                  int64_t(is_v ? row - a.kv_heads : row) * D) * 2;
-                    __builtin_nontemporal_store(__builtin_bit_cast(u32x4, mx4_values(codes[u], mx4_scale(scale[u]))),
+                    __builtin_nontemporal_store(__builtin_bit_cast(u32x4, mx4_values(codes[u], mx4_scale(scale[u] > MX4_MOST ? 255u : scale[u]))),
                                                 reinterpret_cast<u32x4*>(dst + l16 * 16));
                 }
             }
@@ -394,17 +396,17 @@ struct Mx4Decode {
                                          const int (&lim)[NT], float scale2, Places& where) const {
         const int col = lane & 15, g = lane >> 4;
         const Rows r = rows(min(t + WAVES, last), where);
-        uint32_t most = x.vs[0];
+        uint32_t most = max(x.ks[0], x.vs[0]);
 #pragma unroll
-        for (int i = 1; i < SUB; ++i) most = max(most, x.vs[i]);
-        if (__builtin_amdgcn_ballot_w64(most > 252u)) {
+        for (int i = 1; i < SUB; ++i) most = max(most, max(x.ks[i], x.vs[i]));
+        if (__builtin_amdgcn_ballot_w64(most > MX4_MOST)) {
 #pragma unroll
             for (int i = 0; i < SUB; ++i) {
-                const bool none = x.vs[i] > 252u;
+                const bool none = x.vs[i] > MX4_MOST;
                 uint64_t keys_of = __builtin_amdgcn_ballot_w64(none);
                 keys_of |= keys_of >> 32;
                 keys_of |= keys_of >> 16;
-                x.ks[i] = keys_of >> col & 1 ? 255u : x.ks[i];
+                x.ks[i] = x.ks[i] > MX4_MOST || keys_of >> col & 1 ? 255u : x.ks[i];
                 x.vs[i] = none ? 127u : x.vs[i];
                 x.v[i] = none ? u32x4{} : x.v[i];
             }
@@ -717,10 +719,10 @@ struct Mx4Prefill {
                 if (at >= e1) return;
                 const bool in = at * BN + kr < f.keys;
                 const uint32_t ksc = in ? ks : 0u, vsc = in ? vs : 0u;
-                const uint32_t kb = mx4_no_numbers(vsc) ? 255u : ksc >> (8 * block) & 255u;
-                const uint32_t byte = vsc >> (8 * block) & 255u;
-                const bool none = !in || byte > 252u;
-                const float sk = mx4_scale(kb), sv = mx4_scale(none ? 0u : byte);
+                const uint32_t kbyte = ksc >> (8 * block) & 255u, vbyte = vsc >> (8 * block) & 255u;
+                const bool none = !in || vbyte > MX4_MOST;
+                const float sk = mx4_scale(mx4_no_numbers(vsc) || kbyte > MX4_MOST ? 255u : kbyte);
+                const float sv = mx4_scale(none ? 0u : vbyte);
                 unsigned char* k = smem + stage * 2 * TILE_BYTES + kr * ROW_BYTES;
                 unsigned char* v = k + TILE_BYTES;
                 auto put = [](unsigned char* p, bf16x8 x) { *reinterpret_cast<FAV4_LDS bf16x8*>((FAV4_LDS void*)p) = x; };

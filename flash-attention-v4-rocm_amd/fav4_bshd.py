@@ -729,52 +729,51 @@ class Runner:
                      for n in (D // 2, D // 32, D // 2, D // 32))
 
     @staticmethod
-    def _mx4_cache_shape(torch, dev, k_cache, k_scales, v_cache, v_scales):
-        num_pages, kv_heads, page_size, d = shape = k_cache.shape
+    def _mx4_append_block(torch, q, k, v, q_out, k_cache, k_scales, v_cache, v_scales, cu_q, seqlens_k, block_table,
+                          cos, sin, interleaved, positions) -> bytes:
+        bf16, i32, u8, dev = torch.bfloat16, torch.int32, torch.uint8, k.get_device()
+        num_pages, kv_heads, page_size, d = caches = k_cache.shape
         scales = (num_pages, kv_heads, page_size, D // 32)
-        assert d == D // 2 and v_cache.shape == shape and k_scales.shape == v_scales.shape == scales
-        for x in (k_cache, k_scales, v_cache, v_scales):
-            assert x.dtype is torch.uint8 and x.is_contiguous() and x.get_device() == dev, \
-                "uint8, contiguous, all tensors on one device"
-        return num_pages, kv_heads, page_size
-
-    @staticmethod
-    def _mx4_rows(torch, x, tokens, heads, dev):
-        """The stride between the tokens of BF16 rows [tokens, heads, 128] (a single one has none that counts)."""
-        assert x.shape == (tokens, heads, D) and x.dtype is torch.bfloat16 and x.get_device() == dev, \
-            "BF16 rows [tokens, heads, 128] on one device"
-        stride, s1, s2 = x.stride()
-        assert s2 == 1 and (heads == 1 or s1 == D)
-        return stride if tokens > 1 else heads * D
-
-    @staticmethod
-    def _mx4_ints(torch, dev, *arrays):
-        for x, shape in arrays:
-            assert x.dtype is torch.int32 and x.shape == shape and x.is_contiguous() and x.get_device() == dev, \
-                "int32, contiguous, on one device"
-
-    @classmethod
-    def _mx4_append_block(cls, torch, q, k, v, q_out, k_cache, k_scales, v_cache, v_scales, cu_q, seqlens_k,
-                          block_table, cos, sin, interleaved, positions) -> bytes:
-        dev = k.get_device()
-        num_pages, kv_heads, page_size = cls._mx4_cache_shape(torch, dev, k_cache, k_scales, v_cache, v_scales)
+        assert d == D // 2 and v_cache.shape == caches and k_scales.shape == scales and v_scales.shape == scales
+        assert k_cache.dtype is u8 and v_cache.dtype is u8 and k_scales.dtype is u8 and v_scales.dtype is u8
+        assert k_cache.is_contiguous() and v_cache.is_contiguous() and k_scales.is_contiguous() \
+            and v_scales.is_contiguous()
         batch, pages = block_table.shape
-        cls._mx4_ints(torch, dev, (cu_q, (batch + 1,)), (seqlens_k, (batch,)), (block_table, (batch, pages)))
-        tokens, heads = k.shape[0], 1
-        k_stride, v_stride = cls._mx4_rows(torch, k, tokens, kv_heads, dev), cls._mx4_rows(torch, v, tokens, kv_heads, dev)
-        q_stride = o_stride = q_ptr = o_ptr = rows = half = c_ptr = s_ptr = p_ptr = 0
-        assert (q is None) == (q_out is None) and (cos is None) == (sin is None)
+        assert cu_q.dtype is i32 and seqlens_k.dtype is i32 and block_table.dtype is i32
+        assert cu_q.shape == (batch + 1,) and seqlens_k.shape == (batch,)
+        assert cu_q.is_contiguous() and seqlens_k.is_contiguous() and block_table.is_contiguous()
+        assert dev == k_cache.get_device() == k_scales.get_device() == v_cache.get_device() == v_scales.get_device() \
+            == v.get_device() == cu_q.get_device() == seqlens_k.get_device() == block_table.get_device(), \
+            "all tensors on one device"
+        # Rows: any stride between tokens (a single token has none that counts), heads and dims contiguous.
+        tokens = k.shape[0]
+        assert k.shape == v.shape == (tokens, kv_heads, D) and k.dtype is bf16 and v.dtype is bf16
+        k_stride, k1, k2 = k.stride()
+        v_stride, v1, v2 = v.stride()
+        assert k2 == v2 == 1 and (kv_heads == 1 or k1 == v1 == D)
+        heads, q_stride, o_stride, q_ptr, o_ptr = 1, 0, 0, 0, 0
+        assert (q is None) == (q_out is None)
         if q is not None:
             heads = q.shape[1]
-            q_stride, o_stride = cls._mx4_rows(torch, q, tokens, heads, dev), cls._mx4_rows(torch, q_out, tokens, heads, dev)
+            assert q.shape == q_out.shape == (tokens, heads, D) and q.dtype is bf16 and q_out.dtype is bf16
+            assert q.get_device() == q_out.get_device() == dev, "all tensors on one device"
+            q_stride, q1, q2 = q.stride()
+            o_stride, o1, o2 = q_out.stride()
+            assert q2 == o2 == 1 and (heads == 1 or q1 == o1 == D)
             q_ptr, o_ptr = q.data_ptr(), q_out.data_ptr()
+        if tokens == 1:
+            k_stride = v_stride = kv_heads * D
+            q_stride = o_stride = heads * D
+        rows = half = c_ptr = s_ptr = p_ptr = 0
+        assert (cos is None) == (sin is None)
         if cos is not None:
-            rows, half = cos.shape
-            assert sin.shape == cos.shape and cos.dtype is sin.dtype is torch.float32
+            rows, half = angles = cos.shape
+            assert sin.shape == angles and cos.dtype is sin.dtype is torch.float32
             assert cos.is_contiguous() and sin.is_contiguous() and cos.get_device() == sin.get_device() == dev
             c_ptr, s_ptr = cos.data_ptr(), sin.data_ptr()
         if positions is not None:
-            cls._mx4_ints(torch, dev, (positions, (tokens,)))
+            assert positions.dtype is i32 and positions.shape == (tokens,) and positions.is_contiguous()
+            assert positions.get_device() == dev, "all tensors on one device"
             p_ptr = positions.data_ptr()
         return _MX4_APPEND.pack(q_ptr, k.data_ptr(), v.data_ptr(), o_ptr, k_cache.data_ptr(), v_cache.data_ptr(),
                                 c_ptr, s_ptr, cu_q.data_ptr(), seqlens_k.data_ptr(), block_table.data_ptr(), p_ptr,
@@ -793,20 +792,34 @@ class Runner:
         if status:
             raise RuntimeError(f"append paged mx4: HIP status {status}")
 
-    @classmethod
-    def _mx4_gather_block(cls, torch, k_cache, k_scales, v_cache, v_scales, k, v, cu_k, block_table, starts) -> bytes:
-        dev = k.get_device()
-        num_pages, kv_heads, page_size = cls._mx4_cache_shape(torch, dev, k_cache, k_scales, v_cache, v_scales)
+    @staticmethod
+    def _mx4_gather_block(torch, k_cache, k_scales, v_cache, v_scales, k, v, cu_k, block_table, starts) -> bytes:
+        bf16, i32, u8, dev = torch.bfloat16, torch.int32, torch.uint8, k.get_device()
+        num_pages, kv_heads, page_size, d = caches = k_cache.shape
+        scales = (num_pages, kv_heads, page_size, D // 32)
+        assert d == D // 2 and v_cache.shape == caches and k_scales.shape == scales and v_scales.shape == scales
+        assert k_cache.dtype is u8 and v_cache.dtype is u8 and k_scales.dtype is u8 and v_scales.dtype is u8
+        assert k_cache.is_contiguous() and v_cache.is_contiguous() and k_scales.is_contiguous() \
+            and v_scales.is_contiguous()
         batch, pages = block_table.shape
-        cls._mx4_ints(torch, dev, (cu_k, (batch + 1,)), (block_table, (batch, pages)))
+        assert cu_k.dtype is i32 and block_table.dtype is i32 and cu_k.shape == (batch + 1,)
+        assert cu_k.is_contiguous() and block_table.is_contiguous()
+        assert dev == k_cache.get_device() == k_scales.get_device() == v_cache.get_device() == v_scales.get_device() \
+            == v.get_device() == cu_k.get_device() == block_table.get_device(), "all tensors on one device"
+        rows, s_ptr = k.shape[0], 0
+        assert k.shape == v.shape == (rows, kv_heads, D) and k.dtype is bf16 and v.dtype is bf16
+        k_stride, k1, k2 = k.stride()
+        v_stride, v1, v2 = v.stride()
+        assert k2 == v2 == 1 and (kv_heads == 1 or k1 == v1 == D)
+        if rows == 1:                                     # has no stride that counts
+            k_stride = v_stride = kv_heads * D
         if starts is not None:
-            cls._mx4_ints(torch, dev, (starts, (batch,)))
-        rows = k.shape[0]
-        k_stride, v_stride = cls._mx4_rows(torch, k, rows, kv_heads, dev), cls._mx4_rows(torch, v, rows, kv_heads, dev)
+            assert starts.dtype is i32 and starts.shape == (batch,) and starts.is_contiguous()
+            assert starts.get_device() == dev, "all tensors on one device"
+            s_ptr = starts.data_ptr()
         return _MX4_GATHER.pack(k_cache.data_ptr(), k_scales.data_ptr(), v_cache.data_ptr(), v_scales.data_ptr(),
-                                k.data_ptr(), v.data_ptr(), cu_k.data_ptr(), 0 if starts is None else starts.data_ptr(),
-                                block_table.data_ptr(), k_stride, v_stride, batch, kv_heads, rows, num_pages, page_size,
-                                pages)
+                                k.data_ptr(), v.data_ptr(), cu_k.data_ptr(), s_ptr, block_table.data_ptr(), k_stride,
+                                v_stride, batch, kv_heads, rows, num_pages, page_size, pages)
 
     def call_gather_paged_mx4(self, k_cache, k_scales, v_cache, v_scales, k, v, cu_k, block_table, starts=None,
                               stream=None):
@@ -819,16 +832,26 @@ class Runner:
         if status:
             raise RuntimeError(f"gather paged mx4: HIP status {status}")
 
-    @classmethod
-    def _mx4_paged_block(cls, torch, q, k_cache, k_scales, v_cache, v_scales, o, lse, cu_q, seqlens_k, block_table,
-                         max_q, max_k, total_k, scale) -> bytes:
-        dev = q.get_device()
-        num_pages, kv_heads, page_size = cls._mx4_cache_shape(torch, dev, k_cache, k_scales, v_cache, v_scales)
+    @staticmethod
+    def _mx4_paged_block(torch, q, k_cache, k_scales, v_cache, v_scales, o, lse, cu_q, seqlens_k, block_table, max_q,
+                         max_k, total_k, scale) -> bytes:
+        bf16, i32, u8, dev = torch.bfloat16, torch.int32, torch.uint8, q.get_device()
+        num_pages, kv_heads, page_size, d = caches = k_cache.shape
+        scales = (num_pages, kv_heads, page_size, D // 32)
+        assert d == D // 2 and v_cache.shape == caches and k_scales.shape == scales and v_scales.shape == scales
+        assert k_cache.dtype is u8 and v_cache.dtype is u8 and k_scales.dtype is u8 and v_scales.dtype is u8
+        assert k_cache.is_contiguous() and v_cache.is_contiguous() and k_scales.is_contiguous() \
+            and v_scales.is_contiguous()
         batch, pages = block_table.shape
-        cls._mx4_ints(torch, dev, (cu_q, (batch + 1,)), (seqlens_k, (batch,)), (block_table, (batch, pages)))
-        tokens, heads, d = q.shape
-        assert d == D and o.shape == q.shape and q.dtype is torch.bfloat16 and o.dtype is torch.bfloat16
-        assert q.is_contiguous() and o.is_contiguous() and o.get_device() == dev, "all tensors on one device"
+        assert cu_q.dtype is i32 and seqlens_k.dtype is i32 and block_table.dtype is i32
+        assert cu_q.shape == (batch + 1,) and seqlens_k.shape == (batch,)
+        assert cu_q.is_contiguous() and seqlens_k.is_contiguous() and block_table.is_contiguous()
+        tokens, heads, d = rows = q.shape
+        assert d == D and o.shape == rows and q.dtype is bf16 and o.dtype is bf16
+        assert q.is_contiguous() and o.is_contiguous()
+        assert dev == k_cache.get_device() == k_scales.get_device() == v_cache.get_device() == v_scales.get_device() \
+            == o.get_device() == cu_q.get_device() == seqlens_k.get_device() == block_table.get_device(), \
+            "all tensors on one device"
         lse_ptr = 0
         if lse is not None:
             assert lse.shape == (heads, tokens) and lse.is_contiguous() and lse.dtype is torch.float32

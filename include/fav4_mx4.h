@@ -14,9 +14,9 @@
 // codes, dims 2i and 2i + 1 in the low and the high half of byte i, and four E8M0
 // scales: the number in a dim of block j (dims 32j to 32j + 31) is
 // +-{0, 0.5, 1, 1.5, 2, 3, 4, 6}[code & 7] * 2^(scale[j] - 127), negative where
-// code & 8.  A scale of 255 makes its block no numbers (NaN).  Every number with a
-// scale of 2 to 252 is a normal BF16 one, exactly; the products with others may
-// count numbers below 2^-126 as 0 and give infinities above 2^128.
+// code & 8.  Scales of 253 to 255 make their block no numbers (NaN; an append writes 255
+// alone).  All others are exact in BF16; with scales of 0 and 1 numbers below 2^-126 may
+// count as 0.
 // The caches of K and of V are each two tensors, contiguous, head before slot, so
 // that the keys of a page and head that a workgroup reads lie side by side:
 //   codes   uint8 [num_pages, kv_heads, page_size, 64]
@@ -47,7 +47,7 @@ extern "C" int fav4_bshd_append_paged_mx4(const Fav4Mx4AppendArgs* args, hipStre
 // cu_seqlens_k[b + 1]) of k and v get keys starts[b], starts[b] + 1, ... of sequence
 // b (0, 1, ... where starts is NULL).
 //  * A row whose slot is negative or past the table, or whose page number is not in
-//    [0, num_pages), becomes 0.  Blocks of scale 255 become NaN.
+//    [0, num_pages), becomes 0.  Blocks of scales above 252 become NaN.
 //  * Rows in no sequence (behind the last one) are not written.
 struct Fav4Mx4GatherArgs {
     const void *k_cache, *k_scales, *v_cache, *v_scales;
@@ -69,7 +69,7 @@ extern "C" int fav4_bshd_gather_paged_mx4(const Fav4Mx4GatherArgs* args, hipStre
 // queries of each sequence, any number of them, dense (causal 0) or bottom-right causal
 // (2), against its keys.  A sequence without keys, and rows that see no key, get O = 0
 // and LSE = -inf; a sequence without queries writes nothing, nor do rows in no sequence.
-//  * A key with a scale of 255 in any block of its K or V is no number: a row that sees
+//  * A key with a scale above 252 in any block of its K or V is no number: a row that sees
 //    it gets O and LSE of NaN in all dims, and so does one whose query holds a NaN; rows
 //    that do not see the key are not touched by it, nor by what slots behind seqlens_k
 //    and hidden keys hold.

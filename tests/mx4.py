@@ -16,7 +16,7 @@ def values(codes, scales):
     if isinstance(codes, torch.Tensor):
         grid = torch.tensor(np.concatenate([GRID, -GRID]), device=codes.device)
         code = torch.stack((codes & 15, codes >> 4), -1).flatten(-2).long()
-        power = torch.tensor(np.r_[np.ldexp(1.0, np.arange(255) - 127), np.nan], device=codes.device)
+        power = torch.tensor(np.r_[np.ldexp(1.0, np.arange(253) - 127), [np.nan] * 3], device=codes.device)
         return grid[code] * power[scales.long()].repeat_interleave(32, -1)
     return values(torch.from_numpy(codes), torch.from_numpy(scales)).numpy()
 

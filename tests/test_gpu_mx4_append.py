@@ -195,8 +195,7 @@ def test_gather(gpu_runner, kv_heads, page, packed):
             ref[torch.from_numpy(~ok)] = 0
             assert (x[t.n:] == 3).all()
             got = x[:t.n].double()
-            # Numbers below 2^-126 may count as 0; 2^128 and above are infinite in BF16.
-            ref = torch.where(ref.abs() >= 2.0 ** 128, ref * float("inf"), ref)
+            # Numbers below 2^-126 may count as 0.
             same = (got == ref) | (got.isnan() & ref.isnan()) | ((ref.abs() < 2.0 ** -126) & (got == 0))
             assert same.all(), (j, int((~same).sum()))
 
