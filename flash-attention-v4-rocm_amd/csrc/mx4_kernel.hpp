@@ -259,32 +259,6 @@ __device__ __forceinline__ Mx4Seq mx4_seq(const Fav4PagedArgs& pg, int b) {
     return {t0, min(max(t1 - t0, 0), pg.max_seqlen_q), min(max(pg.seqlens_k[b], 0), pg.max_seqlen_k)};
 }
 
-// A sequence's pages, 64 entries of the table in the wave's lanes.
-struct Mx4Pages {
-    const int* table;
-    int entries, num_pages, page_size, slot0, pages;
-    int64_t page_rows, head_row;      // cache rows of a page, and of the head within it
-    __device__ __forceinline__ void load(int slot, int lane) {
-        slot0 = slot;
-        pages = min(max(table[min(slot + lane, entries - 1)], 0), num_pages - 1);
-    }
-    // The cache row of a key (keys in ascending order).
-    __device__ __forceinline__ int64_t row(int key, const FastDiv& by_page, int lane) {
-        const int slot = uniform(by_page(key));
-        if (slot - slot0 >= 64) load(slot, lane);
-        const int page = __builtin_amdgcn_readlane(pages, slot - slot0);
-        return page * page_rows + head_row + (key - slot * page_size);
-    }
-};
-__device__ __forceinline__ Mx4Pages mx4_pages(const Fav4PagedArgs& pg, int b, int kvh, int key, const FastDiv& by_page,
-                                              int lane) {
-    Mx4Pages p{pg.block_table + int64_t(b) * pg.max_pages_per_seq, pg.max_pages_per_seq, pg.num_pages, pg.page_size};
-    p.page_rows = int64_t(pg.kv_heads) * pg.page_size;
-    p.head_row = int64_t(kvh) * pg.page_size;
-    p.load(uniform(by_page(key)), lane);
-    return p;
-}
-
 __device__ __forceinline__ f32x4 mfma16(bf16x8 a, bf16x8 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
 }
@@ -701,27 +675,37 @@ struct Mx4Prefill {
             load_q(pg, f.t0 + token, head, half, qr);
             // This thread's key, and which of its stretches of DWORDS * 8 dims.
             const int kr = wave * KEYS + lane / WAVES, j = lane % WAVES, block = j * DWORDS / 4;
-            const int last = (f.keys - 1) & ~(KEYS - 1);
-            Mx4Pages pages = mx4_pages(pg, b, kvh, min(t * BN + wave * KEYS, last), pl.by_page, lane);
             typedef uint32_t codes_t __attribute__((ext_vector_type(DWORDS)));
             codes_t ck, cv;
             uint32_t ks, vs;
+            // The cache rows of this wave's keys of 64 tiles from `held` on, in the lanes.  (Keys past the sequence's are
+            // masked, and lie in whatever pages the table has there, clamped into the pool.)
+            int held = t, lo = 0, hi = 0;
+            auto hold = [&](int from) {
+                held = from;
+                const int key = min(from + lane, e1 - 1) * BN + wave * KEYS, slot_of = pl.by_page(key);
+                const int entry = pg.block_table[int64_t(b) * pg.max_pages_per_seq + min(slot_of, pg.max_pages_per_seq - 1)];
+                const int64_t r = (int64_t(min(max(entry, 0), pg.num_pages - 1)) * pg.kv_heads + kvh) * pg.page_size +
+                                  (key - slot_of * pg.page_size);
+                lo = int(r), hi = int(r >> 32);
+            };
+            hold(t);
             auto load = [&](int at) {
-                if (at >= e1) return;
-                const int64_t r = pages.row(min(at * BN + wave * KEYS, last), pl.by_page, lane);
+                // Behind the last tile that again, into the stage that no step reads: no branch around the loads.
+                int e = min(at, e1 - 1) - held;
+                if (e >= 64) hold(held + e), e = 0;
+                const int64_t r = int64_t(uint32_t(__builtin_amdgcn_readlane(lo, e))) |
+                                  int64_t(__builtin_amdgcn_readlane(hi, e)) << 32;
                 const uint32_t code = lane * DWORDS * 4, scale = lane / WAVES * MX4_SCALES;
                 ck = *reinterpret_cast<const codes_t*>(static_cast<const char*>(pg.k_cache) + r * MX4_CODES + code);
                 cv = *reinterpret_cast<const codes_t*>(static_cast<const char*>(pg.v_cache) + r * MX4_CODES + code);
                 ks = *reinterpret_cast<const uint32_t*>(static_cast<const char*>(a.k_scales) + r * MX4_SCALES + scale);
                 vs = *reinterpret_cast<const uint32_t*>(static_cast<const char*>(a.v_scales) + r * MX4_SCALES + scale);
             };
-            auto store = [&](int at, int stage) {
-                if (at >= e1) return;
-                const bool in = at * BN + kr < f.keys;
-                const uint32_t ksc = in ? ks : 0u, vsc = in ? vs : 0u;
-                const uint32_t kbyte = ksc >> (8 * block) & 255u, vbyte = vsc >> (8 * block) & 255u;
-                const bool none = !in || vbyte > MX4_MOST;
-                const float sk = mx4_scale(mx4_no_numbers(vsc) || kbyte > MX4_MOST ? 255u : kbyte);
+            auto store = [&](int stage) {
+                const uint32_t kbyte = ks >> (8 * block) & 255u, vbyte = vs >> (8 * block) & 255u;
+                const bool none = vbyte > MX4_MOST;
+                const float sk = mx4_scale(mx4_no_numbers(vs) || kbyte > MX4_MOST ? 255u : kbyte);
                 const float sv = mx4_scale(none ? 0u : vbyte);
                 unsigned char* k = smem + stage * 2 * TILE_BYTES + kr * ROW_BYTES;
                 unsigned char* v = k + TILE_BYTES;
@@ -735,14 +719,14 @@ struct Mx4Prefill {
             const bool idle = qw >= rows, early = WAVES == 4 || wave < 4;
             const int t0 = t;
             load(t);
-            store(t, 0);
+            store(0);
             load(t + 1);
             int stage = 0;
             auto steps = [&](auto masked, int to) {
                 for (; t < to; ++t) {
                     __syncthreads();
                     if (early) {
-                        store(t + 1, stage ^ 1);
+                        store(stage ^ 1);
                         load(t + 2);
                     }
                     const unsigned char* cur = smem + stage * 2 * TILE_BYTES;
@@ -750,7 +734,7 @@ struct Mx4Prefill {
                         attend_fused<BN, decltype(masked)::value, true, LSE, true>(cur, cur + TILE_BYTES, off, qr, st, t == t0,
                                                                                    t * BN, f.keys, lim, half, scale2);
                     if (!early) {
-                        store(t + 1, stage ^ 1);
+                        store(stage ^ 1);
                         load(t + 2);
                     }
                     stage ^= 1;
