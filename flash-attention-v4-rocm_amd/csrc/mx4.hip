@@ -106,13 +106,17 @@ constexpr int LINE_KEYS = 384;
 constexpr int FEW_ROWS = 64;
 
 // Whether every sequence and K/V head (`pairs`) has a workgroup of its own, and no merge.
-// Measured (H32 KVH8 where not said): such a workgroup reads 264 keys a us and starts and
-// ends in 4.5; a line takes 13 and its bytes at 6.3 TB/s.  32 x 4 queries behind 200..4096
-// keys 20.3 us whole, 24.6 cut; 4 sequences of up to 2000 10.8 and 13; 4 of up to 3096,
-// KVH4, 15.1 and 13.1.  With more pairs than CUs whole sequences wait for one another: 48 of
-// 100..4096 23.3 whole, 21.7 cut; 64 of 500..8192 55.8 and 46.0.
-bool whole_sequences(int64_t pairs, int64_t max_keys, double all_keys, int cus) {
-    return pairs <= cus && double(max_keys) < 264 * (8.5 + all_keys * 136 / 6.3e6);
+// Measured, as graphs: such workgroups start and end in 4.2 us, read 290 keys a us (175 with
+// 32 rows) and wait for 0.3 of the time that all bytes take at 6.3 TB/s; a line takes 9.1,
+// 0.3 for each row up to 16, and the bytes' time.  H32 KVH8 and one query where not said,
+// lengths of a third of the longest and more, whole / cut: 1 sequence of 1536 9.4 / 10.1, of
+// 4096 18.4 / 10.2; 16 of up to 2600 14.7 / 16.6, of 4000 20.4 / 18.1; 32 of 4000 22.2 /
+// 24.5, of 4 queries 22.8 / 28.5; 8 x 4 queries of 2500, H8 KVH1, 18.5 / 15.9.  With more
+// pairs than CUs whole sequences wait for one another: 48 of 100..4096 23.3 whole, 20.2
+// cut; 64 of 500..8192 55.8 and 44.5.
+bool whole_sequences(int64_t pairs, int64_t rows, int64_t max_keys, double all_keys, int cus) {
+    const double rate = rows <= 16 ? 290 : 175;
+    return pairs <= cus && double(max_keys) < rate * (4.9 + 0.3 * double(std::min<int64_t>(rows, 16)) + 0.7 * all_keys * 136 / 6.3e6);
 }
 
 // Sequences of many rows: row tiles of eight waves (256 rows, one workgroup a CU) or four
@@ -174,7 +178,7 @@ Sizes paged_sizes(const Fav4Mx4PagedArgs& args, int causal) {
         segs = int64_t(a.batch) * p.tiles;
         const int resident = std::max(1, line_per_cu(p.stride / 16) * cus / a.kv_heads);
         const int64_t keys = a.total_k > 0 ? a.total_k : int64_t(a.batch) * a.max_seqlen_k;
-        s.split = !whole_sequences(segs * a.kv_heads, a.max_seqlen_k, double(keys) * p.tiles * a.kv_heads, cus);
+        s.split = !whole_sequences(segs * a.kv_heads, seq_rows, a.max_seqlen_k, double(keys) * p.tiles * a.kv_heads, cus);
         p.ranges = s.split ? int(std::min<int64_t>(resident, keys * p.tiles / LINE_KEYS + 1)) : 1;
     } else {
         auto row_tiles = [&](int bm) {

@@ -553,7 +553,7 @@ struct Mx4Decode {
 
 // One row tile of a sequence and one K/V head a workgroup (SPLIT false), or a range of
 // the line.
-constexpr int MX4_LEAD = 2;
+constexpr int MX4_LEAD = 10;
 template <int NT, int WAVES, int SUB, int EU, bool SPLIT, bool LSE, bool P64>
 __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(EU, EU)))
 void mx4_decode_kernel(Fav4Mx4PagedArgs a, Mx4Plan pl) {
@@ -634,7 +634,7 @@ void mx4_decode_kernel(Fav4Mx4PagedArgs a, Mx4Plan pl) {
 // four scales, loaded two tiles ahead.  Of the two waves of a SIMD that eight make one
 // converts the next tile before its products and the other behind them, so that one's
 // conversion runs beside the other's products; two workgroups of four do that unasked.
-constexpr int MX4_MANY_LEAD = 2;
+constexpr int MX4_MANY_LEAD = 3;
 constexpr int MX4_LINE_TILES = 1024, MX4_LINE_SEQS = 512;      // of a batch that is cut into ranges
 
 template <int WAVES, bool LSE>
@@ -670,9 +670,6 @@ struct Mx4Prefill {
         RowState st;
         clear(st);
         if (t < e1) {
-            const LdsOffsets off = lds_offsets(lane);
-            bf16x8 qr[8];
-            load_q(pg, f.t0 + token, head, half, qr);
             // This thread's key, and which of its stretches of DWORDS * 8 dims.
             const int kr = wave * KEYS + lane / WAVES, j = lane % WAVES, block = j * DWORDS / 4;
             typedef uint32_t codes_t __attribute__((ext_vector_type(DWORDS)));
@@ -690,6 +687,9 @@ struct Mx4Prefill {
                 lo = int(r), hi = int(r >> 32);
             };
             hold(t);
+            const LdsOffsets off = lds_offsets(lane);
+            bf16x8 qr[8];
+            load_q(pg, f.t0 + token, head, half, qr);
             auto load = [&](int at) {
                 // Behind the last tile that again, into the stage that no step reads: no branch around the loads.
                 int e = min(at, e1 - 1) - held;
@@ -831,6 +831,7 @@ void mx4_prefill_line_kernel(Fav4Mx4PagedArgs a, Mx4Plan pl) {
     constexpr int BM = WAVES * 32, THREADS = WAVES * 64;
     __shared__ int seq_end[MX4_LINE_SEQS], unit_end[MX4_LINE_TILES], waves[WAVES];
     __shared__ uint16_t seq_of[MX4_LINE_TILES];
+    __shared__ Mx4Seq seqs[MX4_LINE_SEQS];
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
     const Mx4Prefill<WAVES, LSE> x{a, pl, smem, lane, wave};
     const Fav4PagedArgs& pg = a.paged;
@@ -852,7 +853,10 @@ void mx4_prefill_line_kernel(Fav4Mx4PagedArgs a, Mx4Plan pl) {
     };
     int tiles = 0;
     for (int b0 = 0; b0 < pg.batch; b0 += THREADS) {
-        const int b = b0 + tid, n = b < pg.batch ? x.tiles_of(mx4_seq(pg, b)) : 0;
+        const int b = b0 + tid;
+        Mx4Seq f{};
+        if (b < pg.batch) seqs[b] = f = mx4_seq(pg, b);
+        const int n = x.tiles_of(f);
         int all;
         const int end = tiles + scan(n, all);
         if (b < pg.batch) seq_end[b] = end;
@@ -867,7 +871,7 @@ void mx4_prefill_line_kernel(Fav4Mx4PagedArgs a, Mx4Plan pl) {
         int c = 0;
         if (i < tiles) {
             const int b = seq_of[i];
-            c = max(1, x.key_tiles(mx4_seq(pg, b), i - (b > 0 ? seq_end[b - 1] : 0))) + MX4_MANY_LEAD;
+            c = max(1, x.key_tiles(seqs[b], i - (b > 0 ? seq_end[b - 1] : 0))) + MX4_MANY_LEAD;
         }
         int all;
         const int end = units + scan(c, all);
@@ -889,7 +893,7 @@ void mx4_prefill_line_kernel(Fav4Mx4PagedArgs a, Mx4Plan pl) {
         const int base = uniform(i > 0 ? unit_end[i - 1] : 0), end = uniform(unit_end[i]);
         if (base >= g1) break;
         const int b = uniform(seq_of[i]), rt = i - uniform(b > 0 ? seq_end[b - 1] : 0);
-        Mx4Seq f = mx4_seq(pg, b);
+        Mx4Seq f = seqs[b];
         f = {uniform(f.t0), uniform(f.tokens), uniform(f.keys)};
         const int n = uniform(x.key_tiles(f, rt)), first = end - max(n, 1);
         if (first >= g1) break;
