@@ -18,6 +18,7 @@ constexpr int BOTTOM_RIGHT = 2;
 constexpr int MAX_KEYS = INT_MAX - 255;       // in whole pages: a position and a tile's width fit an int
 constexpr int MAX_HEADS = 1 << 15;            // the documented limit; indexes need total_q * heads < 2^31 alone
 constexpr int MAX_ROW_TILES = 1 << 22;
+constexpr int MAX_KEY_TILES = 1'000'000'000;
 
 // CU count of the current device (256 if it cannot be read), cached per
 // device after the first query.
@@ -170,7 +171,8 @@ Sizes paged_sizes(const Fav4Mx4PagedArgs& args, int causal) {
     p.br = causal == BOTTOM_RIGHT;
     s.few = seq_rows <= FEW_ROWS;
     // Workgroups of a K/V head that are resident at once, at most: with few rows, and with many.
-    const int few_ranges = std::max(1, line_per_cu(1) * cus / a.kv_heads), many_ranges = std::max(1, 2 * cus / a.kv_heads);
+    const int few_ranges = std::max(1, line_per_cu(1) * cus / a.kv_heads);
+    auto many_ranges = [&](int waves) { return std::max(1, 8 / waves * cus / a.kv_heads); };
     int64_t segs;
     if (s.few) {
         p.stride = seq_rows <= 16 ? 16 : 32;
@@ -192,11 +194,12 @@ Sizes paged_sizes(const Fav4Mx4PagedArgs& args, int causal) {
         segs = row_tiles(p.stride);
         p.tiles = int(std::min<int64_t>(segs, INT_MAX));
         s.split = cut.line && segs <= fav4::MX4_LINE_TILES && a.batch <= fav4::MX4_LINE_SEQS;
-        p.ranges = s.split ? std::max(1, 8 / s.waves * cus / a.kv_heads) : 1;
+        p.ranges = s.split ? many_ranges(s.waves) : 1;
     }
     s.grid = a.kv_heads * (s.split ? int64_t(p.ranges) : segs);
-    s.ok = segs <= MAX_ROW_TILES && s.grid < (int64_t(1) << 30) &&
-           segs * (int64_t(a.max_seqlen_k) / 64 + 1 + std::max(fav4::MX4_LEAD, fav4::MX4_MANY_LEAD)) < (1 << 30);
+    // A grid has less than 2^32 threads, and the units of a line (of 32 keys) end below 2^31.
+    s.ok = segs <= MAX_ROW_TILES && s.grid < (int64_t(1) << 23) &&
+           segs * (int64_t(a.max_seqlen_k) / 64 + 1 + std::max(fav4::MX4_LEAD, fav4::MX4_MANY_LEAD)) < MAX_KEY_TILES;
     p.by_kv_heads = fav4::fast_div(a.kv_heads);
     p.by_group = fav4::fast_div(int(group));
     p.by_page = fav4::fast_div(a.page_size);
@@ -206,7 +209,9 @@ Sizes paged_sizes(const Fav4Mx4PagedArgs& args, int causal) {
     s.merge_grid = int64_t(p.ranges) * a.kv_heads * p.merge_chunks;
     p.by_merge = fav4::fast_div(p.merge_chunks);
     // What a call of either kind could need: more queries or sequences never need less.
-    s.part_rows = int64_t(a.kv_heads) * 2 * (s.few ? few_ranges * 32 : std::max(few_ranges * 32, many_ranges * 128));
+    // (With more K/V heads than CUs a range of 128-row tiles holds less than one of 256.)
+    const int few_part = few_ranges * 32, many_part = std::max(many_ranges(8) * 256, many_ranges(4) * 128);
+    s.part_rows = int64_t(a.kv_heads) * 2 * (s.few ? few_part : std::max(few_part, many_part));
     s.bytes = s.part_rows * (fav4::D * 4 + 8) + int64_t(few_ranges) * 16;
     return s;
 }

@@ -83,13 +83,13 @@ struct Fav4Mx4PagedArgs {
 // Checks: those of Fav4PagedArgs with causal 0 or 2, page_size a multiple of 16,
 // max_seqlen_k <= max_pages_per_seq * page_size and in whole pages < 2^31 - 255, heads
 // <= 2^15, total_q * heads < 2^31, 16-byte aligned scales, caches of less than 2^48
-// bytes, and a plan of fewer than 2^30 key tiles and 2^22 row tiles.  The workspace is
-// caller-owned device memory, 256-byte aligned, of at least
-// fav4_bshd_paged_mx4_workspace_size() bytes and not shared with a concurrent call
-// (two captured graphs that may run at once included); its contents do not matter.  The
-// size query reads only the sizes (pointers may be NULL), returns -1 for rejected
-// arguments, and never less for a larger batch or more queries; it does not depend on
-// the keys.
+// bytes, and a plan of fewer than 10^9 key tiles, at most 2^22 row tiles, and fewer than
+// 2^23 row tiles over all K/V heads.  The workspace is caller-owned device memory,
+// 256-byte aligned, of at least fav4_bshd_paged_mx4_workspace_size() bytes and not shared
+// with a concurrent call (two captured graphs that may run at once included); its
+// contents do not matter.  The size query reads only the sizes (pointers may be NULL),
+// returns -1 for rejected arguments, and never less for a larger batch or more queries:
+// the size follows from kv_heads and from whether a sequence may have more than 64 rows.
 extern "C" int fav4_bshd_forward_paged_mx4(const Fav4Mx4PagedArgs* args, int causal, void* workspace,
                                            size_t workspace_bytes, hipStream_t stream);
 extern "C" long long fav4_bshd_paged_mx4_workspace_size(const Fav4Mx4PagedArgs* args, int causal);

@@ -88,6 +88,21 @@ def test_workspaces_and_padded_batches(gpu_runner, kind, total_k):
     assert torch.equal(first[0][:batch.total], o[:batch.total]) and torch.equal(first[1][:, :batch.total], lse[:, :batch.total])
 
 
+@pytest.mark.parametrize("heads,lens", [(300, [(256, 4000)]), (600, [(130, 1500), (90, 900)]), (800, [(2, 700)])])
+def test_more_heads_than_cus(gpu_runner, heads, lens):
+    """A range for each K/V head, in a workspace of exactly its size between guards."""
+    batch = Cache4(heads, heads, 64, lens)
+    o, lse = batch.outputs(True)
+    need = gpu_runner.paged_mx4_workspace_size(len(lens), heads, heads, batch.max_q, batch.max_k, o.shape[0], 64,
+                                               batch.table.shape[1], batch.caches[0].shape[0], 2)
+    guard = 1 << 20
+    room = torch.full((guard + need + guard,), 0xff, dtype=torch.uint8, device=batch.dev)
+    batch.attend(gpu_runner, o, lse, 2, workspace=room[guard:guard + need])
+    batch.check(o, lse, 2)
+    assert (room[:guard] == 0xff).all() and (room[guard + need:] == 0xff).all()
+    assert_guard_rows_untouched(batch)
+
+
 def test_more_sequences_than_a_line_is_laid_out_for(gpu_runner):
     """600 sequences, some of them of many rows: past what a workgroup keeps in LDS."""
     rng = np.random.default_rng(3)

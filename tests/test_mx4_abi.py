@@ -195,6 +195,25 @@ def test_workspace_grows_with_the_batch(pkg, lib):
         assert size(kv_heads=kvh, heads=max(32, kvh), max_seqlen_k=64) == size(kv_heads=kvh, heads=max(32, kvh))
 
 
+@pytest.mark.parametrize("kv_heads", [1, 8, 200, 257, 300, 512, 513, 2000, 1 << 15])
+def test_workspace_holds_both_parts_of_a_row_tile(pkg, lib, kv_heads):
+    """Every K/V head has a range of its own at least, with two partial blocks of up to 256 rows (32 with few rows): 128
+    numbers of 4 bytes and two sums a row."""
+    for q, rows in ((1, 32), (32, 32), (300, 256)):
+        a = paged_args(pkg, heads=kv_heads, kv_heads=kv_heads, max_seqlen_q=q, total_q=q, batch=1)
+        assert lib.fav4_bshd_paged_mx4_workspace_size(C.byref(a), 2) >= kv_heads * 2 * rows * (128 * 4 + 8) + 16
+
+
+def test_grids_stay_below_the_most_threads(pkg, lib):
+    """2^22 row tiles are too many over 8 K/V heads, not over one."""
+    size = lambda kvh, total: lib.fav4_bshd_paged_mx4_workspace_size(C.byref(paged_args(
+        pkg, batch=1, heads=8, kv_heads=kvh, max_seqlen_q=total, total_q=total, max_seqlen_k=64)), 2)
+    assert size(1, 1 << 23) > 0 and size(8, 1 << 25) > 0
+    many = lambda kvh: lib.fav4_bshd_paged_mx4_workspace_size(C.byref(paged_args(
+        pkg, batch=1 << 21, heads=64, kv_heads=kvh, max_seqlen_q=100, total_q=1 << 24, max_seqlen_k=64)), 2)
+    assert many(64) == -1
+
+
 def test_runner_refuses_host_tensors_and_wrong_ones(pkg):
     import torch
     r = pkg.Runner()
