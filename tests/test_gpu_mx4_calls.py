@@ -159,9 +159,11 @@ def test_graph_follows_the_lengths(gpu_runner, kind):
 def test_two_graphs_with_workspaces_of_their_own(gpu_runner):
     batches = [Cache4(8, 1, 32, [(1, 4000), (1, 900)], seed=s) for s in (1, 2)]
     streams, graphs, outs = [torch.cuda.Stream() for _ in batches], [], []
+    workspaces = []                   # both live as long as the graphs: entering a capture gives unused memory back
     for batch, stream in zip(batches, streams):
         out = batch.outputs(True)
         ws = batch.attend(gpu_runner, *out, 0)
+        workspaces.append(ws)
         torch.cuda.synchronize()
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph, stream=stream):
