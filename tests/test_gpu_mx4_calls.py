@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from tests.mx4 import Cache4, assert_guard_rows_untouched, quantise, values
-from tests.serving import D, angles
+from tests.serving import D, SCALE, angles
 from tests.test_gpu_mx4_append import Tokens
 
 pytestmark = pytest.mark.gpu
@@ -58,6 +58,19 @@ def test_large_scores(gpu_runner, kind):
     o, _ = batch.outputs(False)
     batch.attend(gpu_runner, o, None, 2)
     batch.check(o, None, 2, weight_err=3.2e-3)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_scale(gpu_runner, kind):
+    """A quarter of the scale is a quarter of the queries, bit by bit: powers of two do not change a rounding."""
+    batch = Cache4(8, 2, 16, KINDS[kind])
+    outs = []
+    for scale, q in ((SCALE / 4, batch.q), (None, batch.q / 4)):
+        o, lse = batch.outputs(True)
+        batch.attend(gpu_runner, o, lse, 2, q=q, scale=scale)
+        outs.append((o, lse))
+    assert torch.equal(outs[0][0], outs[1][0]) and torch.equal(outs[0][1], outs[1][1])
+    batch.check(*outs[1], 2, q=batch.q / 4)
 
 
 @pytest.mark.parametrize("kind", KINDS)
