@@ -99,10 +99,17 @@ bool paged_shape_ok(const Fav4Mx4PagedArgs* args, int causal) {
 constexpr int LINE_WAVES = 4, WHOLE_WAVES = 8;
 constexpr int line_per_cu(int row_tiles) { return row_tiles == 1 ? 3 : 2; }
 constexpr int line_subtiles(int row_tiles) { return row_tiles == 1 ? 2 : 4; }
-// Keys that a workgroup of a line should have at least: 24 sequences of 1000..16384, H8
-// KVH1, 17.1 us with 384, 18.3 with 128; 32 x 4 queries behind 200..4096, H32 KVH8, 24.6
-// with 384, 25.5 with 768, 30.1 with 1536.
-constexpr int LINE_KEYS = 384;
+// Keys that a workgroup of a line should have at least: what it takes grows with them, what
+// the merge takes with the longest sequence's parts; their sum is least near the root of its
+// keys.  With 4, 5, 3 times that and with 384: 4 sequences of 100..2000, H32 KVH8, 9.0, 9.5,
+// 9.8 and 10.4 us; 24 of 1000..16384, H8 KVH1, 15.4, 15.1, 15.5 and 15.5; 3 x 6 queries
+// behind 540..8641, H16 KVH2, 15.6, 17.3, 16.0 and 15.6.
+double line_keys(int max_keys) { return std::max(128.0, 4 * std::sqrt(double(max_keys))); }
+// Up to this many parts of the longest sequence's rows four teams of a merge take two parts
+// each at once, above eight teams four: 24 of 1000..16384, H8 KVH1, 15.5 so and 16.5 with
+// four, 48 of 100..4096, H32 KVH8, 19.4 and with eight 20.2 (20.6 with four of eight parts
+// each, many of whose loads find no part).
+constexpr int MERGE_PARTS = 16;
 // Up to this many rows a sequence go by the decode kernel.
 constexpr int FEW_ROWS = 64;
 
@@ -181,7 +188,7 @@ Sizes paged_sizes(const Fav4Mx4PagedArgs& args, int causal) {
         const int resident = std::max(1, line_per_cu(p.stride / 16) * cus / a.kv_heads);
         const int64_t keys = a.total_k > 0 ? a.total_k : int64_t(a.batch) * a.max_seqlen_k;
         s.split = !whole_sequences(segs * a.kv_heads, seq_rows, a.max_seqlen_k, double(keys) * p.tiles * a.kv_heads, cus);
-        p.ranges = s.split ? int(std::min<int64_t>(resident, keys * p.tiles / LINE_KEYS + 1)) : 1;
+        p.ranges = s.split ? int(std::min(double(resident), 1 + double(keys) * p.tiles / line_keys(a.max_seqlen_k))) : 1;
     } else {
         auto row_tiles = [&](int bm) {
             return std::min<int64_t>(a.batch * ((seq_rows + bm - 1) / bm), (rows + int64_t(a.batch) * (bm - 1)) / bm);
@@ -203,8 +210,9 @@ Sizes paged_sizes(const Fav4Mx4PagedArgs& args, int causal) {
     p.by_kv_heads = fav4::fast_div(a.kv_heads);
     p.by_group = fav4::fast_div(int(group));
     p.by_page = fav4::fast_div(a.page_size);
-    // Teams per merged row: many where the row tiles are few and cut into many parts.
-    s.merge_teams = s.few ? 4 : 1;
+    // Teams per merged row, by how many parts the longest sequence's rows are in.
+    const double keys = a.total_k > 0 ? double(a.total_k) : double(a.batch) * a.max_seqlen_k;
+    s.merge_teams = !s.few ? 1 : a.max_seqlen_k * double(p.ranges) <= MERGE_PARTS * keys * p.tiles ? 4 : 8;
     p.merge_chunks = int((std::min<int64_t>(p.stride, seq_rows) * s.merge_teams + 15) / 16);
     s.merge_grid = int64_t(p.ranges) * a.kv_heads * p.merge_chunks;
     p.by_merge = fav4::fast_div(p.merge_chunks);
@@ -307,7 +315,8 @@ extern "C" __attribute__((visibility("default"))) int fav4_bshd_forward_paged_mx
     auto merge = [&](auto kernel) {
         hipLaunchKernelGGL(kernel, dim3(unsigned(s.merge_grid)), dim3(256), 0, stream, *args, p);
     };
-    if (s.merge_teams == 4) merge(fav4::mx4_merge_kernel<4>);
-    else merge(fav4::mx4_merge_kernel<1>);
+    if (s.merge_teams == 8) merge(fav4::mx4_merge_kernel<8, 4>);
+    else if (s.merge_teams == 4) merge(fav4::mx4_merge_kernel<4, 2>);
+    else merge(fav4::mx4_merge_kernel<1, 4>);
     return hipGetLastError();
 }

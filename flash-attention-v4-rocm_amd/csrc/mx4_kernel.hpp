@@ -912,11 +912,12 @@ void mx4_prefill_line_kernel(Fav4Mx4PagedArgs a, Mx4Plan pl) {
 // The row tiles that were cut: workgroup by workgroup 16 / PER rows of a range's, with one
 // K/V head.  PER teams of 16 lanes share a row, 8 dims a lane; a team takes every PER-th
 // part, NS at a time with all their loads in flight, with the running maximum and sums of a
-// softmax over the parts' log-sums.  Bound by latency: the first parts are loaded beside the
-// note that says how many there are.
-template <int PER>
+// softmax over the parts' log-sums.  Bound by latency (3.6 to 5 us, as little as a kernel
+// that follows another and reads what it wrote can take): the first parts are loaded beside
+// the note that says how many there are.
+template <int PER, int NS>
 __global__ __launch_bounds__(256) void mx4_merge_kernel(Fav4Mx4PagedArgs a, Mx4Plan pl) {
-    constexpr int RPB = 16 / PER, NS = PER == 1 ? 4 : 8;
+    constexpr int RPB = 16 / PER;
     __shared__ float4 red[16];
     __shared__ f32x4 red_o[16][32];
     const Fav4PagedArgs& pg = a.paged;
