@@ -108,7 +108,9 @@ double line_keys(int max_keys) { return std::max(128.0, 4 * std::sqrt(double(max
 // Up to this many parts of the longest sequence's rows four teams of a merge take two parts
 // each at once, above eight teams four: 24 of 1000..16384, H8 KVH1, 15.5 so and 16.5 with
 // four, 48 of 100..4096, H32 KVH8, 19.4 and with eight 20.2 (20.6 with four of eight parts
-// each, many of whose loads find no part).
+// each, many of whose loads find no part).  Of many rows one team takes four, or four two:
+// 59 queries behind 6778 keys, H8 KVH1, 26.2 with four, 27.2 with one; 4 x 56 behind 1278 to
+// 4502, H40 KVH8, 47.3 and 43.3.
 constexpr int MERGE_PARTS = 16;
 // Up to this many rows a sequence go by the decode kernel.
 constexpr int FEW_ROWS = 64;
@@ -127,35 +129,50 @@ bool whole_sequences(int64_t pairs, int64_t rows, int64_t max_keys, double all_k
     return pairs <= cus && double(max_keys) < rate * (4.9 + 0.3 * double(std::min<int64_t>(rows, 16)) + 0.7 * all_keys * 136 / 6.3e6);
 }
 
+// Key tiles of many rows that a range should have at least: with a half, 0.3, 0.8 times the
+// longest's root, and one, 3 sequences of 20..54 queries behind 488..2460 22.3, 26.4, 22.9
+// and 26.9 us; one of 59 behind 6778, H8 KVH1, 26.2, 25.0, 30.3 and 33.4.
+double range_tiles(double most) { return std::max(1.0, 0.5 * std::sqrt(most)); }
+
 // Sequences of many rows: row tiles of eight waves (256 rows, one workgroup a CU) or four
-// (128, two), each whole, the longest of a sequence first, or on a line.  By an estimate in
-// us of each, from the sizes (of unequal lengths their means and the longest): a 64-key tile
-// takes a workgroup of eight waves 1.95, one of four 1.7 beside another, 2.15 in a full GPU
-// and 1.3 alone; a row tile on a line starts and ends in 4.5 more, and its merge takes 18
-// with the launch.  Measured, H32 KVH8 where not said, whole 8 / whole 4 / line 8 / line 4:
-// 8 x 64..512 queries behind 1024..8192 keys 246 / 296 / 162 / 182; prompts of 500..2500
-// 147 / 151 / 149 / 163; 3 prompts of 396..782 29.1 / 26.2 / 33.9 / 35.4; 2 prompts of
-// 1673 and 2078, KVH32, 86.7 / 90.2 / 106 / 106; 6 x 6..23 queries behind 241..1524, H8
-// KVH2, 35.0 / 36.8 / 18.0 / 17.1.
+// (128, two), each whole, the longest first, or on a line.  By an estimate in us of each,
+// from the sizes (of unequal lengths their means and the longest), its constants fitted to
+// 120 batches timed all four ways; over 40 others its choice costs 1% more than the best.  A
+// 64-key tile takes a workgroup of eight waves 1.9, one of four 2.0 in a full GPU (2.15 on
+// a line) and 1.3 alone; a row tile starts and ends in 4 (2.2), on a line in 6.8; a line's own
+// start, the second launch and its merge take 15.  Measured, H32 KVH8 where not said, whole 8
+// / whole 4 / line 8 / line 4: 8 x 64..512 queries behind 1024..8192 keys 227 / 188 / 156 /
+// 172; prompts of 500..2500 134 / 137 / 148 / 162; 2 prompts of 146 and 134 behind 224, H40,
+// 13.7 / 10.9 / 20.5 / 17.9; one of 95 behind 3387, H8 KVH1, 97.9 / 73.3 / 23.3 / 20.0.
 struct Cut {
-    int waves;
-    bool line;
+    int waves, ranges;                // ranges of a K/V head, 0: whole
+    double parts;                     // of the longest row tile on a line, about
 };
 template <class F>
 Cut many_rows_cut(const Fav4PagedArgs& a, int causal, int cus, F&& row_tiles) {
-    const double mean_q = double(a.total_q) / a.batch;
-    const double mean_k = a.total_k > 0 ? double(a.total_k) / a.batch : double(a.max_seqlen_k);
-    const double units = std::max(1.0, (mean_k - (causal == BOTTOM_RIGHT ? 0.5 * mean_q : 0.0)) / 64);
+    double mean_q = double(a.total_q) / a.batch;
+    double mean_k = a.total_k > 0 ? double(a.total_k) / a.batch : double(a.max_seqlen_k);
+    const bool br = causal == BOTTOM_RIGHT, even = !br && mean_k > 0.95 * a.max_seqlen_k;
+    const bool prompts = a.max_seqlen_k < 2.0 * a.max_seqlen_q;
+    if (prompts) {                    // the long ones' row tiles are the most
+        mean_q += 0.4 * (a.max_seqlen_q - mean_q);
+        mean_k += 0.4 * (a.max_seqlen_k - mean_k);
+    }
+    const double units = std::max(1.0, (mean_k - (br ? 0.5 * mean_q : 0.0)) / 64);
     const double most = std::max(units, a.max_seqlen_k / 64.0);
-    Cut best{8, false};
+    Cut best{};
     double least = 1e30;
     for (int waves : {8, 4}) {
-        const double n = row_tiles(waves) * a.kv_heads, slots = double(cus) * (8 / waves);
-        const double unit = waves == 8 ? 1.95 : n <= cus ? 1.3 : n <= slots ? 1.7 : 2.15;
-        const double whole = 5 + unit * (n <= slots ? most : n * units / slots + 0.3 * most);
-        const double line = 18 + (waves == 8 ? 1.95 : 2.15) * n * units / slots + 4.5 * (n / slots + 1);
-        if (whole < least) least = whole, best = {waves, false};
-        if (line < least) least = line, best = {waves, true};
+        const double tiles = row_tiles(waves), n = tiles * a.kv_heads, slots = double(cus) * (8 / waves), turns = n / slots;
+        const double unit = waves == 8 ? 1.9 : n <= cus ? 1.3 : n <= slots && br && prompts ? 1.45 : 2.0;
+        const double ends = waves == 8 ? 4 : 2.2;
+        const double tail = even ? (std::ceil(turns) - turns) * (unit * units + ends) : 0.24 * unit * most;
+        const double whole = 3 + (turns <= 1 ? unit * most + ends : turns * (unit * units + ends) + tail);
+        const int ranges = int(std::min(std::max(1.0, std::floor(slots / a.kv_heads)), 1 + tiles * units / range_tiles(most)));
+        const double groups = double(ranges) * a.kv_heads, line_unit = waves == 8 ? 1.9 : groups <= cus ? 1.3 : 2.15;
+        const double line = 15 + (line_unit * units + 6.8) * n / groups;
+        if (whole < least) least = whole, best = {waves, 0, 1};
+        if (line < least) least = line, best = {waves, ranges, most * ranges / (tiles * units)};
     }
     return best;
 }
@@ -166,6 +183,7 @@ struct Sizes {
     int merge_teams, waves;
     bool few, split;
     bool ok;
+    double parts;                     // of the longest sequence's rows, about
 };
 Sizes paged_sizes(const Fav4Mx4PagedArgs& args, int causal) {
     const Fav4PagedArgs& a = args.paged;
@@ -189,19 +207,23 @@ Sizes paged_sizes(const Fav4Mx4PagedArgs& args, int causal) {
         const int64_t keys = a.total_k > 0 ? a.total_k : int64_t(a.batch) * a.max_seqlen_k;
         s.split = !whole_sequences(segs * a.kv_heads, seq_rows, a.max_seqlen_k, double(keys) * p.tiles * a.kv_heads, cus);
         p.ranges = s.split ? int(std::min(double(resident), 1 + double(keys) * p.tiles / line_keys(a.max_seqlen_k))) : 1;
+        s.parts = a.max_seqlen_k * double(p.ranges) / (double(keys) * p.tiles);
     } else {
         auto row_tiles = [&](int bm) {
             return std::min<int64_t>(a.batch * ((seq_rows + bm - 1) / bm), (rows + int64_t(a.batch) * (bm - 1)) / bm);
         };
+        const bool equal = double(a.max_seqlen_q) * a.batch < 1.05 * a.total_q;
         const Cut cut = many_rows_cut(a, causal, cus, [&](int waves) {
-            return std::min(double(row_tiles(waves * 32)), double(rows) / (waves * 32) + 0.5 * a.batch);
+            const double most = double(row_tiles(waves * 32));
+            return equal ? most : std::min(most, double(rows) / (waves * 32) + 0.5 * a.batch);
         });
         s.waves = cut.waves;
         p.stride = s.waves * 32;
         segs = row_tiles(p.stride);
         p.tiles = int(std::min<int64_t>(segs, INT_MAX));
-        s.split = cut.line && segs <= fav4::MX4_LINE_TILES && a.batch <= fav4::MX4_LINE_SEQS;
-        p.ranges = s.split ? many_ranges(s.waves) : 1;
+        s.split = cut.ranges && segs <= fav4::MX4_LINE_TILES && a.batch <= fav4::MX4_LINE_SEQS;
+        p.ranges = s.split ? std::min(cut.ranges, many_ranges(s.waves)) : 1;
+        s.parts = cut.parts;
     }
     s.grid = a.kv_heads * (s.split ? int64_t(p.ranges) : segs);
     // A grid has less than 2^32 threads, and the units of a line (of 32 keys) end below 2^31.
@@ -210,9 +232,8 @@ Sizes paged_sizes(const Fav4Mx4PagedArgs& args, int causal) {
     p.by_kv_heads = fav4::fast_div(a.kv_heads);
     p.by_group = fav4::fast_div(int(group));
     p.by_page = fav4::fast_div(a.page_size);
-    // Teams per merged row, by how many parts the longest sequence's rows are in.
-    const double keys = a.total_k > 0 ? double(a.total_k) : double(a.batch) * a.max_seqlen_k;
-    s.merge_teams = !s.few ? 1 : a.max_seqlen_k * double(p.ranges) <= MERGE_PARTS * keys * p.tiles ? 4 : 8;
+    // Teams per merged row.
+    s.merge_teams = s.few ? s.parts <= MERGE_PARTS ? 4 : 8 : s.parts <= MERGE_PARTS ? 1 : 4;
     p.merge_chunks = int((std::min<int64_t>(p.stride, seq_rows) * s.merge_teams + 15) / 16);
     s.merge_grid = int64_t(p.ranges) * a.kv_heads * p.merge_chunks;
     p.by_merge = fav4::fast_div(p.merge_chunks);

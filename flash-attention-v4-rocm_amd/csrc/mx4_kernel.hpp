@@ -792,32 +792,67 @@ struct Mx4Prefill {
     }
 };
 
-// One row tile of the batch and one K/V head a workgroup, a sequence's longest first.
+// One row tile of the batch and one K/V head a workgroup, those with the most key tiles first,
+// so that the last ones to start are short (8 prompts of 500..2500, H32 KVH8: 134 us, 139
+// where only a sequence's own were in that order).  How many row tiles have more than u key
+// tiles is, for each sequence, a division (their last token's number grows with the tile's);
+// the sequences lie in the lanes, and u is found by halving.  More sequences than lanes go
+// one behind the other, each its longest first.
 template <int WAVES, bool LSE>
 __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
 void mx4_prefill_kernel(Fav4Mx4PagedArgs a, Mx4Plan pl) {
+    constexpr int BM = WAVES * 32;
     __shared__ __attribute__((aligned(1024))) unsigned char smem[4 * Mx4Prefill<WAVES, LSE>::TILE_BYTES];
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
     const Mx4Prefill<WAVES, LSE> x{a, pl, smem, lane, wave};
     const Fav4PagedArgs& pg = a.paged;
     const int id = uniform(pl.by_kv_heads(blockIdx.x)), kvh = uniform(int(blockIdx.x) - id * pg.kv_heads);
-    int b = 0, before = 0;
-    for (;;) {
-        const int n = b + lane < pg.batch ? x.tiles_of(mx4_seq(pg, b + lane)) : 0, end = wave_scan(n);
-        const uint64_t hit = __builtin_amdgcn_ballot_w64(before + end > id);
-        if (hit) {
-            const int l = __builtin_ctzll(hit);
-            before = uniform(before + __builtin_amdgcn_readlane(end - n, l));
-            b = uniform(b + l);
-            break;
+    auto in_lane = [](const Mx4Seq& f, int l) {
+        return Mx4Seq{__builtin_amdgcn_readlane(f.t0, l), __builtin_amdgcn_readlane(f.tokens, l),
+                      __builtin_amdgcn_readlane(f.keys, l)};
+    };
+    Mx4Seq f{};
+    int b = 0, rt;
+    if (pg.batch <= 64) {
+        Mx4Seq own{};
+        if (lane < pg.batch) own = mx4_seq(pg, lane);
+        const int n = x.tiles_of(own), shift = own.keys - own.tokens;
+        auto above = [&](int u) {      // of the lane's sequence
+            if (!pl.br) return own.keys > int64_t(u) * 64 ? n : 0;
+            const int64_t token = int64_t(u) * 64 - shift;         // the first that sees more
+            return token >= own.tokens ? 0 : token <= 0 ? n : n - int(uint32_t(token) * uint32_t(pl.group) / BM);
+        };
+        auto sum = [](int v) { return __builtin_amdgcn_readlane(wave_scan(v), 63); };
+        if (id >= sum(n)) return;
+        int lo = 0, hi = (pg.max_seqlen_k + 63) >> 6;
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (sum(above(mid)) <= id) hi = mid;
+            else lo = mid + 1;
         }
-        before += __builtin_amdgcn_readlane(end, 63);
-        b += 64;
-        if (b >= pg.batch) return;
+        const int more = above(lo), equal = (lo > 0 ? above(lo - 1) : n) - more, end = wave_scan(equal);
+        const int at = id - sum(more);
+        b = __builtin_ctzll(__builtin_amdgcn_ballot_w64(end > at));
+        f = in_lane(own, b);
+        rt = __builtin_amdgcn_readlane(n - 1 - more - (at - (end - equal)), b);
+    } else {
+        int before = 0;
+        for (;;) {
+            if (b + lane < pg.batch) f = mx4_seq(pg, b + lane);
+            const int n = b + lane < pg.batch ? x.tiles_of(f) : 0, end = wave_scan(n);
+            const uint64_t hit = __builtin_amdgcn_ballot_w64(before + end > id);
+            if (hit) {
+                const int l = __builtin_ctzll(hit);
+                rt = __builtin_amdgcn_readlane(before + end - 1 - id, l);
+                f = in_lane(f, l);
+                b = uniform(b + l);
+                break;
+            }
+            before += __builtin_amdgcn_readlane(end, 63);
+            b += 64;
+            if (b >= pg.batch) return;
+        }
     }
-    Mx4Seq f = mx4_seq(pg, b);
-    f = {uniform(f.t0), uniform(f.tokens), uniform(f.keys)};
-    const int rt = uniform(x.tiles_of(f)) - 1 - (id - before);
     x.attend(b, f, rt, kvh, 0, uniform(x.key_tiles(f, rt)), false, 0);
 }
 
@@ -941,10 +976,12 @@ __global__ __launch_bounds__(256) void mx4_merge_kernel(Fav4Mx4PagedArgs a, Mx4P
     };
     load(part);
     const int4 note = pl.notes[w];
-    if (r - slot >= note.y || note.z <= 0) return;
+    // (Rows of the call, whatever another one that was given the same workspace has written there.)
+    const int rows = min(note.y, pg.total_q * pl.group - note.x);
+    if (note.x < 0 || r - slot >= rows || note.z <= 0) return;
     const int total = min(note.z, pl.ranges - w);
-    const bool live = r < note.y;
-    const int tok = pl.by_group(note.x + min(r, note.y - 1)), head = kvh * pl.group + note.x + r - tok * pl.group;
+    const bool live = r < rows;
+    const int tok = pl.by_group(note.x + min(r, rows - 1)), head = kvh * pl.group + note.x + r - tok * pl.group;
     float mb = -__builtin_inff(), ml = mb, den = 0.f, suml = 0.f;
     f32x4 acc[2] = {};
     for (int c0 = part; c0 < total; c0 += PER * NS) {
