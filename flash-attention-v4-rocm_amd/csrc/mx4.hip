@@ -138,7 +138,7 @@ double range_tiles(double most) { return std::max(1.0, 0.5 * std::sqrt(most)); }
 // (128, two), each whole, the longest first, or on a line.  By an estimate in us of each,
 // from the sizes (of unequal lengths their means and the longest), its constants fitted to
 // 120 batches timed all four ways; over 40 others its choice costs 1% more than the best.  A
-// 64-key tile takes a workgroup of eight waves 1.9, one of four 2.0 in a full GPU (2.15 on
+// 64-key tile takes a workgroup of eight waves 1.9, one of four 2.06 in a full GPU (2.15 on
 // a line) and 1.3 alone; a row tile starts and ends in 4 (2.2), on a line in 6.8; a line's own
 // start, the second launch and its merge take 15.  Measured, H32 KVH8 where not said, whole 8
 // / whole 4 / line 8 / line 4: 8 x 64..512 queries behind 1024..8192 keys 227 / 188 / 156 /
@@ -164,7 +164,7 @@ Cut many_rows_cut(const Fav4PagedArgs& a, int causal, int cus, F&& row_tiles) {
     double least = 1e30;
     for (int waves : {8, 4}) {
         const double tiles = row_tiles(waves), n = tiles * a.kv_heads, slots = double(cus) * (8 / waves), turns = n / slots;
-        const double unit = waves == 8 ? 1.9 : n <= cus ? 1.3 : n <= slots && br && prompts ? 1.45 : 2.0;
+        const double unit = waves == 8 ? 1.9 : n <= cus ? 1.3 : n <= slots && br && prompts ? 1.45 : 2.06;
         const double ends = waves == 8 ? 4 : 2.2;
         const double tail = even ? (std::ceil(turns) - turns) * (unit * units + ends) : 0.24 * unit * most;
         const double whole = 3 + (turns <= 1 ? unit * most + ends : turns * (unit * units + ends) + tail);
