@@ -33,8 +33,10 @@ __device__ __forceinline__ bool mx4_no_numbers(uint32_t x) {
 // granules whose dims are rotated together.  The four granules of a block of 32 dims
 // then lie in up to four lanes, so the granules' largest magnitudes go through LDS
 // (as bits, whose order is that of the magnitudes, infinities and NaN above them) and
-// each lane reads its blocks' four.  Bound by memory, for few tokens by the chain of
-// dependent loads.
+// each lane reads its blocks' four.  Bound by memory (16 prompts of 500..4096, H32 KVH8,
+// 626 MB: 128 us, 4.9 TB/s; 123 with all rows of a token a wave and streaming Q stores, but
+// then 4 tokens take 3.6 in place of 3.2; 126 to 164 with one head of eight tokens a wave),
+// for few tokens by the chain offsets -> table -> store.
 // ---------------------------------------------------------------------------
 // The block's scale byte (255: not all numbers are finite) from its largest
 // magnitude's bits: the smallest e with max <= 1.75 * 2^(e + 2), i.e. the exponent,
@@ -286,6 +288,10 @@ __device__ __forceinline__ float quad_sum(float x) {
 //  * Keys are hidden by their scores, so V needs no other care than to be finite: a block
 //    with a scale above 252 becomes 0 there, and its key's scores NaN by way of its K
 //    scale.
+// Bound by memory where the GPU is full (32 sequences of 4096..16384, H32 KVH8: 76 us, 6.4
+// TB/s over the whole kernel), else by a wave's chain of conversions, products, softmax and
+// LDS, 1.8 us for 64 keys.  Two or three tiles ahead, four waves a SIMD, V converted before
+// the scores or read ahead of the softmax, rows of LDS padded by 32 bytes: no quicker.
 template <int NT>
 struct Mx4State {
     f32x4 o[NT][8], lb[NT];           // lb: sums of the BF16 weights, over all lanes
@@ -551,9 +557,12 @@ struct Mx4Decode {
     }
 };
 
+// What a row tile's start and end cost, in key tiles of 32 (64 with 32 rows): 64 sequences of
+// 500..8192, H32 KVH8, 43.3 us, with 8 and 12 43.5; 4 of 100..2000 10.5, 10.6 and 10.8.
+constexpr int MX4_LEAD = 10;
+
 // One row tile of a sequence and one K/V head a workgroup (SPLIT false), or a range of
 // the line.
-constexpr int MX4_LEAD = 10;
 template <int NT, int WAVES, int SUB, int EU, bool SPLIT, bool LSE, bool P64>
 __global__ __launch_bounds__(WAVES * 64) __attribute__((amdgpu_waves_per_eu(EU, EU)))
 void mx4_decode_kernel(Fav4Mx4PagedArgs a, Mx4Plan pl) {
@@ -634,7 +643,9 @@ void mx4_decode_kernel(Fav4Mx4PagedArgs a, Mx4Plan pl) {
 // four scales, loaded two tiles ahead.  Of the two waves of a SIMD that eight make one
 // converts the next tile before its products and the other behind them, so that one's
 // conversion runs beside the other's products; two workgroups of four do that unasked.
-constexpr int MX4_MANY_LEAD = 3;
+// Bound by the MFMAs and what the loop issues beside them: dense 8 x 2048 queries x 8192
+// keys, H32 KVH8, 1104 to 1138 TFLOP/s by the card (BF16 caches 1158 to 1189).
+constexpr int MX4_MANY_LEAD = 3;       // a row tile's start and end, in key tiles of 64
 constexpr int MX4_LINE_TILES = 1024, MX4_LINE_SEQS = 512;      // of a batch that is cut into ranges
 
 template <int WAVES, bool LSE>

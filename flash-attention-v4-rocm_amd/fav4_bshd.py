@@ -131,8 +131,8 @@ def parse_resource_usage(text: str) -> dict:
 def build_library(out: Path = LIB_PATH, verbose: bool = False) -> Path:
     """Compile ``csrc/bshd.hip`` for gfx950 into ``build/libfav4_bshd.so``, the
     serving operators ``csrc/serving.hip`` into ``build/libfav4_serving.so``, those of
-    4-bit caches ``csrc/mx4.hip`` into ``build/libfav4_mx4.so``, the loader probe ``csrc/loader_kat.hip`` into ``build/libfav4_loader_kat.so``
-    (a test library) and the MFMA-only probe ``csrc/mfma_ceiling.hip`` into
+    4-bit caches ``csrc/mx4.hip`` into ``build/libfav4_mx4.so``, the loader probe
+    ``csrc/loader_kat.hip`` into ``build/libfav4_loader_kat.so`` (a test library) and the MFMA-only probe ``csrc/mfma_ceiling.hip`` into
     ``build/libfav4_mfma_ceiling.so`` (a measurement library, read by
     ``bench.py --mfma-ceiling``), keep the compiler's kernel-resource-usage remarks in
     ``build/resource-usage.txt`` and write ``build/build-manifest.json``

@@ -17,7 +17,7 @@ def table():
 # Least waves a SIMD: the workgroups that the launches count on being resident at once.
 @pytest.mark.parametrize("pattern,count,waves", [(r"mx4_decode_kernelILi1ELi4E", 4, 3), (r"mx4_decode_kernelILi1ELi8E", 4, 2),
                                                  (r"mx4_decode_kernelILi2E", 8, 2), (r"mx4_prefill_kernelI", 4, 2),
-                                                 (r"mx4_prefill_line_kernelI", 4, 2), (r"mx4_merge_kernelI", 2, 4),
+                                                 (r"mx4_prefill_line_kernelI", 4, 2), (r"mx4_merge_kernelI", 3, 7),
                                                  (r"mx4_store_kernelI", 2, 7), (r"mx4_read_kernel", 1, 8)])
 def test_kernels_keep_their_waves(table, pattern, count, waves):
     kernels = {n: r for n, r in table.items() if re.search(pattern, n)}
