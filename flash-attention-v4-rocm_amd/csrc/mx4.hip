@@ -220,7 +220,6 @@ Sizes paged_sizes(const Fav4Mx4PagedArgs& args, int causal) {
         s.waves = cut.waves;
         p.stride = s.waves * 32;
         segs = row_tiles(p.stride);
-        p.tiles = int(std::min<int64_t>(segs, INT_MAX));
         s.split = cut.ranges && segs <= fav4::MX4_LINE_TILES && a.batch <= fav4::MX4_LINE_SEQS;
         p.ranges = s.split ? std::min(cut.ranges, many_ranges(s.waves)) : 1;
         s.parts = cut.parts;

@@ -244,7 +244,7 @@ struct Mx4Plan {
     int ranges;                       // of a K/V head
     FastDiv by_kv_heads, by_group, by_page, by_merge;
     int stride, merge_chunks;         // rows of a partial block; workgroups of the merge for those that can be live
-    int tiles;                        // row tiles that a sequence (few rows) or the batch (many) can have
+    int tiles;                        // row tiles that a sequence of few rows can have
     int br;                           // bottom-right causal
 };
 // The partial block of a row tile's part in range w.

@@ -75,6 +75,20 @@ def test_many_sequences(gpu_runner):
     run(gpu_runner, Cache4(4, 2, 16, [(int(q), int(k)) for q, k in zip(rng.integers(0, 60, 100), rng.integers(0, 300, 100))]), 2)
 
 
+@pytest.mark.parametrize("count", [40, 64, 65])
+@pytest.mark.parametrize("causal", [0, 2])
+def test_row_tiles_of_many_lengths(gpu_runner, count, causal):
+    """Row tiles of many rows in the order of their key tiles, among them idle sequences, equal ones, ones without keys and
+    ones with fewer keys than queries."""
+    rng = np.random.default_rng(count)
+    sq = rng.choice([0, 1, 33, 64, 65, 130, 257, 300], count)
+    sk = np.where(rng.random(count) < 0.5, sq, rng.integers(0, 700, count))
+    batch = Cache4(8, 4, 16, [(int(q), int(k)) for q, k in zip(sq, sk)])
+    run(gpu_runner, batch, causal)
+    run(gpu_runner, batch, causal, total_k=1)
+    run(gpu_runner, batch, causal, total_k=int(sk.sum()))
+
+
 def test_results_are_the_same_from_call_to_call(gpu_runner):
     for lens, causal in (([(1, 5000), (1, 77)] * 4, 0), ([(150, 1500)] * 2, 2)):
         batch = Cache4(8, 2, 64, lens)

@@ -27,12 +27,6 @@ def lib(pkg):
     return pkg.load_mx4_library()
 
 
-def _nested(outer, inner, name, over, **own):
-    for k, v in over.items():
-        (own if k in own else inner)[k] = v
-    return outer, inner, own
-
-
 def append_args(pkg, **over):
     """A call that would be accepted (addresses are never read on the host)."""
     inner = dict(q=0x10000, k=0x20000, v=0x30000, q_out=0x40000, k_cache=0x50000, v_cache=0x60000, cos=0x70000,
