@@ -112,8 +112,19 @@ double line_keys(int max_keys) { return std::max(128.0, 4 * std::sqrt(double(max
 // 59 queries behind 6778 keys, H8 KVH1, 26.2 with four, 27.2 with one; 4 x 56 behind 1278 to
 // 4502, H40 KVH8, 47.3 and 43.3.
 constexpr int MERGE_PARTS = 16;
-// Up to this many rows a sequence go by the decode kernel.
+// Whether a call goes by the decode kernel: with up to FEW_ROWS rows a sequence, and with
+// more where its row tiles of 32 are no more than the CUs and read so few keys in all (and
+// what their starts and ends cost) that the GPU is not full.  Decode / prefill kernels: H8
+// KVH1, 64 x 8 queries behind 1000..4000 25.3 / 28.5; H32 KVH8, 32 x 16 behind 2000..8000
+// 78.6 / 90.7, 32 x 20 109 / 94, 8 x 20 behind 500..2000 16.7 / 26.1; prompts, one of 128
+// 6.6 / 7.8, 13 of 26 26.7 / 6.8.
 constexpr int FEW_ROWS = 64;
+bool few_rows(int64_t seq_rows, double rows, double keys, int64_t batch, int kv_heads, int cus) {
+    if (seq_rows <= FEW_ROWS) return true;
+    const int64_t tiles = (seq_rows + 31) / 32;
+    return double(tiles) * double(batch) * kv_heads <= cus &&
+           (keys + 640. * double(batch)) * kv_heads * std::min(double(tiles), rows / 32 / double(batch) + 0.5) <= 750e3;
+}
 
 // Whether every sequence and K/V head (`pairs`) has a workgroup of its own, and no merge.
 // Measured, as graphs: such workgroups start and end in 4.2 us, read 290 keys a us (175 with
@@ -194,7 +205,8 @@ Sizes paged_sizes(const Fav4Mx4PagedArgs& args, int causal) {
     fav4::Mx4Plan& p = s.plan;
     p.group = int(group);
     p.br = causal == BOTTOM_RIGHT;
-    s.few = seq_rows <= FEW_ROWS;
+    const int64_t keys = a.total_k > 0 ? a.total_k : int64_t(a.batch) * a.max_seqlen_k;
+    s.few = few_rows(seq_rows, double(rows), double(keys), a.batch, a.kv_heads, cus);
     // Workgroups of a K/V head that are resident at once, at most: with few rows, and with many.
     const int few_ranges = std::max(1, line_per_cu(1) * cus / a.kv_heads);
     auto many_ranges = [&](int waves) { return std::max(1, 8 / waves * cus / a.kv_heads); };
@@ -204,7 +216,6 @@ Sizes paged_sizes(const Fav4Mx4PagedArgs& args, int causal) {
         p.tiles = int((seq_rows + p.stride - 1) / p.stride);
         segs = int64_t(a.batch) * p.tiles;
         const int resident = std::max(1, line_per_cu(p.stride / 16) * cus / a.kv_heads);
-        const int64_t keys = a.total_k > 0 ? a.total_k : int64_t(a.batch) * a.max_seqlen_k;
         s.split = !whole_sequences(segs * a.kv_heads, seq_rows, a.max_seqlen_k, double(keys) * p.tiles * a.kv_heads, cus);
         p.ranges = s.split ? int(std::min(double(resident), 1 + double(keys) * p.tiles / line_keys(a.max_seqlen_k))) : 1;
         s.parts = a.max_seqlen_k * double(p.ranges) / (double(keys) * p.tiles);
@@ -239,7 +250,7 @@ Sizes paged_sizes(const Fav4Mx4PagedArgs& args, int causal) {
     // What a call of either kind could need: more queries or sequences never need less.
     // (With more K/V heads than CUs a range of 128-row tiles holds less than one of 256.)
     const int few_part = few_ranges * 32, many_part = std::max(many_ranges(8) * 256, many_ranges(4) * 128);
-    s.part_rows = int64_t(a.kv_heads) * 2 * (s.few ? few_part : std::max(few_part, many_part));
+    s.part_rows = int64_t(a.kv_heads) * 2 * (seq_rows <= FEW_ROWS ? few_part : std::max(few_part, many_part));
     s.bytes = s.part_rows * (fav4::D * 4 + 8) + int64_t(few_ranges) * 16;
     return s;
 }

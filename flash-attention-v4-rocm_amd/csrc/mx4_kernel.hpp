@@ -227,8 +227,8 @@ __global__ __launch_bounds__(256) void mx4_read_kernel(Fav4Mx4GatherArgs a, Fast
 
 // ---------------------------------------------------------------------------
 // Attention.  Rows are (token, query head of the K/V head's group), r = token *
-// group + head.  Sequences of up to 64 rows (decode, drafts) go by mx4_decode_kernel,
-// longer ones by mx4_prefill_kernel.
+// group + head.  Sequences of up to 64 rows (decode, drafts), and of more where the call
+// does not fill the GPU, go by mx4_decode_kernel, others by mx4_prefill_kernel.
 // ---------------------------------------------------------------------------
 // Sequences' row tiles and their key tiles lie end to end on a line, a few units more
 // before each row tile for what its start and end cost, and the line is cut into equal

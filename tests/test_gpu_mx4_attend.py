@@ -75,6 +75,12 @@ def test_many_sequences(gpu_runner):
     run(gpu_runner, Cache4(4, 2, 16, [(int(q), int(k)) for q, k in zip(rng.integers(0, 60, 100), rng.integers(0, 300, 100))]), 2)
 
 
+@pytest.mark.parametrize("lse", [False, True])
+def test_a_row_tile_for_every_cu(gpu_runner, lse):
+    """256 row tiles of 256 rows."""
+    run(gpu_runner, Cache4(32, 8, 64, [(512, 2000)] * 4), 0, lse)
+
+
 @pytest.mark.parametrize("count", [40, 64, 65])
 @pytest.mark.parametrize("causal", [0, 2])
 def test_row_tiles_of_many_lengths(gpu_runner, count, causal):

@@ -15,7 +15,8 @@ pytestmark = pytest.mark.gpu
 KINDS = {"whole": [(1, 300), (1, 77), (1, 640)], "line": [(1, 5000), (1, 300), (1, 2100)] * 3,
          "drafts": [(5, 400), (5, 90)], "drafts_line": [(5, 6000), (5, 90), (3, 3500)],
          "prompts": [(150, 150), (200, 333)], "chunks": [(100, 4000), (40, 1500), (70, 70)],
-         "long_chunks": [(300, 9000), (250, 2000)]}
+         "long_chunks": [(300, 9000), (250, 2000)], "many_prompts": [(150, 150), (200, 333)] * 4,
+         "many_chunks": [(100, 4000), (40, 1500), (70, 70)] * 4}
 
 
 @pytest.mark.parametrize("kind", KINDS)
@@ -58,6 +59,18 @@ def test_large_scores(gpu_runner, kind):
     o, _ = batch.outputs(False)
     batch.attend(gpu_runner, o, None, 2)
     batch.check(o, None, 2, weight_err=3.2e-3)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_without_lse(gpu_runner, kind):
+    """O does not depend on whether the LSE is asked for."""
+    batch = Cache4(8, 2, 64, KINDS[kind])
+    with_lse = batch.outputs(True)
+    batch.attend(gpu_runner, *with_lse, 2)
+    o, _ = batch.outputs(False)
+    batch.attend(gpu_runner, o, None, 2)
+    batch.check(*with_lse, 2)
+    assert torch.equal(o, with_lse[0])
 
 
 @pytest.mark.parametrize("kind", KINDS)
@@ -130,7 +143,7 @@ def test_more_sequences_than_a_line_is_laid_out_for(gpu_runner):
 def test_lengths_and_pages_out_of_range(gpu_runner, page):
     """Key counts past max_seqlen_k are cut to it, negative ones are none; entries behind a sequence's keys are not used,
     whatever they are, also where a tile reaches past them."""
-    for kind in ("whole", "line", "drafts", "chunks"):
+    for kind in ("whole", "line", "drafts", "chunks", "many_prompts", "many_chunks"):
         batch = Cache4(8, 2, page, KINDS[kind] + [(1, 0)])
         most = max(sk for _, sk in batch.lens)
         want, got = batch.outputs(True), None
