@@ -38,6 +38,7 @@ KAT_LIB_PATH = ROOT / "build" / "libfav4_loader_kat.so"
 CEILING_LIB_PATH = ROOT / "build" / "libfav4_mfma_ceiling.so"
 SERVING_LIB_PATH = ROOT / "build" / "libfav4_serving.so"
 MX4_LIB_PATH = ROOT / "build" / "libfav4_mx4.so"
+MX4_BLOCKS_PATH = ROOT / "build" / "fav4_mx4_blocks.so"
 RESOURCE_LOG = ROOT / "build" / "resource-usage.txt"
 MANIFEST = ROOT / "build" / "build-manifest.json"
 
@@ -101,11 +102,6 @@ class Mx4PagedArgs(C.Structure):
     _fields_ = [("paged", PagedArgs)] + [(n, C.c_void_p) for n in ("k_scales", "v_scales")]
 
 
-_MX4_APPEND = struct.Struct("@12P4q10i2P")
-_MX4_GATHER = struct.Struct("@9P2q6i")
-_MX4_PAGED = struct.Struct("@8P10if2P")
-
-
 class Strides(C.Structure):
     """``struct Fav4Strides`` (include/fav4_bshd.h): element strides of a [B, S, H, 128] view."""
     _fields_ = [(n, C.c_longlong) for n in ("batch", "seq", "head")]
@@ -128,11 +124,26 @@ def parse_resource_usage(text: str) -> dict:
     return table
 
 
+def _extension_command(src: Path) -> list:
+    """The host compiler's command for a Python extension that reads torch tensors."""
+    import sysconfig
+    import torch
+    home = Path(torch.__file__).parent
+    system = ["/opt/rocm/include", home / "include", home / "include/torch/csrc/api/include",
+              sysconfig.get_paths()["include"]]
+    return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+            "-D__HIP_PLATFORM_AMD__", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{INCLUDE}",
+            *(x for d in system for x in ("-isystem", str(d))), str(src), f"-L{home / 'lib'}", "-ltorch_python",
+            "-ltorch_cpu", "-lc10"]
+
+
 def build_library(out: Path = LIB_PATH, verbose: bool = False) -> Path:
     """Compile ``csrc/bshd.hip`` for gfx950 into ``build/libfav4_bshd.so``, the
     serving operators ``csrc/serving.hip`` into ``build/libfav4_serving.so``, those of
-    4-bit caches ``csrc/mx4.hip`` into ``build/libfav4_mx4.so``, the loader probe
-    ``csrc/loader_kat.hip`` into ``build/libfav4_loader_kat.so`` (a test library) and the MFMA-only probe ``csrc/mfma_ceiling.hip`` into
+    4-bit caches ``csrc/mx4.hip`` into ``build/libfav4_mx4.so`` and their binding's argument
+    blocks ``csrc/mx4_blocks.cpp`` into ``build/fav4_mx4_blocks.so``, the loader probe
+    ``csrc/loader_kat.hip`` into ``build/libfav4_loader_kat.so`` (a test library) and the
+    MFMA-only probe ``csrc/mfma_ceiling.hip`` into
     ``build/libfav4_mfma_ceiling.so`` (a measurement library, read by
     ``bench.py --mfma-ceiling``), keep the compiler's kernel-resource-usage remarks in
     ``build/resource-usage.txt`` and write ``build/build-manifest.json``
@@ -145,16 +156,19 @@ def build_library(out: Path = LIB_PATH, verbose: bool = False) -> Path:
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
     jobs = {out: CSRC / "bshd.hip", SERVING_LIB_PATH: CSRC / "serving.hip", MX4_LIB_PATH: CSRC / "mx4.hip",
             KAT_LIB_PATH: CSRC / "loader_kat.hip", CEILING_LIB_PATH: CSRC / "mfma_ceiling.hip"}
+    commands = {lib: [hipcc, *HIPCC_FLAGS, str(src)] for lib, src in jobs.items()}
+    jobs[MX4_BLOCKS_PATH] = CSRC / "mx4_blocks.cpp"
+    commands[MX4_BLOCKS_PATH] = _extension_command(jobs[MX4_BLOCKS_PATH])
     procs = {}
-    for lib, src in jobs.items():
+    for lib, command in commands.items():
         tmp = lib.with_suffix(".so.tmp")
-        procs[lib] = (tmp, subprocess.Popen([hipcc, *HIPCC_FLAGS, str(src), "-o", str(tmp)],
+        procs[lib] = (tmp, subprocess.Popen([*command, "-o", str(tmp)],
                                             stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True))
     remarks = []
     for lib, (tmp, proc) in procs.items():
         _, err = proc.communicate()
         if proc.returncode != 0:
-            raise RuntimeError(f"hipcc failed ({proc.returncode}) on {jobs[lib].name}:\n{err[-4000:]}")
+            raise RuntimeError(f"{Path(commands[lib][0]).name} failed ({proc.returncode}) on {jobs[lib].name}:\n{err[-4000:]}")
         if verbose and err:
             print(err)
         remarks.append(err)
@@ -163,7 +177,7 @@ def build_library(out: Path = LIB_PATH, verbose: bool = False) -> Path:
     RESOURCE_LOG.write_text(text)
     sha = lambda p: hashlib.sha256(Path(p).read_bytes()).hexdigest()
     version = subprocess.run([hipcc, "--version"], capture_output=True, text=True).stdout
-    sources = sorted(CSRC.glob("*.hip")) + sorted(CSRC.glob("*.hpp")) + sorted(INCLUDE.glob("*.h"))
+    sources = sorted(p for ext in ("hip", "hpp", "cpp") for p in CSRC.glob(f"*.{ext}")) + sorted(INCLUDE.glob("*.h"))
     manifest = {
         "built_at": time.strftime("%Y-%m-%dT%H:%M:%SZ", time.gmtime()),
         "host": platform.node(),
@@ -298,6 +312,26 @@ def load_mx4_library(path: Path = MX4_LIB_PATH) -> C.CDLL:
         lib.fav4_bshd_paged_mx4_workspace_size.restype = C.c_longlong
         _MX4 = lib
     return _MX4
+
+
+_MX4_BLOCKS = None
+
+
+def load_mx4_blocks(path: Path = MX4_BLOCKS_PATH):
+    """The module that checks torch tensors and packs them into the argument blocks of the 4-bit caches' calls (raises
+    OSError if it is missing)."""
+    global _MX4_BLOCKS
+    if _MX4_BLOCKS is None:
+        if not Path(path).exists():
+            raise OSError(f"{path} not built; run __graft_entry__.build() first")
+        import importlib.machinery
+        import importlib.util
+        import torch  # noqa: F401
+        loader = importlib.machinery.ExtensionFileLoader("fav4_mx4_blocks", str(path))
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("fav4_mx4_blocks", loader))
+        loader.exec_module(module)
+        _MX4_BLOCKS = module
+    return _MX4_BLOCKS
 
 
 class Runner:
@@ -720,6 +754,13 @@ class Runner:
             lib = self._mx4 = load_mx4_library()
         return lib
 
+    @property
+    def mx4_blocks(self):
+        blocks = self.__dict__.get("_mx4_blocks")
+        if blocks is None:
+            blocks = self._mx4_blocks = load_mx4_blocks()
+        return blocks
+
     @staticmethod
     def mx4_caches(num_pages, kv_heads, page_size, device="cuda"):
         """(k_cache, k_scales, v_cache, v_scales) of zeros."""
@@ -728,98 +769,16 @@ class Runner:
         return tuple(torch.zeros((*shape, n), dtype=torch.uint8, device=device)
                      for n in (D // 2, D // 32, D // 2, D // 32))
 
-    @staticmethod
-    def _mx4_append_block(torch, q, k, v, q_out, k_cache, k_scales, v_cache, v_scales, cu_q, seqlens_k, block_table,
-                          cos, sin, interleaved, positions) -> bytes:
-        bf16, i32, u8, dev = torch.bfloat16, torch.int32, torch.uint8, k.get_device()
-        num_pages, kv_heads, page_size, d = caches = k_cache.shape
-        scales = (num_pages, kv_heads, page_size, D // 32)
-        assert d == D // 2 and v_cache.shape == caches and k_scales.shape == scales and v_scales.shape == scales
-        assert k_cache.dtype is u8 and v_cache.dtype is u8 and k_scales.dtype is u8 and v_scales.dtype is u8
-        assert k_cache.is_contiguous() and v_cache.is_contiguous() and k_scales.is_contiguous() \
-            and v_scales.is_contiguous()
-        batch, pages = block_table.shape
-        assert cu_q.dtype is i32 and seqlens_k.dtype is i32 and block_table.dtype is i32
-        assert cu_q.shape == (batch + 1,) and seqlens_k.shape == (batch,)
-        assert cu_q.is_contiguous() and seqlens_k.is_contiguous() and block_table.is_contiguous()
-        assert dev == k_cache.get_device() == k_scales.get_device() == v_cache.get_device() == v_scales.get_device() \
-            == v.get_device() == cu_q.get_device() == seqlens_k.get_device() == block_table.get_device(), \
-            "all tensors on one device"
-        # Rows: any stride between tokens (a single token has none that counts), heads and dims contiguous.
-        tokens = k.shape[0]
-        assert k.shape == v.shape == (tokens, kv_heads, D) and k.dtype is bf16 and v.dtype is bf16
-        k_stride, k1, k2 = k.stride()
-        v_stride, v1, v2 = v.stride()
-        assert k2 == v2 == 1 and (kv_heads == 1 or k1 == v1 == D)
-        heads, q_stride, o_stride, q_ptr, o_ptr = 1, 0, 0, 0, 0
-        assert (q is None) == (q_out is None)
-        if q is not None:
-            heads = q.shape[1]
-            assert q.shape == q_out.shape == (tokens, heads, D) and q.dtype is bf16 and q_out.dtype is bf16
-            assert q.get_device() == q_out.get_device() == dev, "all tensors on one device"
-            q_stride, q1, q2 = q.stride()
-            o_stride, o1, o2 = q_out.stride()
-            assert q2 == o2 == 1 and (heads == 1 or q1 == o1 == D)
-            q_ptr, o_ptr = q.data_ptr(), q_out.data_ptr()
-        if tokens == 1:
-            k_stride = v_stride = kv_heads * D
-            q_stride = o_stride = heads * D
-        rows = half = c_ptr = s_ptr = p_ptr = 0
-        assert (cos is None) == (sin is None)
-        if cos is not None:
-            rows, half = angles = cos.shape
-            assert sin.shape == angles and cos.dtype is sin.dtype is torch.float32
-            assert cos.is_contiguous() and sin.is_contiguous() and cos.get_device() == sin.get_device() == dev
-            c_ptr, s_ptr = cos.data_ptr(), sin.data_ptr()
-        if positions is not None:
-            assert positions.dtype is i32 and positions.shape == (tokens,) and positions.is_contiguous()
-            assert positions.get_device() == dev, "all tensors on one device"
-            p_ptr = positions.data_ptr()
-        return _MX4_APPEND.pack(q_ptr, k.data_ptr(), v.data_ptr(), o_ptr, k_cache.data_ptr(), v_cache.data_ptr(),
-                                c_ptr, s_ptr, cu_q.data_ptr(), seqlens_k.data_ptr(), block_table.data_ptr(), p_ptr,
-                                q_stride, k_stride, v_stride, o_stride, batch, heads, kv_heads, tokens, num_pages,
-                                page_size, pages, 2 * half, rows, 1 if interleaved else 0, k_scales.data_ptr(),
-                                v_scales.data_ptr())
-
     def call_append_paged_mx4(self, q, k, v, q_out, k_cache, k_scales, v_cache, v_scales, cu_q, seqlens_k, block_table,
                               cos=None, sin=None, interleaved=False, positions=None, stream=None):
         """fav4_bshd_append_paged_mx4: call_append_paged into 4-bit caches (see mx4_caches); the other tensors as
         there."""
         import torch
-        block = self._mx4_append_block(torch, q, k, v, q_out, k_cache, k_scales, v_cache, v_scales, cu_q, seqlens_k,
-                                       block_table, cos, sin, interleaved, positions)
+        block = self.mx4_blocks.append(q, k, v, q_out, k_cache, k_scales, v_cache, v_scales, cu_q, seqlens_k, block_table,
+                                       cos, sin, interleaved, positions)
         status = self.mx4.fav4_bshd_append_paged_mx4(block, self._stream(torch, k.get_device(), stream))
         if status:
             raise RuntimeError(f"append paged mx4: HIP status {status}")
-
-    @staticmethod
-    def _mx4_gather_block(torch, k_cache, k_scales, v_cache, v_scales, k, v, cu_k, block_table, starts) -> bytes:
-        bf16, i32, u8, dev = torch.bfloat16, torch.int32, torch.uint8, k.get_device()
-        num_pages, kv_heads, page_size, d = caches = k_cache.shape
-        scales = (num_pages, kv_heads, page_size, D // 32)
-        assert d == D // 2 and v_cache.shape == caches and k_scales.shape == scales and v_scales.shape == scales
-        assert k_cache.dtype is u8 and v_cache.dtype is u8 and k_scales.dtype is u8 and v_scales.dtype is u8
-        assert k_cache.is_contiguous() and v_cache.is_contiguous() and k_scales.is_contiguous() \
-            and v_scales.is_contiguous()
-        batch, pages = block_table.shape
-        assert cu_k.dtype is i32 and block_table.dtype is i32 and cu_k.shape == (batch + 1,)
-        assert cu_k.is_contiguous() and block_table.is_contiguous()
-        assert dev == k_cache.get_device() == k_scales.get_device() == v_cache.get_device() == v_scales.get_device() \
-            == v.get_device() == cu_k.get_device() == block_table.get_device(), "all tensors on one device"
-        rows, s_ptr = k.shape[0], 0
-        assert k.shape == v.shape == (rows, kv_heads, D) and k.dtype is bf16 and v.dtype is bf16
-        k_stride, k1, k2 = k.stride()
-        v_stride, v1, v2 = v.stride()
-        assert k2 == v2 == 1 and (kv_heads == 1 or k1 == v1 == D)
-        if rows == 1:                                     # has no stride that counts
-            k_stride = v_stride = kv_heads * D
-        if starts is not None:
-            assert starts.dtype is i32 and starts.shape == (batch,) and starts.is_contiguous()
-            assert starts.get_device() == dev, "all tensors on one device"
-            s_ptr = starts.data_ptr()
-        return _MX4_GATHER.pack(k_cache.data_ptr(), k_scales.data_ptr(), v_cache.data_ptr(), v_scales.data_ptr(),
-                                k.data_ptr(), v.data_ptr(), cu_k.data_ptr(), s_ptr, block_table.data_ptr(), k_stride,
-                                v_stride, batch, kv_heads, rows, num_pages, page_size, pages)
 
     def call_gather_paged_mx4(self, k_cache, k_scales, v_cache, v_scales, k, v, cu_k, block_table, starts=None,
                               stream=None):
@@ -827,41 +786,10 @@ class Runner:
         [total_k, kv_heads, 128] (any stride between rows), of which [cu_k[b], cu_k[b + 1]) get keys starts[b], ... of
         sequence b; cu_k: int32 [batch+1]; block_table: int32 [batch, max_pages]; starts: int32 [batch] or None (0)."""
         import torch
-        block = self._mx4_gather_block(torch, k_cache, k_scales, v_cache, v_scales, k, v, cu_k, block_table, starts)
+        block = self.mx4_blocks.gather(k_cache, k_scales, v_cache, v_scales, k, v, cu_k, block_table, starts)
         status = self.mx4.fav4_bshd_gather_paged_mx4(block, self._stream(torch, k.get_device(), stream))
         if status:
             raise RuntimeError(f"gather paged mx4: HIP status {status}")
-
-    @staticmethod
-    def _mx4_paged_block(torch, q, k_cache, k_scales, v_cache, v_scales, o, lse, cu_q, seqlens_k, block_table, max_q,
-                         max_k, total_k, scale) -> bytes:
-        bf16, i32, u8, dev = torch.bfloat16, torch.int32, torch.uint8, q.get_device()
-        num_pages, kv_heads, page_size, d = caches = k_cache.shape
-        scales = (num_pages, kv_heads, page_size, D // 32)
-        assert d == D // 2 and v_cache.shape == caches and k_scales.shape == scales and v_scales.shape == scales
-        assert k_cache.dtype is u8 and v_cache.dtype is u8 and k_scales.dtype is u8 and v_scales.dtype is u8
-        assert k_cache.is_contiguous() and v_cache.is_contiguous() and k_scales.is_contiguous() \
-            and v_scales.is_contiguous()
-        batch, pages = block_table.shape
-        assert cu_q.dtype is i32 and seqlens_k.dtype is i32 and block_table.dtype is i32
-        assert cu_q.shape == (batch + 1,) and seqlens_k.shape == (batch,)
-        assert cu_q.is_contiguous() and seqlens_k.is_contiguous() and block_table.is_contiguous()
-        tokens, heads, d = rows = q.shape
-        assert d == D and o.shape == rows and q.dtype is bf16 and o.dtype is bf16
-        assert q.is_contiguous() and o.is_contiguous()
-        assert dev == k_cache.get_device() == k_scales.get_device() == v_cache.get_device() == v_scales.get_device() \
-            == o.get_device() == cu_q.get_device() == seqlens_k.get_device() == block_table.get_device(), \
-            "all tensors on one device"
-        lse_ptr = 0
-        if lse is not None:
-            assert lse.shape == (heads, tokens) and lse.is_contiguous() and lse.dtype is torch.float32
-            assert lse.get_device() == dev, "all tensors on one device"
-            lse_ptr = lse.data_ptr()
-        return _MX4_PAGED.pack(q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), o.data_ptr(), lse_ptr,
-                               cu_q.data_ptr(), seqlens_k.data_ptr(), block_table.data_ptr(), batch, heads, kv_heads,
-                               int(max_q), int(max_k), tokens, 0 if total_k is None else int(total_k), num_pages,
-                               page_size, pages, SCALE if scale is None else scale, k_scales.data_ptr(),
-                               v_scales.data_ptr())
 
     def paged_mx4_workspace_size(self, batch, heads, kv_heads, max_q, max_k, total_q, page_size, max_pages, num_pages,
                                  causal=0) -> int:
@@ -876,8 +804,8 @@ class Runner:
         paged_args.  causal 0 dense, 2 bottom-right.  `workspace` as for call_splitkv (None: allocated here); returned
         for the next call."""
         import torch
-        block = self._mx4_paged_block(torch, q, k_cache, k_scales, v_cache, v_scales, o, lse, cu_q, seqlens_k,
-                                      block_table, max_q, max_k, total_k, scale)
+        block = self.mx4_blocks.paged(q, k_cache, k_scales, v_cache, v_scales, o, lse, cu_q, seqlens_k, block_table,
+                                      max_q, max_k, total_k, scale)
         raw = self._stream(torch, q.get_device(), stream)
         causal = int(causal)
         if workspace is None:

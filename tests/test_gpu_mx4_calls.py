@@ -129,6 +129,23 @@ def test_more_heads_than_cus(gpu_runner, heads, lens):
     assert_guard_rows_untouched(batch)
 
 
+def test_one_device(gpu_runner):
+    """A host tensor among the GPU's is refused, whichever it is."""
+    t = Tokens([(3, 10), (2, 5)])
+    blocks, (k, v) = gpu_runner.mx4_blocks, (torch.empty_like(x[:t.n]) for x in (t.k, t.v))
+    cos, sin = angles(64, 128, t.dev)
+    o, lse = torch.empty_like(t.q), torch.empty(t.q.shape[1], t.q.shape[0], device=t.dev)
+    positions = torch.zeros(t.q.shape[0], dtype=torch.int32, device=t.dev)
+    for call, args in ((blocks.append, [t.q, t.k, t.v, t.q_out, *t.caches, t.cu, t.seqlens, t.table_d, cos, sin, False, positions]),
+                       (blocks.gather, [*t.caches, k, v, t.cu, t.table_d, t.seqlens]),
+                       (blocks.paged, [t.q, *t.caches, o, lse, t.cu, t.seqlens, t.table_d, 3, 10, None, None])):
+        call(*args)
+        for i, x in enumerate(args):
+            if isinstance(x, torch.Tensor):
+                with pytest.raises(AssertionError, match="one device"):
+                    call(*args[:i], x.cpu(), *args[i + 1:])
+
+
 def test_more_sequences_than_a_line_is_laid_out_for(gpu_runner):
     """600 sequences, some of them of many rows: past what a workgroup keeps in LDS."""
     rng = np.random.default_rng(3)

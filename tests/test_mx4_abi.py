@@ -84,17 +84,82 @@ def test_ctypes_layout_matches_the_header(pkg, name, tmp_path):
 
 
 def test_packed_blocks_match_the_structs(pkg):
-    """The blocks that Runner packs in one step lie as the ctypes structs do."""
-    b = pkg.fav4_bshd
-    for packer, block in ((b._MX4_APPEND, append_args(pkg, positions=0xc0000)),
-                          (b._MX4_GATHER, gather_args(pkg, starts=0xa0000)),
-                          (b._MX4_PAGED, paged_args(pkg, lse=0xb0000))):
-        assert packer.size == C.sizeof(block)
-        flat = []
-        for name, *_ in block._fields_:
-            value = getattr(block, name)
-            flat += [getattr(value, n) for n, *_ in value._fields_] if isinstance(value, C.Structure) else [value]
-        assert packer.pack(*flat) == bytes(block)
+    """The blocks that the binding packs, field by field."""
+    import torch
+    blocks = pkg.fav4_bshd.load_mx4_blocks()
+    bf16 = lambda *s: torch.zeros(s, dtype=torch.bfloat16)
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32)
+    caches = pkg.Runner.mx4_caches(7, 2, 48, device="cpu")
+    qkv, q_out = bf16(5, 6 + 4, 128), bf16(5, 6, 128)
+    q, k, v = qkv[:, :6], qkv[:, 6:8], qkv[:, 8:]
+    cu, seqlens, table, positions, starts = i32(4), i32(3), i32(3, 9), i32(5), i32(3)
+    cos, sin = torch.zeros(300, 32), torch.zeros(300, 32)
+    ptrs = {n: x.data_ptr() for n, x in zip(("k_cache", "k_scales", "v_cache", "v_scales"), caches)}
+    sizes = dict(batch=3, kv_heads=2, num_pages=7, page_size=48, max_pages_per_seq=9, block_table=table.data_ptr())
+
+    def check(cls, block, **want):
+        assert len(block) == C.sizeof(cls)
+        got, a = {}, cls.from_buffer_copy(block)
+        for name, *_ in a._fields_:
+            value = getattr(a, name)
+            got.update({n: getattr(value, n) for n, *_ in value._fields_} if isinstance(value, C.Structure)
+                       else {name: value})
+        assert got == want
+
+    new = dict(cu_seqlens_q=cu.data_ptr(), seqlens_k=seqlens.data_ptr(), **sizes)
+    check(pkg.Mx4AppendArgs, blocks.append(q, k, v, q_out, *caches, cu, seqlens, table, cos, sin, True, positions),
+          q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), q_out=q_out.data_ptr(), cos=cos.data_ptr(), sin=sin.data_ptr(),
+          positions=positions.data_ptr(), q_stride=1280, k_stride=1280, v_stride=1280, q_out_stride=768, heads=6,
+          total_q=5, rotary_dim=64, rotary_rows=300, interleaved=1, **ptrs, **new)
+    check(pkg.Mx4AppendArgs, blocks.append(None, k[:1], v[:1], None, *caches, cu, seqlens, table, None, None, False, None),
+          q=None, k=k.data_ptr(), v=v.data_ptr(), q_out=None, cos=None, sin=None, positions=None, q_stride=0, k_stride=256,
+          v_stride=256, q_out_stride=0, heads=1, total_q=1, rotary_dim=0, rotary_rows=0, interleaved=0, **ptrs, **new)
+    for given in (starts, None):
+        check(pkg.Mx4GatherArgs, blocks.gather(*caches, k, v, cu, table, given), k=k.data_ptr(), v=v.data_ptr(),
+              cu_seqlens_k=cu.data_ptr(), starts=None if given is None else starts.data_ptr(), k_stride=1280,
+              v_stride=1280, total_k=5, **ptrs, **sizes)
+    lse = torch.zeros(6, 5)
+    for given, total, scale, want in ((lse, None, None, 128 ** -0.5), (None, 77, 0.25, 0.25)):
+        check(pkg.Mx4PagedArgs, blocks.paged(q_out, *caches, q_out, given, cu, seqlens, table, 2, 400, total, scale),
+              q=q_out.data_ptr(), o=q_out.data_ptr(), lse=None if given is None else lse.data_ptr(), heads=6,
+              max_seqlen_q=2, max_seqlen_k=400, total_q=5, total_k=total or 0, scale=C.c_float(want).value, **ptrs, **new)
+
+
+def test_blocks_refuse_wrong_tensors(pkg):
+    """Every tensor with another type, shape or layout, and numbers that do not fit."""
+    import torch
+    blocks = pkg.fav4_bshd.load_mx4_blocks()
+    bf16 = lambda *s: torch.zeros(s, dtype=torch.bfloat16)
+    i32 = lambda *s: torch.zeros(s, dtype=torch.int32)
+    caches = pkg.Runner.mx4_caches(7, 2, 48, device="cpu")
+    q, k, v, cu, seqlens, table = bf16(5, 6, 128), bf16(5, 2, 128), bf16(5, 2, 128), i32(4), i32(3), i32(3, 9)
+    cos, sin = torch.zeros(300, 32), torch.zeros(300, 32)
+    calls = {blocks.append: [q, k, v, bf16(5, 6, 128), *caches, cu, seqlens, table, cos, sin, False, i32(5)],
+             blocks.gather: [*caches, k, v, cu, table, i32(3)],
+             blocks.paged: [q, *caches, bf16(5, 6, 128), torch.zeros(6, 5), cu, seqlens, table, 1, 99, None, None]}
+    wrong = (lambda x: x.double(), lambda x: x[:-1], lambda x: x.unsqueeze(0), lambda x: torch.stack((x, x), -1)[..., 0])
+    for call, args in calls.items():
+        call(*args)
+        for i, x in enumerate(args):
+            if not isinstance(x, torch.Tensor):
+                continue
+            for change in wrong:
+                with pytest.raises(AssertionError):
+                    call(*args[:i], change(x), *args[i + 1:])
+            with pytest.raises(TypeError):
+                call(*args[:i], 5, *args[i + 1:])
+        with pytest.raises(TypeError):
+            call(*args[:-1])
+    append, paged = calls[blocks.append], calls[blocks.paged]
+    for i in (0, 3, 11, 12):
+        with pytest.raises(AssertionError):
+            blocks.append(*append[:i], None, *append[i + 1:])
+    for i in (10, 11, 12):
+        for bad, error in ((1 << 31, OverflowError), (1 << 80, OverflowError), ("x", ValueError), ([], TypeError)):
+            with pytest.raises(error):
+                blocks.paged(*paged[:i], bad, *paged[i + 1:])
+    with pytest.raises(TypeError):
+        blocks.paged(*paged[:13], "1")
 
 
 APPEND_BAD = [{n: None} for n in ("k", "v", "q", "q_out", "k_cache", "v_cache", "cos", "sin", "cu_seqlens_q",
