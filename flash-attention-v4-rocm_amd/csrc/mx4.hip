@@ -95,8 +95,10 @@ bool paged_shape_ok(const Fav4Mx4PagedArgs* args, int causal) {
 
 // The decode kernel's workgroups on a line (cut): four waves of 32-key tiles, three a CU,
 // with up to 16 rows; of 64-key tiles, two a CU, with 32.  Whole sequences: eight waves of
-// 64-key tiles, one a CU.
-constexpr int LINE_WAVES = 4, WHOLE_WAVES = 8;
+// 32-key tiles, one a CU, or twelve with up to 16 rows and more than LONG_KEYS keys: 1
+// sequence of 800, H32 KVH8, 6.8 and 7.2 us (8.0 with eight of 64-key tiles), 16 of 500..2500
+// 14.5 and 13.6 (14.8), 32 x 4 queries of 200..4096 21.2 and 19.6 (21.3).
+constexpr int LINE_WAVES = 4, WHOLE_WAVES = 8, LONG_WAVES = 12, LONG_KEYS = 2048;
 constexpr int line_per_cu(int row_tiles) { return row_tiles == 1 ? 3 : 2; }
 constexpr int line_subtiles(int row_tiles) { return row_tiles == 1 ? 2 : 4; }
 // Keys that a workgroup of a line should have at least: what it takes grows with them, what
@@ -129,15 +131,17 @@ bool few_rows(int64_t seq_rows, double rows, double keys, int64_t batch, int kv_
 // Whether every sequence and K/V head (`pairs`) has a workgroup of its own, and no merge.
 // Measured, as graphs: such workgroups start and end in 4.2 us, read 290 keys a us (175 with
 // 32 rows) and wait for 0.3 of the time that all bytes take at 6.3 TB/s; a line takes 9.1,
-// 0.3 for each row up to 16, and the bytes' time.  H32 KVH8 and one query where not said,
-// lengths of a third of the longest and more, whole / cut: 1 sequence of 1536 9.4 / 10.1, of
-// 4096 18.4 / 10.2; 16 of up to 2600 14.7 / 16.6, of 4000 20.4 / 18.1; 32 of 4000 22.2 /
-// 24.5, of 4 queries 22.8 / 28.5; 8 x 4 queries of 2500, H8 KVH1, 18.5 / 15.9.  With more
-// pairs than CUs whole sequences wait for one another: 48 of 100..4096 23.3 whole, 20.2
+// 0.05 to 0.3 for each row up to 16 (by how many pairs write parts), and the bytes' time.  H32
+// KVH8 and one query where not said, whole / cut: 1 sequence of 2500, 4 queries, 13.6 / 10.9;
+// 4 of 500..2000, H16 KVH2, 2 queries, 12.3 / 10.7; 16 of 500..2500, 4 queries, 14.2 / 17.7;
+// 32 of 200..4096, 4 queries, 19.6 / 21.5; 32 of 3500..4000, 8 queries, 28.5 / 41.5.  With
+// more pairs than CUs whole sequences wait for one another: 48 of 100..4096 23.3 whole, 20.2
 // cut; 64 of 500..8192 55.8 and 44.5.
 bool whole_sequences(int64_t pairs, int64_t rows, int64_t max_keys, double all_keys, int cus) {
     const double rate = rows <= 16 ? 290 : 175;
-    return pairs <= cus && double(max_keys) < rate * (4.9 + 0.3 * double(std::min<int64_t>(rows, 16)) + 0.7 * all_keys * 136 / 6.3e6);
+    const double row = 0.05 + 0.25 * double(pairs) / cus;
+    return pairs <= cus &&
+           double(max_keys) < rate * (4.9 + row * double(std::min<int64_t>(rows, 16)) + 0.7 * all_keys * 136 / 6.3e6);
 }
 
 // Key tiles of many rows that a range should have at least: with a half, 0.3, 0.8 times the
@@ -264,8 +268,10 @@ void launch_few(const Fav4Mx4PagedArgs& a, const Sizes& s, hipStream_t stream) {
         constexpr bool L = decltype(lse)::value, P = decltype(p64)::value;
         if (s.split)
             go(fav4::mx4_decode_kernel<NT, LINE_WAVES, line_subtiles(NT), line_per_cu(NT), true, L, P>, LINE_WAVES);
+        else if (NT == 1 && a.paged.max_seqlen_k > LONG_KEYS)
+            go(fav4::mx4_decode_kernel<1, LONG_WAVES, 2, 3, false, L, P>, LONG_WAVES);
         else
-            go(fav4::mx4_decode_kernel<NT, WHOLE_WAVES, 4, 2, false, L, P>, WHOLE_WAVES);
+            go(fav4::mx4_decode_kernel<NT, WHOLE_WAVES, 2, 2, false, L, P>, WHOLE_WAVES);
     };
     const bool p64 = a.paged.page_size % 64 == 0;
     if (a.paged.lse) p64 ? with(std::true_type{}, std::true_type{}) : with(std::true_type{}, std::false_type{});

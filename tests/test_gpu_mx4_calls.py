@@ -13,6 +13,7 @@ pytestmark = pytest.mark.gpu
 # The kinds of call: whole sequences and lines of few rows, of one row tile and two, row tiles of 128 and of 256 rows,
 # whole and on a line.
 KINDS = {"whole": [(1, 300), (1, 77), (1, 640)], "line": [(1, 5000), (1, 300), (1, 2100)] * 3,
+         "long_whole": [(4, 2100), (3, 1500), (4, 900), (1, 2099)] * 8,
          "drafts": [(5, 400), (5, 90)], "drafts_line": [(5, 6000), (5, 90), (3, 3500)],
          "prompts": [(150, 150), (200, 333)], "chunks": [(100, 4000), (40, 1500), (70, 70)],
          "long_chunks": [(300, 9000), (250, 2000)], "many_prompts": [(150, 150), (200, 333)] * 4,

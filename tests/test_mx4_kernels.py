@@ -16,6 +16,7 @@ def table():
 
 # Least waves a SIMD: the workgroups that the launches count on being resident at once.
 @pytest.mark.parametrize("pattern,count,waves", [(r"mx4_decode_kernelILi1ELi4E", 4, 3), (r"mx4_decode_kernelILi1ELi8E", 4, 2),
+                                                 (r"mx4_decode_kernelILi1ELi12E", 4, 3),
                                                  (r"mx4_decode_kernelILi2E", 8, 2), (r"mx4_prefill_kernelI", 4, 2),
                                                  (r"mx4_prefill_line_kernelI", 4, 2), (r"mx4_merge_kernelI", 3, 7),
                                                  (r"mx4_store_kernelI", 2, 7), (r"mx4_read_kernel", 1, 8)])
@@ -30,7 +31,7 @@ def test_kernels_keep_their_waves(table, pattern, count, waves):
 def test_workgroups_fit_a_cu(table):
     """LDS: 160 KiB a CU, for three workgroups of a decode line, two of a prefill one."""
     for pattern, each in ((r"mx4_decode_kernelILi1ELi4E", 3), (r"mx4_decode_kernelILi2ELi4E", 2),
-                          (r"mx4_decode_kernelILi\dELi8E", 1), (r"mx4_prefill_(line_)?kernelILi4E", 2),
+                          (r"mx4_decode_kernelILi\dELi(8|12)E", 1), (r"mx4_prefill_(line_)?kernelILi4E", 2),
                           (r"mx4_prefill_(line_)?kernelILi8E", 1)):
         kernels = {n: r for n, r in table.items() if re.search(pattern, n)}
         assert kernels
