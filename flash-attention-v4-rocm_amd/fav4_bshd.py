@@ -125,13 +125,20 @@ def parse_resource_usage(text: str) -> dict:
 
 
 def _extension_command(src: Path) -> list:
-    """The host compiler's command for a Python extension that reads torch tensors."""
+    """The host compiler's command for a Python extension that reads torch tensors (ImportError or FileNotFoundError,
+    naming what is missing, where it cannot be built)."""
+    import shutil
     import sysconfig
     import torch
-    home = Path(torch.__file__).parent
-    system = ["/opt/rocm/include", home / "include", home / "include/torch/csrc/api/include",
-              sysconfig.get_paths()["include"]]
-    return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+    home, python = Path(torch.__file__).parent, Path(sysconfig.get_paths()["include"])
+    compiler = os.environ.get("CXX", "g++")
+    if shutil.which(compiler) is None:
+        raise FileNotFoundError(f"no compiler {compiler}")
+    for header in (home / "include/torch/csrc/autograd/python_variable.h", python / "Python.h"):
+        if not header.exists():
+            raise FileNotFoundError(f"no header {header}")
+    system = ["/opt/rocm/include", home / "include", home / "include/torch/csrc/api/include", python]
+    return [compiler, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
             "-D__HIP_PLATFORM_AMD__", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{INCLUDE}",
             *(x for d in system for x in ("-isystem", str(d))), str(src), f"-L{home / 'lib'}", "-ltorch_python",
             "-ltorch_cpu", "-lc10"]
@@ -147,25 +154,36 @@ def build_library(out: Path = LIB_PATH, verbose: bool = False) -> Path:
     ``build/libfav4_mfma_ceiling.so`` (a measurement library, read by
     ``bench.py --mfma-ceiling``), keep the compiler's kernel-resource-usage remarks in
     ``build/resource-usage.txt`` and write ``build/build-manifest.json``
-    (toolchain, flags, source and library sha256, per-kernel resources)."""
+    (toolchain, flags, source and library sha256, per-kernel resources).
+
+    The extension alone needs torch, its headers and a host compiler.  Where one of them is
+    missing it is left out, with a warning, and loading it says why."""
     import hashlib
     import json
     import platform
     import time
+    import warnings
     out.parent.mkdir(parents=True, exist_ok=True)
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
     jobs = {out: CSRC / "bshd.hip", SERVING_LIB_PATH: CSRC / "serving.hip", MX4_LIB_PATH: CSRC / "mx4.hip",
             KAT_LIB_PATH: CSRC / "loader_kat.hip", CEILING_LIB_PATH: CSRC / "mfma_ceiling.hip"}
     commands = {lib: [hipcc, *HIPCC_FLAGS, str(src)] for lib, src in jobs.items()}
-    jobs[MX4_BLOCKS_PATH] = CSRC / "mx4_blocks.cpp"
-    commands[MX4_BLOCKS_PATH] = _extension_command(jobs[MX4_BLOCKS_PATH])
+    left_out = {}
+    extension = CSRC / "mx4_blocks.cpp"
+    MX4_BLOCKS_PATH.unlink(missing_ok=True)       # an earlier build's may pack other argument blocks
+    try:
+        commands[MX4_BLOCKS_PATH] = _extension_command(extension)
+        jobs[MX4_BLOCKS_PATH] = extension
+    except (ImportError, FileNotFoundError) as e:
+        left_out[MX4_BLOCKS_PATH.name] = str(e)
+        warnings.warn(f"{MX4_BLOCKS_PATH.name} is left out: {e}")
     procs = {}
     for lib, command in commands.items():
         tmp = lib.with_suffix(".so.tmp")
         procs[lib] = (tmp, subprocess.Popen([*command, "-o", str(tmp)],
                                             stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True))
     remarks = []
-    for lib, (tmp, proc) in procs.items():
+    for lib, (tmp, proc) in procs.items():        # the extension last: the libraries are in place if it fails
         _, err = proc.communicate()
         if proc.returncode != 0:
             raise RuntimeError(f"{Path(commands[lib][0]).name} failed ({proc.returncode}) on {jobs[lib].name}:\n{err[-4000:]}")
@@ -186,6 +204,7 @@ def build_library(out: Path = LIB_PATH, verbose: bool = False) -> Path:
         "sources": {str(p.relative_to(ROOT)): sha(p) for p in sources},
         "libraries": {lib.name: {"sha256": sha(lib), "bytes": lib.stat().st_size, "source": jobs[lib].name}
                       for lib in jobs},
+        "left_out": left_out,
         "kernel_resources": parse_resource_usage(text),
     }
     MANIFEST.write_text(json.dumps(manifest, indent=1))
@@ -317,13 +336,23 @@ def load_mx4_library(path: Path = MX4_LIB_PATH) -> C.CDLL:
 _MX4_BLOCKS = None
 
 
+def _left_out(path: Path) -> str:
+    """Why the last build left a library out (empty: it did not)."""
+    import json
+    try:
+        why = json.loads(MANIFEST.read_text()).get("left_out", {}).get(Path(path).name)
+    except (OSError, ValueError):
+        why = None
+    return f" ({why})" if why else ""
+
+
 def load_mx4_blocks(path: Path = MX4_BLOCKS_PATH):
     """The module that checks torch tensors and packs them into the argument blocks of the 4-bit caches' calls (raises
     OSError if it is missing)."""
     global _MX4_BLOCKS
     if _MX4_BLOCKS is None:
         if not Path(path).exists():
-            raise OSError(f"{path} not built; run __graft_entry__.build() first")
+            raise OSError(f"{path} not built{_left_out(path)}; run __graft_entry__.build() first")
         import importlib.machinery
         import importlib.util
         import torch  # noqa: F401
