@@ -220,4 +220,13 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "fav4_mx4_blocks", nullptr, -1, met
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit_fav4_mx4_blocks() { return PyModule_Create(&module); }
+// torch_version: of the torch that this file was compiled against.  Its tensors' C++ layout
+// is no stable interface, so the loader compares it with the one in the process.
+PyMODINIT_FUNC PyInit_fav4_mx4_blocks() {
+    PyObject* m = PyModule_Create(&module);
+    if (m && PyModule_AddStringConstant(m, "torch_version", FAV4_TORCH) < 0) {
+        Py_DECREF(m);
+        return nullptr;
+    }
+    return m;
+}

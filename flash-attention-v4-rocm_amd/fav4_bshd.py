@@ -139,7 +139,8 @@ def _extension_command(src: Path) -> list:
             raise FileNotFoundError(f"no header {header}")
     system = ["/opt/rocm/include", home / "include", home / "include/torch/csrc/api/include", python]
     return [compiler, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
-            "-D__HIP_PLATFORM_AMD__", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{INCLUDE}",
+            "-D__HIP_PLATFORM_AMD__", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+            f'-DFAV4_TORCH="{torch.__version__}"', f"-I{INCLUDE}",
             *(x for d in system for x in ("-isystem", str(d))), str(src), f"-L{home / 'lib'}", "-ltorch_python",
             "-ltorch_cpu", "-lc10"]
 
@@ -168,12 +169,14 @@ def build_library(out: Path = LIB_PATH, verbose: bool = False) -> Path:
     jobs = {out: CSRC / "bshd.hip", SERVING_LIB_PATH: CSRC / "serving.hip", MX4_LIB_PATH: CSRC / "mx4.hip",
             KAT_LIB_PATH: CSRC / "loader_kat.hip", CEILING_LIB_PATH: CSRC / "mfma_ceiling.hip"}
     commands = {lib: [hipcc, *HIPCC_FLAGS, str(src)] for lib, src in jobs.items()}
-    left_out = {}
+    left_out, extension_build = {}, None
     extension = CSRC / "mx4_blocks.cpp"
     MX4_BLOCKS_PATH.unlink(missing_ok=True)       # an earlier build's may pack other argument blocks
     try:
         commands[MX4_BLOCKS_PATH] = _extension_command(extension)
+        import torch
         jobs[MX4_BLOCKS_PATH] = extension
+        extension_build = {"command": commands[MX4_BLOCKS_PATH], "torch": torch.__version__}
     except (ImportError, FileNotFoundError) as e:
         left_out[MX4_BLOCKS_PATH.name] = str(e)
         warnings.warn(f"{MX4_BLOCKS_PATH.name} is left out: {e}")
@@ -205,6 +208,7 @@ def build_library(out: Path = LIB_PATH, verbose: bool = False) -> Path:
         "libraries": {lib.name: {"sha256": sha(lib), "bytes": lib.stat().st_size, "source": jobs[lib].name}
                       for lib in jobs},
         "left_out": left_out,
+        "extension": extension_build,
         "kernel_resources": parse_resource_usage(text),
     }
     MANIFEST.write_text(json.dumps(manifest, indent=1))
@@ -348,17 +352,23 @@ def _left_out(path: Path) -> str:
 
 def load_mx4_blocks(path: Path = MX4_BLOCKS_PATH):
     """The module that checks torch tensors and packs them into the argument blocks of the 4-bit caches' calls (raises
-    OSError if it is missing)."""
+    OSError if it is missing, or was built against another torch than the one in the process)."""
     global _MX4_BLOCKS
     if _MX4_BLOCKS is None:
         if not Path(path).exists():
             raise OSError(f"{path} not built{_left_out(path)}; run __graft_entry__.build() first")
         import importlib.machinery
         import importlib.util
-        import torch  # noqa: F401
+        import torch
         loader = importlib.machinery.ExtensionFileLoader("fav4_mx4_blocks", str(path))
-        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("fav4_mx4_blocks", loader))
-        loader.exec_module(module)
+        try:
+            module = importlib.util.module_from_spec(importlib.util.spec_from_loader("fav4_mx4_blocks", loader))
+            loader.exec_module(module)
+        except ImportError as e:
+            raise OSError(f"{path} does not load with torch {torch.__version__} ({e}); run __graft_entry__.build() again") from e
+        if module.torch_version != torch.__version__:
+            raise OSError(f"{path} was built against torch {module.torch_version}, not {torch.__version__}; run "
+                          "__graft_entry__.build() again")
         _MX4_BLOCKS = module
     return _MX4_BLOCKS
 

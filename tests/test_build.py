@@ -1,6 +1,7 @@
 """Host-only checks of build_library(): what it needs for what it builds.  The compilers are stand-ins that write their
 output file; the package's own paths are turned to a folder of the test's."""
 import json
+import re
 import sys
 import warnings
 
@@ -82,3 +83,48 @@ def test_an_extension_that_does_not_compile_is_an_error(tree, monkeypatch, tmp_p
         tree.build_library(tree.LIB_PATH)
     assert c_libraries(tree) <= {p.name for p in tree.LIB_PATH.parent.glob("*.so")}
     assert not tree.MX4_BLOCKS_PATH.exists()
+
+
+@pytest.fixture(scope="module")
+def extension():
+    """The built extension's path (built here where one of the two is missing)."""
+    pkg = load_package()
+    if not pkg.fav4_bshd.MX4_BLOCKS_PATH.exists() or not pkg.MX4_LIB_PATH.exists():
+        pkg.build_library()
+    return pkg.fav4_bshd.MX4_BLOCKS_PATH
+
+
+def test_an_extension_of_another_torch_is_refused(extension, monkeypatch):
+    """It reads tensors by the C++ layout of the torch that it was built against."""
+    import torch
+    module = load_package().fav4_bshd
+    monkeypatch.setattr(module, "_MX4_BLOCKS", None)
+    built_for = module.load_mx4_blocks(extension).torch_version
+    assert built_for == torch.__version__
+    monkeypatch.setattr(module, "_MX4_BLOCKS", None)
+    monkeypatch.setattr(torch, "__version__", "1.0.0")
+    with pytest.raises(OSError, match=f"torch {re.escape(built_for)}, not 1.0.0"):
+        module.load_mx4_blocks(extension)
+    assert module._MX4_BLOCKS is None
+
+
+def test_an_extension_that_does_not_load_is_an_oserror(tmp_path, monkeypatch):
+    """As a build against another torch ends whose symbols are gone."""
+    module = load_package().fav4_bshd
+    monkeypatch.setattr(module, "_MX4_BLOCKS", None)
+    path = tmp_path / "fav4_mx4_blocks.so"
+    path.write_bytes(b"no library")
+    with pytest.raises(OSError, match="does not load"):
+        module.load_mx4_blocks(path)
+
+
+def test_the_manifest_says_how_the_extension_was_built(tree):
+    import torch
+    manifest = built(tree)[2]["extension"]
+    assert manifest["torch"] == torch.__version__
+    assert manifest["command"][0].endswith("cxx") and any("mx4_blocks.cpp" in x for x in manifest["command"])
+
+
+def test_the_manifest_of_a_build_without_it(tree, monkeypatch):
+    monkeypatch.setitem(sys.modules, "torch", None)
+    assert built(tree)[2]["extension"] is None
