@@ -1,0 +1,101 @@
+"""Each form of the 4-bit caches' attention kernels (row tiles of 16, 32, 128 and 256 rows, whole and on a line), over
+caches past 4 GiB, keys and queries that are no numbers, and again.  tests/test_mx4_launches.py holds every
+batch to the form that it is here for."""
+import numpy as np
+import pytest
+import torch
+
+from tests.mx4 import Cache4
+
+pytestmark = pytest.mark.gpu
+
+# Form: (kernel, whole or line, rows of a row tile, threads), and a batch that gets it: heads, K/V heads, (queries, keys).
+FORMS = {
+    "few": (("decode", "whole", 16, 512), 16, 8, [(1, 300), (1, 77), (1, 640)]),
+    "few_long": (("decode", "whole", 16, 768), 16, 8, [(4, 2100), (3, 1500), (4, 900), (1, 2099)] * 4),
+    "few_line": (("decode", "line", 16, 256), 16, 8, [(1, 5000), (1, 300), (1, 2100)] * 3),
+    "drafts": (("decode", "whole", 32, 512), 16, 8, [(9, 400), (9, 90)]),
+    "drafts_line": (("decode", "line", 32, 256), 16, 8, [(9, 6000), (9, 90), (6, 3500)]),
+    "many_128": (("prefill", "whole", 128, 256), 16, 8, [(150, 150), (200, 333)] * 4),
+    "many_256": (("prefill", "whole", 256, 512), 32, 8, [(512, 2000)] * 3 + [(512, 1777)]),
+    "many_line_128": (("prefill", "line", 128, 256), 16, 8, [(100, 4000), (40, 1500), (70, 70)] * 2),
+    "many_line_256": (("prefill", "line", 256, 512), 16, 8, [(300, 9000), (250, 2000)]),
+}
+PAGES = [64, 128]
+
+
+def batch_of(form, page, **more):
+    _, heads, kv_heads, lens = FORMS[form]
+    return Cache4(heads, kv_heads, page, lens, **more)
+
+
+@pytest.fixture(scope="module")
+def room():
+    """Codes of K and V of a little more than 2^32 bytes each, and their scales."""
+    extra = 1 << 26
+    return [torch.zeros(((1 << 32) + extra) * n // 64, dtype=torch.uint8, device="cuda:0") for n in (64, 4, 64, 4)]
+
+
+@pytest.mark.parametrize("page", [64, 128])
+@pytest.mark.parametrize("form", FORMS)
+def test_pages_on_both_sides_of_4_gib(gpu_runner, room, form, page):
+    """Half of the pool's pages in use begin below 2^32 bytes of codes and half above."""
+    batch = batch_of(form, page)
+    kv_heads, pool = batch.kv_heads, batch.caches[0].shape[0]
+    border = (1 << 32) // (page * kv_heads * 64)
+    first = border - pool // 2
+    caches = []
+    for x, own, width in zip(room, batch.caches, (64, 4, 64, 4)):
+        n = x.numel() // (page * kv_heads * width)
+        whole = x[:n * page * kv_heads * width].view(n, kv_heads, page, width)
+        whole[first:first + pool] = own
+        caches.append(whole)
+    assert first + pool <= caches[0].shape[0]
+    used = np.zeros(batch.table.shape, dtype=bool)
+    for b, pages in enumerate(batch.pages):
+        used[b, :len(pages)] = True
+    batch.table[used] += first
+    batch.pages = [p + first for p in batch.pages]
+    assert (batch.table[used] < border).any() and (batch.table[used] >= border).any()
+    batch.table_d.copy_(torch.from_numpy(batch.table))
+    batch.caches = caches
+    o, lse = batch.outputs(True)
+    batch.attend(gpu_runner, o, lse, 2)
+    batch.check(o, lse, 2)
+    for x in caches:
+        x[first:first + pool] = 0
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_the_same_bits_again(gpu_runner, form):
+    """Eager calls one behind the other in one workspace, which holds any bytes, then what the call before left there."""
+    batch = batch_of(form, 64)
+    o, lse = batch.outputs(True)
+    ws = batch.attend(gpu_runner, o, lse, 2)
+    batch.check(o, lse, 2)
+    first = o.clone(), lse.clone()
+    for fill in (None, 0xff, None, 0x3f):
+        if fill is not None:
+            ws.fill_(fill)
+        o, lse = batch.outputs(True)
+        assert batch.attend(gpu_runner, o, lse, 2, workspace=ws) is ws
+        assert torch.equal(o, first[0]) and torch.equal(lse, first[1])
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("which,scale", [(1, 255), (3, 254)])
+def test_keys_and_queries_that_are_no_numbers(gpu_runner, form, which, scale):
+    """Rows that see such a key, or are one, get NaN; all others what they get without it."""
+    batch = batch_of(form, 64)
+    g = batch.heads // batch.kv_heads
+    nan = torch.zeros(batch.total, batch.heads, dtype=torch.bool, device=batch.dev)
+    for b, (sq, sk) in enumerate(batch.lens):
+        key, head = (sk - 1, 1) if b % 2 == 0 else (sk - sq // 2 - 1, 6)
+        batch.caches[which][batch.table[b, key // 64], head, key % 64, b % 4] = scale
+        at, end = int(batch.offsets[b]), int(batch.offsets[b + 1])
+        nan[at + max(0, key - (sk - sq)):end, head * g:head * g + g] = True
+        batch.q[at, 4 * g, 100] = float("nan")
+        nan[at, 4 * g] = True
+    o, lse = batch.outputs(True)
+    batch.attend(gpu_runner, o, lse, 2)
+    batch.check(o, lse, 2, nan_rows=nan)
