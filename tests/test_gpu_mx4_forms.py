@@ -1,11 +1,11 @@
 """Each form of the 4-bit caches' attention kernels (row tiles of 16, 32, 128 and 256 rows, whole and on a line), over
-caches past 4 GiB, keys and queries that are no numbers, and again.  tests/test_mx4_launches.py holds every
+large pages, caches past 4 GiB, keys and queries that are no numbers, and again.  tests/test_mx4_launches.py holds every
 batch to the form that it is here for."""
 import numpy as np
 import pytest
 import torch
 
-from tests.mx4 import Cache4
+from tests.mx4 import Cache4, assert_guard_rows_untouched
 
 pytestmark = pytest.mark.gpu
 
@@ -21,12 +21,23 @@ FORMS = {
     "many_line_128": (("prefill", "line", 128, 256), 16, 8, [(100, 4000), (40, 1500), (70, 70)] * 2),
     "many_line_256": (("prefill", "line", 256, 512), 16, 8, [(300, 9000), (250, 2000)]),
 }
-PAGES = [64, 128]
+PAGES = [64, 128, 192, 1024]
 
 
 def batch_of(form, page, **more):
     _, heads, kv_heads, lens = FORMS[form]
     return Cache4(heads, kv_heads, page, lens, **more)
+
+
+@pytest.mark.parametrize("causal", [0, 2])
+@pytest.mark.parametrize("page", PAGES[1:])
+@pytest.mark.parametrize("form", FORMS)
+def test_pages_of_more_than_a_tile(gpu_runner, form, page, causal):
+    batch = batch_of(form, page)
+    o, lse = batch.outputs(True)
+    batch.attend(gpu_runner, o, lse, causal)
+    batch.check(o, lse, causal)
+    assert_guard_rows_untouched(batch)
 
 
 @pytest.fixture(scope="module")
