@@ -110,3 +110,39 @@ def test_keys_and_queries_that_are_no_numbers(gpu_runner, form, which, scale):
     o, lse = batch.outputs(True)
     batch.attend(gpu_runner, o, lse, 2)
     batch.check(o, lse, 2, nan_rows=nan)
+
+
+# Heads of one K/V head that fill more than a row tile, so that a token's rows lie in several.
+WIDE = [(96, 1, [(1, 700), (1, 0), (1, 65)]), (300, 1, [(1, 700), (3, 2), (2, 1300)]), (512, 1, [(1, 3000), (5, 90)]),
+        (516, 2, [(7, 2000), (0, 3), (1, 1)] * 3), (2000, 1, [(30, 500)])]
+
+
+@pytest.mark.parametrize("causal", [0, 2])
+@pytest.mark.parametrize("heads,kv_heads,lens", WIDE, ids=str)
+def test_wide_groups(gpu_runner, heads, kv_heads, lens, causal):
+    batch = Cache4(heads, kv_heads, 32, lens)
+    o, lse = batch.outputs(True)
+    batch.attend(gpu_runner, o, lse, causal)
+    batch.check(o, lse, causal)
+    assert_guard_rows_untouched(batch)
+
+
+@pytest.mark.parametrize("sequences", [1, 600_000])
+def test_queries_past_4_gib(gpu_runner, sequences):
+    """600000 tokens of 32 heads, of one sequence or of one each; looked at are some at both ends and in the middle."""
+    tokens, keys = 600_000, 70
+    batch = Cache4(32, 8, 64, [(1, keys)])
+    gen = torch.Generator(device=batch.dev).manual_seed(2)
+    q = torch.randn(tokens, 32, 128, generator=gen, device=batch.dev, dtype=torch.bfloat16)
+    assert q.nbytes > 1 << 32
+    o, lse = torch.full_like(q, float("nan")), torch.full((32, tokens), float("nan"), device=batch.dev)
+    cu = torch.arange(0, tokens + 1, tokens // sequences, dtype=torch.int32, device=batch.dev)
+    table = batch.table_d.expand(sequences, -1).contiguous()
+    seqlens = batch.seqlens.expand(sequences).contiguous()
+    gpu_runner.call_paged_mx4(q, *batch.caches, o, lse, cu, seqlens, table, tokens // sequences, keys, causal=0)
+    middle = (1 << 32) // (32 * 256)
+    for at in (0, middle - 150, tokens - 300):
+        part = slice(at, at + 300)
+        batch.lens, batch.offsets, batch.total = [(300, keys)], np.array([0, 300]), 300
+        batch.check(o[part], lse[:, part], 0, q=q[part])
+    assert not o.isnan().any() and not lse.isnan().any()

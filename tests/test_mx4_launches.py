@@ -4,7 +4,7 @@ import pytest
 
 from tests import launches
 from tests.test_gpu_mx4_calls import KINDS
-from tests.test_gpu_mx4_forms import FORMS, PAGES
+from tests.test_gpu_mx4_forms import FORMS, PAGES, WIDE
 
 
 @pytest.fixture(scope="module")
@@ -41,6 +41,19 @@ CALLS = {"whole": ("decode", "whole", 16, 512), "line": ("decode", "line", 16, 2
 def test_kinds(lib, name, page):
     for lse in (False, True):
         assert form(launches.attention(lib, 8, 2, page, KINDS[name], 2, lse=lse)) == CALLS[name]
+
+
+def test_wide_groups(lib):
+    """More rows a token than a row tile has, in three of the kernels."""
+    got = [launches.kind(launches.attention(lib, h, kvh, 32, lens, 2)) for h, kvh, lens in WIDE]
+    assert {k for k, *_ in got} == {"decode", "prefill"} and {c for _, c, _ in got} == {"whole", "line"}, got
+    assert all(h // kvh > rows for (h, kvh, _), (*_, rows) in zip(WIDE, got)), got
+
+
+def test_queries_past_4_gib(lib):
+    one = launches.attention(lib, 32, 8, 64, [(600_000, 70)], 0)
+    each = launches.attention(lib, 32, 8, 64, [(1, 70)] * 600_000, 0)
+    assert launches.kind(one)[0] == "prefill" and launches.kind(each)[0] == "decode"
 
 
 def test_launches_fit_a_grid(lib):
