@@ -288,7 +288,7 @@ __device__ __forceinline__ float quad_sum(float x) {
 //  * Keys are hidden by their scores, so V needs no other care than to be finite: a block
 //    with a scale above 252 becomes 0 there, and its key's scores NaN by way of its K
 //    scale.
-// Bound by memory where the GPU is full (32 sequences of 4096..16384, H32 KVH8: 76 us, 6.4
+// Bound by memory where the GPU is full (32 sequences of 4096..32768, H32 KVH8: 76 us, 6.4
 // TB/s over the whole kernel), else by a wave's chain of conversions, products, softmax and
 // LDS, 1.8 us for 64 keys.  Two or three tiles ahead, four waves a SIMD, V converted before
 // the scores or read ahead of the softmax, rows of LDS padded by 32 bytes: no quicker.
