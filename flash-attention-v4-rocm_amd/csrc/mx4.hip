@@ -111,15 +111,20 @@ double line_keys(int max_keys) { return std::max(128.0, 4 * std::sqrt(double(max
 // each at once, above eight teams four: 24 of 1000..16384, H8 KVH1, 15.5 so and 16.5 with
 // four, 48 of 100..4096, H32 KVH8, 19.4 and with eight 20.2 (20.6 with four of eight parts
 // each, many of whose loads find no part).  Of many rows one team takes four, or four two:
-// 59 queries behind 6778 keys, H8 KVH1, 26.2 with four, 27.2 with one; 4 x 56 behind 1278 to
-// 4502, H40 KVH8, 47.3 and 43.3.
+// 5 x 329 queries behind 329..1216 keys, H16 KVH1, 31.1 with one and 34.3 with four; 2 x
+// 30..99 behind 4503, H40 KVH8, 36.1 and 39.6; 3 x 7..15 behind 29006..77731, H32 KVH1, 61.5
+// and 47.7; one of 30 behind 26965, H32 KVH8, 45.4 and 41.1.  Over 40 such batches the limit
+// costs 6% less than one team for all, and 1% less than four.
 constexpr int MERGE_PARTS = 16;
 // Whether a call goes by the decode kernel: with up to FEW_ROWS rows a sequence, and with
 // more where its row tiles of 32 are no more than the CUs and read so few keys in all (and
 // what their starts and ends cost) that the GPU is not full.  Decode / prefill kernels: H8
 // KVH1, 64 x 8 queries behind 1000..4000 25.3 / 28.5; H32 KVH8, 32 x 16 behind 2000..8000
 // 78.6 / 90.7, 32 x 20 109 / 94, 8 x 20 behind 500..2000 16.7 / 26.1; prompts, one of 128
-// 6.6 / 7.8, 13 of 26 26.7 / 6.8.
+// 6.6 / 7.8, 13 of 26 26.7 / 6.8.  The two limits are what parts such measurements, and have
+// no other reason.  Over 60 batches of 100 to 800 pairs of a row tile of 32 and a K/V head,
+// drawn apart from those (19 of them go by the decode kernel), the choice costs 0.9% more than
+// the quicker kernel; at the worst, one of 1022 behind 2730, H8 KVH1, 20.2 / 32.8.
 constexpr int FEW_ROWS = 64;
 bool few_rows(int64_t seq_rows, double rows, double keys, int64_t batch, int kv_heads, int cus) {
     if (seq_rows <= FEW_ROWS) return true;
@@ -145,20 +150,25 @@ bool whole_sequences(int64_t pairs, int64_t rows, int64_t max_keys, double all_k
 }
 
 // Key tiles of many rows that a range should have at least: with a half, 0.3, 0.8 times the
-// longest's root, and one, 3 sequences of 20..54 queries behind 488..2460 22.3, 26.4, 22.9
-// and 26.9 us; one of 59 behind 6778, H8 KVH1, 26.2, 25.0, 30.3 and 33.4.
+// longest's root, and one, 3 sequences of 14 queries behind 28774..109665, H8 KVH1, 48.4, 54.4,
+// 60.2 and 54.8 us; 3 of 18..42 behind 14379..85937, H8 KVH1, 59.4, 52.0, 78.5 and 52.1; one of
+// 30 behind 26965, H32 KVH8, 41.1, 35.9, 38.1 and 35.9.  Over 40 batches whose ranges it
+// decides 0.3 and one cost 1% less than a half, 0.8 costs 10% more.
 double range_tiles(double most) { return std::max(1.0, 0.5 * std::sqrt(most)); }
 
 // Sequences of many rows: row tiles of eight waves (256 rows, one workgroup a CU) or four
 // (128, two), each whole, the longest first, or on a line.  By an estimate in us of each,
 // from the sizes (of unequal lengths their means and the longest), its constants fitted to
-// 120 batches timed all four ways; over 40 others its choice costs 1% more than the best.  A
+// 120 batches timed all four ways, among them some that few_rows has since sent to the decode
+// kernel; over 60 others that come here its choice costs 1.2% more than the best (at the
+// worst 16%: one of 797 behind 1059, dense, H16 KVH16, 36.3 / 27.8 / 33.2 / 32.2).  A
 // 64-key tile takes a workgroup of eight waves 1.9, one of four 2.06 in a full GPU (2.15 on
 // a line) and 1.3 alone; a row tile starts and ends in 4 (2.2), on a line in 6.8; a line's own
 // start, the second launch and its merge take 15.  Measured, H32 KVH8 where not said, whole 8
 // / whole 4 / line 8 / line 4: 8 x 64..512 queries behind 1024..8192 keys 227 / 188 / 156 /
 // 172; prompts of 500..2500 134 / 137 / 148 / 162; 2 prompts of 146 and 134 behind 224, H40,
-// 13.7 / 10.9 / 20.5 / 17.9; one of 95 behind 3387, H8 KVH1, 97.9 / 73.3 / 23.3 / 20.0.
+// 13.7 / 10.9 / 20.5 / 17.9; 5 x 144..316 behind 1590..11482 319 / 249 / 136 / 146; 4 x 84
+// behind 3328..14065, dense, 390 / 290 / 83.9 / 80.6.
 struct Cut {
     int waves, ranges;                // ranges of a K/V head, 0: whole
     double parts;                     // of the longest row tile on a line, about
