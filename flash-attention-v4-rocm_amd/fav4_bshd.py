@@ -840,8 +840,9 @@ class Runner:
     def call_paged_mx4(self, q, k_cache, k_scales, v_cache, v_scales, o, lse, cu_q, seqlens_k, block_table, max_q,
                        max_k, workspace=None, total_k=None, scale=None, stream=None, causal=0):
         """fav4_bshd_forward_paged_mx4: attention over 4-bit caches (see mx4_caches); the other tensors as for
-        paged_args.  causal 0 dense, 2 bottom-right.  `workspace` as for call_splitkv (None: allocated here); returned
-        for the next call."""
+        paged_args, but for total_k: the sum of seqlens_k, which steers the cut alone; None (0) takes every sequence
+        for max_k long.  causal 0 dense, 2 bottom-right.  `workspace` as for call_splitkv (None: allocated here);
+        returned for the next call."""
         import torch
         block = self.mx4_blocks.paged(q, k_cache, k_scales, v_cache, v_scales, o, lse, cu_q, seqlens_k, block_table,
                                       max_q, max_k, total_k, scale)

@@ -43,6 +43,17 @@ def test_kinds(lib, name, page):
         assert form(launches.attention(lib, 8, 2, page, KINDS[name], 2, lse=lse)) == CALLS[name]
 
 
+def test_a_sum_that_is_not_known(lib):
+    """total_k 0 is taken as batch * max_seqlen_k; the rule of the BF16 call, one less, is not this one's."""
+    for lens, causal in (([(1, 32768)] + [(1, 300)] * 31, 0), ([(4, 3000), (4, 100)] * 9, 2), ([(300, 4000), (20, 30)] * 5, 2)):
+        most = len(lens) * max(k for _, k in lens)
+        not_known = launches.attention(lib, 32, 8, 64, lens, causal)
+        assert not_known == launches.attention(lib, 32, 8, 64, lens, causal, total_k=most)
+    skewed = [(1, 32768)] + [(1, 300)] * 31
+    assert launches.kind(launches.attention(lib, 32, 8, 64, skewed, 0))[1] == "whole"
+    assert launches.kind(launches.attention(lib, 32, 8, 64, skewed, 0, total_k=32768 + 31 * 300))[1] == "line"
+
+
 def test_wide_groups(lib):
     """More rows a token than a row tile has, in three of the kernels."""
     got = [launches.kind(launches.attention(lib, h, kvh, 32, lens, 2)) for h, kvh, lens in WIDE]
