@@ -73,17 +73,22 @@ extern "C" int fav4_bshd_gather_paged_mx4(const Fav4Mx4GatherArgs* args, hipStre
 //    it gets O and LSE of NaN in all dims, and so does one whose query holds a NaN; rows
 //    that do not see the key are not touched by it, nor by what slots behind seqlens_k
 //    and hidden keys hold.
+//  * A query that holds an infinity has no finite score: its row's O and LSE are NaN, or as
+//    without keys where all its scores are -inf.
+//  * Scores and sums are FP32.  Where one passes 3.4e38, which needs keys of more than some
+//    1e36 (an append stores numbers of up to 2.6e38), O and LSE of the rows that see the key
+//    are infinite or NaN, and of no others.
 //  * K and V enter the matrix products as BF16, which holds their numbers exactly;
 //    weights are rounded to BF16 and O is divided by the sum of the rounded ones, as in
 //    the forward.  Results are the same from call to call.
 //  * total_k, the sum of seqlens_k, steers how the call is cut and nothing else, by a rule
 //    that is not fav4_bshd.h's: 0 says that the sum is not known, and every sequence is then
 //    taken for max_seqlen_k long, as with batch * max_seqlen_k; one less than that is a sum
-//    like any other.  The cut is chosen on the host, so a captured call keeps it.  Short
-//    batches of up to as many sequences and K/V heads as CUs get a workgroup for each whole
-//    sequence where all are taken for long: 32 x 1 queries, 32 / 8 heads, max_seqlen_k 32768,
-//    with the sum and without: one of 32768 keys and 31 of 300 19 and 116 us, all of 300
-//    18 and 6, all of 32768 169 both.
+//    like any other.  The cut is chosen on the host, so a captured call keeps it.  Where
+//    all sequences are taken for long and there are no more pairs of one and a K/V head than
+//    CUs, each pair gets a workgroup: 32 x 1 queries, 32 / 8 heads, max_seqlen_k 32768, with
+//    the sum and without: one of 32768 keys and 31 of 300 19 and 116 us, all of 300 18 and 6,
+//    all of 32768 169 both.
 struct Fav4Mx4PagedArgs {
     Fav4PagedArgs paged;               // k_cache, v_cache: codes
     const void *k_scales, *v_scales;

@@ -146,3 +146,53 @@ def test_queries_past_4_gib(gpu_runner, sequences):
         batch.lens, batch.offsets, batch.total = [(300, keys)], np.array([0, 300]), 300
         batch.check(o[part], lse[:, part], 0, q=q[part])
     assert not o.isnan().any() and not lse.isnan().any()
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_infinite_queries(gpu_runner, form):
+    """Scores are then infinite or no numbers: O and LSE are NaN, or where all of a row's are -inf those of a row that sees
+    no key.  Other rows do not notice."""
+    batch = batch_of(form, 64)
+    g, dim, head = batch.heads // batch.kv_heads, 37, 5
+    kinds = torch.zeros(batch.total, dtype=torch.long, device=batch.dev)       # 1: no number, 2: as without keys
+    for b, (sq, sk) in enumerate(batch.lens):
+        k = batch.keys(b)[0][:, head // g, dim]
+        gain = float("inf") if b % 2 else float("-inf")
+        rows = slice(int(batch.offsets[b]), int(batch.offsets[b + 1]))
+        batch.q[rows, head, dim] = gain
+        sees_other = torch.cumsum((k * np.sign(gain) >= 0).long(), 0)[sk - sq:] > 0    # a key whose score is not -inf
+        kinds[rows] = torch.where(sees_other, 1, 2)
+    o, lse = batch.outputs(True)
+    batch.attend(gpu_runner, o, lse, 2)
+    assert o[kinds == 1, head].isnan().all() and lse[head, kinds == 1].isnan().all()
+    assert (o[kinds == 2, head] == 0).all() and torch.isneginf(lse[head, kinds == 2]).all()
+    # The others, with those rows as any.
+    want, want_lse = batch.outputs(True)
+    batch.q[:, head, dim] = 1
+    batch.attend(gpu_runner, want, want_lse, 2)
+    o[:, head], lse[head] = want[:, head], want_lse[head]
+    assert torch.equal(o, want) and torch.equal(lse, want_lse)
+    batch.check(want, want_lse, 2)
+
+
+@pytest.mark.parametrize("form", FORMS)
+def test_the_largest_keys_touch_only_rows_that_see_them(gpu_runner, form):
+    """Keys of 6 * 2^125 in all dims, whose scores and weighted sums pass FP32: whatever the rows get that see them, the
+    others get the bits that they get without."""
+    batch = batch_of(form, 64)
+    want = [x.clone() for x in batch.outputs(True)]
+    batch.attend(gpu_runner, *want, 2)
+    batch.check(*want, 2)
+    sees = torch.zeros(batch.total, batch.heads, dtype=torch.bool, device=batch.dev)
+    g = batch.heads // batch.kv_heads
+    for b, (sq, sk) in enumerate(batch.lens):
+        key, head = sk - max(1, sq // 3), b % batch.kv_heads
+        page, slot = batch.table[b, key // 64], key % 64
+        for x, byte in zip(batch.caches, (0xf7, 252, 0x7f, 252)):
+            x[page, head, slot] = byte
+        at, end = int(batch.offsets[b]), int(batch.offsets[b + 1])
+        sees[at + max(0, key - (sk - sq)):end, head * g:head * g + g] = True
+    o, lse = batch.outputs(True)
+    batch.attend(gpu_runner, o, lse, 2)
+    assert torch.equal(o[~sees], want[0][~sees]) and torch.equal(lse.T[~sees], want[1].T[~sees])
+    assert (~sees).any() and not torch.equal(o[sees], want[0][sees])
