@@ -285,6 +285,11 @@ __device__ __forceinline__ float quad_sum(float x) {
 //    holding keys 4g + e of both subtiles of 32 keys.  V is converted as K is and goes
 //    through LDS of the wave's own, from where ds_read_b64_tr_b16 reads it turned.  The
 //    sums of the weights come from one more MFMA, against ones.
+//  * The weights are rounded to BF16 for that product, as the forward's are, because FP32
+//    MFMAs take 16 times as long and a second BF16 part of the weights twice: O is off by
+//    0.0020 to 0.0023 of its size against 64 bits, with FP32 weights by 0.0017 (its own
+//    rounding alone).  O is divided by the sum of the rounded ones; that, the LSE's sum and
+//    all parts stay FP32.
 //  * Keys are hidden by their scores, so V needs no other care than to be finite: a block
 //    with a scale above 252 becomes 0 there, and its key's scores NaN by way of its K
 //    scale.

@@ -75,9 +75,9 @@ extern "C" int fav4_bshd_gather_paged_mx4(const Fav4Mx4GatherArgs* args, hipStre
 //    and hidden keys hold.
 //  * A query that holds an infinity has no finite score: its row's O and LSE are NaN, or as
 //    without keys where all its scores are -inf.
-//  * Scores and sums are FP32.  Where one passes 3.4e38, which needs keys of more than some
-//    1e36 (an append stores numbers of up to 2.6e38), O and LSE of the rows that see the key
-//    are infinite or NaN, and of no others.
+//  * Scores and sums are FP32.  Where one passes 3.4e38 (with queries of about 1 that takes
+//    keys of some 1e36, and an append stores numbers of up to 2.6e38), O and LSE of the rows
+//    that see the key are infinite or NaN, and of no others.
 //  * K and V enter the matrix products as BF16, which holds their numbers exactly;
 //    weights are rounded to BF16 and O is divided by the sum of the rounded ones, as in
 //    the forward.  Results are the same from call to call.
